@@ -15,7 +15,7 @@ import torch  # noqa: F401  (must precede CDLL, see module docstring)
 
 MAX_PATHS = 128
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libictc_hip.so")
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 
 class TpDesc(ctypes.Structure):
@@ -40,6 +40,19 @@ class DegreeLinearDesc(ctypes.Structure):
         ("channels", ctypes.c_int32),
         ("out_channels", ctypes.c_int32),
         ("counts", ctypes.c_int32 * 8),
+    ]
+
+
+class AdamwDesc(ctypes.Structure):
+    """Mirror of ``ictc_adamw_desc``."""
+    _fields_ = [
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("lr", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("seed", ctypes.c_uint32),
+        ("moment_bits", ctypes.c_int32),
     ]
 
 
@@ -121,6 +134,10 @@ _SIGNATURES = {
     "ictc_hip_gates_input_grad": (ctypes.c_int, [_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P]),
     "ictc_hip_gates_weight_grad_workspace": (_I64, [_I64, _I64]),
     "ictc_hip_gates_weight_grad": (ctypes.c_int, [_P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P]),
+    "ictc_hip_gradient_norm_workspace": (_I64, [_I64]),
+    "ictc_hip_gradient_norm": (ctypes.c_int, [_P, _P, _I64, ctypes.c_float, _P, _I64, _P, _P]),
+    "ictc_hip_adamw_step": (ctypes.c_int, [_P, _P, _P, _I64, ctypes.POINTER(AdamwDesc)] + [_P] * 8),
+    "ictc_hip_moment_values": (ctypes.c_int, [_P] * 6 + [_I64, _P]),
     "ictc_hip_sgemm": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _I64, _I64, _I64, ctypes.c_float, _P, _I64, _P,
                                       _I64, ctypes.c_float, _P, _I64, _P]),
     "ictc_hip_radius_graph_bins": (ctypes.c_int, [ctypes.POINTER(CellGrid), _P, _I64, _P, _P, _P, _P, _P, _P]),

@@ -1,0 +1,177 @@
+"""The optimizer step on ``libictc_hip.so``: the norm of all gradients and one AdamW update of many
+tensors (``ictc_hip_gradient_norm``, ``ictc_hip_adamw_step``; no counterpart in the reference, whose
+training loop uses torch's optimizers).  Formulas and the 8-bit format stand in ``ictc_hip.h``.
+
+Nothing here reads from the device or copies to it: the tensors' addresses are kernel arguments, and
+steps, clipping coefficient and (where it is a tensor) the learning rate stay on the device, so a step
+can be captured into a HIP graph.  ``ictc_o3.optim.AdamW`` is the optimizer on top.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from contextlib import nullcontext
+
+import torch
+
+from ictc_o3 import _lib
+
+MOMENT_BLOCK = 256
+
+
+def _on(device: torch.device):
+    """The launch's device made current where it is not (streams belong to a device)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _flat(tensors, what: str) -> torch.device:
+    """Checks FP32 GPU tensors (None allowed) on one device; their device."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or t.dtype is not torch.float32 or t.layout is not torch.strided:
+            raise ValueError(f"{what} must be dense FP32 tensors on a ROCm GPU")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"{what} must be on the same GPU")
+    return device
+
+
+def state_values(sizes) -> int:
+    """Values of the flat moments for tensors of these sizes (each padded to whole blocks)."""
+    return sum(-(-n // MOMENT_BLOCK) for n in sizes) * MOMENT_BLOCK
+
+
+def new_state(params, moment_bits: int = 32):
+    """(exp_avg, exp_avg_sq, progress) before the first step: zeros, and no steps for each tensor.
+    8-bit moments are (codes, block exponents) pairs."""
+    params = list(params)
+    device = _flat(params, "parameters")
+    if device is None:
+        raise ValueError("expected at least one parameter")
+    total = state_values([p.numel() for p in params])
+    if moment_bits == 32:
+        moments = [torch.zeros(total, device=device) for _ in range(2)]
+    elif moment_bits == 8:
+        moments = [(torch.zeros(total, device=device, dtype=torch.uint8),
+                    torch.zeros(total // MOMENT_BLOCK, device=device, dtype=torch.uint8)) for _ in range(2)]
+    else:
+        raise ValueError("moment_bits must be 32 or 8")
+    progress = torch.zeros(len(params) + 1, 3, device=device, dtype=torch.float64)
+    progress[:-1, 1:] = 1.0
+    return moments[0], moments[1], progress
+
+
+def gradient_norm(grads, max_norm=None) -> torch.Tensor:
+    """[norm, coefficient] on the device: the 2-norm of all gradients together and min(1, max_norm /
+    norm) (1 without max_norm; not-a-number for a norm that is not finite, with which ``adamw_step``
+    leaves everything as it is).  The gradients are not changed; entries that are None are left out."""
+    grads = [g for g in grads if g is not None]
+    device = _flat(grads, "gradients")
+    if device is None:
+        raise ValueError("expected at least one gradient")
+    if max_norm is not None and not float(max_norm) > 0.0:
+        raise ValueError("max_norm must be positive, or None for no limit")
+    limit = 0.0 if max_norm is None or math.isinf(max_norm) else float(max_norm)
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    n = len(grads)
+    out = torch.empty(2, device=device)
+    lib = _lib.lib()
+    doubles = lib.ictc_hip_gradient_norm_workspace(n)
+    workspace = torch.empty(doubles, device=device, dtype=torch.float64)
+    with _on(device):
+        _lib.check(lib.ictc_hip_gradient_norm(
+            (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_int64 * n)(*[g.numel() for g in grads]), n,
+            limit, workspace.data_ptr(), doubles, out.data_ptr(), _lib.stream_of(device)), "ictc_hip_gradient_norm")
+    return out
+
+
+def _moments(state, values: int, device, what: str):
+    """(address of the values or codes, address of the exponents or None, bits)."""
+    if isinstance(state, torch.Tensor):
+        if state.dtype is not torch.float32 or state.numel() != values or not state.is_contiguous() \
+                or state.device != device:
+            raise ValueError(f"{what} must be a contiguous FP32 tensor of {values} values beside the parameters")
+        return state.data_ptr(), None, 32
+    codes, top = state
+    if (codes.dtype is not torch.uint8 or top.dtype is not torch.uint8 or codes.numel() != values
+            or top.numel() * MOMENT_BLOCK != values or not codes.is_contiguous() or not top.is_contiguous()
+            or codes.device != device or top.device != device):
+        raise ValueError(f"{what} must be contiguous uint8 codes ({values}) and exponents "
+                         f"({values // MOMENT_BLOCK}) beside the parameters")
+    return codes.data_ptr(), top.data_ptr(), 8
+
+
+def _number(value, name: str, below: float = math.inf) -> float:
+    if isinstance(value, bool) or not isinstance(value, (int, float)) or not 0.0 <= value < below:
+        raise ValueError(f"{name} must be a number in [0, {below})")
+    return float(value)
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, progress, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               clip=None, seed=0) -> None:
+    """One AdamW step of every parameter with a gradient, in place (a None gradient leaves its
+    parameter, moments and steps as they are).
+
+    exp_avg, exp_avg_sq, progress: as ``new_state`` makes them (float32 moments, or pairs of 8-bit codes
+    and block exponents).  lr: a number, or a one-element float32 tensor on the device.  clip:
+    ``gradient_norm``'s result, whose coefficient scales the gradients.  seed: of the 8-bit rounding."""
+    params, grads = list(params), list(grads)
+    n = len(params)
+    if n == 0 or len(grads) != n:
+        raise ValueError("expected one gradient (or None) for each parameter")
+    device = _flat(params, "parameters")
+    sizes = []
+    for p, g in zip(params, grads):
+        if p is None or not p.is_contiguous():
+            raise ValueError("parameters must be contiguous")
+        if g is not None and g.shape != p.shape:
+            raise ValueError("a gradient must have its parameter's shape")
+        sizes.append(p.numel())
+    if _flat(grads, "gradients") not in (None, device):
+        raise ValueError("parameters and gradients must be on the same GPU")
+    grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
+    values = state_values(sizes)
+    m, m_top, bits = _moments(exp_avg, values, device, "exp_avg")
+    v, v_top, v_bits = _moments(exp_avg_sq, values, device, "exp_avg_sq")
+    if bits != v_bits:
+        raise ValueError("exp_avg and exp_avg_sq must have the same number of bits")
+    if progress.shape != (n + 1, 3) or progress.dtype is not torch.float64 or not progress.is_contiguous() \
+            or progress.device != device:
+        raise ValueError(f"progress must be a contiguous float64 tensor [{n + 1}, 3] beside the parameters")
+    if clip is not None and (clip.dtype is not torch.float32 or clip.shape != (2,) or clip.device != device
+                             or not clip.is_contiguous()):
+        raise ValueError("clip must be gradient_norm's result")
+    lr_device = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.device != device:
+            raise ValueError("a learning rate tensor must hold one FP32 value beside the parameters")
+        lr_device, lr = lr.data_ptr(), 0.0
+    desc = _lib.AdamwDesc(_number(betas[0], "beta1", 1.0), _number(betas[1], "beta2", 1.0),
+                          _number(weight_decay, "weight_decay"), _number(lr, "lr"), _number(eps, "eps"),
+                          int(seed) & 0xFFFFFFFF, bits)
+    with _on(device):
+        _lib.check(_lib.lib().ictc_hip_adamw_step(
+            (ctypes.c_void_p * n)(*[p.data_ptr() for p in params]),
+            (ctypes.c_void_p * n)(*[None if g is None else g.data_ptr() or 16 for g in grads]),
+            (ctypes.c_int64 * n)(*sizes), n, ctypes.byref(desc), m, v, m_top, v_top, progress.data_ptr(),
+            _lib.ptr(clip), lr_device, _lib.stream_of(device)), "ictc_hip_adamw_step")
+    # the kernel writes through addresses: tell autograd (and caches keyed on versions) of the change
+    torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+
+
+def moment_values(exp_avg, exp_avg_sq):
+    """8-bit moments as the values they stand for, bfloat16 (which holds them exactly)."""
+    codes = exp_avg[0]
+    values, device = codes.numel(), codes.device
+    if not codes.is_cuda or values % MOMENT_BLOCK:
+        raise ValueError("expected 8-bit moments on a ROCm GPU")
+    m, m_top, _ = _moments(exp_avg, values, device, "exp_avg")
+    v, v_top, _ = _moments(exp_avg_sq, values, device, "exp_avg_sq")
+    out = [torch.empty(values, device=device, dtype=torch.bfloat16) for _ in range(2)]
+    with _on(device):
+        _lib.check(_lib.lib().ictc_hip_moment_values(m, m_top, v, v_top, out[0].data_ptr(), out[1].data_ptr(), values,
+                                                     _lib.stream_of(device)), "ictc_hip_moment_values")
+    return out[0], out[1]

@@ -690,6 +690,61 @@ int ictc_hip_gates_weight_grad(const float *grad, int64_t grad_row_stride, const
                                int64_t edges, int64_t width, hipStream_t stream);
 
 /*
+ * The optimizer step of training (no counterpart in the reference, whose training loop uses torch's
+ * optimizers).  `params`, `grads`, `elements` and their like are host arrays of `count` entries; the
+ * device addresses in them are read before the call returns.
+ *
+ * ictc_hip_gradient_norm: out[0] = the 2-norm of all gradients together (sums of squares in 64 bits, in
+ * a fixed order), out[1] = the coefficient that brings it to max_norm, min(1, max_norm / norm); 1 for
+ * max_norm <= 0, and not-a-number where the norm is not finite.  The gradients are not changed.
+ * workspace: ictc_hip_gradient_norm_workspace(count) doubles (negative: -ictc_status).
+ *
+ * ictc_hip_adamw_step: for every tensor with a gradient (a null one is left out, and its moments and
+ * steps stay as they are), with g = clip[1] * grad (clip null: grad),
+ *   m <- beta1 m + (1 - beta1) g         v <- beta2 v + (1 - beta2) g^2
+ *   p <- (1 - lr weight_decay) p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+ * A clip[1] that is not a number leaves everything as it is.  lr_device, if not null, is one float on the
+ * device that takes the place of desc->lr.  A tensor and its gradient may have any float alignment.
+ *
+ * exp_avg and exp_avg_sq are flat arrays over all `count` tensors (those without a gradient too), each
+ * tensor's values starting at the next multiple of ICTC_MOMENT_BLOCK; the values behind a tensor's end
+ * stay zero.  moment_bits 32: float, 16-byte aligned.  moment_bits 8: one byte a value, 4-byte aligned,
+ * and one exponent byte for each block in exp_avg_top and exp_avg_sq_top.  With f the block's byte, a
+ * value whose code has the low 3 bits a and the bits above them e (m: 4 bits below a sign bit; v: 5 bits) is
+ *   m = +-(e ? 8 + a : a) 2^(max(e,1) - 18) 2^(f - 127)      v = (e ? 8 + a : a) 2^(max(e,1) - 34) 2^(f - 127)
+ * (m 0x7f and v 0xff: not a number).  New values are rounded up or down at random, by 16 bits each of a
+ * hash of desc->seed, the tensor's step and the value's place; a v above zero is never stored as zero.
+ *
+ * progress: 3 (count + 1) doubles, per tensor its number of steps, beta1^steps and beta2^steps (0, 1, 1
+ * before the first); the last three are the kernel's own and start as zero.
+ *
+ * ictc_hip_moment_values: 8-bit moments (values: a multiple of ICTC_MOMENT_BLOCK) as bfloat16, which
+ * holds them exactly.
+ */
+#define ICTC_MOMENT_BLOCK 256
+
+typedef struct ictc_adamw_desc {
+    double beta1;              /* [0, 1) */
+    double beta2;              /* [0, 1) */
+    double weight_decay;       /* >= 0 */
+    float lr;                  /* >= 0 */
+    float eps;                 /* >= 0 */
+    uint32_t seed;             /* of the 8-bit rounding */
+    int32_t moment_bits;       /* 32 or 8 */
+} ictc_adamw_desc;
+
+int64_t ictc_hip_gradient_norm_workspace(int64_t count);
+int ictc_hip_gradient_norm(const float* const* grads, const int64_t* elements, int64_t count, float max_norm,
+                           double* workspace, int64_t workspace_doubles, float* out, hipStream_t stream);
+int ictc_hip_adamw_step(float* const* params, const float* const* grads, const int64_t* elements, int64_t count,
+                        const ictc_adamw_desc* desc, void* exp_avg, void* exp_avg_sq, uint8_t* exp_avg_top,
+                        uint8_t* exp_avg_sq_top, double* progress, const float* clip, const float* lr_device,
+                        hipStream_t stream);
+int ictc_hip_moment_values(const uint8_t* exp_avg, const uint8_t* exp_avg_top, const uint8_t* exp_avg_sq,
+                           const uint8_t* exp_avg_sq_top, void* exp_avg_bf16, void* exp_avg_sq_bf16,
+                           int64_t values, hipStream_t stream);
+
+/*
  * Row-major fp32 product C[m,n] = alpha * op(A) op(B) + beta * C on rocBLAS, for the dense
  * channel linears around the operators.  op(A) is [m,k]: A is stored [m,k] (lda >= k) or,
  * with trans_a != 0, [k,m] (lda >= m); likewise B with op(B) [k,n].  Each host thread uses
