@@ -10,7 +10,9 @@ Steps:
      degree-generic kernels);
   3. compile every TU to an object in parallel, largest first;
   4. link the objects and the API TUs into ``ictc_o3/lib/libictc_hip.so``;
-  5. build ``libictc_stream_probe.so`` beside bench.py from the repository root's
+  5. compile ``host_tensors.cpp`` (host code only: lists of torch tensors as arrays of addresses) against
+     torch's headers into the Python module ``ictc_o3/lib/ictc_host_tensors.so``;
+  6. build ``libictc_stream_probe.so`` beside bench.py from the repository root's
      ``stream_probe.hip`` (bench.py's streaming-bandwidth and FMA-rate reference; not part of
      the operator library).
 
@@ -29,6 +31,7 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+import sysconfig
 import time
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -39,6 +42,8 @@ GEN = os.path.join(HERE, "generated")
 OBJ = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(PKG, "ictc_o3", "lib")
 LIB = os.path.join(LIB_DIR, "libictc_hip.so")
+HOST_SRC = os.path.join(HERE, "host_tensors.cpp")
+HOST_LIB = os.path.join(LIB_DIR, "ictc_host_tensors.so")
 PROBE_SRC = os.path.join(REPO, "stream_probe.hip")
 PROBE_LIB = os.path.join(REPO, "libictc_stream_probe.so")
 
@@ -204,6 +209,19 @@ def _compile(src: str, incremental: bool = False) -> str:
     return obj
 
 
+def _build_host() -> None:
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(root, "include"),
+           "-I", sysconfig.get_paths()["include"], HOST_SRC, "-o", HOST_LIB + ".tmp", "-L", os.path.join(root, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-Wl,-rpath," + os.path.join(root, "lib")]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"host module build failed:\n{res.stderr}")
+    os.replace(HOST_LIB + ".tmp", HOST_LIB)
+
+
 def build(jobs: int | None = None, verbose: bool = True, incremental: bool = False) -> str:
     """Compile every unit (incremental: only units whose object is older than the unit or
     anything it includes) and link the library."""
@@ -211,9 +229,11 @@ def build(jobs: int | None = None, verbose: bool = True, incremental: bool = Fal
     combos = _combos()
     units = [os.path.join(HERE, s) for s in API_SOURCES] + _generate(combos)
     jobs = jobs or max(1, min(len(units), os.cpu_count() or 1))
-    with cf.ThreadPoolExecutor(max_workers=jobs) as pool:
-        objs = list(pool.map(lambda u: _compile(u, incremental), units))
     os.makedirs(LIB_DIR, exist_ok=True)
+    with cf.ThreadPoolExecutor(max_workers=jobs) as pool:
+        host = pool.submit(_build_host)
+        objs = list(pool.map(lambda u: _compile(u, incremental), units))
+        host.result()
     tmp = LIB + ".tmp"
     res = subprocess.run([HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", *objs, *LINK_LIBS, "-o", tmp],
                          capture_output=True, text=True)

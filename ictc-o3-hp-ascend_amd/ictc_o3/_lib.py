@@ -8,6 +8,8 @@ There is no fallback: if the library is missing every operator raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
@@ -15,6 +17,7 @@ import torch  # noqa: F401  (must precede CDLL, see module docstring)
 
 MAX_PATHS = 128
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libictc_hip.so")
+HOST_PATH = os.path.join(os.path.dirname(LIB_PATH), "ictc_host_tensors.so")
 ABI_VERSION = 27
 
 
@@ -178,6 +181,27 @@ def lib() -> ctypes.CDLL:
                 raise RuntimeError("libictc_hip.so ABI version mismatch; rebuild the library")
             _lib = handle
     return _lib
+
+
+_host = None
+
+
+def host():
+    """The host module that reads lists of tensors (``csrc/host_tensors.cpp``), opened once."""
+    global _host
+    if _host is not None:
+        return _host
+    with _lock:
+        if _host is None:
+            if not os.path.isfile(HOST_PATH):
+                raise RuntimeError(f"{os.path.basename(HOST_PATH)} not found beside {LIB_PATH}; build it with "
+                                   "`python ictc-o3-hp-ascend_amd/csrc/build.py`")
+            loader = importlib.machinery.ExtensionFileLoader("ictc_host_tensors", HOST_PATH)
+            spec = importlib.util.spec_from_loader("ictc_host_tensors", loader)
+            module = importlib.util.module_from_spec(spec)
+            loader.exec_module(module)
+            _host = module
+    return _host
 
 
 def check(status: int, what: str) -> None:

@@ -17,26 +17,12 @@ import torch
 from ictc_o3 import _lib
 
 MOMENT_BLOCK = 256
+_HERE = nullcontext()
 
 
 def _on(device: torch.device):
     """The launch's device made current where it is not (streams belong to a device)."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _flat(tensors, what: str) -> torch.device:
-    """Checks FP32 GPU tensors (None allowed) on one device; their device."""
-    device = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda or t.dtype is not torch.float32 or t.layout is not torch.strided:
-            raise ValueError(f"{what} must be dense FP32 tensors on a ROCm GPU")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f"{what} must be on the same GPU")
-    return device
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def state_values(sizes) -> int:
@@ -48,9 +34,9 @@ def new_state(params, moment_bits: int = 32):
     """(exp_avg, exp_avg_sq, progress) before the first step: zeros, and no steps for each tensor.
     8-bit moments are (codes, block exponents) pairs."""
     params = list(params)
-    device = _flat(params, "parameters")
-    if device is None:
+    if not params:
         raise ValueError("expected at least one parameter")
+    device = torch.device("cuda", _lib.host().addresses(params, "parameters")[0])
     total = state_values([p.numel() for p in params])
     if moment_bits == 32:
         moments = [torch.zeros(total, device=device) for _ in range(2)]
@@ -69,22 +55,23 @@ def gradient_norm(grads, max_norm=None) -> torch.Tensor:
     norm) (1 without max_norm; not-a-number for a norm that is not finite, with which ``adamw_step``
     leaves everything as it is).  The gradients are not changed; entries that are None are left out."""
     grads = [g for g in grads if g is not None]
-    device = _flat(grads, "gradients")
-    if device is None:
+    if not grads:
         raise ValueError("expected at least one gradient")
     if max_norm is not None and not float(max_norm) > 0.0:
         raise ValueError("max_norm must be positive, or None for no limit")
     limit = 0.0 if max_norm is None or math.isinf(max_norm) else float(max_norm)
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    n = len(grads)
+    _, at, sizes, contiguous = _lib.host().addresses(grads, "gradients")
+    if not contiguous:
+        grads = [g.contiguous() for g in grads]
+        _, at, sizes, _ = _lib.host().addresses(grads, "gradients")
+    n, device = len(grads), grads[0].device
     out = torch.empty(2, device=device)
     lib = _lib.lib()
     doubles = lib.ictc_hip_gradient_norm_workspace(n)
     workspace = torch.empty(doubles, device=device, dtype=torch.float64)
     with _on(device):
         _lib.check(lib.ictc_hip_gradient_norm(
-            (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_int64 * n)(*[g.numel() for g in grads]), n,
-            limit, workspace.data_ptr(), doubles, out.data_ptr(), _lib.stream_of(device)), "ictc_hip_gradient_norm")
+            at, sizes, n, limit, workspace.data_ptr(), doubles, out.data_ptr(), _lib.stream_of(device)), "ictc_hip_gradient_norm")
     return out
 
 
@@ -119,21 +106,11 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, progress, *, lr, betas=(0.9, 
     and block exponents).  lr: a number, or a one-element float32 tensor on the device.  clip:
     ``gradient_norm``'s result, whose coefficient scales the gradients.  seed: of the 8-bit rounding."""
     params, grads = list(params), list(grads)
-    n = len(params)
-    if n == 0 or len(grads) != n:
-        raise ValueError("expected one gradient (or None) for each parameter")
-    device = _flat(params, "parameters")
-    sizes = []
-    for p, g in zip(params, grads):
-        if p is None or not p.is_contiguous():
-            raise ValueError("parameters must be contiguous")
-        if g is not None and g.shape != p.shape:
-            raise ValueError("a gradient must have its parameter's shape")
-        sizes.append(p.numel())
-    if _flat(grads, "gradients") not in (None, device):
-        raise ValueError("parameters and gradients must be on the same GPU")
-    grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
-    values = state_values(sizes)
+    _, p_at, g_at, sizes, values, contiguous = _lib.host().pairs(params, grads, MOMENT_BLOCK)
+    if not contiguous:
+        grads = [g if g is None else g.contiguous() for g in grads]
+        _, p_at, g_at, sizes, values, _ = _lib.host().pairs(params, grads, MOMENT_BLOCK)
+    n, device = len(params), params[0].device
     m, m_top, bits = _moments(exp_avg, values, device, "exp_avg")
     v, v_top, v_bits = _moments(exp_avg_sq, values, device, "exp_avg_sq")
     if bits != v_bits:
@@ -154,12 +131,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, progress, *, lr, betas=(0.9, 
                           int(seed) & 0xFFFFFFFF, bits)
     with _on(device):
         _lib.check(_lib.lib().ictc_hip_adamw_step(
-            (ctypes.c_void_p * n)(*[p.data_ptr() for p in params]),
-            (ctypes.c_void_p * n)(*[None if g is None else g.data_ptr() or 16 for g in grads]),
-            (ctypes.c_int64 * n)(*sizes), n, ctypes.byref(desc), m, v, m_top, v_top, progress.data_ptr(),
+            p_at, g_at, sizes, n, ctypes.byref(desc), m, v, m_top, v_top, progress.data_ptr(),
             _lib.ptr(clip), lr_device, _lib.stream_of(device)), "ictc_hip_adamw_step")
     # the kernel writes through addresses: tell autograd (and caches keyed on versions) of the change
-    torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+    _lib.host().written(params, grads)
 
 
 def moment_values(exp_avg, exp_avg_sq):
