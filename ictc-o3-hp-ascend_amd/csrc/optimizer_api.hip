@@ -34,27 +34,41 @@ namespace {
 constexpr int kWaveSize = 64;
 constexpr int kThreads = 256;
 constexpr int kQuant = ICTC_MOMENT_BLOCK;        // values that share a scale: one wave, 4 a lane
-constexpr int kChunk = kQuant * (kThreads / kWaveSize);
-constexpr int kTensors = 96;                     // 40 bytes each, within the 4 KB of kernel arguments
-constexpr int kMaxBlocks = 2048;                 // 8 workgroups for each of 256 CUs
-constexpr int kNormTensors = 160;
-constexpr int kNormChunk = 4096;
-constexpr int kNormBlocks = 1024;
+constexpr int kWaves = kThreads / kWaveSize;
+constexpr int kTensors = 184;                    // 21 bytes each, within the 4 KB of kernel arguments
+constexpr int kMaskTensors = 16384;
+constexpr float kFastEps = 1e-11f;               // times 2^-24 above the root of the smallest normal float
+constexpr int64_t kStream = int64_t{1} << 24;     // values of a launch that no cache holds until their next use
+constexpr int64_t kMostGroups = int64_t{1} << 24;  // workgroups of a launch that streams
 
-struct StepTensor {
-  float* param;
-  const float* grad;
-  int64_t elements;
-  int64_t state;     // first value in the flat state
-  int32_t chunk;     // first chunk of this tensor in the launch
-  int32_t row;       // its row in progress
+// Blocks that a wave takes at a time.
+constexpr int step_blocks(bool small, bool past) { return small && past ? 4 : 1; }
+
+constexpr int kSkip = 4096;                      // 1 M values
+constexpr int kMaxBlocks = 2048;                 // 8 workgroups for each of 256 CUs (a launch that does not stream)
+constexpr int kNormTensors = 200;                // 20 bytes each
+constexpr int kNormChunk = 4096;
+constexpr int kNormBlocks = 2048;
+
+// The tensors of one launch, in the order of the flat state without gaps (one without a gradient has a
+// null address there).  Tensor i has the state's blocks [start[i], start[i + 1]), counted from the
+// launch's first, and its last block holds tail[i] values (256: 0).
+struct StepTable {
+  float* param[kTensors];
+  const float* grad[kTensors];
+  uint32_t start[kTensors + 1];
+  uint8_t tail[kTensors];
+  int64_t state;     // the launch's first block
+  int64_t row;       // the first tensor's row in progress
+  int32_t count;     // (of the host's)
+  uint32_t blocks;
 };
 
-struct StepTable {
-  StepTensor t[kTensors];
+// The tensors that take part in a step, one bit each.
+struct RowMask {
+  uint32_t bits[kMaskTensors / 32];
+  int64_t first;
   int32_t count;
-  int32_t chunks;
-  int32_t per_block;
 };
 
 struct StepArgs {
@@ -63,7 +77,6 @@ struct StepArgs {
   uint8_t* exp_avg_top;
   uint8_t* exp_avg_sq_top;
   double* progress;
-  unsigned* ticket;
   const float* clip;
   const float* lr_device;
   double beta1, beta2, weight_decay;
@@ -71,7 +84,7 @@ struct StepArgs {
   uint32_t seed;
 };
 
-static_assert(sizeof(StepTable) + sizeof(StepArgs) <= 4096, "kernel arguments are limited to 4 KB");
+static_assert(sizeof(StepTable) + sizeof(StepArgs) + 16 <= 4096, "kernel arguments are limited to 4 KB");
 
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
   x ^= x >> 16;
@@ -97,242 +110,380 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
   return ab > cd ? ab : cd;
 }
 
-// Exponent byte of a block from its largest finite magnitude.
-__device__ __forceinline__ int block_top(uint32_t largest) {
+// The codes of 4 values, a byte each.  m is the hardware's 8-bit float with 4 exponent bits (the largest
+// exponent's last code is its not-a-number), 2^8 the first power of two above it.
+__device__ __forceinline__ void decode_signed(uint32_t codes, int top, float* m) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes), false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes), true);
+  m[0] = ldexpf(lo[0], top - 135);
+  m[1] = ldexpf(lo[1], top - 135);
+  m[2] = ldexpf(hi[0], top - 135);
+  m[3] = ldexpf(hi[1], top - 135);
+}
+
+// v: 5 exponent and 3 mantissa bits; 0xff is not a number (looked for in all four at once).
+__device__ __forceinline__ void decode_unsigned(uint32_t codes, int top, float* v) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = ldexpf(__uint_as_float(((codes >> (8 * k)) & 0xFFu) << 20), top - 31);
+  if (((codes & 0x7F7F7F7Fu) + 0x01010101u) & codes & 0x80808080u) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (((codes >> (8 * k)) & 0xFFu) == 0xFFu) v[k] = __uint_as_float(0x7FC00000u);
+  }
+}
+
+__device__ __forceinline__ uint32_t max3(uint32_t a, uint32_t b, uint32_t c) {
+  const uint32_t ab = a > b ? a : b;
+  return ab > c ? ab : c;
+}
+
+constexpr uint32_t kInf = 0x7F800000u;
+
+// Exponent byte of a block from its values' magnitudes as integers; not finite: those left out (uniform).
+__device__ __forceinline__ int block_top(const float* x, bool& finite) {
+  uint32_t b[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) b[k] = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+  uint32_t largest = wave_max(max3(max3(b[0], b[1], b[2]), b[3], 0u));
+  finite = largest < kInf;
+  if (!finite) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) b[k] = b[k] < kInf ? b[k] : 0u;
+    largest = wave_max(max3(max3(b[0], b[1], b[2]), b[3], 0u));
+  }
   const int f = static_cast<int>((largest + 0x1FFFFFu) >> 23);
   return f < 1 ? 1 : f;
 }
 
-__device__ __forceinline__ uint32_t finite_magnitude(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
-  return b < 0x7F800000u ? b : 0u;
+// Four codes from values, their block's exponent byte and 16 random bits each.
+__device__ __forceinline__ uint32_t encode_signed(const float* m, int top, bool finite, const uint32_t* random) {
+  uint32_t out = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t x = __float_as_uint(ldexpf(fabsf(m[k]), 15 - top));
+    uint32_t code = (x + ((random[k] & 0xFFFFu) << 4)) >> 20;
+    if (!finite && !(fabsf(m[k]) < INFINITY)) code = 0x7Fu;
+    code |= (__float_as_uint(m[k]) >> 24) & 0x80u;
+    out |= code << (8 * k);
+  }
+  return out;
 }
 
-// m: sign, 4 exponent bits, 3 mantissa bits; top code 0x7e, 0x7f not a number
-__device__ __forceinline__ float decode_signed(uint32_t code, int top) {
-  const uint32_t size = code & 0x7Fu;
-  const float x = ldexpf(__uint_as_float(size << 20), top - 15);
-  const float y = size == 0x7Fu ? __uint_as_float(0x7FC00000u) : x;
-  return (code & 0x80u) ? -y : y;
+__device__ __forceinline__ uint32_t encode_unsigned(const float* v, int top, bool finite, const uint32_t* random) {
+  uint32_t out = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t b = __float_as_uint(v[k]), least = b < 1u ? b : 1u;    // above zero: at least code 1
+    uint32_t code = (__float_as_uint(ldexpf(v[k], 31 - top)) + ((random[k] >> 16) << 4)) >> 20;
+    code = code > least ? code : least;
+    if (!finite && !(v[k] < INFINITY)) code = 0xFFu;
+    out |= code << (8 * k);
+  }
+  return out;
 }
 
-__device__ __forceinline__ uint32_t encode_signed(float m, int top, uint32_t random16) {
-  const float x = ldexpf(fabsf(m), 15 - top);
-  const uint32_t code = (__float_as_uint(x) + (random16 << 4)) >> 20;
-  const uint32_t size = fabsf(m) < INFINITY ? code : 0x7Fu;
-  return size | ((__float_as_uint(m) >> 24) & 0x80u);
-}
-
-// v: 5 exponent bits, 3 mantissa bits; top code 0xfe, 0xff not a number
-__device__ __forceinline__ float decode_unsigned(uint32_t code, int top) {
-  const float x = ldexpf(__uint_as_float(code << 20), top - 31);
-  return code == 0xFFu ? __uint_as_float(0x7FC00000u) : x;
-}
-
-__device__ __forceinline__ uint32_t encode_unsigned(float v, int top, uint32_t random16) {
-  const float x = ldexpf(v, 31 - top);
-  uint32_t code = (__float_as_uint(x) + (random16 << 4)) >> 20;
-  code = code < 1u && v > 0.f ? 1u : code;
-  return v < INFINITY ? code : 0xFFu;
-}
-
-template <bool SMALL>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const StepTable table, const StepArgs a) {
+// Index of the last entry that is at most `value` (start[0] is, the unused ones are the largest number):
+// every lane compares its share and the ones are counted.
+template <int MOST>
+__device__ __forceinline__ int entry_of(const uint32_t* start, uint32_t value) {
   const int lane = threadIdx.x & (kWaveSize - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-  const float coefficient = a.clip ? a.clip[1] : 1.f;
-  const bool live = coefficient == coefficient;     // a norm that is not finite: nothing changes
-  if (live) {
-    int chunk = blockIdx.x * table.per_block;
-    const int end = chunk + table.per_block < table.chunks ? chunk + table.per_block : table.chunks;
-    int i = 0;
-    for (int step = 64; step; step >>= 1)            // the last tensor that starts at or before the chunk
-      if (i + step < table.count && table.t[i + step].chunk <= chunk) i += step;
-    const float lr = a.lr_device ? *a.lr_device : a.lr;
-    const float keep = static_cast<float>(1.0 - static_cast<double>(lr) * a.weight_decay);
-    const float b1 = static_cast<float>(a.beta1), b2 = static_cast<float>(a.beta2);
-    const float n1 = static_cast<float>(1.0 - a.beta1), n2 = static_cast<float>(1.0 - a.beta2);
-    int loaded = -1;
-    float rate = 0.f, inv2 = 0.f;
-    uint32_t key = 0;
-    bool wide = false;
-    StepTensor t = table.t[i];
-    for (; chunk < end; ++chunk) {
-      while (i + 1 < table.count && table.t[i + 1].chunk <= chunk) ++i;
-      if (i != loaded) {
-        t = table.t[i];
-        const double* row = a.progress + 3 * static_cast<int64_t>(t.row);
-        rate = lr / static_cast<float>(1.0 - row[1] * a.beta1);
-        inv2 = 1.f / static_cast<float>(1.0 - row[2] * a.beta2);
-        if constexpr (SMALL)
-          key = mix(a.seed + static_cast<uint32_t>(static_cast<int64_t>(row[0]) + 1) * 0x9E3779B9u);
-        wide = ((reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad)) & 15) == 0;
-        loaded = i;
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < MOST; k += kWaveSize)
+    n += __popcll(__ballot(k + lane < MOST && start[k + lane < MOST ? k + lane : 0] <= value));
+  return __builtin_amdgcn_readfirstlane(n - 1);
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
+template <typename T>
+__device__ __forceinline__ T* uniform(T* p) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<T*>((static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32) |
+                              uniform(static_cast<uint32_t>(x)));
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <bool STREAM>
+__device__ __forceinline__ void load4(const float* p, float* v) {
+  const f32x4* q = reinterpret_cast<const f32x4*>(p);
+  const f32x4 x = STREAM ? __builtin_nontemporal_load(q) : *q;
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+}
+
+template <bool STREAM>
+__device__ __forceinline__ void store4(float* p, const float* v) {
+  const f32x4 x = {v[0], v[1], v[2], v[3]};
+  f32x4* q = reinterpret_cast<f32x4*>(p);
+  if constexpr (STREAM) __builtin_nontemporal_store(x, q); else *q = x;
+}
+
+// What the blocks of one tensor share.
+struct StepScalars {
+  float coefficient, keep, rate, inv2, b1, b2, n1, n2, eps;
+  uint32_t key;
+};
+
+// The update of U whole blocks (or, with U = 1, of the first `left` of each lane's values): four values a
+// lane and block, all loads before the first store.
+template <bool SMALL, bool STREAM, int U, bool WHOLE>
+__device__ __forceinline__ void update(const StepArgs& a, const StepScalars& c, float* param, const float* grad,
+                                       int64_t block, int left) {
+  const int lane = threadIdx.x & (kWaveSize - 1);
+  const int64_t s = block * kQuant + lane * 4;
+  uint8_t* const codes_m = static_cast<uint8_t*>(a.exp_avg) + s;
+  uint8_t* const codes_v = static_cast<uint8_t*>(a.exp_avg_sq) + s;
+  float* const values_m = static_cast<float*>(a.exp_avg) + s;
+  float* const values_v = static_cast<float*>(a.exp_avg_sq) + s;
+  float p[U][4] = {}, g[U][4] = {}, m[U][4], v[U][4];
+  uint32_t cm[U], cv[U];
+  int tm[U], tv[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if constexpr (WHOLE) {
+      load4<STREAM>(param + u * kQuant, p[u]);
+      load4<STREAM>(grad + u * kQuant, g[u]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < left) p[u][k] = param[k], g[u][k] = grad[k];
+    }
+    if constexpr (SMALL) {
+      cm[u] = *reinterpret_cast<const uint32_t*>(codes_m + u * kQuant);
+      cv[u] = *reinterpret_cast<const uint32_t*>(codes_v + u * kQuant);
+      tm[u] = a.exp_avg_top[block + u], tv[u] = a.exp_avg_sq_top[block + u];
+    } else {
+      load4<STREAM>(values_m + u * kQuant, m[u]);
+      load4<STREAM>(values_v + u * kQuant, v[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if constexpr (SMALL) {
+      decode_signed(cm[u], tm[u], m[u]);
+      decode_unsigned(cv[u], tv[u], v[u]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float gk = c.coefficient * g[u][k];
+      m[u][k] = c.b1 * m[u][k] + c.n1 * gk;
+      v[u][k] = c.b2 * v[u][k] + c.n2 * (gk * gk);
+    }
+    if (SMALL && c.eps >= kFastEps) {
+      // Roots and reciprocals to the last bit but one, without the steps for denormal roots (eps covers
+      // them): the exact ones are a quarter of this variant's instructions, which bound it.
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        p[u][k] = c.keep * p[u][k] -
+                  c.rate * m[u][k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[u][k] * c.inv2) + c.eps);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        p[u][k] = c.keep * p[u][k] - c.rate * m[u][k] / (sqrtf(v[u][k] * c.inv2) + c.eps);
+    }
+    if constexpr (WHOLE) {
+      store4<STREAM>(param + u * kQuant, p[u]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < left) param[k] = p[u][k];
+    }
+    if constexpr (SMALL) {
+      bool fm, fv;
+      tm[u] = block_top(m[u], fm), tv[u] = block_top(v[u], fv);
+      uint32_t random[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) random[k] = mix(static_cast<uint32_t>(s) + u * kQuant + k + c.key);
+      *reinterpret_cast<uint32_t*>(codes_m + u * kQuant) = encode_signed(m[u], tm[u], fm, random);
+      *reinterpret_cast<uint32_t*>(codes_v + u * kQuant) = encode_unsigned(v[u], tv[u], fv, random);
+      if (lane == 0) {
+        a.exp_avg_top[block + u] = static_cast<uint8_t>(tm[u]);
+        a.exp_avg_sq_top[block + u] = static_cast<uint8_t>(tv[u]);
       }
-      const int64_t first = static_cast<int64_t>(chunk - t.chunk) * kChunk + wave * kQuant;
-      if (first >= t.elements) continue;
-      const int64_t at = first + lane * 4;
-      float p[4] = {}, g[4] = {}, m[4], v[4];
-      const bool whole = wide && first + kQuant <= t.elements;
-      if (whole) {
-        const float4 p4 = *reinterpret_cast<const float4*>(t.param + at);
-        const float4 g4 = *reinterpret_cast<const float4*>(t.grad + at);
-        p[0] = p4.x, p[1] = p4.y, p[2] = p4.z, p[3] = p4.w;
-        g[0] = g4.x, g[1] = g4.y, g[2] = g4.z, g[3] = g4.w;
+    } else {
+      store4<STREAM>(values_m + u * kQuant, m[u]);
+      store4<STREAM>(values_v + u * kQuant, v[u]);
+    }
+  }
+}
+
+// One wave to U consecutive blocks of 256 values; the launch's waves sweep over the blocks side by side,
+// so a wave changes tensors often: the table and each tensor's scalars are in LDS.
+//
+// Bound by memory: 28 bytes a value (8-bit moments 16). 150 M values in 120 tensors: 705 us (5.9 TB/s) with
+// float32 moments and 401 us (6.0 TB/s) with 8-bit ones, a copy of the same size runs at 5.3 to 5.9.  What
+// that took, from 835 and 535 us with a contiguous range of blocks for each of 2,048 workgroups: lookups
+// from LDS and waves side by side (the ranges met on the same memory channels), no reuse asked of the
+// caches (`STREAM`, from kStream values on; below, the caches hold a model: 8 M values 37 us against
+// 40), a workgroup for each piece of work instead of 2,048 that go on, and with 8-bit moments four blocks a
+// wave at a time (292 us at 100 M against 254; with float32 moments one is the better: 448 against 469).
+// The 8-bit variant was bound by its instructions at first (66 % of issue slots): hardware conversions of
+// m, codes of four values handled together, and approximate roots took 40 % of them.
+template <bool SMALL, bool STREAM>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const StepTable table, const StepArgs a) {
+  constexpr int U = step_blocks(SMALL, STREAM);
+  __shared__ float* params[kTensors];
+  __shared__ const float* grads[kTensors];
+  __shared__ uint32_t starts[kTensors + 1];
+  __shared__ uint32_t tails[kTensors];
+  __shared__ float rates[kTensors], inv2s[kTensors];
+  __shared__ uint32_t keys[kTensors];
+  const int thread = threadIdx.x, lane = thread & (kWaveSize - 1);
+  StepScalars c;
+  c.coefficient = a.clip ? a.clip[1] : 1.f;
+  const float lr = a.lr_device ? *a.lr_device : a.lr;
+  if (thread < table.count) {
+    const double* row = a.progress + 3 * (table.row + thread);
+    const double steps = row[0], power1 = row[1], power2 = row[2];
+    params[thread] = table.param[thread];
+    grads[thread] = table.grad[thread];
+    tails[thread] = table.tail[thread];
+    rates[thread] = lr / static_cast<float>(1.0 - power1 * a.beta1);
+    inv2s[thread] = 1.f / static_cast<float>(1.0 - power2 * a.beta2);
+    keys[thread] = mix(a.seed + static_cast<uint32_t>(static_cast<int64_t>(steps) + 1) * 0x9E3779B9u);
+  }
+  if (thread <= kTensors) starts[thread] = table.start[thread];
+  __syncthreads();
+  if (c.coefficient != c.coefficient) return;    // a norm that is not finite: nothing changes
+  c.keep = static_cast<float>(1.0 - static_cast<double>(lr) * a.weight_decay);
+  c.b1 = static_cast<float>(a.beta1), c.b2 = static_cast<float>(a.beta2);
+  c.n1 = static_cast<float>(1.0 - a.beta1), c.n2 = static_cast<float>(1.0 - a.beta2);
+  c.eps = a.eps;
+  const uint32_t blocks = table.blocks, stride = gridDim.x * (kWaves * U);
+  int last = 0;
+  uint32_t start = 0, next = 0;
+  float* param = nullptr;
+  const float* grad = nullptr;
+  bool wide = false;
+  for (uint32_t first = (blockIdx.x * kWaves + uniform(static_cast<uint32_t>(thread / kWaveSize))) * U; first < blocks;
+       first += stride) {
+    const uint32_t end = blocks - first < U ? blocks : first + U;
+    for (uint32_t b = first; b < end;) {
+      if (b >= next) {
+        const int i = entry_of<kTensors>(starts, b);
+        start = uniform(starts[i]), next = uniform(starts[i + 1]);
+        param = uniform(params[i]), grad = uniform(grads[i]), last = uniform(tails[i]);
+        wide = ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
+        c.rate = rates[i], c.inv2 = inv2s[i], c.key = keys[i];
+      }
+      const int64_t at = static_cast<int64_t>(b - start) * kQuant + lane * 4;
+      const uint32_t whole = wide ? next - (last != 0) : 0u;     // blocks before it can be read four values at a time
+      if (!grad) {
+        b = next < end ? next : end;
+      } else if (U > 1 && b + U <= whole && b + U <= end) {
+        update<SMALL, STREAM, U, true>(a, c, param + at, grad + at, table.state + b, 4);
+        b += U;
+      } else if (b < whole) {
+        update<SMALL, STREAM, 1, true>(a, c, param + at, grad + at, table.state + b, 4);
+        ++b;
       } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (at + k < t.elements) p[k] = t.param[at + k], g[k] = t.grad[at + k];
-      }
-      const int64_t s = t.state + at;
-      [[maybe_unused]] const int64_t block = (t.state + first) / kQuant;
-      if constexpr (SMALL) {
-        const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.exp_avg) + s);
-        const uint32_t cv = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.exp_avg_sq) + s);
-        const int tm = a.exp_avg_top[block], tv = a.exp_avg_sq_top[block];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          m[k] = decode_signed((cm >> (8 * k)) & 0xFFu, tm);
-          v[k] = decode_unsigned((cv >> (8 * k)) & 0xFFu, tv);
-        }
-      } else {
-        const float4 m4 = *reinterpret_cast<const float4*>(static_cast<const float*>(a.exp_avg) + s);
-        const float4 v4 = *reinterpret_cast<const float4*>(static_cast<const float*>(a.exp_avg_sq) + s);
-        m[0] = m4.x, m[1] = m4.y, m[2] = m4.z, m[3] = m4.w;
-        v[0] = v4.x, v[1] = v4.y, v[2] = v4.z, v[3] = v4.w;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float gk = coefficient * g[k];
-        m[k] = b1 * m[k] + n1 * gk;
-        v[k] = b2 * v[k] + n2 * (gk * gk);
-        p[k] = keep * p[k] - rate * m[k] / (sqrtf(v[k] * inv2) + a.eps);
-      }
-      if (whole) {
-        *reinterpret_cast<float4*>(t.param + at) = make_float4(p[0], p[1], p[2], p[3]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (at + k < t.elements) t.param[at + k] = p[k];
-      }
-      if constexpr (SMALL) {
-        uint32_t lm = 0, lv = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t fm = finite_magnitude(m[k]), fv = finite_magnitude(v[k]);
-          lm = lm > fm ? lm : fm;
-          lv = lv > fv ? lv : fv;
-        }
-        const int tm = block_top(wave_max(lm)), tv = block_top(wave_max(lv));
-        uint32_t cm = 0, cv = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t bits = mix(static_cast<uint32_t>(s) + k + key);
-          cm |= encode_signed(m[k], tm, bits & 0xFFFFu) << (8 * k);
-          cv |= encode_unsigned(v[k], tv, bits >> 16) << (8 * k);
-        }
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.exp_avg) + s) = cm;
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.exp_avg_sq) + s) = cv;
-        if (lane == 0) {
-          a.exp_avg_top[block] = static_cast<uint8_t>(tm);
-          a.exp_avg_sq_top[block] = static_cast<uint8_t>(tv);
-        }
-      } else {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.exp_avg) + s) = make_float4(m[0], m[1], m[2], m[3]);
-        *reinterpret_cast<float4*>(static_cast<float*>(a.exp_avg_sq) + s) = make_float4(v[0], v[1], v[2], v[3]);
+        const int left = (b + 1 == next && last ? last : kQuant) - lane * 4;
+        update<SMALL, STREAM, 1, false>(a, c, param + at, grad + at, table.state + b, left);
+        ++b;
       }
     }
   }
-  // the workgroup that ends last advances the tensors' steps: every other one has read them by then
-  __shared__ unsigned last;
-  __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
-  __syncthreads();
-  if (!last) return;
-  if (live)
-    for (int k = threadIdx.x; k < table.count; k += kThreads) {
-      double* row = a.progress + 3 * static_cast<int64_t>(table.t[k].row);
-      row[0] += 1.0;
-      row[1] *= a.beta1;
-      row[2] *= a.beta2;
-    }
-  if (threadIdx.x == 0) *a.ticket = 0u;
 }
 
-// Eight-bit moments as the values they stand for: 4 significant bits (m) and a power of two, exact in bfloat16.
+// One more step for every tensor that took part.  A launch of its own: the update kernels read the steps
+// in every workgroup, and a count of the workgroups that are done costs more (14 ns each, one address).
+__global__ void __launch_bounds__(kThreads)
+advance_kernel(const RowMask mask, double* __restrict__ progress, double beta1, double beta2,
+               const float* __restrict__ clip) {
+  if (clip && clip[1] != clip[1]) return;
+  const int k = blockIdx.x * kThreads + threadIdx.x;
+  if (k >= mask.count || !((mask.bits[k >> 5] >> (k & 31)) & 1u)) return;
+  double* row = progress + 3 * (mask.first + k);
+  row[0] += 1.0;
+  row[1] *= beta1;
+  row[2] *= beta2;
+}
+
+// Eight-bit moments as the values they stand for: 4 significant bits (m and v) and a power of two, exact in
+// bfloat16.  Eight codes a thread, so that the stores are 16 bytes wide.  Bound by memory: 6 bytes a value.
 __global__ void __launch_bounds__(kThreads)
 moment_values_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ m_top, const uint8_t* __restrict__ v,
                      const uint8_t* __restrict__ v_top, uint16_t* __restrict__ m_out, uint16_t* __restrict__ v_out,
-                     int64_t blocks) {
-  const int lane = threadIdx.x & (kWaveSize - 1);
-  const int64_t waves = static_cast<int64_t>(gridDim.x) * (kThreads / kWaveSize);
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * (kThreads / kWaveSize) + threadIdx.x / kWaveSize; b < blocks;
-       b += waves) {
-    const int64_t s = b * kQuant + lane * 4;
-    const uint32_t cm = *reinterpret_cast<const uint32_t*>(m + s), cv = *reinterpret_cast<const uint32_t*>(v + s);
-    const int tm = m_top[b], tv = v_top[b];
-    ushort4 om, ov;
-    uint16_t* pm = reinterpret_cast<uint16_t*>(&om);
-    uint16_t* pv = reinterpret_cast<uint16_t*>(&ov);
+                     int64_t values) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads * 8;
+  for (int64_t s = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 8; s < values; s += stride) {
+    const u32x2 cm = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(m + s));
+    const u32x2 cv = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(v + s));
+    const int tm = m_top[s / kQuant], tv = v_top[s / kQuant];
+    float x[8], y[8];
+    decode_signed(cm.x, tm, x);
+    decode_signed(cm.y, tm, x + 4);
+    decode_unsigned(cv.x, tv, y);
+    decode_unsigned(cv.y, tv, y + 4);
+    u32x4 om, ov;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      pm[k] = static_cast<uint16_t>(__float_as_uint(decode_signed((cm >> (8 * k)) & 0xFFu, tm)) >> 16);
-      pv[k] = static_cast<uint16_t>(__float_as_uint(decode_unsigned((cv >> (8 * k)) & 0xFFu, tv)) >> 16);
+      om[k] = (__float_as_uint(x[2 * k]) >> 16) | (__float_as_uint(x[2 * k + 1]) & 0xFFFF0000u);
+      ov[k] = (__float_as_uint(y[2 * k]) >> 16) | (__float_as_uint(y[2 * k + 1]) & 0xFFFF0000u);
     }
-    *reinterpret_cast<ushort4*>(m_out + s) = om;
-    *reinterpret_cast<ushort4*>(v_out + s) = ov;
+    __builtin_nontemporal_store(om, reinterpret_cast<u32x4*>(m_out + s));
+    __builtin_nontemporal_store(ov, reinterpret_cast<u32x4*>(v_out + s));
   }
 }
 
-struct NormTensor {
-  const float* grad;
-  int64_t elements;
-  int64_t chunk;
-};
-
 struct NormTable {
-  NormTensor t[kNormTensors];
-  int64_t chunks;
-  int64_t per_block;
-  int32_t count;
+  const float* grad[kNormTensors];
+  int64_t elements[kNormTensors];
+  uint32_t start[kNormTensors + 1];    // a tensor's first chunk of kNormChunk values
+  int32_t count;     // (of the host's)
+  uint32_t chunks;
 };
 
 __device__ __forceinline__ double block_sum(double x) {
-  __shared__ double part[kThreads / kWaveSize];
+  __shared__ double part[kWaves];
 #pragma unroll
   for (int d = kWaveSize / 2; d; d >>= 1) x += __shfl_xor(x, d);
   if ((threadIdx.x & (kWaveSize - 1)) == 0) part[threadIdx.x / kWaveSize] = x;
   __syncthreads();
   double sum = 0.0;
 #pragma unroll
-  for (int w = 0; w < kThreads / kWaveSize; ++w) sum += part[w];
+  for (int w = 0; w < kWaves; ++w) sum += part[w];
   return sum;
 }
 
 // Sums of squares in 64 bits (a float's square neither overflows nor vanishes there), one for each
 // workgroup; a second launch adds them in order.
+template <bool STREAM>
 __global__ void __launch_bounds__(kThreads) norm_partial_kernel(const NormTable table, double* __restrict__ partial) {
-  int64_t chunk = blockIdx.x * table.per_block;
-  const int64_t end = chunk + table.per_block < table.chunks ? chunk + table.per_block : table.chunks;
-  int i = 0;
-  for (int step = 128; step; step >>= 1)
-    if (i + step < table.count && table.t[i + step].chunk <= chunk) i += step;
+  __shared__ const float* grads[kNormTensors];
+  __shared__ int64_t sizes[kNormTensors];
+  __shared__ uint32_t starts[kNormTensors + 1];
+  if (threadIdx.x < kNormTensors) {
+    grads[threadIdx.x] = table.grad[threadIdx.x];
+    sizes[threadIdx.x] = table.elements[threadIdx.x];
+  }
+  if (threadIdx.x <= kNormTensors) starts[threadIdx.x] = table.start[threadIdx.x];
+  __syncthreads();
   double sum = 0.0;
-  for (; chunk < end; ++chunk) {
-    while (i + 1 < table.count && table.t[i + 1].chunk <= chunk) ++i;
-    const NormTensor t = table.t[i];
-    const int64_t first = (chunk - t.chunk) * kNormChunk;
-    if ((reinterpret_cast<uintptr_t>(t.grad) & 15) == 0 && first + kNormChunk <= t.elements) {
+  uint32_t start = 0, next = 0;
+  const float* grad = nullptr;
+  int64_t elements = 0;
+  for (uint32_t chunk = blockIdx.x; chunk < table.chunks; chunk += gridDim.x) {
+    if (chunk >= next) {
+      const int i = entry_of<kNormTensors>(starts, chunk);
+      start = uniform(starts[i]), next = uniform(starts[i + 1]);
+      grad = uniform(grads[i]), elements = sizes[i];
+    }
+    const int64_t first = static_cast<int64_t>(chunk - start) * kNormChunk;
+    if ((reinterpret_cast<uintptr_t>(grad) & 15) == 0 && first + kNormChunk <= elements) {
+      float g[kNormChunk / kThreads];
 #pragma unroll
-      for (int k = 0; k < kNormChunk / (4 * kThreads); ++k) {
-        const float4 g = *reinterpret_cast<const float4*>(t.grad + first + (k * kThreads + threadIdx.x) * 4);
-        const double x = g.x, y = g.y, z = g.z, w = g.w;
-        sum += x * x + y * y + z * z + w * w;
-      }
+      for (int k = 0; k < kNormChunk / (4 * kThreads); ++k)
+        load4<STREAM>(grad + first + (k * kThreads + threadIdx.x) * 4, g + 4 * k);
+#pragma unroll
+      for (int k = 0; k < kNormChunk / kThreads; ++k) sum += static_cast<double>(g[k]) * static_cast<double>(g[k]);
     } else {
-      const int64_t stop = first + kNormChunk < t.elements ? first + kNormChunk : t.elements;
+      const int64_t stop = first + kNormChunk < elements ? first + kNormChunk : elements;
       for (int64_t k = first + threadIdx.x; k < stop; k += kThreads) {
-        const double x = t.grad[k];
+        const double x = grad[k];
         sum += x * x;
       }
     }
@@ -350,8 +501,18 @@ norm_finish_kernel(const double* __restrict__ partial, int count, float max_norm
     const double norm = sqrt(sum);
     const double ratio = static_cast<double>(max_norm) / norm;
     out[0] = static_cast<float>(norm);
-    out[1] = !(norm < INFINITY) ? __uint_as_float(0x7FC00000u) : max_norm > 0.f && ratio < 1.0 ? static_cast<float>(ratio) : 1.f;
+    const float coefficient = max_norm > 0.f && ratio < 1.0 ? static_cast<float>(ratio) : 1.f;
+    out[1] = norm < INFINITY ? coefficient : __uint_as_float(0x7FC00000u);
   }
+}
+
+constexpr int64_t kMostElements = int64_t{1} << 38;     // of one tensor: 2^30 blocks
+constexpr int64_t kMostUnits = int64_t{3} << 30;        // blocks or chunks of one launch, within 32 bits
+
+// The end of the last tensor, and entries that no search finds.
+void close_starts(uint32_t* start, int count, int most, int64_t end) {
+  start[count] = static_cast<uint32_t>(end);
+  for (int i = count + 1; i <= most; ++i) start[i] = ~0u;
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -376,21 +537,28 @@ int ictc_hip_gradient_norm(const float* const* grads, const int64_t* elements, i
       workspace_doubles < ictc_hip_gradient_norm_workspace(count) || max_norm != max_norm)
     return ICTC_ERR_INVALID_ARGUMENT;
   for (int64_t k = 0; k < count; ++k)
-    if (elements[k] < 0 || (elements[k] && !grads[k])) return ICTC_ERR_INVALID_ARGUMENT;
+    if (elements[k] < 0 || elements[k] > kMostElements || (elements[k] && !grads[k])) return ICTC_ERR_INVALID_ARGUMENT;
   int partials = 0;
   for (int64_t k = 0; k < count;) {
     NormTable table;
     table.count = 0;
-    table.chunks = 0;
+    int64_t chunks = 0;
     for (; k < count && table.count < kNormTensors; ++k) {
       if (!elements[k]) continue;
-      table.t[table.count++] = {grads[k], elements[k], table.chunks};
-      table.chunks += ceil_div(elements[k], kNormChunk);
+      const int64_t more = ceil_div(elements[k], kNormChunk);
+      if (chunks + more > kMostUnits) break;         // the next launch takes it
+      table.grad[table.count] = grads[k];
+      table.elements[table.count] = elements[k];
+      table.start[table.count++] = static_cast<uint32_t>(chunks);
+      chunks += more;
     }
     if (!table.count) continue;
-    table.per_block = ceil_div(table.chunks, kNormBlocks);
-    const int blocks = static_cast<int>(ceil_div(table.chunks, table.per_block));
-    hipLaunchKernelGGL(norm_partial_kernel, dim3(blocks), dim3(kThreads), 0, stream, table, workspace + partials);
+    close_starts(table.start, table.count, kNormTensors, chunks);
+    table.chunks = static_cast<uint32_t>(chunks);
+    const int blocks = static_cast<int>(chunks < kNormBlocks ? chunks : kNormBlocks);
+    if (partials + blocks > workspace_doubles) return ICTC_ERR_UNSUPPORTED;
+    const auto kernel = chunks * kNormChunk >= kStream ? norm_partial_kernel<true> : norm_partial_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, stream, table, workspace + partials);
     if (const int rc = launched()) return rc;
     partials += blocks;
   }
@@ -416,7 +584,7 @@ int ictc_hip_adamw_step(float* const* params, const float* const* grads, const i
   if ((reinterpret_cast<uintptr_t>(exp_avg) | reinterpret_cast<uintptr_t>(exp_avg_sq)) & (small ? 3 : 15))
     return ICTC_ERR_INVALID_ARGUMENT;
   for (int64_t k = 0; k < count; ++k)
-    if (elements[k] < 0 || elements[k] > (int64_t{1} << 40) || (elements[k] && grads[k] && !params[k]))
+    if (elements[k] < 0 || elements[k] > kMostElements || (elements[k] && grads[k] && !params[k]))
       return ICTC_ERR_INVALID_ARGUMENT;
   if (count > 0x7fffffff) return ICTC_ERR_INVALID_ARGUMENT;
   StepArgs args;
@@ -425,7 +593,6 @@ int ictc_hip_adamw_step(float* const* params, const float* const* grads, const i
   args.exp_avg_top = exp_avg_top;
   args.exp_avg_sq_top = exp_avg_sq_top;
   args.progress = progress;
-  args.ticket = reinterpret_cast<unsigned*>(progress + 3 * count);
   args.clip = clip;
   args.lr_device = lr_device;
   args.beta1 = desc->beta1;
@@ -434,32 +601,49 @@ int ictc_hip_adamw_step(float* const* params, const float* const* grads, const i
   args.lr = desc->lr;
   args.eps = desc->eps;
   args.seed = desc->seed;
-  int64_t state = 0;
+  int64_t state = 0;    // blocks of the tensors before k
   for (int64_t k = 0; k < count;) {
-    StepTable table;
-    table.count = 0;
-    int64_t chunks = 0;
-    for (; k < count && table.count < kTensors; ++k) {
-      const int64_t at = state;
-      const int64_t more = ceil_div(elements[k], kChunk);
-      state += ceil_div(elements[k], kQuant) * kQuant;
-      if (!grads[k]) continue;                       // not part of this step
-      if (chunks + more > 0x7fffffff - kMaxBlocks) { // the next launch takes it
-        state = at;
-        break;
-      }
-      table.t[table.count++] = {params[k], grads[k], elements[k], at, static_cast<int32_t>(chunks),
-                                static_cast<int32_t>(k)};
-      chunks += more;
+    if (!grads[k]) {    // a launch begins with a tensor that takes part
+      state += ceil_div(elements[k++], kQuant);
+      continue;
     }
-    if (!table.count) continue;
-    table.chunks = static_cast<int32_t>(chunks);
-    table.per_block = static_cast<int32_t>(chunks ? ceil_div(chunks, kMaxBlocks) : 1);
-    const int blocks = static_cast<int>(chunks ? ceil_div(chunks, table.per_block) : 1);
-    if (small)
-      hipLaunchKernelGGL(adamw_kernel<true>, dim3(blocks), dim3(kThreads), 0, stream, table, args);
-    else
-      hipLaunchKernelGGL(adamw_kernel<false>, dim3(blocks), dim3(kThreads), 0, stream, table, args);
+    StepTable table;
+    table.state = state;
+    table.row = k;
+    table.count = 0;
+    int64_t blocks = 0;
+    for (; k < count && table.count < kTensors; ++k) {
+      const int64_t more = ceil_div(elements[k], kQuant);
+      // a large tensor that takes no part ends the launch: its blocks would go by without work
+      if (blocks + more > kMostUnits || (!grads[k] && more > kSkip)) break;
+      table.param[table.count] = params[k];
+      table.grad[table.count] = grads[k];
+      table.tail[table.count] = static_cast<uint8_t>(elements[k] % kQuant);
+      table.start[table.count++] = static_cast<uint32_t>(blocks);
+      blocks += more;
+    }
+    state += blocks;
+    if (!blocks) continue;
+    close_starts(table.start, table.count, kTensors, blocks);
+    table.blocks = static_cast<uint32_t>(blocks);
+    const bool past = blocks * kQuant >= kStream;
+    const int64_t groups = ceil_div(blocks, kWaves * step_blocks(small, past)), most = past ? kMostGroups : kMaxBlocks;
+    const int grid = static_cast<int>(groups < most ? groups : most);
+    const auto kernel = small ? past ? adamw_kernel<true, true> : adamw_kernel<true, false>
+                              : past ? adamw_kernel<false, true> : adamw_kernel<false, false>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, stream, table, args);
+    if (const int rc = launched()) return rc;
+  }
+  for (int64_t first = 0; first < count; first += kMaskTensors) {
+    RowMask mask = {};
+    mask.first = first;
+    mask.count = static_cast<int32_t>(count - first < kMaskTensors ? count - first : kMaskTensors);
+    bool any = false;
+    for (int k = 0; k < mask.count; ++k)
+      if (grads[first + k]) mask.bits[k >> 5] |= 1u << (k & 31), any = true;
+    if (!any) continue;
+    hipLaunchKernelGGL(advance_kernel, dim3(static_cast<unsigned>(ceil_div(mask.count, kThreads))), dim3(kThreads), 0,
+                       stream, mask, progress, desc->beta1, desc->beta2, clip);
     if (const int rc = launched()) return rc;
   }
   return ICTC_OK;
@@ -472,14 +656,13 @@ int ictc_hip_moment_values(const uint8_t* exp_avg, const uint8_t* exp_avg_top, c
   if (values < 0 || values % kQuant) return ICTC_ERR_INVALID_ARGUMENT;
   if (values == 0) return ICTC_OK;
   if (!exp_avg || !exp_avg_top || !exp_avg_sq || !exp_avg_sq_top || !exp_avg_bf16 || !exp_avg_sq_bf16 ||
-      ((reinterpret_cast<uintptr_t>(exp_avg) | reinterpret_cast<uintptr_t>(exp_avg_sq)) & 3) ||
-      ((reinterpret_cast<uintptr_t>(exp_avg_bf16) | reinterpret_cast<uintptr_t>(exp_avg_sq_bf16)) & 7))
+      ((reinterpret_cast<uintptr_t>(exp_avg) | reinterpret_cast<uintptr_t>(exp_avg_sq)) & 7) ||
+      ((reinterpret_cast<uintptr_t>(exp_avg_bf16) | reinterpret_cast<uintptr_t>(exp_avg_sq_bf16)) & 15))
     return ICTC_ERR_INVALID_ARGUMENT;
-  const int64_t blocks = values / kQuant;
-  const int64_t groups = ceil_div(blocks, kThreads / kWaveSize);
-  hipLaunchKernelGGL(moment_values_kernel, dim3(static_cast<unsigned>(groups < 4096 ? groups : 4096)), dim3(kThreads),
-                     0, stream, exp_avg, exp_avg_top, exp_avg_sq, exp_avg_sq_top,
-                     static_cast<uint16_t*>(exp_avg_bf16), static_cast<uint16_t*>(exp_avg_sq_bf16), blocks);
+  const int64_t groups = ceil_div(values, 8 * kThreads);
+  hipLaunchKernelGGL(moment_values_kernel, dim3(static_cast<unsigned>(groups < kMostGroups ? groups : kMostGroups)),
+                     dim3(kThreads), 0, stream, exp_avg, exp_avg_top, exp_avg_sq, exp_avg_sq_top,
+                     static_cast<uint16_t*>(exp_avg_bf16), static_cast<uint16_t*>(exp_avg_sq_bf16), values);
   return launched();
 }
 

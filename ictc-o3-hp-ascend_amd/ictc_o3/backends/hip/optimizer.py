@@ -45,8 +45,8 @@ def new_state(params, moment_bits: int = 32):
                     torch.zeros(total // MOMENT_BLOCK, device=device, dtype=torch.uint8)) for _ in range(2)]
     else:
         raise ValueError("moment_bits must be 32 or 8")
-    progress = torch.zeros(len(params) + 1, 3, device=device, dtype=torch.float64)
-    progress[:-1, 1:] = 1.0
+    progress = torch.ones(len(params), 3, device=device, dtype=torch.float64)
+    progress[:, 0] = 0.0
     return moments[0], moments[1], progress
 
 
@@ -103,7 +103,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, progress, *, lr, betas=(0.9, 
     parameter, moments and steps as they are).
 
     exp_avg, exp_avg_sq, progress: as ``new_state`` makes them (float32 moments, or pairs of 8-bit codes
-    and block exponents).  lr: a number, or a one-element float32 tensor on the device.  clip:
+    and block exponents; for each parameter its steps t, beta1^t and beta2^t, further rows are left alone).  lr: a number, or a one-element float32 tensor on the device.  clip:
     ``gradient_norm``'s result, whose coefficient scales the gradients.  seed: of the 8-bit rounding."""
     params, grads = list(params), list(grads)
     _, p_at, g_at, sizes, values, contiguous = _lib.host().pairs(params, grads, MOMENT_BLOCK)
@@ -115,9 +115,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, progress, *, lr, betas=(0.9, 
     v, v_top, v_bits = _moments(exp_avg_sq, values, device, "exp_avg_sq")
     if bits != v_bits:
         raise ValueError("exp_avg and exp_avg_sq must have the same number of bits")
-    if progress.shape != (n + 1, 3) or progress.dtype is not torch.float64 or not progress.is_contiguous() \
+    if progress.dim() != 2 or progress.shape[0] < n or progress.shape[1] != 3 or progress.dtype is not torch.float64 or not progress.is_contiguous() \
             or progress.device != device:
-        raise ValueError(f"progress must be a contiguous float64 tensor [{n + 1}, 3] beside the parameters")
+        raise ValueError(f"progress must be a contiguous float64 tensor of at least {n} rows of 3 beside the "
+                         "parameters")
     if clip is not None and (clip.dtype is not torch.float32 or clip.shape != (2,) or clip.device != device
                              or not clip.is_contiguous()):
         raise ValueError("clip must be gradient_norm's result")

@@ -715,11 +715,11 @@ int ictc_hip_gates_weight_grad(const float *grad, int64_t grad_row_stride, const
  * (m 0x7f and v 0xff: not a number).  New values are rounded up or down at random, by 16 bits each of a
  * hash of desc->seed, the tensor's step and the value's place; a v above zero is never stored as zero.
  *
- * progress: 3 (count + 1) doubles, per tensor its number of steps, beta1^steps and beta2^steps (0, 1, 1
- * before the first); the last three are the kernel's own and start as zero.
+ * progress: 3 count doubles, per tensor its number of steps, beta1^steps and beta2^steps (0, 1, 1 before
+ * the first).
  *
- * ictc_hip_moment_values: 8-bit moments (values: a multiple of ICTC_MOMENT_BLOCK) as bfloat16, which
- * holds them exactly.
+ * ictc_hip_moment_values: 8-bit moments (values: a multiple of ICTC_MOMENT_BLOCK; 8-byte aligned) as
+ * bfloat16 (16-byte aligned), which holds them exactly.
  */
 #define ICTC_MOMENT_BLOCK 256
 

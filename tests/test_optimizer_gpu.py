@@ -105,8 +105,7 @@ def test_steps_match_the_formula(gpu, name, offset):
                 assert np.all(np.abs(got - value) <= tol), (k, n, np.max(np.abs(got - value) - tol))
             assert not m[at[k] + n:at[k + 1]].any() and not v[at[k] + n:at[k + 1]].any()
         progress = state[2].cpu().numpy()
-        np.testing.assert_allclose(progress[:-1], [[step, BETAS[0] ** step, BETAS[1] ** step]] * len(sizes), rtol=1e-14)
-        assert not progress[-1].any()
+        np.testing.assert_allclose(progress, [[step, BETAS[0] ** step, BETAS[1] ** step]] * len(sizes), rtol=1e-14)
 
 
 @pytest.mark.parametrize("offset", [0, 3])
@@ -189,7 +188,7 @@ def test_a_tensor_without_a_gradient_keeps_its_state(gpu):
         adamw_step(params, [grads[0], None, grads[2]], *state, lr=LR)
         after = [t for part in state for t in ((part,) if isinstance(part, torch.Tensor) else part)]
         assert torch.equal(params[1], kept)
-        assert state[2][:, 0].tolist() == [2.0, 1.0, 2.0, 0.0]
+        assert state[2][:, 0].tolist() == [2.0, 1.0, 2.0]
         for a, b in zip(after[:-1], before[:-1]):
             s = slice(512, 768) if a.numel() == 512 + 256 + 768 else slice(2, 3)
             assert torch.equal(a[s], b[s])
@@ -305,7 +304,7 @@ def test_refusals(gpu):
     for args, more in ((([p], [g[:5]], m, v, progress), ok), (([p], [], m, v, progress), ok),
                        (([p], [g.double()], m, v, progress), ok), (([p.cpu()], [g], m, v, progress), ok),
                        (([p.view(20, 15).t()], [g.view(20, 15).t()], m, v, progress), ok),
-                       (([p], [g], m[:256], v, progress), ok), (([p], [g], m, v, progress[:1]), ok),
+                       (([p], [g], m[:256], v, progress), ok), (([p], [g], m, v, progress[:0]), ok),
                        (([p], [g], m, v, progress.float()), ok), (([p], [g], m, new_state([p], 8)[1], progress), ok),
                        (([p], [g], m, v, progress), dict(lr=-1.0)), (([p], [g], m, v, progress), dict(lr=float("nan"))),
                        (([p], [g], m, v, progress), dict(lr=1e-3, betas=(1.0, 0.9))),
