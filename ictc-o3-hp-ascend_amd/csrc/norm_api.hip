@@ -1,0 +1,684 @@
+// Norms of a residual block on equivariant node features, gfx950: the norm before a block, and the block's
+// end in one pass (norm of its output, gate, residual sum, norm before the next block), each with its
+// gradients and with the gradients of those (forces are gradients, and training on them asks for more).
+//
+// A row v holds degrees l = 0..L, per degree a [C, 2l+1] block.  With a_l = 1 / ((L+1) C (2l+1)),
+//   q(v) = sum a_l v_lcm^2     rho(v) = (q + eps)^(-1/2)     N(v; w)_lcm = w_lc v_lcm rho(v)
+// one statistic for the row: rotations mix only the components m of one l and c, on which neither q nor
+// w depends, so N commutes with them; and every degree has the same share in q.
+//
+//   forward   h = x + k . b rho(b), k_lc = s sigmoid(g_lc) post_lc      y = N(h; pre)
+//
+//   VJP of V(v; e) = rho e - rho^3 a v <e, v>, the adjoint of N at cotangent e / w, is what both norms' gradients
+//   are made of.  With cotangents dh, dy:
+//     r = dh + V(h; pre dy)      dx = r      db = V(b; k r)
+//     dg = s sigmoid' post rho_b <r, b>_lc   dpost = sum_n s sigmoid rho_b <r, b>_lc   dpre = sum_n rho_h <dy, h>_lc
+//
+//   second order, cotangents X, B, G of dx, db, dg.  For Phi = <B, V(v; e)>, S1 = <B, e>, S2 = <a B, v>, S3 = <e, v>:
+//     dPhi/de = rho B - rho^3 S2 v
+//     dPhi/dv = -rho^3 a v S1 + 3 rho^5 a v S2 S3 - rho^3 (a B S3 + e S2)
+//   once at the block (v = b, e = k r), whose dPhi/de gives r's cotangent R = X + k dPhi/de + (G's part), and
+//   once at the next norm (v = h, e = pre dy, R in B's place).
+//
+// All of it is bound by memory: a row is read into registers once, its sums are taken there, and its results
+// are written once.  The gradients' sums and projections are in 64 bits: they take away the part of a
+// cotangent along v (all but eps / (q + eps) of it for a row with one large entry), and the difference is
+// as exact as the operands.  One thread holds one channel's (L+1)^2 components of every operand, so weights, gates and
+// their gradients need no exchange between threads; its 1, 3, 5 and 7 components are loaded with vectors of
+// that many words, which side by side fill whole lines.  A row's threads are part of a wave (up to 64
+// channels: a power of two of them) or up to 16 waves, whose sums meet in LDS.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "ictc_hip.h"
+
+namespace ictc {
+namespace {
+
+constexpr int kNormWave = 64;
+constexpr int kNormThreads = 256;            // of a workgroup whose rows fit into a wave
+constexpr int kNormMaxThreads = ICTC_NORM_MAX_CHANNELS;
+constexpr int kNormGroups = 1024;            // workgroups that leave partial weight gradients
+
+typedef float nf4 __attribute__((ext_vector_type(4), aligned(4)));
+
+struct NormArgs {
+  const float *x, *block, *gate, *post, *pre, *h, *dh, *dy, *cx, *cb, *cg;
+  float *out_h, *out_y, *dx, *db, *dg;
+  float *gh, *gb, *gg, *gdh, *gdy;
+  float* partial;             // per workgroup [2][L+1][C]: post's and pre's gradients
+  int64_t rows;
+  int64_t width_x;            // floats of a row of x, dx and cx
+  int channels;
+  int input_lmax;             // degrees of x that a row takes part with (at most L)
+  int threads;                // of a row
+  int groups;                 // rows of a workgroup at a time
+  float scale, eps;
+};
+
+template <int N>
+__device__ __forceinline__ void load_n(const float* p, float* v) {
+  if constexpr (N == 1) {
+    v[0] = *p;
+  } else if constexpr (N == 3) {
+    v[0] = p[0], v[1] = p[1], v[2] = p[2];      // (a vector type of three would take up four)
+  } else {
+    const nf4 t = *reinterpret_cast<const nf4*>(p);
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+    load_n<N - 4>(p + 4, v + 4);
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void store_n(float* p, const float* v) {
+  if constexpr (N == 1) {
+    *p = v[0];
+  } else if constexpr (N == 3) {
+    p[0] = v[0], p[1] = v[1], p[2] = v[2];
+  } else {
+    const nf4 t = {v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<nf4*>(p) = t;
+    store_n<N - 4>(p + 4, v + 4);
+  }
+}
+
+// Channel c of a row's degrees up to `most`; the others are zero.
+template <int L, int l = 0>
+__device__ __forceinline__ void load_row(const float* row, int C, int c, int most, float* v) {
+  if constexpr (l <= L) {
+    if (l <= most) {
+      load_n<2 * l + 1>(row + C * l * l + c * (2 * l + 1), v + l * l);
+    } else {
+#pragma unroll
+      for (int m = 0; m < 2 * l + 1; ++m) v[l * l + m] = 0.f;
+    }
+    load_row<L, l + 1>(row, C, c, most, v);
+  }
+}
+
+template <int L, int l = 0>
+__device__ __forceinline__ void store_row(float* row, int C, int c, int most, const float* v) {
+  if constexpr (l <= L) {
+    if (l <= most) store_n<2 * l + 1>(row + C * l * l + c * (2 * l + 1), v + l * l);
+    store_row<L, l + 1>(row, C, c, most, v);
+  }
+}
+
+template <int L>
+__device__ __forceinline__ void clear_row(float* v) {
+#pragma unroll
+  for (int i = 0; i < (L + 1) * (L + 1); ++i) v[i] = 0.f;
+}
+
+constexpr int degree_of(int i) { return i < 1 ? 0 : i < 4 ? 1 : i < 9 ? 2 : 3; }
+
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+
+template <int CTRL>
+__device__ __forceinline__ double add_dpp(double x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, 0xf, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, 0xf, 0xf, false);
+  return x + __hiloint2double(hi, lo);
+}
+
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
+__device__ __forceinline__ double lane_value(double x, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), lane),
+                          __builtin_amdgcn_readlane(__double2loint(x), lane));
+}
+
+constexpr int kMaxWaves = kNormMaxThreads / kNormWave;
+constexpr int kSums = 4;             // of a round at most
+
+// Sums over a row's threads, in all of them and in a fixed order.
+template <int S, int WIDE, typename T>
+__device__ __forceinline__ void row_sums(T (&x)[S], int threads, double* lds, int& turn) {
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    if (WIDE || threads >= 2) x[s] = add_dpp<0xB1>(x[s]);         // quad_perm 1 0 3 2
+    if (WIDE || threads >= 4) x[s] = add_dpp<0x4E>(x[s]);         // quad_perm 2 3 0 1
+    if (WIDE || threads >= 8) x[s] = add_dpp<0x141>(x[s]);        // row_half_mirror
+    if (WIDE || threads >= 16) x[s] = add_dpp<0x140>(x[s]);       // row_mirror
+    if (WIDE || threads == 64)
+      x[s] = (lane_value(x[s], 0) + lane_value(x[s], 16)) + (lane_value(x[s], 32) + lane_value(x[s], 48));
+    else if (threads == 32)
+      x[s] += __shfl_xor(x[s], 16);
+  }
+  if constexpr (WIDE) {
+    // two slots in turn: a wave is at most one round ahead of another
+    T* slot = reinterpret_cast<T*>(lds + turn * (kSums * kMaxWaves));
+    turn ^= 1;
+    const int waves = threads / kNormWave, wave = threadIdx.x / kNormWave;
+    if ((threadIdx.x & (kNormWave - 1)) == 0) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) slot[s * kMaxWaves + wave] = x[s];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      T sum = 0;
+      for (int w = 0; w < waves; ++w) sum += slot[s * kMaxWaves + w];
+      x[s] = sum;
+    }
+  }
+}
+
+// The rows of a workgroup: which of them is this thread's, and the channel that it holds.
+struct Place {
+  int c, group;
+  bool holds;
+};
+
+template <int WIDE>
+__device__ __forceinline__ Place place(const NormArgs& a) {
+  Place p;
+  p.group = WIDE ? 0 : threadIdx.x / a.threads;
+  p.c = WIDE ? threadIdx.x : threadIdx.x & (a.threads - 1);
+  p.holds = p.c < a.channels;
+  return p;
+}
+
+template <int L>
+__device__ __forceinline__ void load_weight(const float* w, int C, const Place& t, float* out) {
+#pragma unroll
+  for (int l = 0; l <= L; ++l) out[l] = w && t.holds ? w[l * C + t.c] : 0.f;
+}
+
+template <int L, typename T>
+__device__ __forceinline__ void shares(int C, T* a) {
+#pragma unroll
+  for (int l = 0; l <= L; ++l) a[l] = T(1) / static_cast<T>((L + 1) * (2 * l + 1) * C);
+}
+
+// Sums over a thread's components of products, by degree.
+template <int L>
+__device__ __forceinline__ void products(const float* u, const float* v, double* out) {
+#pragma unroll
+  for (int l = 0; l <= L; ++l) out[l] = 0.0;
+#pragma unroll
+  for (int i = 0; i < (L + 1) * (L + 1); ++i)
+    out[degree_of(i)] += static_cast<double>(u[i]) * static_cast<double>(v[i]);
+}
+
+// Gates of one row and what they leave, sigmoid(g) and sigmoid(-g), both to their last bits.
+template <int L>
+__device__ __forceinline__ void gates(const NormArgs& a, int64_t row, const Place& t, bool on, float* open,
+                                      float* closed) {
+#pragma unroll
+  for (int l = 0; l <= L; ++l) {
+    open[l] = 1.f, closed[l] = 0.f;
+    if (a.gate && on) {
+      const float g = a.gate[(row * (L + 1) + l) * a.channels + t.c];
+      const float z = expf(-fabsf(g)), inv = 1.f / (1.f + z);
+      open[l] = g < 0.f ? z * inv : inv;
+      closed[l] = g < 0.f ? inv : z * inv;
+    }
+  }
+}
+
+template <int L, int WIDE, bool BLOCK, bool NEXT>
+__global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) norm_forward_kernel(const NormArgs a) {
+  constexpr int D = (L + 1) * (L + 1);
+  __shared__ double lds[WIDE ? 2 * kSums * kMaxWaves : 1];
+  int turn = 0;
+  const Place t = place<WIDE>(a);
+  const int C = a.channels;
+  const int64_t width = static_cast<int64_t>(C) * D;
+  float post[L + 1], pre[L + 1], share[L + 1];
+  load_weight<L>(BLOCK ? a.post : nullptr, C, t, post);
+  load_weight<L>(NEXT ? a.pre : nullptr, C, t, pre);
+  shares<L>(C, share);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * a.groups;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.groups; base < a.rows; base += step) {
+    const int64_t row = base + t.group;
+    const bool on = t.holds && row < a.rows;
+    float h[D], b[D];
+    clear_row<L>(h);
+    clear_row<L>(b);
+    if (on) {
+      if constexpr (BLOCK) load_row<L>(a.block + row * width, C, t.c, L, b);
+      load_row<L>(a.x + row * a.width_x, C, t.c, a.input_lmax, h);
+    }
+    if constexpr (BLOCK) {
+      float open[L + 1], closed[L + 1];
+      gates<L>(a, row, t, on, open, closed);
+      float sums[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < D; ++i) sums[0] += share[degree_of(i)] * b[i] * b[i];
+      row_sums<1, WIDE>(sums, a.threads, lds, turn);
+      const float rho = 1.f / sqrtf(sums[0] + a.eps);
+#pragma unroll
+      for (int i = 0; i < D; ++i) h[i] += a.scale * open[degree_of(i)] * post[degree_of(i)] * rho * b[i];
+      if (on) store_row<L>(a.out_h + row * width, C, t.c, L, h);
+    }
+    if constexpr (NEXT) {
+      float sums[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < D; ++i) sums[0] += share[degree_of(i)] * h[i] * h[i];
+      row_sums<1, WIDE>(sums, a.threads, lds, turn);
+      const float rho = 1.f / sqrtf(sums[0] + a.eps);
+#pragma unroll
+      for (int i = 0; i < D; ++i) h[i] *= pre[degree_of(i)] * rho;
+      if (on) store_row<L>(a.out_y + row * width, C, t.c, L, h);
+    }
+  }
+}
+
+// A workgroup's weight gradients: each thread's over its rows, then over the workgroup's row groups, in order.
+template <int L, int WIDE>
+__device__ __forceinline__ void write_partial(const NormArgs& a, const Place& t, const float* post, const float* pre,
+                                              double* lds) {
+  float* stage = reinterpret_cast<float*>(lds);
+  const int C = a.channels;
+  float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * (L + 1) * C;
+#pragma unroll
+  for (int l = 0; l <= L; ++l)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float mine = w ? pre[l] : post[l];
+      if constexpr (WIDE) {
+        if (t.holds) out[(w * (L + 1) + l) * C + t.c] = mine;
+      } else {
+        __syncthreads();
+        stage[threadIdx.x] = mine;
+        __syncthreads();
+        if (t.group == 0 && t.holds) {
+          float sum = 0.f;
+          for (int g = 0; g < a.groups; ++g) sum += stage[g * a.threads + t.c];
+          out[(w * (L + 1) + l) * C + t.c] = sum;
+        }
+      }
+    }
+}
+
+template <int L, int WIDE, bool BLOCK, bool NEXT>
+__global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) norm_backward_kernel(const NormArgs a) {
+  constexpr int D = (L + 1) * (L + 1);
+  __shared__ double lds[WIDE ? 2 * kSums * kMaxWaves : kNormThreads / 2];
+  int turn = 0;
+  const Place t = place<WIDE>(a);
+  const int C = a.channels;
+  const int64_t width = static_cast<int64_t>(C) * D;
+  float post[L + 1], pre[L + 1], dpost[L + 1] = {}, dpre[L + 1] = {};
+  double share[L + 1];
+  load_weight<L>(BLOCK ? a.post : nullptr, C, t, post);
+  load_weight<L>(NEXT ? a.pre : nullptr, C, t, pre);
+  shares<L>(C, share);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * a.groups;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.groups; base < a.rows; base += step) {
+    const int64_t row = base + t.group;
+    const bool on = t.holds && row < a.rows;
+    float h[D], b[D], r[D], dy[D];
+    clear_row<L>(h);
+    clear_row<L>(b);
+    clear_row<L>(r);
+    clear_row<L>(dy);
+    if (on) {
+      if constexpr (NEXT) {
+        load_row<L>(a.h + row * width, C, t.c, L, h);
+        load_row<L>(a.dy + row * width, C, t.c, L, dy);
+      }
+      if constexpr (BLOCK) load_row<L>(a.block + row * width, C, t.c, L, b);
+      if (a.dh) load_row<L>(a.dh + row * width, C, t.c, L, r);
+    }
+    double hh[L + 1], yh[L + 1], bb[L + 1];
+    products<L>(h, h, hh);
+    products<L>(dy, h, yh);
+    products<L>(b, b, bb);
+    double sums[3] = {};      // q(h), <pre dy, h>, q(b)
+#pragma unroll
+    for (int l = 0; l <= L; ++l) {
+      sums[0] += share[l] * hh[l];
+      sums[1] += pre[l] * yh[l];
+      sums[2] += share[l] * bb[l];
+    }
+    row_sums<3, WIDE>(sums, a.threads, lds, turn);
+    if constexpr (NEXT) {
+      const double rho = 1.0 / sqrt(sums[0] + a.eps), pull = rho * rho * rho * sums[1];
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        const int l = degree_of(i);
+        r[i] = static_cast<float>(r[i] + pre[l] * rho * dy[i] - share[l] * pull * h[i]);
+      }
+#pragma unroll
+      for (int l = 0; l <= L; ++l) dpre[l] += static_cast<float>(rho * yh[l]);
+    }
+    if (on && a.dx) {
+      float* out = a.dx + row * a.width_x;
+      store_row<L>(out, C, t.c, a.input_lmax, r);
+      for (int64_t i = width + t.c; i < a.width_x; i += C) out[i] = 0.f;     // degrees of x beyond the block's
+    }
+    if constexpr (BLOCK) {
+      float open[L + 1], closed[L + 1];
+      gates<L>(a, row, t, on, open, closed);
+      double e[L + 1], k[L + 1], dot[1] = {0.0};
+      products<L>(r, b, e);
+#pragma unroll
+      for (int l = 0; l <= L; ++l) {
+        k[l] = a.scale * open[l] * post[l];
+        dot[0] += k[l] * e[l];
+      }
+      row_sums<1, WIDE>(dot, a.threads, lds, turn);
+      const double rho = 1.0 / sqrt(sums[2] + a.eps), pull = rho * rho * rho * dot[0];
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        const int l = degree_of(i);
+        r[i] = static_cast<float>(rho * k[l] * r[i] - share[l] * pull * b[i]);
+      }
+      if (on && a.db) store_row<L>(a.db + row * width, C, t.c, L, r);
+#pragma unroll
+      for (int l = 0; l <= L; ++l) {
+        const float along = a.scale * static_cast<float>(rho * e[l]) * open[l];
+        dpost[l] += along;
+        if (on && a.dg) a.dg[(row * (L + 1) + l) * C + t.c] = along * closed[l] * post[l];
+      }
+    }
+  }
+  if (a.partial) write_partial<L, WIDE>(a, t, dpost, dpre, lds);
+}
+
+template <int L, int WIDE, bool BLOCK, bool NEXT>
+__global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) norm_second_kernel(const NormArgs a) {
+  constexpr int D = (L + 1) * (L + 1);
+  __shared__ double lds[WIDE ? 2 * kSums * kMaxWaves : kNormThreads / 2];
+  int turn = 0;
+  const Place t = place<WIDE>(a);
+  const int C = a.channels;
+  const int64_t width = static_cast<int64_t>(C) * D;
+  float post[L + 1], pre[L + 1], gpost[L + 1] = {}, gpre[L + 1] = {};
+  double share[L + 1];
+  load_weight<L>(BLOCK ? a.post : nullptr, C, t, post);
+  load_weight<L>(NEXT ? a.pre : nullptr, C, t, pre);
+  shares<L>(C, share);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * a.groups;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.groups; base < a.rows; base += step) {
+    const int64_t row = base + t.group;
+    const bool on = t.holds && row < a.rows;
+    float h[D], b[D], r[D], dy[D], cb[D], R[D];
+    clear_row<L>(h);
+    clear_row<L>(b);
+    clear_row<L>(r);
+    clear_row<L>(dy);
+    clear_row<L>(cb);
+    clear_row<L>(R);
+    if (on) {
+      if constexpr (NEXT) {
+        load_row<L>(a.h + row * width, C, t.c, L, h);
+        load_row<L>(a.dy + row * width, C, t.c, L, dy);
+      }
+      if constexpr (BLOCK) {
+        load_row<L>(a.block + row * width, C, t.c, L, b);
+        if (a.cb) load_row<L>(a.cb + row * width, C, t.c, L, cb);
+        if (a.dh) load_row<L>(a.dh + row * width, C, t.c, L, r);
+      }
+      if (a.cx) load_row<L>(a.cx + row * a.width_x, C, t.c, a.input_lmax, R);
+    }
+    double hh[L + 1], yh[L + 1], bb[L + 1], cbb[L + 1];
+    products<L>(h, h, hh);
+    products<L>(dy, h, yh);
+    products<L>(b, b, bb);
+    products<L>(cb, b, cbb);
+    double sums[4] = {};      // q(h), <pre dy, h>, q(b), <a B, b>
+#pragma unroll
+    for (int l = 0; l <= L; ++l) {
+      sums[0] += share[l] * hh[l];
+      sums[1] += pre[l] * yh[l];
+      sums[2] += share[l] * bb[l];
+      sums[3] += share[l] * cbb[l];
+    }
+    row_sums<4, WIDE>(sums, a.threads, lds, turn);
+    const double rho_h = 1.0 / sqrt(sums[0] + a.eps), cube_h = rho_h * rho_h * rho_h;
+    if constexpr (BLOCK) {
+      if constexpr (NEXT) {
+        const double pull = cube_h * sums[1];
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+          const int l = degree_of(i);
+          r[i] = static_cast<float>(r[i] + pre[l] * rho_h * dy[i] - share[l] * pull * h[i]);
+        }
+      }
+      float open[L + 1], closed[L + 1];
+      double cg[L + 1];
+      gates<L>(a, row, t, on, open, closed);
+      double e[L + 1], f[L + 1], k[L + 1];
+      products<L>(r, b, e);
+      products<L>(r, cb, f);
+      double dots[2] = {};     // S1 and G's part of dPhi/dv's first factor together, S3
+      const double s2 = sums[3], rho = 1.0 / sqrt(sums[2] + a.eps), cube = rho * rho * rho;
+      float slope[L + 1];      // s sigmoid' post: the gate's derivative of k
+#pragma unroll
+      for (int l = 0; l <= L; ++l) {
+        cg[l] = a.cg && on ? a.cg[(row * (L + 1) + l) * C + t.c] : 0.0;
+        k[l] = a.scale * open[l] * post[l];
+        slope[l] = a.scale * open[l] * closed[l] * post[l];
+        dots[0] += k[l] * f[l] + cg[l] * slope[l] * e[l];
+        dots[1] += k[l] * e[l];
+      }
+      row_sums<2, WIDE>(dots, a.threads, lds, turn);
+      const double along = -cube * dots[0] + 3.0 * cube * rho * rho * s2 * dots[1];
+      float gb[D];
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        const int l = degree_of(i);
+        const double through = rho * slope[l] * cg[l];
+        gb[i] = static_cast<float>(share[l] * (along * b[i] - cube * dots[1] * cb[i]) +
+                                   (through - cube * s2 * k[l]) * r[i]);
+        R[i] = static_cast<float>(R[i] + k[l] * rho * cb[i] + (through - cube * s2 * k[l]) * b[i]);
+      }
+      if (on && a.gb) store_row<L>(a.gb + row * width, C, t.c, L, gb);
+#pragma unroll
+      for (int l = 0; l <= L; ++l) {
+        const float ck = static_cast<float>(rho * f[l] - cube * s2 * e[l]);     // k's cotangent
+        const float pass = static_cast<float>(rho * e[l] * cg[l]);              // G's product
+        gpost[l] += a.scale * open[l] * (ck + closed[l] * pass);
+        if (on && a.gg) a.gg[(row * (L + 1) + l) * C + t.c] = slope[l] * (ck + (closed[l] - open[l]) * pass);
+      }
+      if (on && a.gdh) store_row<L>(a.gdh + row * width, C, t.c, L, R);
+    }
+    if constexpr (NEXT) {
+      double ry[L + 1], rh[L + 1], dots[2] = {};    // <R, pre dy>, <a R, h>
+      products<L>(R, dy, ry);
+      products<L>(R, h, rh);
+#pragma unroll
+      for (int l = 0; l <= L; ++l) {
+        dots[0] += pre[l] * ry[l];
+        dots[1] += share[l] * rh[l];
+      }
+      row_sums<2, WIDE>(dots, a.threads, lds, turn);
+      const double along = -cube_h * dots[0] + 3.0 * cube_h * rho_h * rho_h * dots[1] * sums[1];
+      const double pull = cube_h * dots[1], turned = cube_h * sums[1];
+#pragma unroll
+      for (int l = 0; l <= L; ++l) gpre[l] += static_cast<float>(rho_h * ry[l] - pull * yh[l]);
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        const int l = degree_of(i);
+        const double ce = rho_h * R[i] - pull * h[i];                // the cotangent of e = pre dy
+        h[i] = static_cast<float>(share[l] * (along * h[i] - turned * R[i]) - pull * pre[l] * dy[i]);
+        R[i] = static_cast<float>(pre[l] * ce);
+      }
+      if (on && a.gh) store_row<L>(a.gh + row * width, C, t.c, L, h);
+      if (on && a.gdy) store_row<L>(a.gdy + row * width, C, t.c, L, R);
+    }
+  }
+  if (a.partial) write_partial<L, WIDE>(a, t, gpost, gpre, lds);
+}
+
+// Column sums of the workgroups' partial weight gradients, in order: 64 columns a workgroup, 16 slices.
+constexpr int kSlices = 16;
+
+__global__ void __launch_bounds__(kNormWave* kSlices)
+norm_weight_kernel(const float* __restrict__ partial, float* __restrict__ dpost, float* __restrict__ dpre, int groups,
+                   int columns) {
+  __shared__ double part[kSlices][kNormWave];
+  const int lane = threadIdx.x & (kNormWave - 1), slice = threadIdx.x / kNormWave;
+  const int column = blockIdx.x * kNormWave + lane;       // of post's, then of pre's
+  const int per = (groups + kSlices - 1) / kSlices;
+  double sum = 0.0;
+  if (column < 2 * columns)
+    for (int g = slice * per; g < groups && g < (slice + 1) * per; ++g)
+      sum += partial[static_cast<int64_t>(g) * 2 * columns + column];
+  part[slice][lane] = sum;
+  __syncthreads();
+  if (slice || column >= 2 * columns) return;
+  for (int s = 1; s < kSlices; ++s) sum += part[s][lane];
+  float* out = column < columns ? dpost : dpre;
+  if (out) out[column < columns ? column : column - columns] = static_cast<float>(sum);
+}
+
+struct NormShape {
+  int threads, groups, block;
+  int64_t grid;
+  int wide;                   // 0: within a wave; 1: up to kNormThreads; 2: up to kNormMaxThreads
+};
+
+NormShape shape_of(int channels, int64_t rows) {
+  NormShape s;
+  s.wide = channels <= kNormWave ? 0 : channels <= kNormThreads ? 1 : 2;
+  if (s.wide) {
+    s.threads = (channels + kNormWave - 1) / kNormWave * kNormWave;
+    s.groups = 1;
+    s.block = s.threads;
+  } else {
+    s.threads = 1;
+    while (s.threads < channels) s.threads *= 2;
+    s.block = kNormThreads;
+    s.groups = kNormThreads / s.threads;
+  }
+  s.grid = (rows + s.groups - 1) / s.groups;
+  return s;
+}
+
+int64_t partial_groups(const NormShape& s) { return s.grid < kNormGroups ? s.grid : kNormGroups; }
+
+using NormKernel = void (*)(NormArgs);
+
+template <int L, int WIDE, bool BLOCK, bool NEXT>
+NormKernel kernel_of(int order) {
+  return order == 0 ? norm_forward_kernel<L, WIDE, BLOCK, NEXT>
+                    : order == 1 ? norm_backward_kernel<L, WIDE, BLOCK, NEXT> : norm_second_kernel<L, WIDE, BLOCK, NEXT>;
+}
+
+template <int L, int WIDE>
+NormKernel kernel_of(int order, bool block, bool next) {
+  return !block ? kernel_of<L, WIDE, false, true>(order)
+                : next ? kernel_of<L, WIDE, true, true>(order) : kernel_of<L, WIDE, true, false>(order);
+}
+
+template <int L>
+NormKernel kernel_of(int order, int wide, bool block, bool next) {
+  return wide == 0 ? kernel_of<L, 0>(order, block, next)
+                   : wide == 1 ? kernel_of<L, 1>(order, block, next) : kernel_of<L, 2>(order, block, next);
+}
+
+bool valid(const ictc_norm_desc* d, int64_t rows) {
+  return d && rows >= 0 && d->channels >= 1 && d->channels <= ICTC_NORM_MAX_CHANNELS && d->lmax >= 0 && d->lmax <= 3 &&
+         d->input_lmax >= 0 && d->input_lmax <= 127 && d->eps > 0.f && rows <= (int64_t{1} << 40);
+}
+
+int run(int order, const ictc_norm_desc* d, NormArgs a, int64_t rows, bool block, bool next, float* dpost, float* dpre,
+        hipStream_t stream) {
+  const NormShape s = shape_of(d->channels, rows);
+  a.rows = rows;
+  a.channels = d->channels;
+  a.width_x = static_cast<int64_t>(d->channels) * (d->input_lmax + 1) * (d->input_lmax + 1);
+  a.input_lmax = d->input_lmax < d->lmax ? d->input_lmax : d->lmax;
+  a.threads = s.threads;
+  a.groups = s.groups;
+  a.scale = d->residual_scale;
+  a.eps = d->eps;
+  const bool weights = dpost || dpre;
+  if (!weights) a.partial = nullptr;
+  const int64_t most = weights ? partial_groups(s) : int64_t{1} << 30;
+  const int64_t grid = s.grid < most ? s.grid : most;
+  const NormKernel kernel = d->lmax == 0   ? kernel_of<0>(order, s.wide, block, next)
+                            : d->lmax == 1 ? kernel_of<1>(order, s.wide, block, next)
+                            : d->lmax == 2 ? kernel_of<2>(order, s.wide, block, next)
+                                           : kernel_of<3>(order, s.wide, block, next);
+  if (grid) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(s.block), 0, stream, a);
+    if (hipGetLastError() != hipSuccess) return ICTC_ERR_LAUNCH;
+  }
+  if (weights) {
+    const int columns = d->channels * (d->lmax + 1);
+    hipLaunchKernelGGL(norm_weight_kernel, dim3((2 * columns + kNormWave - 1) / kNormWave), dim3(kNormWave * kSlices), 0,
+                       stream, a.partial, dpost, dpre, static_cast<int>(grid), columns);
+    if (hipGetLastError() != hipSuccess) return ICTC_ERR_LAUNCH;
+  }
+  return ICTC_OK;
+}
+
+}  // namespace
+}  // namespace ictc
+
+extern "C" {
+
+int64_t ictc_hip_norm_workspace(const ictc_norm_desc* desc, int64_t rows) {
+  using namespace ictc;
+  if (!valid(desc, rows)) return -ICTC_ERR_INVALID_ARGUMENT;
+  const int64_t groups = partial_groups(shape_of(desc->channels, rows));
+  return (groups ? groups : 1) * 2 * desc->channels * (desc->lmax + 1);
+}
+
+int ictc_hip_norm_forward(const ictc_norm_desc* desc, const float* x, const float* block, const float* gate,
+                          const float* post, const float* pre, float* h, float* y, int64_t rows, hipStream_t stream) {
+  using namespace ictc;
+  if (!valid(desc, rows) || (!block && (gate || post || h || !pre || desc->input_lmax != desc->lmax)) ||
+      (block && !post))
+    return ICTC_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return ICTC_OK;
+  if (!x || (block && !h) || (!pre != !y)) return ICTC_ERR_INVALID_ARGUMENT;
+  NormArgs a = {};
+  a.x = x, a.block = block, a.gate = gate, a.post = post, a.pre = pre, a.out_h = h, a.out_y = y;
+  return run(0, desc, a, rows, block != nullptr, pre != nullptr, nullptr, nullptr, stream);
+}
+
+int ictc_hip_norm_backward(const ictc_norm_desc* desc, const float* h, const float* block, const float* gate,
+                           const float* post, const float* pre, const float* grad_h, const float* grad_y, float* dx,
+                           float* dblock, float* dgate, float* dpost, float* dpre, float* workspace,
+                           int64_t workspace_floats, int64_t rows, hipStream_t stream) {
+  using namespace ictc;
+  if (!valid(desc, rows) || (!block && (gate || post || grad_h || dblock || dpost || !pre || desc->input_lmax != desc->lmax)) ||
+      (block && !post) || (dgate && !gate) || (dpre && !pre) || (!pre && grad_y))
+    return ICTC_ERR_INVALID_ARGUMENT;
+  if ((dpost || dpre) && (!workspace || workspace_floats < ictc_hip_norm_workspace(desc, rows)))
+    return ICTC_ERR_INVALID_ARGUMENT;
+  if (rows == 0 && !dpost && !dpre) return ICTC_OK;
+  const bool next = pre && grad_y;
+  if (rows && ((next && !h) || (!grad_y && !grad_h) || (!block && !grad_y))) return ICTC_ERR_INVALID_ARGUMENT;
+  NormArgs a = {};
+  a.h = h, a.block = block, a.gate = gate, a.post = post, a.pre = pre, a.dh = grad_h, a.dy = grad_y;
+  a.dx = dx, a.db = dblock, a.dg = dgate, a.partial = workspace;
+  return run(1, desc, a, rows, block != nullptr, next, dpost, dpre, stream);
+}
+
+int ictc_hip_norm_second(const ictc_norm_desc* desc, const float* h, const float* block, const float* gate,
+                         const float* post, const float* pre, const float* grad_h, const float* grad_y,
+                         const float* cot_x, const float* cot_block, const float* cot_gate, float* dh, float* dblock,
+                         float* dgate, float* dgrad_h, float* dgrad_y, float* dpost, float* dpre, float* workspace,
+                         int64_t workspace_floats, int64_t rows, hipStream_t stream) {
+  using namespace ictc;
+  const bool next = pre && grad_y;
+  if (!valid(desc, rows) ||
+      (!block && (gate || post || grad_h || cot_block || cot_gate || dblock || dgate || dgrad_h || dpost || !next ||
+                  desc->input_lmax != desc->lmax)) ||
+      (block && !post) || ((dgate || cot_gate) && !gate) || (dpre && !next) || ((dh || dgrad_y) && !next) ||
+      (!pre && grad_y) || (!grad_y && !grad_h))
+    return ICTC_ERR_INVALID_ARGUMENT;
+  if ((dpost || dpre) && (!workspace || workspace_floats < ictc_hip_norm_workspace(desc, rows)))
+    return ICTC_ERR_INVALID_ARGUMENT;
+  if (rows == 0 && !dpost && !dpre) return ICTC_OK;
+  if (rows && next && !h) return ICTC_ERR_INVALID_ARGUMENT;
+  NormArgs a = {};
+  a.h = h, a.block = block, a.gate = gate, a.post = post, a.pre = pre, a.dh = grad_h, a.dy = grad_y;
+  a.cx = cot_x, a.cb = cot_block, a.cg = cot_gate;
+  a.gh = dh, a.gb = dblock, a.gg = dgate, a.gdh = dgrad_h, a.gdy = dgrad_y, a.partial = workspace;
+  return run(2, desc, a, rows, block != nullptr, next, dpost, dpre, stream);
+}
+
+}  // extern "C"

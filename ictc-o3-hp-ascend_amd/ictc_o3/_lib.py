@@ -59,6 +59,17 @@ class AdamwDesc(ctypes.Structure):
     ]
 
 
+class NormDesc(ctypes.Structure):
+    """Mirror of ``ictc_norm_desc``."""
+    _fields_ = [
+        ("channels", ctypes.c_int32),
+        ("lmax", ctypes.c_int32),
+        ("input_lmax", ctypes.c_int32),
+        ("residual_scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+    ]
+
+
 class CellGrid(ctypes.Structure):
     """Mirror of ``ictc_cell_grid``."""
     _fields_ = [
@@ -141,6 +152,10 @@ _SIGNATURES = {
     "ictc_hip_gradient_norm": (ctypes.c_int, [_P, _P, _I64, ctypes.c_float, _P, _I64, _P, _P]),
     "ictc_hip_adamw_step": (ctypes.c_int, [_P, _P, _P, _I64, ctypes.POINTER(AdamwDesc)] + [_P] * 8),
     "ictc_hip_moment_values": (ctypes.c_int, [_P] * 6 + [_I64, _P]),
+    "ictc_hip_norm_workspace": (_I64, [ctypes.POINTER(NormDesc), _I64]),
+    "ictc_hip_norm_forward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_P] * 7 + [_I64, _P]),
+    "ictc_hip_norm_backward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_P] * 13 + [_I64, _I64, _P]),
+    "ictc_hip_norm_second": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_P] * 18 + [_I64, _I64, _P]),
     "ictc_hip_sgemm": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _I64, _I64, _I64, ctypes.c_float, _P, _I64, _P,
                                       _I64, ctypes.c_float, _P, _I64, _P]),
     "ictc_hip_radius_graph_bins": (ctypes.c_int, [ctypes.POINTER(CellGrid), _P, _I64, _P, _P, _P, _P, _P, _P]),

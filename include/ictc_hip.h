@@ -745,6 +745,49 @@ int ictc_hip_moment_values(const uint8_t* exp_avg, const uint8_t* exp_avg_top, c
                            int64_t values, hipStream_t stream);
 
 /*
+ * Norms of a residual block on node features (no counterpart in the reference, whose layers have none).
+ * Rows in mul_ir order: per degree l <= lmax a [C, 2l+1] block.  Weights and gates [(lmax+1) C], per degree C.
+ *   N(v; w)_lcm = w_lc v_lcm rho(v),  rho(v) = (q + eps)^(-1/2),  q = mean over l, c and m of v^2, each
+ *                                     degree with the same weight (N commutes with rotations)
+ *   forward:  h = x + residual_scale sigmoid(gate) N(block; post)      y = N(h; pre)
+ * x has the degrees up to input_lmax: those beyond lmax are left out, missing ones are zero.  gate may be
+ * null (no gate), pre and y may be null (no norm behind the block).  Without a block (block, gate, post and
+ * h null; input_lmax = lmax) it is the norm alone, y = N(x; pre), and `h` stands for x below.
+ *
+ *   backward: from grad_h (may be null) and grad_y (null without pre; may be null) the gradients to x, block,
+ *             gate, post and pre; any output may be null.  h is forward's result.
+ *   second:   the gradients of <cot_x, dx> + <cot_block, dblock> + <cot_gate, dgate> (any may be null), dx,
+ *             dblock and dgate being backward's, to h (taken as an argument of its own), block, gate, grad_h,
+ *             grad_y, post and pre; any output may be null, those to h, grad_y and pre must be without grad_y.
+ *
+ * Weight gradients need a workspace of ictc_hip_norm_workspace(desc, rows) floats (negative: -ictc_status)
+ * and are summed in a fixed order; they are zero for rows = 0.  1 <= channels <= ICTC_NORM_MAX_CHANNELS,
+ * lmax <= 3, eps > 0.
+ */
+#define ICTC_NORM_MAX_CHANNELS 1024
+
+typedef struct ictc_norm_desc {
+    int32_t channels;
+    int32_t lmax;
+    int32_t input_lmax;
+    float residual_scale;
+    float eps;
+} ictc_norm_desc;
+
+int64_t ictc_hip_norm_workspace(const ictc_norm_desc* desc, int64_t rows);
+int ictc_hip_norm_forward(const ictc_norm_desc* desc, const float* x, const float* block, const float* gate,
+                          const float* post, const float* pre, float* h, float* y, int64_t rows, hipStream_t stream);
+int ictc_hip_norm_backward(const ictc_norm_desc* desc, const float* h, const float* block, const float* gate,
+                           const float* post, const float* pre, const float* grad_h, const float* grad_y, float* dx,
+                           float* dblock, float* dgate, float* dpost, float* dpre, float* workspace,
+                           int64_t workspace_floats, int64_t rows, hipStream_t stream);
+int ictc_hip_norm_second(const ictc_norm_desc* desc, const float* h, const float* block, const float* gate,
+                         const float* post, const float* pre, const float* grad_h, const float* grad_y,
+                         const float* cot_x, const float* cot_block, const float* cot_gate, float* dh, float* dblock,
+                         float* dgate, float* dgrad_h, float* dgrad_y, float* dpost, float* dpre, float* workspace,
+                         int64_t workspace_floats, int64_t rows, hipStream_t stream);
+
+/*
  * Row-major fp32 product C[m,n] = alpha * op(A) op(B) + beta * C on rocBLAS, for the dense
  * channel linears around the operators.  op(A) is [m,k]: A is stored [m,k] (lda >= k) or,
  * with trans_a != 0, [k,m] (lda >= m); likewise B with op(B) [k,n].  Each host thread uses
