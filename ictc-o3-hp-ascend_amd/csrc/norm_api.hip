@@ -42,6 +42,11 @@ constexpr int kNormGroups = 1024;            // workgroups that leave partial we
 
 typedef float nf4 __attribute__((ext_vector_type(4), aligned(4)));
 
+// Threads of a workgroup by where a row's threads are: 0 within a wave, else in up to 4, 8 or 16 waves of their own.
+constexpr int most_threads(int wide) {
+  return wide < 2 ? kNormThreads : wide == 2 ? 2 * kNormThreads : kNormMaxThreads;
+}
+
 struct NormArgs {
   const float *x, *block, *gate, *post, *pre, *h, *dh, *dy, *cx, *cb, *cg;
   float *out_h, *out_y, *dx, *db, *dg;
@@ -82,25 +87,49 @@ __device__ __forceinline__ void store_n(float* p, const float* v) {
   }
 }
 
-// Channel c of a row's degrees up to `most`; the others are zero.
+// Where a thread's components of each degree are, in bytes from the workgroup's first row: 32 bits beside a
+// uniform address.
+template <int L>
+struct Offsets {
+  uint32_t at[L + 1];
+};
+
+template <int L>
+__device__ __forceinline__ Offsets<L> offsets(int64_t width, int C, int c, int group) {
+  Offsets<L> o;
+#pragma unroll
+  for (int l = 0; l <= L; ++l)
+    o.at[l] = (static_cast<uint32_t>(group) * static_cast<uint32_t>(width) + C * l * l + c * (2 * l + 1)) * 4u;
+  return o;
+}
+
+__device__ __forceinline__ const float* at_bytes(const float* p, uint32_t bytes) {
+  return reinterpret_cast<const float*>(reinterpret_cast<const char*>(p) + bytes);
+}
+
+__device__ __forceinline__ float* at_bytes(float* p, uint32_t bytes) {
+  return reinterpret_cast<float*>(reinterpret_cast<char*>(p) + bytes);
+}
+
+// A thread's components of the degrees up to `most`; the others are zero.
 template <int L, int l = 0>
-__device__ __forceinline__ void load_row(const float* row, int C, int c, int most, float* v) {
+__device__ __forceinline__ void load_row(const float* rows, const Offsets<L>& o, int most, float* v) {
   if constexpr (l <= L) {
     if (l <= most) {
-      load_n<2 * l + 1>(row + C * l * l + c * (2 * l + 1), v + l * l);
+      load_n<2 * l + 1>(at_bytes(rows, o.at[l]), v + l * l);
     } else {
 #pragma unroll
       for (int m = 0; m < 2 * l + 1; ++m) v[l * l + m] = 0.f;
     }
-    load_row<L, l + 1>(row, C, c, most, v);
+    load_row<L, l + 1>(rows, o, most, v);
   }
 }
 
 template <int L, int l = 0>
-__device__ __forceinline__ void store_row(float* row, int C, int c, int most, const float* v) {
+__device__ __forceinline__ void store_row(float* rows, const Offsets<L>& o, int most, const float* v) {
   if constexpr (l <= L) {
-    if (l <= most) store_n<2 * l + 1>(row + C * l * l + c * (2 * l + 1), v + l * l);
-    store_row<L, l + 1>(row, C, c, most, v);
+    if (l <= most) store_n<2 * l + 1>(at_bytes(rows, o.at[l]), v + l * l);
+    store_row<L, l + 1>(rows, o, most, v);
   }
 }
 
@@ -196,6 +225,36 @@ __device__ __forceinline__ void shares(int C, T* a) {
   for (int l = 0; l <= L; ++l) a[l] = T(1) / static_cast<T>((L + 1) * (2 * l + 1) * C);
 }
 
+// One degree's sum of products of a thread's components.
+template <int l>
+__device__ __forceinline__ double product(const float* u, const float* v) {
+  double s = 0.0;
+#pragma unroll
+  for (int m = 0; m < 2 * l + 1; ++m) s += static_cast<double>(u[l * l + m]) * static_cast<double>(v[l * l + m]);
+  return s;
+}
+
+// f(Degree<0>{}), ..., f(Degree<L>{})
+template <int l>
+struct Degree {
+  static constexpr int value = l;
+};
+
+template <int L, int l = 0, typename F>
+__device__ __forceinline__ void degrees(F&& f) {
+  if constexpr (l <= L) {
+    f(Degree<l>{});
+    degrees<L, l + 1>(f);
+  }
+}
+
+// Values that the compiler does not carry over in the 64-bit form it has of them (twice the registers).
+template <int N>
+__device__ __forceinline__ void narrow(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
+}
+
 // Sums over a thread's components of products, by degree.
 template <int L>
 __device__ __forceinline__ void products(const float* u, const float* v, double* out) {
@@ -208,13 +267,13 @@ __device__ __forceinline__ void products(const float* u, const float* v, double*
 
 // Gates of one row and what they leave, sigmoid(g) and sigmoid(-g), both to their last bits.
 template <int L>
-__device__ __forceinline__ void gates(const NormArgs& a, int64_t row, const Place& t, bool on, float* open,
+__device__ __forceinline__ void gates(const NormArgs& a, int64_t base, uint32_t own_gate, bool on, float* open,
                                       float* closed) {
 #pragma unroll
   for (int l = 0; l <= L; ++l) {
     open[l] = 1.f, closed[l] = 0.f;
     if (a.gate && on) {
-      const float g = a.gate[(row * (L + 1) + l) * a.channels + t.c];
+      const float g = *at_bytes(a.gate + (base * (L + 1) + l) * a.channels, own_gate);
       const float z = expf(-fabsf(g)), inv = 1.f / (1.f + z);
       open[l] = g < 0.f ? z * inv : inv;
       closed[l] = g < 0.f ? inv : z * inv;
@@ -223,7 +282,7 @@ __device__ __forceinline__ void gates(const NormArgs& a, int64_t row, const Plac
 }
 
 template <int L, int WIDE, bool BLOCK, bool NEXT>
-__global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) norm_forward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(most_threads(WIDE)) norm_forward_kernel(const NormArgs a) {
   constexpr int D = (L + 1) * (L + 1);
   __shared__ double lds[WIDE ? 2 * kSums * kMaxWaves : 1];
   int turn = 0;
@@ -234,6 +293,8 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
   load_weight<L>(BLOCK ? a.post : nullptr, C, t, post);
   load_weight<L>(NEXT ? a.pre : nullptr, C, t, pre);
   shares<L>(C, share);
+  const Offsets<L> own = offsets<L>(width, C, t.c, t.group), own_x = offsets<L>(a.width_x, C, t.c, t.group);
+  const uint32_t own_gate = (static_cast<uint32_t>(t.group) * (L + 1) * C + t.c) * 4u;
   const int64_t step = static_cast<int64_t>(gridDim.x) * a.groups;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.groups; base < a.rows; base += step) {
     const int64_t row = base + t.group;
@@ -242,12 +303,12 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
     clear_row<L>(h);
     clear_row<L>(b);
     if (on) {
-      if constexpr (BLOCK) load_row<L>(a.block + row * width, C, t.c, L, b);
-      load_row<L>(a.x + row * a.width_x, C, t.c, a.input_lmax, h);
+      if constexpr (BLOCK) load_row<L>(a.block + base * width, own, L, b);
+      load_row<L>(a.x + base * a.width_x, own_x, a.input_lmax, h);
     }
     if constexpr (BLOCK) {
       float open[L + 1], closed[L + 1];
-      gates<L>(a, row, t, on, open, closed);
+      gates<L>(a, base, own_gate, on, open, closed);
       float sums[1] = {0.f};
 #pragma unroll
       for (int i = 0; i < D; ++i) sums[0] += share[degree_of(i)] * b[i] * b[i];
@@ -255,7 +316,7 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
       const float rho = 1.f / sqrtf(sums[0] + a.eps);
 #pragma unroll
       for (int i = 0; i < D; ++i) h[i] += a.scale * open[degree_of(i)] * post[degree_of(i)] * rho * b[i];
-      if (on) store_row<L>(a.out_h + row * width, C, t.c, L, h);
+      if (on) store_row<L>(a.out_h + base * width, own, L, h);
     }
     if constexpr (NEXT) {
       float sums[1] = {0.f};
@@ -265,7 +326,7 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
       const float rho = 1.f / sqrtf(sums[0] + a.eps);
 #pragma unroll
       for (int i = 0; i < D; ++i) h[i] *= pre[degree_of(i)] * rho;
-      if (on) store_row<L>(a.out_y + row * width, C, t.c, L, h);
+      if (on) store_row<L>(a.out_y + base * width, own, L, h);
     }
   }
 }
@@ -298,7 +359,7 @@ __device__ __forceinline__ void write_partial(const NormArgs& a, const Place& t,
 }
 
 template <int L, int WIDE, bool BLOCK, bool NEXT>
-__global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) norm_backward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(most_threads(WIDE)) norm_backward_kernel(const NormArgs a) {
   constexpr int D = (L + 1) * (L + 1);
   __shared__ double lds[WIDE ? 2 * kSums * kMaxWaves : kNormThreads / 2];
   int turn = 0;
@@ -310,6 +371,8 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
   load_weight<L>(BLOCK ? a.post : nullptr, C, t, post);
   load_weight<L>(NEXT ? a.pre : nullptr, C, t, pre);
   shares<L>(C, share);
+  const Offsets<L> own = offsets<L>(width, C, t.c, t.group), own_x = offsets<L>(a.width_x, C, t.c, t.group);
+  const uint32_t own_gate = (static_cast<uint32_t>(t.group) * (L + 1) * C + t.c) * 4u;
   const int64_t step = static_cast<int64_t>(gridDim.x) * a.groups;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.groups; base < a.rows; base += step) {
     const int64_t row = base + t.group;
@@ -321,11 +384,11 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
     clear_row<L>(dy);
     if (on) {
       if constexpr (NEXT) {
-        load_row<L>(a.h + row * width, C, t.c, L, h);
-        load_row<L>(a.dy + row * width, C, t.c, L, dy);
+        load_row<L>(a.h + base * width, own, L, h);
+        load_row<L>(a.dy + base * width, own, L, dy);
       }
-      if constexpr (BLOCK) load_row<L>(a.block + row * width, C, t.c, L, b);
-      if (a.dh) load_row<L>(a.dh + row * width, C, t.c, L, r);
+      if constexpr (BLOCK) load_row<L>(a.block + base * width, own, L, b);
+      if (a.dh) load_row<L>(a.dh + base * width, own, L, r);
     }
     double hh[L + 1], yh[L + 1], bb[L + 1];
     products<L>(h, h, hh);
@@ -338,6 +401,7 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
       sums[1] += pre[l] * yh[l];
       sums[2] += share[l] * bb[l];
     }
+    narrow(h), narrow(b), narrow(dy);
     row_sums<3, WIDE>(sums, a.threads, lds, turn);
     if constexpr (NEXT) {
       const double rho = 1.0 / sqrt(sums[0] + a.eps), pull = rho * rho * rho * sums[1];
@@ -350,13 +414,13 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
       for (int l = 0; l <= L; ++l) dpre[l] += static_cast<float>(rho * yh[l]);
     }
     if (on && a.dx) {
+      store_row<L>(a.dx + base * a.width_x, own_x, a.input_lmax, r);
       float* out = a.dx + row * a.width_x;
-      store_row<L>(out, C, t.c, a.input_lmax, r);
       for (int64_t i = width + t.c; i < a.width_x; i += C) out[i] = 0.f;     // degrees of x beyond the block's
     }
     if constexpr (BLOCK) {
       float open[L + 1], closed[L + 1];
-      gates<L>(a, row, t, on, open, closed);
+      gates<L>(a, base, own_gate, on, open, closed);
       double e[L + 1], k[L + 1], dot[1] = {0.0};
       products<L>(r, b, e);
 #pragma unroll
@@ -364,6 +428,7 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
         k[l] = a.scale * open[l] * post[l];
         dot[0] += k[l] * e[l];
       }
+      narrow(r), narrow(b);
       row_sums<1, WIDE>(dot, a.threads, lds, turn);
       const double rho = 1.0 / sqrt(sums[2] + a.eps), pull = rho * rho * rho * dot[0];
 #pragma unroll
@@ -371,12 +436,12 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
         const int l = degree_of(i);
         r[i] = static_cast<float>(rho * k[l] * r[i] - share[l] * pull * b[i]);
       }
-      if (on && a.db) store_row<L>(a.db + row * width, C, t.c, L, r);
+      if (on && a.db) store_row<L>(a.db + base * width, own, L, r);
 #pragma unroll
       for (int l = 0; l <= L; ++l) {
         const float along = a.scale * static_cast<float>(rho * e[l]) * open[l];
         dpost[l] += along;
-        if (on && a.dg) a.dg[(row * (L + 1) + l) * C + t.c] = along * closed[l] * post[l];
+        if (on && a.dg) *at_bytes(a.dg + (base * (L + 1) + l) * C, own_gate) = along * closed[l] * post[l];
       }
     }
   }
@@ -384,7 +449,8 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
 }
 
 template <int L, int WIDE, bool BLOCK, bool NEXT>
-__global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) norm_second_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(most_threads(WIDE)) __attribute__((amdgpu_waves_per_eu(WIDE == 1 && L == 3 ? 2 : 1)))
+norm_second_kernel(const NormArgs a) {
   constexpr int D = (L + 1) * (L + 1);
   __shared__ double lds[WIDE ? 2 * kSums * kMaxWaves : kNormThreads / 2];
   int turn = 0;
@@ -396,6 +462,8 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
   load_weight<L>(BLOCK ? a.post : nullptr, C, t, post);
   load_weight<L>(NEXT ? a.pre : nullptr, C, t, pre);
   shares<L>(C, share);
+  const Offsets<L> own = offsets<L>(width, C, t.c, t.group), own_x = offsets<L>(a.width_x, C, t.c, t.group);
+  const uint32_t own_gate = (static_cast<uint32_t>(t.group) * (L + 1) * C + t.c) * 4u;
   const int64_t step = static_cast<int64_t>(gridDim.x) * a.groups;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * a.groups; base < a.rows; base += step) {
     const int64_t row = base + t.group;
@@ -409,124 +477,143 @@ __global__ void __launch_bounds__(WIDE == 2 ? kNormMaxThreads : kNormThreads) no
     clear_row<L>(R);
     if (on) {
       if constexpr (NEXT) {
-        load_row<L>(a.h + row * width, C, t.c, L, h);
-        load_row<L>(a.dy + row * width, C, t.c, L, dy);
+        load_row<L>(a.h + base * width, own, L, h);
+        load_row<L>(a.dy + base * width, own, L, dy);
       }
       if constexpr (BLOCK) {
-        load_row<L>(a.block + row * width, C, t.c, L, b);
-        if (a.cb) load_row<L>(a.cb + row * width, C, t.c, L, cb);
-        if (a.dh) load_row<L>(a.dh + row * width, C, t.c, L, r);
+        load_row<L>(a.block + base * width, own, L, b);
+        if (a.cb) load_row<L>(a.cb + base * width, own, L, cb);
+        if (a.dh) load_row<L>(a.dh + base * width, own, L, r);
       }
-      if (a.cx) load_row<L>(a.cx + row * a.width_x, C, t.c, a.input_lmax, R);
+      if (a.cx) load_row<L>(a.cx + base * a.width_x, own_x, a.input_lmax, R);
     }
-    double hh[L + 1], yh[L + 1], bb[L + 1], cbb[L + 1];
-    products<L>(h, h, hh);
-    products<L>(dy, h, yh);
-    products<L>(b, b, bb);
-    products<L>(cb, b, cbb);
     double sums[4] = {};      // q(h), <pre dy, h>, q(b), <a B, b>
-#pragma unroll
-    for (int l = 0; l <= L; ++l) {
-      sums[0] += share[l] * hh[l];
-      sums[1] += pre[l] * yh[l];
-      sums[2] += share[l] * bb[l];
-      sums[3] += share[l] * cbb[l];
-    }
+    degrees<L>([&](auto d) {
+      constexpr int l = decltype(d)::value;
+      if constexpr (NEXT) {
+        sums[0] += share[l] * product<l>(h, h);
+        sums[1] += pre[l] * product<l>(dy, h);
+      }
+      if constexpr (BLOCK) {
+        sums[2] += share[l] * product<l>(b, b);
+        sums[3] += share[l] * product<l>(cb, b);
+      }
+    });
+    narrow(h), narrow(b), narrow(dy), narrow(cb);
     row_sums<4, WIDE>(sums, a.threads, lds, turn);
     const double rho_h = 1.0 / sqrt(sums[0] + a.eps), cube_h = rho_h * rho_h * rho_h;
     if constexpr (BLOCK) {
       if constexpr (NEXT) {
         const double pull = cube_h * sums[1];
+        degrees<L>([&](auto d) {
+          constexpr int l = decltype(d)::value;
+          const double up = pre[l] * rho_h, down = share[l] * pull;
 #pragma unroll
-        for (int i = 0; i < D; ++i) {
-          const int l = degree_of(i);
-          r[i] = static_cast<float>(r[i] + pre[l] * rho_h * dy[i] - share[l] * pull * h[i]);
-        }
+          for (int i = l * l; i < (l + 1) * (l + 1); ++i) r[i] = static_cast<float>(r[i] + up * dy[i] - down * h[i]);
+        });
+        narrow(r), narrow(h), narrow(dy);
       }
-      float open[L + 1], closed[L + 1];
-      double cg[L + 1];
-      gates<L>(a, row, t, on, open, closed);
-      double e[L + 1], f[L + 1], k[L + 1];
-      products<L>(r, b, e);
-      products<L>(r, cb, f);
+      float open[L + 1], closed[L + 1], cg[L + 1];
+      gates<L>(a, base, own_gate, on, open, closed);
+      double e[L + 1], f[L + 1];
       double dots[2] = {};     // S1 and G's part of dPhi/dv's first factor together, S3
       const double s2 = sums[3], rho = 1.0 / sqrt(sums[2] + a.eps), cube = rho * rho * rho;
-      float slope[L + 1];      // s sigmoid' post: the gate's derivative of k
-#pragma unroll
-      for (int l = 0; l <= L; ++l) {
-        cg[l] = a.cg && on ? a.cg[(row * (L + 1) + l) * C + t.c] : 0.0;
-        k[l] = a.scale * open[l] * post[l];
-        slope[l] = a.scale * open[l] * closed[l] * post[l];
-        dots[0] += k[l] * f[l] + cg[l] * slope[l] * e[l];
-        dots[1] += k[l] * e[l];
-      }
+      degrees<L>([&](auto d) {
+        constexpr int l = decltype(d)::value;
+        cg[l] = a.cg && on ? *at_bytes(a.cg + (base * (L + 1) + l) * C, own_gate) : 0.f;
+        e[l] = product<l>(r, b);
+        f[l] = product<l>(r, cb);
+        const double k = a.scale * open[l] * post[l], slope = a.scale * open[l] * closed[l] * post[l];
+        dots[0] += k * f[l] + cg[l] * slope * e[l];      // (slope: the gate's derivative of k)
+        dots[1] += k * e[l];
+      });
+      narrow(r), narrow(b), narrow(cb);
       row_sums<2, WIDE>(dots, a.threads, lds, turn);
-      const double along = -cube * dots[0] + 3.0 * cube * rho * rho * s2 * dots[1];
-      float gb[D];
-#pragma unroll
-      for (int i = 0; i < D; ++i) {
-        const int l = degree_of(i);
-        const double through = rho * slope[l] * cg[l];
-        gb[i] = static_cast<float>(share[l] * (along * b[i] - cube * dots[1] * cb[i]) +
-                                   (through - cube * s2 * k[l]) * r[i]);
-        R[i] = static_cast<float>(R[i] + k[l] * rho * cb[i] + (through - cube * s2 * k[l]) * b[i]);
-      }
-      if (on && a.gb) store_row<L>(a.gb + row * width, C, t.c, L, gb);
-#pragma unroll
-      for (int l = 0; l <= L; ++l) {
+      const double along = -cube * dots[0] + 3.0 * cube * rho * rho * s2 * dots[1], away = cube * dots[1];
+      degrees<L>([&](auto d) {
+        constexpr int l = decltype(d)::value;
+        const double k = a.scale * open[l] * post[l], slope = a.scale * open[l] * closed[l] * post[l];
+        const double through = rho * cg[l] * slope - cube * s2 * k;
         const float ck = static_cast<float>(rho * f[l] - cube * s2 * e[l]);     // k's cotangent
         const float pass = static_cast<float>(rho * e[l] * cg[l]);              // G's product
         gpost[l] += a.scale * open[l] * (ck + closed[l] * pass);
-        if (on && a.gg) a.gg[(row * (L + 1) + l) * C + t.c] = slope[l] * (ck + (closed[l] - open[l]) * pass);
-      }
-      if (on && a.gdh) store_row<L>(a.gdh + row * width, C, t.c, L, R);
+        if (on && a.gg)
+          *at_bytes(a.gg + (base * (L + 1) + l) * C, own_gate) =
+              static_cast<float>(slope) * (ck + (closed[l] - open[l]) * pass);
+        const double ab = share[l] * along, ac = share[l] * away, up = k * rho;
+        float gb[2 * l + 1];
+#pragma unroll
+        for (int m = 0; m < 2 * l + 1; ++m) {
+          const int i = l * l + m;
+          gb[m] = static_cast<float>(ab * b[i] - ac * cb[i] + through * r[i]);
+          R[i] = static_cast<float>(R[i] + up * cb[i] + through * b[i]);
+        }
+        if (on && a.gb) store_n<2 * l + 1>(at_bytes(a.gb + base * width, own.at[l]), gb);
+      });
+      if (on && a.gdh) store_row<L>(a.gdh + base * width, own, L, R);
     }
     if constexpr (NEXT) {
-      double ry[L + 1], rh[L + 1], dots[2] = {};    // <R, pre dy>, <a R, h>
-      products<L>(R, dy, ry);
-      products<L>(R, h, rh);
-#pragma unroll
-      for (int l = 0; l <= L; ++l) {
-        dots[0] += pre[l] * ry[l];
-        dots[1] += share[l] * rh[l];
-      }
+      double dots[2] = {};    // <R, pre dy>, <a R, h>
+      degrees<L>([&](auto d) {
+        constexpr int l = decltype(d)::value;
+        dots[0] += pre[l] * product<l>(R, dy);
+        dots[1] += share[l] * product<l>(R, h);
+      });
+      narrow(R), narrow(h), narrow(dy);
       row_sums<2, WIDE>(dots, a.threads, lds, turn);
       const double along = -cube_h * dots[0] + 3.0 * cube_h * rho_h * rho_h * dots[1] * sums[1];
       const double pull = cube_h * dots[1], turned = cube_h * sums[1];
+      degrees<L>([&](auto d) {
+        constexpr int l = decltype(d)::value;
+        const double ah = share[l] * along, ar = share[l] * turned, ay = pull * pre[l];
+        float gh[2 * l + 1], gdy[2 * l + 1];
+        double sum = 0.0;
 #pragma unroll
-      for (int l = 0; l <= L; ++l) gpre[l] += static_cast<float>(rho_h * ry[l] - pull * yh[l]);
-#pragma unroll
-      for (int i = 0; i < D; ++i) {
-        const int l = degree_of(i);
-        const double ce = rho_h * R[i] - pull * h[i];                // the cotangent of e = pre dy
-        h[i] = static_cast<float>(share[l] * (along * h[i] - turned * R[i]) - pull * pre[l] * dy[i]);
-        R[i] = static_cast<float>(pre[l] * ce);
-      }
-      if (on && a.gh) store_row<L>(a.gh + row * width, C, t.c, L, h);
-      if (on && a.gdy) store_row<L>(a.gdy + row * width, C, t.c, L, R);
+        for (int m = 0; m < 2 * l + 1; ++m) {
+          const int i = l * l + m;
+          const double ce = rho_h * R[i] - pull * h[i];                // the cotangent of e = pre dy
+          sum += ce * dy[i];
+          gh[m] = static_cast<float>(ah * h[i] - ar * R[i] - ay * dy[i]);
+          gdy[m] = static_cast<float>(pre[l] * ce);
+        }
+        gpre[l] += static_cast<float>(sum);
+        if (on && a.gh) store_n<2 * l + 1>(at_bytes(a.gh + base * width, own.at[l]), gh);
+        if (on && a.gdy) store_n<2 * l + 1>(at_bytes(a.gdy + base * width, own.at[l]), gdy);
+      });
     }
   }
   if (a.partial) write_partial<L, WIDE>(a, t, gpost, gpre, lds);
 }
 
-// Column sums of the workgroups' partial weight gradients, in order: 64 columns a workgroup, 16 slices.
-constexpr int kSlices = 16;
+// Column sums of the workgroups' partial weight gradients, in order: 16 columns a workgroup, and 32 slices
+// of the partials side by side, eight of whose loads are on their way at a time.
+constexpr int kSlices = 32, kColumns = 16;
 
-__global__ void __launch_bounds__(kNormWave* kSlices)
+__global__ void __launch_bounds__(kSlices* kColumns)
 norm_weight_kernel(const float* __restrict__ partial, float* __restrict__ dpost, float* __restrict__ dpre, int groups,
                    int columns) {
-  __shared__ double part[kSlices][kNormWave];
-  const int lane = threadIdx.x & (kNormWave - 1), slice = threadIdx.x / kNormWave;
-  const int column = blockIdx.x * kNormWave + lane;       // of post's, then of pre's
+  __shared__ double part[kSlices][kColumns];
+  const int at = threadIdx.x % kColumns, slice = threadIdx.x / kColumns;
+  const int column = blockIdx.x * kColumns + at;          // of post's, then of pre's
   const int per = (groups + kSlices - 1) / kSlices;
+  const int end = groups < (slice + 1) * per ? groups : (slice + 1) * per;
   double sum = 0.0;
-  if (column < 2 * columns)
-    for (int g = slice * per; g < groups && g < (slice + 1) * per; ++g)
-      sum += partial[static_cast<int64_t>(g) * 2 * columns + column];
-  part[slice][lane] = sum;
+  if (column < 2 * columns) {
+    const float* p = partial + column;
+    int g = slice * per;
+    for (; g + 8 <= end; g += 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = p[static_cast<int64_t>(g + k) * 2 * columns];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += v[k];
+    }
+    for (; g < end; ++g) sum += p[static_cast<int64_t>(g) * 2 * columns];
+  }
+  part[slice][at] = sum;
   __syncthreads();
   if (slice || column >= 2 * columns) return;
-  for (int s = 1; s < kSlices; ++s) sum += part[s][lane];
+  for (int s = 1; s < kSlices; ++s) sum += part[s][at];
   float* out = column < columns ? dpost : dpre;
   if (out) out[column < columns ? column : column - columns] = static_cast<float>(sum);
 }
@@ -534,12 +621,12 @@ norm_weight_kernel(const float* __restrict__ partial, float* __restrict__ dpost,
 struct NormShape {
   int threads, groups, block;
   int64_t grid;
-  int wide;                   // 0: within a wave; 1: up to kNormThreads; 2: up to kNormMaxThreads
+  int wide;                   // see most_threads
 };
 
 NormShape shape_of(int channels, int64_t rows) {
   NormShape s;
-  s.wide = channels <= kNormWave ? 0 : channels <= kNormThreads ? 1 : 2;
+  s.wide = channels <= kNormWave ? 0 : channels <= most_threads(1) ? 1 : channels <= most_threads(2) ? 2 : 3;
   if (s.wide) {
     s.threads = (channels + kNormWave - 1) / kNormWave * kNormWave;
     s.groups = 1;
@@ -560,8 +647,9 @@ using NormKernel = void (*)(NormArgs);
 
 template <int L, int WIDE, bool BLOCK, bool NEXT>
 NormKernel kernel_of(int order) {
-  return order == 0 ? norm_forward_kernel<L, WIDE, BLOCK, NEXT>
-                    : order == 1 ? norm_backward_kernel<L, WIDE, BLOCK, NEXT> : norm_second_kernel<L, WIDE, BLOCK, NEXT>;
+  return order == 0   ? norm_forward_kernel<L, WIDE, BLOCK, NEXT>
+         : order == 1 ? norm_backward_kernel<L, WIDE, BLOCK, NEXT>
+                      : norm_second_kernel<L, WIDE, BLOCK, NEXT>;
 }
 
 template <int L, int WIDE>
@@ -572,8 +660,9 @@ NormKernel kernel_of(int order, bool block, bool next) {
 
 template <int L>
 NormKernel kernel_of(int order, int wide, bool block, bool next) {
-  return wide == 0 ? kernel_of<L, 0>(order, block, next)
-                   : wide == 1 ? kernel_of<L, 1>(order, block, next) : kernel_of<L, 2>(order, block, next);
+  return wide == 0   ? kernel_of<L, 0>(order, block, next)
+         : wide == 1 ? kernel_of<L, 1>(order, block, next)
+         : wide == 2 ? kernel_of<L, 2>(order, block, next) : kernel_of<L, 3>(order, block, next);
 }
 
 bool valid(const ictc_norm_desc* d, int64_t rows) {
@@ -606,7 +695,7 @@ int run(int order, const ictc_norm_desc* d, NormArgs a, int64_t rows, bool block
   }
   if (weights) {
     const int columns = d->channels * (d->lmax + 1);
-    hipLaunchKernelGGL(norm_weight_kernel, dim3((2 * columns + kNormWave - 1) / kNormWave), dim3(kNormWave * kSlices), 0,
+    hipLaunchKernelGGL(norm_weight_kernel, dim3((2 * columns + kColumns - 1) / kColumns), dim3(kColumns * kSlices), 0,
                        stream, a.partial, dpost, dpre, static_cast<int>(grid), columns);
     if (hipGetLastError() != hipSuccess) return ICTC_ERR_LAUNCH;
   }
@@ -643,7 +732,8 @@ int ictc_hip_norm_backward(const ictc_norm_desc* desc, const float* h, const flo
                            float* dblock, float* dgate, float* dpost, float* dpre, float* workspace,
                            int64_t workspace_floats, int64_t rows, hipStream_t stream) {
   using namespace ictc;
-  if (!valid(desc, rows) || (!block && (gate || post || grad_h || dblock || dpost || !pre || desc->input_lmax != desc->lmax)) ||
+  if (!valid(desc, rows) ||
+      (!block && (gate || post || grad_h || dblock || dpost || !pre || desc->input_lmax != desc->lmax)) ||
       (block && !post) || (dgate && !gate) || (dpre && !pre) || (!pre && grad_y))
     return ICTC_ERR_INVALID_ARGUMENT;
   if ((dpost || dpre) && (!workspace || workspace_floats < ictc_hip_norm_workspace(desc, rows)))

@@ -95,6 +95,12 @@ def _second(desc, h, block, gate, post, pre, dh, dy, cx, cb, cg, need):
     return out
 
 
+def _weights_run(post, pre, declared) -> bool:
+    """Whether the engine will use a weight's gradient (not so where forces are taken from positions).  One
+    answer decides for both, and rows are not asked about: a question costs as much as the call."""
+    return any(n and required_gradients((w,), (True,))[0] for w, n in zip((post, pre), declared))
+
+
 class _Layout:
     """Index of each column's degree and (degree, channel) place, and its share in the mean."""
 
@@ -161,7 +167,9 @@ class _Gradient(torch.autograd.Function):
         inputs = ctx.saved_tensors
         desc = ctx.desc
         h, block, gate, post, pre, dh, dy = inputs
-        need = required_gradients(inputs, ctx.needs_input_grad[2:])
+        need = list(ctx.needs_input_grad[2:])
+        if not _weights_run(post, pre, need[3:5]):
+            need[3] = need[4] = False
         if not any(need) or all(c is None for c in cots):
             return (None,) * 9
         graph = torch.is_grad_enabled()
@@ -186,6 +194,11 @@ class _Gradient(torch.autograd.Function):
         return (None, None, *_second(desc, *inputs, cx, cb, cg, need))
 
 
+def _gradients(desc, need, *inputs):
+    """The gradients, recorded where a graph is (a function of its own costs 15 us a call)."""
+    return _Gradient.apply(desc, need, *inputs) if torch.is_grad_enabled() else _backward(desc, *inputs, need)
+
+
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, desc, x, pre):
@@ -196,11 +209,11 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x, pre = ctx.saved_tensors
-        need = required_gradients((x, pre), ctx.needs_input_grad[1:])
+        need = (ctx.needs_input_grad[1], _weights_run(None, pre, (False, ctx.needs_input_grad[2])))
         if not any(need):
             return None, None, None
-        dx, _, _, _, dpre = _Gradient.apply(ctx.desc, (need[0], False, False, False, need[1]), x, None, None, None,
-                                            pre, None, dy.contiguous())
+        dx, _, _, _, dpre = _gradients(ctx.desc, (need[0], False, False, False, need[1]), x, None, None, None, pre,
+                                       None, dy.contiguous())
         return None, dx, dpre
 
 
@@ -218,7 +231,9 @@ class _BlockEnd(torch.autograd.Function):
         h, block, gate, post, pre = ctx.saved_tensors
         if dh is None and dy is None:
             return (None,) * 6
-        need = [ctx.needs_input_grad[1], *required_gradients((block, gate, post, pre), ctx.needs_input_grad[2:])]
+        need = list(ctx.needs_input_grad[1:])
+        if not _weights_run(post, pre, need[3:5]):
+            need[3] = need[4] = False
         dx = None
         if dy is None:
             need[4] = False
@@ -226,7 +241,7 @@ class _BlockEnd(torch.autograd.Function):
                 dx, need[0] = dh, False
         if not any(need):
             return None, dx, None, None, None, None
-        grads = _Gradient.apply(ctx.desc, tuple(need), h, block, gate, post, pre, _cont(dh), _cont(dy))
+        grads = _gradients(ctx.desc, tuple(need), h, block, gate, post, pre, _cont(dh), _cont(dy))
         return (None, grads[0] if dx is None else dx, *grads[1:])
 
 
