@@ -378,7 +378,8 @@ class MaceICTC(nn.Module):
                 e = self.layer_readouts[t](scalars)
             elif deferred is not None:
                 lin1, _, lin2 = self.last_readout
-                e = readout(deferred, h, self.layer_readouts[t - 1].weight, lin1.weight, lin2.weight, SILU_SCALE)
+                e = readout(deferred, h, self.layer_readouts[t - 1].weight, lin1.weight, lin2.weight,
+                            SILU_SCALE).unsqueeze(1)     # as the layers' [N, 1]
             else:
                 e = self.last_readout(h)
             energy = e if energy is None else energy + e
