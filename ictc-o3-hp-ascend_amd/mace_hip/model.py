@@ -17,6 +17,15 @@ Architecture (reference ``mace_ictc/models/pure_cartesian_ictd_fix.py``; factory
     energy  += readout_t(h_{t+1})                                (:3095-3101)
   layer 0 has input degree 0 (paths (0,l,l)); the last product targets l = 0.
 
+``block_norm=True`` (no counterpart in the reference; off by default) makes each interaction and product a
+block of a residual stream, for stacks of more interactions than plain sums carry well:
+
+  r_0 = h_0, y_0 = norm(r_0);   b_t = product_t(interaction_t(y_t))
+  r_{t+1} = r_t + s sigmoid(gate_t(y_t's scalars)) norm(b_t),   y_{t+1} = norm(r_{t+1})
+
+with s = 1 / sqrt(interactions), the readouts on y_{t+1}, and the norms, gate and sum of a block's end in one
+kernel (``gated_residual_norm``).
+
 Dense layers (radial MLP, channel linears, readouts) go through ``mace_hip.linear`` (one GEMM
 per layer and degree; weight gradients reduced in row blocks).  The edge directions and the
 Bessel x cutoff embedding come from ``mace_hip.embedding`` (one HIP kernel per derivative order).
@@ -46,6 +55,7 @@ from ictc_o3.backends.hip.degree_linear import (DegreeLinearPlan, degree_linear,
                                                  degree_linear_mul_ir)
 from ictc_o3.backends.hip.graph_message import message_bonds, packed_graph_message
 from ictc_o3.backends.hip.harmonics import direction_harmonics_packed
+from ictc_o3.backends.hip.norms import equivariant_norm, gated_residual_norm
 from ictc_o3.backends.hip.radial_message import fold_projection, packed_radial_graph_message
 from ictc_o3.basis.ictd_irreps import EdgeWeightedPathPreservingTensorProduct
 from ictc_o3.ops.symmetric_contraction import ICTDBridgeUSymmetricContractionSO3
@@ -282,7 +292,7 @@ def _side_stream(device: torch.device) -> "torch.cuda.Stream":
 class MaceICTC(nn.Module):
     def __init__(self, *, channels: int = 128, lmax: int = 3, num_interactions: int = 2, correlation: int = 3,
                  atomic_numbers=tuple(range(1, 11)), cutoff: float = 5.0, avg_num_neighbors: float = 50.0,
-                 num_basis: int = 8, cutoff_p: int = 5, readout_hidden: int = 16):
+                 num_basis: int = 8, cutoff_p: int = 5, readout_hidden: int = 16, block_norm: bool = False):
         super().__init__()
         self.channels, self.lmax, self.cutoff = int(channels), int(lmax), float(cutoff)
         self.num_basis, self.cutoff_p = int(num_basis), int(cutoff_p)
@@ -309,6 +319,17 @@ class MaceICTC(nn.Module):
         self.layer_readouts = nn.ModuleList([_mace_linear(self.channels, 1) for _ in range(num_interactions - 1)])
         self.last_readout = nn.Sequential(_mace_linear(self.channels, readout_hidden), NormalizedSiLU(),
                                           _mace_linear(readout_hidden, 1))
+        self.block_norm = bool(block_norm)
+        if self.block_norm:
+            ones = lambda target: nn.Parameter(torch.ones(target + 1, self.channels))      # noqa: E731
+            self.residual_scale = 1.0 / math.sqrt(num_interactions)
+            self.input_norm = ones(0)
+            self.block_post_norms = nn.ParameterList([ones(target) for target in targets])
+            self.block_pre_norms = nn.ParameterList([ones(target) for target in targets])   # behind each block
+            self.block_gates = nn.ModuleList([Linear(self.channels, (target + 1) * self.channels)
+                                              for target in targets])
+            for gate in self.block_gates:
+                nn.init.zeros_(gate.weight)          # every gate half open
 
     def set_message_streaming(self, edge_chunk_size: Optional[int]) -> None:
         """Radial streaming in every interaction (receiver ranges of at most ``edge_chunk_size``
@@ -360,6 +381,8 @@ class MaceICTC(nn.Module):
             h = self.node_embedding.weight.t().index_select(0, species)
         side = self._side_work(edge_feats, harmonics)
         energy = None
+        if self.block_norm:
+            stream, h = h, equivariant_norm(h, self.input_norm, channels=self.channels)
         scalars = h
         last = len(self.interactions) - 1
         deferred = None   # the second-to-last layer's scalars, read out with the last layer's
@@ -370,7 +393,14 @@ class MaceICTC(nn.Module):
                 torch.cuda.current_stream(pos.device).wait_event(ready)
             message, sc = interaction(h, harmonics, edge_feats, edge_src, edge_dst, mask, species, scalars,
                                       gates, bonds)
-            h, scalars = product(message, sc, species)
+            if self.block_norm:
+                gate = self.block_gates[t](scalars)
+                stream, h = gated_residual_norm(stream, product(message, sc, species)[0], gate,
+                                                self.block_post_norms[t], self.block_pre_norms[t],
+                                                channels=self.channels, residual_scale=self.residual_scale)
+                scalars = h[:, :self.channels]
+            else:
+                h, scalars = product(message, sc, species)
             if t == last - 1 and self._fused_readout(scalars, h):
                 deferred = scalars
                 continue

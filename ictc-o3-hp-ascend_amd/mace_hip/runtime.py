@@ -28,7 +28,9 @@ from .model import MaceICTC
 
 def create_model(*, channels=64, lmax=3, edge_lmax=None, num_interactions=2, correlation=3,
                  atomic_numbers=(1, 6, 8), cutoff=5.0, avg_num_neighbors=50.0, device="cuda",
-                 dtype=torch.float32, seed=None) -> MaceICTC:
+                 dtype=torch.float32, seed=None, block_norm=False) -> MaceICTC:
+    """The model with the reference's arguments; ``block_norm`` (no counterpart there) gives every block norms
+    before and after it, a gate and a residual stream (see ``mace_hip.model``)."""
     if dtype != torch.float32:
         raise ValueError("the HIP operators compute in float32")
     if not isinstance(num_interactions, int) or isinstance(num_interactions, bool) or num_interactions < 1:
@@ -44,7 +46,8 @@ def create_model(*, channels=64, lmax=3, edge_lmax=None, num_interactions=2, cor
     if seed is not None:
         torch.manual_seed(int(seed))
     model = MaceICTC(channels=channels, lmax=lmax, num_interactions=num_interactions, correlation=correlation,
-                     atomic_numbers=atomic_numbers, cutoff=cutoff, avg_num_neighbors=avg_num_neighbors)
+                     atomic_numbers=atomic_numbers, cutoff=cutoff, avg_num_neighbors=avg_num_neighbors,
+                     block_norm=block_norm)
     return model.to(device=device, dtype=dtype)
 
 
@@ -237,8 +240,8 @@ class CapturedEnergyAndForces:
 class CapturedTrainingStep:
     """One force-loss training step (energy + forces with create_graph, loss backward, optimizer
     step) captured once and replayed on new positions.  The optimizer must keep its state on
-    the device (``torch.optim.AdamW(..., capturable=True)``, which may also be ``fused=True``: one
-    update kernel for all parameters, 0.3 ms less per cfg-4 step); gradients are released before
+    the device (``ictc_o3.optim.AdamW``, or ``torch.optim.AdamW(..., capturable=True)``, which may also be
+    ``fused=True``: one update kernel for all parameters, 0.3 ms less per cfg-4 step); gradients are released before
     capture so that backward writes them into the graph's own buffers on every replay."""
 
     def __init__(self, model, optimizer, graph: dict, *, species=None, warmup: int = 3):
