@@ -18,7 +18,9 @@
 //     dPhi/de = rho B - rho^3 S2 v
 //     dPhi/dv = -rho^3 a v S1 + 3 rho^5 a v S2 S3 - rho^3 (a B S3 + e S2)
 //   once at the block (v = b, e = k r), whose dPhi/de gives r's cotangent R = X + k dPhi/de + (G's part), and
-//   once at the next norm (v = h, e = pre dy, R in B's place).
+//   once at the next norm (v = h, e = pre dy, R in B's place).  h's own cotangent H then goes back through the
+//   forward pass in the same kernel: H to x, V(b; k H) to b, and so on (another pass over b and H otherwise,
+//   and sums of two gradients of every operand: 100 us of 414 for 8,192 rows of C = 128, L = 3).
 //
 // All of it is bound by memory: a row is read into registers once, its sums are taken there, and its results
 // are written once.  The gradients' sums and projections are in 64 bits: they take away the part of a
@@ -50,7 +52,7 @@ constexpr int most_threads(int wide) {
 struct NormArgs {
   const float *x, *block, *gate, *post, *pre, *h, *dh, *dy, *cx, *cb, *cg;
   float *out_h, *out_y, *dx, *db, *dg;
-  float *gh, *gb, *gg, *gdh, *gdy;
+  float *gx, *gb, *gg, *gdh, *gdy;
   float* partial;             // per workgroup [2][L+1][C]: post's and pre's gradients
   int64_t rows;
   int64_t width_x;            // floats of a row of x, dx and cx
@@ -248,7 +250,8 @@ __device__ __forceinline__ void degrees(F&& f) {
   }
 }
 
-// Values that the compiler does not carry over in the 64-bit form it has of them (twice the registers).
+// Values that are what they are from here on: the compiler neither carries them over in the 64-bit form it has
+// of them nor moves the operations that make them behind a condition (all their operands would stay).
 template <int N>
 __device__ __forceinline__ void narrow(float (&v)[N]) {
 #pragma unroll
@@ -413,6 +416,7 @@ __global__ void __launch_bounds__(most_threads(WIDE)) norm_backward_kernel(const
 #pragma unroll
       for (int l = 0; l <= L; ++l) dpre[l] += static_cast<float>(rho * yh[l]);
     }
+    narrow(r);
     if (on && a.dx) {
       store_row<L>(a.dx + base * a.width_x, own_x, a.input_lmax, r);
       float* out = a.dx + row * a.width_x;
@@ -436,6 +440,7 @@ __global__ void __launch_bounds__(most_threads(WIDE)) norm_backward_kernel(const
         const int l = degree_of(i);
         r[i] = static_cast<float>(rho * k[l] * r[i] - share[l] * pull * b[i]);
       }
+      narrow(r);
       if (on && a.db) store_row<L>(a.db + base * width, own, L, r);
 #pragma unroll
       for (int l = 0; l <= L; ++l) {
@@ -502,6 +507,8 @@ norm_second_kernel(const NormArgs a) {
     narrow(h), narrow(b), narrow(dy), narrow(cb);
     row_sums<4, WIDE>(sums, a.threads, lds, turn);
     const double rho_h = 1.0 / sqrt(sums[0] + a.eps), cube_h = rho_h * rho_h * rho_h;
+    const double rho = 1.0 / sqrt(sums[2] + a.eps);
+    [[maybe_unused]] float open[L + 1], closed[L + 1], gg[L + 1];
     if constexpr (BLOCK) {
       if constexpr (NEXT) {
         const double pull = cube_h * sums[1];
@@ -513,11 +520,11 @@ norm_second_kernel(const NormArgs a) {
         });
         narrow(r), narrow(h), narrow(dy);
       }
-      float open[L + 1], closed[L + 1], cg[L + 1];
+      float cg[L + 1];
       gates<L>(a, base, own_gate, on, open, closed);
       double e[L + 1], f[L + 1];
       double dots[2] = {};     // S1 and G's part of dPhi/dv's first factor together, S3
-      const double s2 = sums[3], rho = 1.0 / sqrt(sums[2] + a.eps), cube = rho * rho * rho;
+      const double s2 = sums[3], cube = rho * rho * rho;
       degrees<L>([&](auto d) {
         constexpr int l = decltype(d)::value;
         cg[l] = a.cg && on ? *at_bytes(a.cg + (base * (L + 1) + l) * C, own_gate) : 0.f;
@@ -537,19 +544,15 @@ norm_second_kernel(const NormArgs a) {
         const float ck = static_cast<float>(rho * f[l] - cube * s2 * e[l]);     // k's cotangent
         const float pass = static_cast<float>(rho * e[l] * cg[l]);              // G's product
         gpost[l] += a.scale * open[l] * (ck + closed[l] * pass);
-        if (on && a.gg)
-          *at_bytes(a.gg + (base * (L + 1) + l) * C, own_gate) =
-              static_cast<float>(slope) * (ck + (closed[l] - open[l]) * pass);
+        gg[l] = static_cast<float>(slope) * (ck + (closed[l] - open[l]) * pass);
         const double ab = share[l] * along, ac = share[l] * away, up = k * rho;
-        float gb[2 * l + 1];
 #pragma unroll
-        for (int m = 0; m < 2 * l + 1; ++m) {
-          const int i = l * l + m;
-          gb[m] = static_cast<float>(ab * b[i] - ac * cb[i] + through * r[i]);
+        for (int i = l * l; i < (l + 1) * (l + 1); ++i) {
           R[i] = static_cast<float>(R[i] + up * cb[i] + through * b[i]);
+          r[i] = static_cast<float>(ab * b[i] - ac * cb[i] + through * r[i]);      // b's gradient from here on
         }
-        if (on && a.gb) store_n<2 * l + 1>(at_bytes(a.gb + base * width, own.at[l]), gb);
       });
+      narrow(R), narrow(r);
       if (on && a.gdh) store_row<L>(a.gdh + base * width, own, L, R);
     }
     if constexpr (NEXT) {
@@ -566,20 +569,50 @@ norm_second_kernel(const NormArgs a) {
       degrees<L>([&](auto d) {
         constexpr int l = decltype(d)::value;
         const double ah = share[l] * along, ar = share[l] * turned, ay = pull * pre[l];
-        float gh[2 * l + 1], gdy[2 * l + 1];
         double sum = 0.0;
 #pragma unroll
-        for (int m = 0; m < 2 * l + 1; ++m) {
-          const int i = l * l + m;
+        for (int i = l * l; i < (l + 1) * (l + 1); ++i) {
           const double ce = rho_h * R[i] - pull * h[i];                // the cotangent of e = pre dy
           sum += ce * dy[i];
-          gh[m] = static_cast<float>(ah * h[i] - ar * R[i] - ay * dy[i]);
-          gdy[m] = static_cast<float>(pre[l] * ce);
+          h[i] = static_cast<float>(ah * h[i] - ar * R[i] - ay * dy[i]);           // H from here on
+          R[i] = static_cast<float>(pre[l] * ce);
         }
         gpre[l] += static_cast<float>(sum);
-        if (on && a.gh) store_n<2 * l + 1>(at_bytes(a.gh + base * width, own.at[l]), gh);
-        if (on && a.gdy) store_n<2 * l + 1>(at_bytes(a.gdy + base * width, own.at[l]), gdy);
       });
+      narrow(R), narrow(h);
+      if (on && a.gdy) store_row<L>(a.gdy + base * width, own, L, R);
+      if (on && a.gx) {
+        store_row<L>(a.gx + base * a.width_x, own_x, a.input_lmax, h);
+        float* out = a.gx + row * a.width_x;
+        for (int64_t i = width + t.c; i < a.width_x; i += C) out[i] = 0.f;         // degrees of x beyond the block's
+      }
+    }
+    if constexpr (BLOCK) {
+      if constexpr (NEXT) {
+        double e[L + 1], dot[1] = {0.0};
+        degrees<L>([&](auto d) {
+          constexpr int l = decltype(d)::value;
+          e[l] = product<l>(h, b);
+          dot[0] += static_cast<double>(a.scale * open[l] * post[l]) * e[l];
+        });
+        narrow(h), narrow(b);
+        row_sums<1, WIDE>(dot, a.threads, lds, turn);
+        const double pull = rho * rho * rho * dot[0];
+        degrees<L>([&](auto d) {
+          constexpr int l = decltype(d)::value;
+          const double up = rho * static_cast<double>(a.scale * open[l] * post[l]), down = share[l] * pull;
+#pragma unroll
+          for (int i = l * l; i < (l + 1) * (l + 1); ++i) r[i] = static_cast<float>(r[i] + up * h[i] - down * b[i]);
+          const float pass = a.scale * static_cast<float>(rho * e[l]) * open[l];
+          gpost[l] += pass;
+          gg[l] += pass * closed[l] * post[l];
+        });
+      }
+      narrow(r), narrow(gg);
+      if (on && a.gb) store_row<L>(a.gb + base * width, own, L, r);
+#pragma unroll
+      for (int l = 0; l <= L; ++l)
+        if (on && a.gg) *at_bytes(a.gg + (base * (L + 1) + l) * C, own_gate) = gg[l];
     }
   }
   if (a.partial) write_partial<L, WIDE>(a, t, gpost, gpre, lds);
@@ -749,7 +782,7 @@ int ictc_hip_norm_backward(const ictc_norm_desc* desc, const float* h, const flo
 
 int ictc_hip_norm_second(const ictc_norm_desc* desc, const float* h, const float* block, const float* gate,
                          const float* post, const float* pre, const float* grad_h, const float* grad_y,
-                         const float* cot_x, const float* cot_block, const float* cot_gate, float* dh, float* dblock,
+                         const float* cot_x, const float* cot_block, const float* cot_gate, float* dx, float* dblock,
                          float* dgate, float* dgrad_h, float* dgrad_y, float* dpost, float* dpre, float* workspace,
                          int64_t workspace_floats, int64_t rows, hipStream_t stream) {
   using namespace ictc;
@@ -757,7 +790,7 @@ int ictc_hip_norm_second(const ictc_norm_desc* desc, const float* h, const float
   if (!valid(desc, rows) ||
       (!block && (gate || post || grad_h || cot_block || cot_gate || dblock || dgate || dgrad_h || dpost || !next ||
                   desc->input_lmax != desc->lmax)) ||
-      (block && !post) || ((dgate || cot_gate) && !gate) || (dpre && !next) || ((dh || dgrad_y) && !next) ||
+      (block && !post) || ((dgate || cot_gate) && !gate) || (dpre && !next) || ((dx || dgrad_y) && !next) ||
       (!pre && grad_y) || (!grad_y && !grad_h))
     return ICTC_ERR_INVALID_ARGUMENT;
   if ((dpost || dpre) && (!workspace || workspace_floats < ictc_hip_norm_workspace(desc, rows)))
@@ -767,7 +800,7 @@ int ictc_hip_norm_second(const ictc_norm_desc* desc, const float* h, const float
   NormArgs a = {};
   a.h = h, a.block = block, a.gate = gate, a.post = post, a.pre = pre, a.dh = grad_h, a.dy = grad_y;
   a.cx = cot_x, a.cb = cot_block, a.cg = cot_gate;
-  a.gh = dh, a.gb = dblock, a.gg = dgate, a.gdh = dgrad_h, a.gdy = dgrad_y, a.partial = workspace;
+  a.gx = dx, a.gb = dblock, a.gg = dgate, a.gdh = dgrad_h, a.gdy = dgrad_y, a.partial = workspace;
   return run(2, desc, a, rows, block != nullptr, next, dpost, dpre, stream);
 }
 

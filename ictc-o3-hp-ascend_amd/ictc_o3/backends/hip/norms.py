@@ -75,21 +75,20 @@ def _backward(desc, h, block, gate, post, pre, dh, dy, need):
     return dx, db, dg, dpost, dpre
 
 
-def _second(desc, h, block, gate, post, pre, dh, dy, cx, cb, cg, need):
-    """Gradients to (h, block, gate, post, pre, dh, dy), None where not needed."""
+def _second(desc, x, h, block, gate, post, pre, dh, dy, cx, cb, cg, need):
+    """Gradients to (x, block, gate, post, pre, dh, dy), None where not needed."""
     p = _lib.ptr
-    like = h if block is None else block
-    rows, device = like.shape[0], like.device
-    out = [torch.empty_like(t) if n else None for t, n in zip((h, block, gate, post, pre, dh, dy), need)]
+    rows, device = x.shape[0], x.device
+    out = [torch.empty_like(t) if n else None for t, n in zip((x, block, gate, post, pre, dh, dy), need)]
     if rows == 0:
         for w in out[3:5]:
             if w is not None:
                 w.zero_()
         return out
     ws = _workspace(desc, rows, device) if need[3] or need[4] else None
-    gh, gb, gg, gpost, gpre, gdh, gdy = out
+    gx, gb, gg, gpost, gpre, gdh, gdy = out
     _lib.check(_lib.lib().ictc_hip_norm_second(
-        ctypes.byref(desc), p(h), p(block), p(gate), p(post), p(pre), p(dh), p(dy), p(cx), p(cb), p(cg), p(gh), p(gb),
+        ctypes.byref(desc), p(h), p(block), p(gate), p(post), p(pre), p(dh), p(dy), p(cx), p(cb), p(cg), p(gx), p(gb),
         p(gg), p(gdh), p(gdy), p(gpost), p(gpre), p(ws), 0 if ws is None else ws.numel(), rows,
         _lib.stream_of(device)), "ictc_hip_norm_second")
     return out
@@ -119,11 +118,14 @@ class _Layout:
         return v.new_zeros(v.shape[0], self.places).index_add(1, self.place, v)
 
 
-def gradient_formula(desc, h, block, gate, post, pre, dh, dy):
-    """(dx, dblock, dgate, dpost, dpre) of torch operations: what ``ictc_hip_norm_backward`` computes."""
-    like = h if block is None else block
-    lay = _Layout(desc.channels, desc.lmax, like.device)
-    r, dpre = dh, None
+def gradient_formula(desc, x, block, gate, post, pre, dh, dy):
+    """(dx, dblock, dgate, dpost, dpre) of torch operations: what ``ictc_hip_norm_backward`` computes, from the
+    forward pass's arguments."""
+    lay = _Layout(desc.channels, desc.lmax, x.device)
+    width, wide = desc.channels * (desc.lmax + 1) ** 2, x.shape[1]
+
+    def fit(v, columns):
+        return v[:, :columns] if columns <= v.shape[1] else torch.nn.functional.pad(v, (0, columns - v.shape[1]))
 
     def root(v):
         return ((v * v * lay.share).sum(1, keepdim=True) + desc.eps).rsqrt()
@@ -131,47 +133,45 @@ def gradient_formula(desc, h, block, gate, post, pre, dh, dy):
     def adjoint(v, rho, e):
         return rho * e - rho ** 3 * lay.share * v * (e * v).sum(1, keepdim=True)
 
+    if block is not None:
+        open_ = torch.ones_like(block[:, :1]) if gate is None else torch.sigmoid(gate)
+        k, rho_b = desc.residual_scale * post.reshape(1, -1) * open_, root(block)
+    r, dpre = dh, None
     if dy is not None:
+        h = x if block is None else fit(x, width) + lay.spread(k.expand(x.shape[0], -1)) * rho_b * block
         rho = root(h)
         through = adjoint(h, rho, lay.spread(pre) * dy)
         r = through if dh is None else dh + through
         dpre = lay.gather(rho * dy * h).sum(0).view_as(pre)
-    dx = r
-    wide = desc.channels * (desc.input_lmax + 1) ** 2
-    if wide != r.shape[1]:
-        dx = r[:, :wide] if wide < r.shape[1] else torch.nn.functional.pad(r, (0, wide - r.shape[1]))
+    dx = fit(r, wide)
     if block is None:
         return dx, None, None, None, dpre
-    rho = root(block)
-    open_ = None if gate is None else torch.sigmoid(gate)
-    k = desc.residual_scale * post.reshape(1, -1) * (1.0 if gate is None else open_)
-    db = adjoint(block, rho, lay.spread(k) * r)
-    along = rho * lay.gather(r * block) * desc.residual_scale
+    db = adjoint(block, rho_b, lay.spread(k.expand(x.shape[0], -1)) * r)
+    along = rho_b * lay.gather(r * block) * desc.residual_scale
     dgate = None if gate is None else along * open_ * (1.0 - open_) * post.reshape(1, -1)
-    dpost = (along if gate is None else along * open_).sum(0).view_as(post)
-    return dx, db, dgate, dpost, dpre
+    return dx, db, dgate, (along * open_).sum(0).view_as(post), dpre
 
 
 class _Gradient(torch.autograd.Function):
-    """The gradients as a function of (h, block, gate, post, pre, dh, dy)."""
+    """The gradients as a function of (x, block, gate, post, pre, dh, dy); h is the forward pass's result."""
 
     @staticmethod
-    def forward(ctx, desc, need, *inputs):
+    def forward(ctx, desc, need, h, *inputs):
         ctx.set_materialize_grads(False)
         ctx.desc = desc
-        ctx.save_for_backward(*inputs)
-        return _backward(desc, *inputs, need)
+        ctx.save_for_backward(h, *inputs)
+        return _backward(desc, h, *inputs[1:], need)
 
     @staticmethod
     def backward(ctx, *cots):
-        inputs = ctx.saved_tensors
+        h, *inputs = ctx.saved_tensors
         desc = ctx.desc
-        h, block, gate, post, pre, dh, dy = inputs
-        need = list(ctx.needs_input_grad[2:])
+        x, block, gate, post, pre, dh, dy = inputs
+        need = list(ctx.needs_input_grad[3:])
         if not _weights_run(post, pre, need[3:5]):
             need[3] = need[4] = False
         if not any(need) or all(c is None for c in cots):
-            return (None,) * 9
+            return (None,) * 10
         graph = torch.is_grad_enabled()
         if graph or cots[3] is not None or cots[4] is not None:
             with torch.enable_grad():
@@ -184,19 +184,21 @@ class _Gradient(torch.autograd.Function):
                     grads = torch.autograd.grad([o for o, _ in heads], leaves, [c for _, c in heads],
                                                 create_graph=graph, allow_unused=True)
             grads = iter(grads)
-            return (None, None, *[next(grads) if n else None for n in need])
-        # h, dy and pre take part through the norm behind the block, h and x then linearly
+            return (None, None, None, *[next(grads) if n else None for n in need])
+        # x, dy and pre take part through the norm behind the block
         follows = dy is not None
         need = [n and (follows or i not in (0, 4, 6)) for i, n in enumerate(need)]
         if block is None:
             need[5] = False
         cx, cb, cg = (_cont(c) for c in cots[:3])
-        return (None, None, *_second(desc, *inputs, cx, cb, cg, need))
+        return (None, None, None, *_second(desc, x, h, *inputs[1:], cx, cb, cg, need))
 
 
-def _gradients(desc, need, *inputs):
+def _gradients(desc, need, h, x, *inputs):
     """The gradients, recorded where a graph is (a function of its own costs 15 us a call)."""
-    return _Gradient.apply(desc, need, *inputs) if torch.is_grad_enabled() else _backward(desc, *inputs, need)
+    if torch.is_grad_enabled():
+        return _Gradient.apply(desc, need, h.detach(), x, *inputs)
+    return _backward(desc, h, *inputs, need)
 
 
 class _Norm(torch.autograd.Function):
@@ -212,8 +214,8 @@ class _Norm(torch.autograd.Function):
         need = (ctx.needs_input_grad[1], _weights_run(None, pre, (False, ctx.needs_input_grad[2])))
         if not any(need):
             return None, None, None
-        dx, _, _, _, dpre = _gradients(ctx.desc, (need[0], False, False, False, need[1]), x, None, None, None, pre,
-                                       None, dy.contiguous())
+        dx, _, _, _, dpre = _gradients(ctx.desc, (need[0], False, False, False, need[1]), x, x, None, None, None,
+                                       pre, None, dy.contiguous())
         return None, dx, dpre
 
 
@@ -223,12 +225,12 @@ class _BlockEnd(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.desc = desc
         h, y = _forward(desc, x, block, gate, post, pre)
-        ctx.save_for_backward(h, block, gate, post, pre)
+        ctx.save_for_backward(x, h, block, gate, post, pre)
         return h, y
 
     @staticmethod
     def backward(ctx, dh, dy):
-        h, block, gate, post, pre = ctx.saved_tensors
+        x, h, block, gate, post, pre = ctx.saved_tensors
         if dh is None and dy is None:
             return (None,) * 6
         need = list(ctx.needs_input_grad[1:])
@@ -241,7 +243,7 @@ class _BlockEnd(torch.autograd.Function):
                 dx, need[0] = dh, False
         if not any(need):
             return None, dx, None, None, None, None
-        grads = _gradients(ctx.desc, tuple(need), h, block, gate, post, pre, _cont(dh), _cont(dy))
+        grads = _gradients(ctx.desc, tuple(need), h, x, block, gate, post, pre, _cont(dh), _cont(dy))
         return (None, grads[0] if dx is None else dx, *grads[1:])
 
 

@@ -757,8 +757,8 @@ int ictc_hip_moment_values(const uint8_t* exp_avg, const uint8_t* exp_avg_top, c
  *   backward: from grad_h (may be null) and grad_y (null without pre; may be null) the gradients to x, block,
  *             gate, post and pre; any output may be null.  h is forward's result.
  *   second:   the gradients of <cot_x, dx> + <cot_block, dblock> + <cot_gate, dgate> (any may be null), dx,
- *             dblock and dgate being backward's, to h (taken as an argument of its own), block, gate, grad_h,
- *             grad_y, post and pre; any output may be null, those to h, grad_y and pre must be without grad_y.
+ *             dblock and dgate being backward's as functions of forward's arguments, to x, block, gate, grad_h,
+ *             grad_y, post and pre; any output may be null, those to x, grad_y and pre must be without grad_y.
  *
  * Weight gradients need a workspace of ictc_hip_norm_workspace(desc, rows) floats (negative: -ictc_status)
  * and are summed in a fixed order; they are zero for rows = 0.  1 <= channels <= ICTC_NORM_MAX_CHANNELS,
@@ -783,7 +783,7 @@ int ictc_hip_norm_backward(const ictc_norm_desc* desc, const float* h, const flo
                            int64_t workspace_floats, int64_t rows, hipStream_t stream);
 int ictc_hip_norm_second(const ictc_norm_desc* desc, const float* h, const float* block, const float* gate,
                          const float* post, const float* pre, const float* grad_h, const float* grad_y,
-                         const float* cot_x, const float* cot_block, const float* cot_gate, float* dh, float* dblock,
+                         const float* cot_x, const float* cot_block, const float* cot_gate, float* dx, float* dblock,
                          float* dgate, float* dgrad_h, float* dgrad_y, float* dpost, float* dpre, float* workspace,
                          int64_t workspace_floats, int64_t rows, hipStream_t stream);
 
