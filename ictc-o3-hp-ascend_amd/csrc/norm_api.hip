@@ -453,11 +453,42 @@ __global__ void __launch_bounds__(most_threads(WIDE)) norm_backward_kernel(const
   if (a.partial) write_partial<L, WIDE>(a, t, dpost, dpre, lds);
 }
 
+// Two operands of every thread, put away in LDS (in place of others, where they are taken back).
+template <int N>
+__device__ __forceinline__ void put_away(float* stash, const float (&u)[N], const float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    stash[i * blockDim.x] = u[i];
+    stash[(N + i) * blockDim.x] = v[i];
+  }
+  asm volatile("" ::: "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void take_back(const float* stash, float (&u)[N], float (&v)[N]) {
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    u[i] = stash[i * blockDim.x];
+    v[i] = stash[(N + i) * blockDim.x];
+  }
+}
+
+// Where two of the second derivatives' operands wait in LDS: with all degrees to 3 a thread has 112 values, which with
+// what goes beside them did not fit into 256 registers (132 bytes of scratch memory a thread, 212 us for 8,192
+// rows of C = 128 against 172; one wave to a SIMD and 512 registers: 209).  With degrees to 2 they fit (109 us against
+// 112 for 16,384 rows of C = 64), rows within a wave gain nothing (127 us against 130 at C = 32), and more than 256
+// threads would take 64 KB and more.
+constexpr bool stashes(int lmax, int wide, bool block, bool next) { return lmax == 3 && wide == 1 && block && next; }
+
 template <int L, int WIDE, bool BLOCK, bool NEXT>
 __global__ void __launch_bounds__(most_threads(WIDE)) __attribute__((amdgpu_waves_per_eu(WIDE == 1 && L == 3 ? 2 : 1)))
 norm_second_kernel(const NormArgs a) {
   constexpr int D = (L + 1) * (L + 1);
   __shared__ double lds[WIDE ? 2 * kSums * kMaxWaves : kNormThreads / 2];
+  constexpr bool STASH = stashes(L, WIDE, BLOCK, NEXT);
+  extern __shared__ float kept[];
+  [[maybe_unused]] float* const stash = kept + threadIdx.x;
   int turn = 0;
   const Place t = place<WIDE>(a);
   const int C = a.channels;
@@ -519,6 +550,7 @@ norm_second_kernel(const NormArgs a) {
           for (int i = l * l; i < (l + 1) * (l + 1); ++i) r[i] = static_cast<float>(r[i] + up * dy[i] - down * h[i]);
         });
         narrow(r), narrow(h), narrow(dy);
+        if constexpr (STASH) put_away(stash, h, dy);
       }
       float cg[L + 1];
       gates<L>(a, base, own_gate, on, open, closed);
@@ -556,6 +588,10 @@ norm_second_kernel(const NormArgs a) {
       if (on && a.gdh) store_row<L>(a.gdh + base * width, own, L, R);
     }
     if constexpr (NEXT) {
+      if constexpr (STASH) {
+        take_back(stash, h, dy);
+        put_away(stash, b, r);
+      }
       double dots[2] = {};    // <R, pre dy>, <a R, h>
       degrees<L>([&](auto d) {
         constexpr int l = decltype(d)::value;
@@ -589,6 +625,7 @@ norm_second_kernel(const NormArgs a) {
     }
     if constexpr (BLOCK) {
       if constexpr (NEXT) {
+        if constexpr (STASH) take_back(stash, b, r);
         double e[L + 1], dot[1] = {0.0};
         degrees<L>([&](auto d) {
           constexpr int l = decltype(d)::value;
@@ -723,7 +760,9 @@ int run(int order, const ictc_norm_desc* d, NormArgs a, int64_t rows, bool block
                             : d->lmax == 2 ? kernel_of<2>(order, s.wide, block, next)
                                            : kernel_of<3>(order, s.wide, block, next);
   if (grid) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(s.block), 0, stream, a);
+    const int columns = (d->lmax + 1) * (d->lmax + 1);
+    const size_t lds = order == 2 && stashes(d->lmax, s.wide, block, next) ? 2 * sizeof(float) * columns * s.block : 0;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(s.block), lds, stream, a);
     if (hipGetLastError() != hipSuccess) return ICTC_ERR_LAUNCH;
   }
   if (weights) {
