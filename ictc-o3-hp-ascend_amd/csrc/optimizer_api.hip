@@ -225,6 +225,18 @@ struct StepScalars {
   uint32_t key;
 };
 
+// The moving averages, each product and sum rounded for itself: the same bits as float32 arithmetic gives
+// elsewhere.  With products fused into the sums one in 2 million 8-bit codes would be rounded the other way.
+__device__ __forceinline__ void moments(const StepScalars& c, const float* g, float* m, float* v) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float gk = c.coefficient * g[k];
+    m[k] = c.b1 * m[k] + c.n1 * gk;
+    v[k] = c.b2 * v[k] + c.n2 * (gk * gk);
+  }
+}
+
 // The update of U whole blocks (or, with U = 1, of the first `left` of each lane's values): four values a
 // lane and block, all loads before the first store.
 template <bool SMALL, bool STREAM, int U, bool WHOLE>
@@ -264,12 +276,7 @@ __device__ __forceinline__ void update(const StepArgs& a, const StepScalars& c, 
       decode_signed(cm[u], tm[u], m[u]);
       decode_unsigned(cv[u], tv[u], v[u]);
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float gk = c.coefficient * g[u][k];
-      m[u][k] = c.b1 * m[u][k] + c.n1 * gk;
-      v[u][k] = c.b2 * v[u][k] + c.n2 * (gk * gk);
-    }
+    moments(c, g[u], m[u], v[u]);
     if (SMALL && c.eps >= kFastEps) {
       // Roots and reciprocals to the last bit but one, without the steps for denormal roots (eps covers
       // them): the exact ones are a quarter of this variant's instructions, which bound it.
@@ -498,10 +505,9 @@ norm_finish_kernel(const double* __restrict__ partial, int count, float max_norm
   for (int k = threadIdx.x; k < count; k += kThreads) sum += partial[k];
   sum = block_sum(sum);
   if (threadIdx.x == 0) {
-    const double norm = sqrt(sum);
-    const double ratio = static_cast<double>(max_norm) / norm;
-    out[0] = static_cast<float>(norm);
-    const float coefficient = max_norm > 0.f && ratio < 1.0 ? static_cast<float>(ratio) : 1.f;
+    const float norm = static_cast<float>(sqrt(sum)), ratio = max_norm / norm;     // of the norm that is returned
+    out[0] = norm;
+    const float coefficient = max_norm > 0.f && ratio < 1.f ? ratio : 1.f;
     out[1] = norm < INFINITY ? coefficient : __uint_as_float(0x7FC00000u);
   }
 }
