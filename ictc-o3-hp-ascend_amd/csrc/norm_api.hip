@@ -28,7 +28,13 @@
 // as exact as the operands.  One thread holds one channel's (L+1)^2 components of every operand, so weights, gates and
 // their gradients need no exchange between threads; its 1, 3, 5 and 7 components are loaded with vectors of
 // that many words, which side by side fill whole lines.  A row's threads are part of a wave (up to 64
-// channels: a power of two of them) or up to 16 waves, whose sums meet in LDS.
+// channels: a power of two of them) or up to 16 waves, whose sums meet in LDS.  (One degree to a wave, all of a
+// row's in one workgroup: 325 us for the second derivatives of 8,192 rows of C = 128, L = 3; eight waves at each
+// barrier.)
+//
+// Measured at C = 128, L = 3 (bytes as each kernel reads and writes them): forward of 32,768 rows 204 us, 5.6 TB/s;
+// of 8,192 rows 48 us (6.0), gradients 81 us with weight gradients (5.4), second derivatives 158 us (4.6: two waves to
+// a SIMD, and 1,900 instructions a wave and row).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

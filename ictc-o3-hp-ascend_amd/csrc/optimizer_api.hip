@@ -318,8 +318,8 @@ __device__ __forceinline__ void update(const StepArgs& a, const StepScalars& c, 
 // One wave to U consecutive blocks of 256 values; the launch's waves sweep over the blocks side by side,
 // so a wave changes tensors often: the table and each tensor's scalars are in LDS.
 //
-// Bound by memory: 28 bytes a value (8-bit moments 16). 150 M values in 120 tensors: 705 us (5.9 TB/s) with
-// float32 moments and 401 us (6.0 TB/s) with 8-bit ones, a copy of the same size runs at 5.3 to 5.9.  What
+// Bound by memory: 28 bytes a value (8-bit moments 16). 150 M values in 120 tensors: 694 us (6.0 TB/s) with
+// float32 moments and 377 us (6.4 TB/s) with 8-bit ones, a copy of the same size runs at 5.3 to 5.9.  What
 // that took, from 835 and 535 us with a contiguous range of blocks for each of 2,048 workgroups: lookups
 // from LDS and waves side by side (the ranges met on the same memory channels), no reuse asked of the
 // caches (`STREAM`, from kStream values on; below, the caches hold a model: 8 M values 37 us against
@@ -457,7 +457,8 @@ __device__ __forceinline__ double block_sum(double x) {
 }
 
 // Sums of squares in 64 bits (a float's square neither overflows nor vanishes there), one for each
-// workgroup; a second launch adds them in order.
+// workgroup; a second launch adds them in order.  Bound by memory: 150 M values in 92 us (6.5 TB/s, past the caches;
+// 150 us with the tables read from the kernel's arguments at every change of tensors), 1.5 M in 5 us.
 template <bool STREAM>
 __global__ void __launch_bounds__(kThreads) norm_partial_kernel(const NormTable table, double* __restrict__ partial) {
   __shared__ const float* grads[kNormTensors];
