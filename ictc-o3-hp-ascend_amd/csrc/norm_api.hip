@@ -85,19 +85,17 @@ __device__ __forceinline__ void load_n(const float* p, float* v) {
 // The gradients' kernels store past the caches (8,192 rows of C = 128, L = 3: 77 us against 86, second
 // derivatives 166 against 172; 2,048 rows: 24.0 against 24.3), the forward pass does not (51 us either way, 203
 // against 207 for 32,768 rows), and no loads do (214, and 29 against 24 for the gradients of 2,048).
-template <bool PAST, typename T>
-__device__ __forceinline__ void put(T* p, T v) {
-  if constexpr (PAST) __builtin_nontemporal_store(v, p); else *p = v;
-}
-
 template <bool PAST, int N>
 __device__ __forceinline__ void store_n(float* p, const float* v) {
   if constexpr (N == 1 || N == 3) {
 #pragma unroll
-    for (int m = 0; m < N; ++m) put<PAST>(p + m, v[m]);
+    for (int m = 0; m < N; ++m) {
+      if constexpr (PAST) __builtin_nontemporal_store(v[m], p + m); else p[m] = v[m];
+    }
   } else {
     const nf4 t = {v[0], v[1], v[2], v[3]};
-    put<PAST>(reinterpret_cast<nf4*>(p), t);
+    nf4* q = reinterpret_cast<nf4*>(p);
+    if constexpr (PAST) __builtin_nontemporal_store(t, q); else *q = t;
     store_n<PAST, N - 4>(p + 4, v + 4);
   }
 }
@@ -766,7 +764,7 @@ int run(int order, const ictc_norm_desc* d, NormArgs a, int64_t rows, bool block
   a.eps = d->eps;
   const bool weights = dpost || dpre;
   if (!weights) a.partial = nullptr;
-  const int64_t most = weights ? partial_groups(s) : int64_t{1} << 30;
+  const int64_t most = weights ? partial_groups(s) : (int64_t{1} << 31) / s.block;      // threads within 32 bits
   const int64_t grid = s.grid < most ? s.grid : most;
   const NormKernel kernel = d->lmax == 0   ? kernel_of<0>(order, s.wide, block, next)
                             : d->lmax == 1 ? kernel_of<1>(order, s.wide, block, next)

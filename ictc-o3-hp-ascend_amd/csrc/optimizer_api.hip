@@ -39,7 +39,7 @@ constexpr int kTensors = 184;                    // 21 bytes each, within the 4 
 constexpr int kMaskTensors = 16384;
 constexpr float kFastEps = 1e-11f;               // times 2^-24 above the root of the smallest normal float
 constexpr int64_t kStream = int64_t{1} << 24;     // values of a launch that no cache holds until their next use
-constexpr int64_t kMostGroups = int64_t{1} << 24;  // workgroups of a launch that streams
+constexpr int64_t kMostGroups = int64_t{1} << 23;  // workgroups of a launch that streams (threads within 32 bits)
 
 // Blocks that a wave takes at a time.
 constexpr int step_blocks(bool small, bool past) { return small && past ? 4 : 1; }

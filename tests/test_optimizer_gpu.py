@@ -176,6 +176,24 @@ def test_eight_bit_averages_are_kept(gpu):
     assert abs(float((m.double() / g.double()).mean()) - 1) <= 5 * 0.5 / 128
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-12, 1e-3])
+def test_small_gradients_and_other_eps(gpu, bits, eps):
+    """Gradients far below the usual eps, on either side of where the 8-bit kernel takes approximate roots."""
+    from ictc_o3.backends.hip.optimizer import adamw_step, new_state
+    params, grads = _inputs([700, 64], 11, gpu)
+    grads = [g * 1e-10 for g in grads]
+    state = new_state(params, bits)
+    before, values = _host(params), _host(grads)
+    adamw_step(params, grads, *state, lr=LR, betas=BETAS, eps=eps, weight_decay=DECAY)
+    for p, old, g in zip(_host(params), before, values):
+        m, v = (1 - BETAS[0]) * g, (1 - BETAS[1]) * g * g
+        denom = np.sqrt(v / (1 - BETAS[1])) + eps
+        rate = LR / (1 - BETAS[0])
+        want = (1 - LR * DECAY) * old - rate * m / denom
+        assert np.all(np.abs(p - want) <= U * (3 * np.abs(old) + 16 * rate * np.abs(m) / denom))
+
+
 def test_a_tensor_without_a_gradient_keeps_its_state(gpu):
     from ictc_o3.backends.hip.optimizer import adamw_step, new_state
     sizes = [300, 5, 700]
