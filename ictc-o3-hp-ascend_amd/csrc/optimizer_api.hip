@@ -279,7 +279,7 @@ __device__ __forceinline__ void update(const StepArgs& a, const StepScalars& c, 
     moments(c, g[u], m[u], v[u]);
     if (SMALL && c.eps >= kFastEps) {
       // Roots and reciprocals to the last bit but one, without the steps for denormal roots (eps covers
-      // them): the exact ones are a quarter of this variant's instructions, which bound it.
+      // them): with the exact ones instructions bound this variant (100 M values: 279 us against 250).
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         p[u][k] = c.keep * p[u][k] -

@@ -115,6 +115,22 @@ def test_training_captured_and_eager(gpu, bits):
     assert not torch.allclose(got, first)
 
 
+def test_captured_inference(gpu):
+    from mace_hip import CapturedEnergyAndForces, energy_and_forces
+    model, graph = _setup(gpu)
+    model.requires_grad_(False)
+    step = CapturedEnergyAndForces(model, **graph)
+    for k in range(3):
+        gen = torch.Generator(device=gpu).manual_seed(k)
+        pos = graph["positions"] + 0.05 * torch.randn(graph["positions"].shape, device=gpu, generator=gen)
+        eager = energy_and_forces(model, **dict(graph, positions=pos))
+        torch.cuda.synchronize(gpu)
+        got = step(pos)
+        torch.cuda.synchronize(gpu)
+        assert_rel(got["energy"], eager["energy"], what=f"replay {k} energy")
+        assert_rel(got["forces"], eager["forces"], what=f"replay {k} forces")
+
+
 def test_default_model_has_no_norms(gpu):
     from mace_hip import create_model
     model = create_model(channels=8, lmax=1, correlation=1, device=gpu)

@@ -213,6 +213,34 @@ def test_a_tensor_without_a_gradient_keeps_its_state(gpu):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_large_tensors_without_gradients(gpu, bits):
+    """Tensors that end a launch because they take no part: the ones around them as in steps of their own."""
+    from ictc_o3.backends.hip.optimizer import adamw_step, moment_values, new_state
+    sizes = [300, 1_500_000, 700, 5, 1_200_000, 2_000_000, 40]
+    params, grads = _inputs(sizes, 12, gpu)
+    for k in (1, 4, 5):
+        grads[k] = None
+    before = [p.clone() for p in params]
+    state = new_state(params, bits)
+    adamw_step(params, grads, *state, lr=LR, seed=3)
+    at = _starts(sizes)
+    m, v = state[:2] if bits == 32 else moment_values(*state[:2])
+    for k, g in enumerate(grads):
+        part = slice(int(at[k]), int(at[k]) + sizes[k])
+        if g is None:
+            assert torch.equal(params[k], before[k]) and not m[part].any() and not v[part].any()
+            continue
+        alone, own = [before[k].clone()], new_state([before[k]], bits)
+        adamw_step(alone, [g], *own, lr=LR, seed=3)
+        assert torch.equal(params[k], alone[0])           # (a first step's update does not see the rounding)
+        # 8-bit moments are rounded by their place in the state: within one code step of 1/8
+        for got, want in zip((m, v), own[:2] if bits == 32 else moment_values(*own[:2])):
+            exact = dict(rtol=0, atol=0) if bits == 32 else dict(rtol=0.125, atol=1e-4)
+            torch.testing.assert_close(got[part], want[:sizes[k]], **exact)
+    assert state[2][:, 0].tolist() == [1.0, 0.0, 1.0, 1.0, 0.0, 0.0, 1.0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_values_that_are_not_finite(gpu, bits, bad):
     """Unclipped they go where the formula takes them and nowhere else; with the norm taken, the whole step is left out."""
