@@ -488,8 +488,8 @@ __device__ __forceinline__ void take_back(const float* stash, float (&u)[N], flo
 // Where two of the second derivatives' operands wait in LDS: with all degrees to 3 a thread has 112 values, which with
 // what goes beside them did not fit into 256 registers (132 bytes of scratch memory a thread, 212 us for 8,192
 // rows of C = 128 against 172; one wave to a SIMD and 512 registers: 209).  With degrees to 2 they fit (109 us against
-// 112 for 16,384 rows of C = 64), rows within a wave gain nothing (127 us against 130 at C = 32), and more than 256
-// threads would take 64 KB and more.
+// 112 for 16,384 rows of C = 64), rows that share a wave gain nothing (127 us against 130 at C = 32), and more than
+// 256 threads would take 64 KB and more.
 constexpr bool stashes(int lmax, int wide, bool block, bool next) { return lmax == 3 && wide == 1 && block && next; }
 
 template <int L, int WIDE, bool BLOCK, bool NEXT>
@@ -705,9 +705,13 @@ struct NormShape {
   int wide;                   // see most_threads
 };
 
-NormShape shape_of(int channels, int64_t rows) {
+// Rows of up to 64 channels share a wave, but for those of more than 32 with every degree to 3, which have one of their
+// own: the second derivatives then keep two operands in LDS (16,384 rows of 64 channels: 160 us against 206, their
+// gradients 74 against 82; with degrees to 2 98 against 96).
+NormShape shape_of(int channels, int lmax, int64_t rows) {
   NormShape s;
-  s.wide = channels <= kNormWave ? 0 : channels <= most_threads(1) ? 1 : channels <= most_threads(2) ? 2 : 3;
+const bool shared = channels <= (lmax == 3 ? kNormWave / 2 : kNormWave);
+  s.wide = shared ? 0 : channels <= most_threads(1) ? 1 : channels <= most_threads(2) ? 2 : 3;
   if (s.wide) {
     s.threads = (channels + kNormWave - 1) / kNormWave * kNormWave;
     s.groups = 1;
@@ -722,7 +726,15 @@ NormShape shape_of(int channels, int64_t rows) {
   return s;
 }
 
-int64_t partial_groups(const NormShape& s) { return s.grid < kNormGroups ? s.grid : kNormGroups; }
+// Workgroups that leave partial weight gradients: more of them fill the chip, fewer leave less to add up.  Those of one
+// wave are twice as many (second derivatives of 2,048 rows of 64 channels: 29 us against 33 with 1,024; gradients
+// 21.4 against 20.9); second derivatives fit fewer large ones at a time (256 threads: 92 us with 512, 104 with 1,024).
+int64_t partial_groups(const NormShape& s, int order) {
+  int64_t most = kNormGroups;
+  if (s.block == kNormWave) most *= 2;
+  if (order == 2 && s.block >= kNormThreads) most /= 2;
+  return s.grid < most ? s.grid : most;
+}
 
 using NormKernel = void (*)(NormArgs);
 
@@ -753,7 +765,7 @@ bool valid(const ictc_norm_desc* d, int64_t rows) {
 
 int run(int order, const ictc_norm_desc* d, NormArgs a, int64_t rows, bool block, bool next, float* dpost, float* dpre,
         hipStream_t stream) {
-  const NormShape s = shape_of(d->channels, rows);
+  const NormShape s = shape_of(d->channels, d->lmax, rows);
   a.rows = rows;
   a.channels = d->channels;
   a.width_x = static_cast<int64_t>(d->channels) * (d->input_lmax + 1) * (d->input_lmax + 1);
@@ -764,7 +776,7 @@ int run(int order, const ictc_norm_desc* d, NormArgs a, int64_t rows, bool block
   a.eps = d->eps;
   const bool weights = dpost || dpre;
   if (!weights) a.partial = nullptr;
-  const int64_t most = weights ? partial_groups(s) : (int64_t{1} << 31) / s.block;      // threads within 32 bits
+  const int64_t most = weights ? partial_groups(s, order) : (int64_t{1} << 31) / s.block;      // threads within 32 bits
   const int64_t grid = s.grid < most ? s.grid : most;
   const NormKernel kernel = d->lmax == 0   ? kernel_of<0>(order, s.wide, block, next)
                             : d->lmax == 1 ? kernel_of<1>(order, s.wide, block, next)
@@ -793,7 +805,7 @@ extern "C" {
 int64_t ictc_hip_norm_workspace(const ictc_norm_desc* desc, int64_t rows) {
   using namespace ictc;
   if (!valid(desc, rows)) return -ICTC_ERR_INVALID_ARGUMENT;
-  const int64_t groups = partial_groups(shape_of(desc->channels, rows));
+  const int64_t groups = partial_groups(shape_of(desc->channels, desc->lmax, rows), 1);
   return (groups ? groups : 1) * 2 * desc->channels * (desc->lmax + 1);
 }
 
