@@ -16,8 +16,8 @@ pytestmark = pytest.mark.gpu
 
 EPS = 1e-5
 # channels (a part of a wave, a whole one, two waves with six or all of the second's lanes, more than four), lmax, rows
-SHAPES = [(1, 0, 1), (3, 1, 5), (16, 2, 33), (48, 3, 20), (64, 3, 7), (40, 1, 9), (70, 2, 130), (128, 3, 65), (129, 1, 17), (300, 3, 9),
-          (1024, 0, 3), (5, 3, 3000)]
+SHAPES = [(1, 0, 1), (3, 1, 5), (16, 2, 33), (48, 3, 20), (64, 3, 7), (40, 1, 9), (70, 2, 130), (128, 3, 65),
+          (129, 1, 17), (300, 3, 9), (1024, 0, 3), (5, 3, 3000)]
 
 
 def _degrees(x, c, lmax):
