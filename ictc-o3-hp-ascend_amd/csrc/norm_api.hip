@@ -27,8 +27,8 @@
 // cotangent along v (all but eps / (q + eps) of it for a row with one large entry), and the difference is
 // as exact as the operands.  One thread holds one channel's (L+1)^2 components of every operand, so weights, gates and
 // their gradients need no exchange between threads; its 1, 3, 5 and 7 components are loaded with vectors of
-// that many words, which side by side fill whole lines.  A row's threads are part of a wave (up to 64
-// channels: a power of two of them) or up to 16 waves, whose sums meet in LDS.  (One degree to a wave, all of a
+// that many words, which side by side fill whole lines.  A row's threads are a power of two of
+// a wave's (for few channels, see shape_of) or up to 16 waves, whose sums meet in LDS.  (One degree to a wave, all of a
 // row's in one workgroup: 325 us for the second derivatives of 8,192 rows of C = 128, L = 3; eight waves at each
 // barrier.)
 //
