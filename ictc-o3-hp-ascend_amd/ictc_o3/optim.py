@@ -85,8 +85,9 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
-        """Restores hyperparameters, moments and steps; moments that exist are overwritten in place, so a
-        captured step goes on from what was loaded."""
+        """Restores hyperparameters, moments and steps.  Moments and learning rate tensors that exist are
+        overwritten in place, so a captured step goes on from what was loaded (numbers among its
+        hyperparameters are part of the graph: a rate that has to follow is a tensor)."""
         if state_dict.get("moment_bits") != self.moment_bits or len(state_dict["moments"]) != len(self.param_groups):
             raise ValueError("the state has another number of moment bits or of parameter groups")
         new = []
@@ -99,7 +100,18 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError("the state belongs to parameters of other sizes")
                     a.copy_(b)
             new.append(own)
+        rates = [group["lr"] for group in self.param_groups]
+        loaded = {}                  # groups may share a tensor (the default's): one value for all of them
+        for rate, group in zip(rates, state_dict["param_groups"]):
+            if isinstance(rate, torch.Tensor) and loaded.setdefault(id(rate), float(group["lr"])) != float(group["lr"]):
+                raise ValueError("groups that share a learning rate tensor cannot take different learning rates")
         super().load_state_dict({k: state_dict[k] for k in ("state", "param_groups")})
+        for rate, group in zip(rates, self.param_groups):
+            if isinstance(rate, torch.Tensor):
+                rate.copy_(torch.as_tensor(group["lr"]).reshape(rate.shape))
+                group["lr"] = rate
+            elif isinstance(group["lr"], torch.Tensor):
+                group["lr"] = group["lr"].to(group["params"][0].device)
         self.seed = int(state_dict["seed"])
         for i, own in enumerate(new):
             if self._moments[i] is None:

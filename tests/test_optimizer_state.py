@@ -1,0 +1,46 @@
+"""The optimizer's own bookkeeping, without a GPU: what a loaded state, a copy and a capture do to it."""
+import pytest
+import torch
+
+from ictc_o3.optim import AdamW
+
+
+def _params(count=2):
+    return [torch.nn.Parameter(torch.full((3,), float(k))) for k in range(count)]
+
+
+def test_a_loaded_state_keeps_the_rate_tensors():
+    """A captured step reads the rate at its tensor's address: the loaded value goes there."""
+    own, shared = torch.tensor([1e-2]), torch.tensor(1e-3)
+    make = lambda a, b: AdamW([{"params": p[:1], "lr": a}, {"params": p[1:]}], lr=b)      # noqa: E731
+    p = _params(3)
+    optimizer = make(own, shared)
+    other = make(torch.tensor(0.5), torch.tensor(0.25))
+    optimizer.load_state_dict(other.state_dict())
+    assert optimizer.param_groups[0]["lr"] is own and optimizer.param_groups[1]["lr"] is shared
+    assert own.item() == 0.5 and shared.item() == 0.25
+    optimizer.load_state_dict(make(0.125, 2.0).state_dict())        # numbers, into the tensors
+    assert optimizer.param_groups[0]["lr"] is own and own.item() == 0.125 and shared.item() == 2.0
+    assert other.param_groups[0]["lr"].item() == 0.5                # the saved state's own is not shared
+
+
+def test_a_loaded_rate_tensor_goes_beside_the_parameters():
+    """From a state on another device, into a group whose rate was a number."""
+    p = _params(1)
+    saved = AdamW(p, lr=torch.tensor(0.5)).state_dict()
+    optimizer = AdamW([torch.nn.Parameter(torch.empty(3, device="meta"))], lr=1e-3)
+    optimizer.load_state_dict(saved)
+    assert optimizer.param_groups[0]["lr"].device.type == "meta"
+
+
+def test_groups_that_share_a_rate_tensor_take_one_value():
+    p, rate = _params(2), torch.tensor(1e-3)
+    optimizer = AdamW([{"params": p[:1]}, {"params": p[1:]}], lr=rate, weight_decay=0.25)
+    same = AdamW([{"params": p[:1]}, {"params": p[1:]}], lr=0.5)
+    optimizer.load_state_dict(same.state_dict())
+    assert all(g["lr"] is rate for g in optimizer.param_groups) and rate.item() == 0.5
+    two = AdamW([{"params": p[:1], "lr": 1.0}, {"params": p[1:], "lr": 2.0}], weight_decay=0.125)
+    before = optimizer.param_groups[0]["weight_decay"]
+    with pytest.raises(ValueError, match="share"):
+        optimizer.load_state_dict(two.state_dict())
+    assert rate.item() == 0.5 and optimizer.param_groups[0]["weight_decay"] == before     # nothing was taken over
