@@ -6,7 +6,8 @@
     mace_hip.CapturedTrainingStep(model, optimizer, graph)
 
 The step reads nothing back and keeps its state on the device, so it can be captured as it is (a learning
-rate that changes between replays is given as a one-element float32 tensor).
+rate that changes between replays is given as a one-element float32 tensor; the first step of a group makes
+its moments and is taken outside of the capture).
 """
 from __future__ import annotations
 
@@ -51,6 +52,10 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         grads = [[p.grad for p in group["params"]] for group in self.param_groups]
+        first = any(state is None and any(g is not None for g in gs) for state, gs in zip(self._moments, grads))
+        if first and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a group's first step makes its moments and cannot be captured: every replay would be a "
+                               "first step (take a step, or load a state, before the capture)")
         clip = None
         if self.max_grad_norm is not None and any(g is not None for gs in grads for g in gs):
             clip = self.grad_norm = gradient_norm([g for gs in grads for g in gs], self.max_grad_norm)

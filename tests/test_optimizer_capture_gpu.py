@@ -62,3 +62,49 @@ def test_a_captured_step_goes_on_from_a_loaded_state(gpu, bits, where):
         for a, b in zip(params, others):
             assert torch.equal(a, b), step
     assert float(optimizer.moments(params[2])[2]) == 5.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_first_step_cannot_be_captured(gpu, bits):
+    """Neither a new optimizer's nor that of a group without a gradient until now; the refusal changes nothing."""
+    params, optimizer = _optimizer(gpu, bits)
+    before = [p.detach().clone() for p in params]
+    with pytest.raises(RuntimeError, match="first step"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            optimizer.step()
+    late = torch.nn.Parameter(torch.ones(40, device=gpu))
+    optimizer.add_param_group({"params": [late]})
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(params, before)) and optimizer.moments(params[0]) is None
+    graph = _captured(optimizer)                 # the second group has no gradient: not part of it
+    late.grad = torch.ones_like(late)
+    with pytest.raises(RuntimeError, match="first step"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            optimizer.step()
+    late.grad = None
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+    assert float(optimizer.moments(params[1])[2]) == 4.0
+
+
+def test_a_training_step_needs_a_step_before_its_capture(gpu):
+    from ictc_o3.optim import AdamW
+    from mace_hip import CapturedTrainingStep, training_step
+    from test_mace_gpu import _setup
+    model, graph, _, _ = _setup(gpu, atoms=32)
+    species = model.species_index(graph["atomic_numbers"])
+    optimizer = AdamW(model.parameters(), lr=1e-3)
+    # the model's own first call (its checks read from the device)
+    training_step(model, torch.optim.SGD(model.parameters(), lr=0.0), dict(graph), species=species)
+    with pytest.raises(RuntimeError, match="first step"):
+        CapturedTrainingStep(model, optimizer, graph, species=species, warmup=0)
+    model.zero_grad(set_to_none=True)
+    training_step(model, optimizer, dict(graph))
+    first = next(p for p in model.parameters() if p.requires_grad)
+    assert float(optimizer.moments(first)[2]) == 1.0
+    captured = CapturedTrainingStep(model, optimizer, graph, warmup=1)
+    for _ in range(2):
+        captured(graph["positions"])
+        torch.cuda.synchronize(gpu)
+    assert float(optimizer.moments(first)[2]) == 4.0

@@ -44,3 +44,18 @@ def test_groups_that_share_a_rate_tensor_take_one_value():
     with pytest.raises(ValueError, match="share"):
         optimizer.load_state_dict(two.state_dict())
     assert rate.item() == 0.5 and optimizer.param_groups[0]["weight_decay"] == before     # nothing was taken over
+
+
+def test_a_first_step_is_refused_in_a_capture(monkeypatch):
+    """The moments' zeros would be part of the graph, and every replay a first step."""
+    p = _params(1)
+    p[0].grad = torch.ones(3)
+    for clipped in (None, 1.0):
+        optimizer = AdamW(p, max_grad_norm=clipped)
+        monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="first step"):
+            optimizer.step()
+        assert optimizer.moments(p[0]) is None
+    p[0].grad = None
+    optimizer.step()                                     # nothing to do
