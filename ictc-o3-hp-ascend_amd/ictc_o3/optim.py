@@ -45,6 +45,11 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         self._moments.append(None)
 
+    def __getstate__(self):
+        """For copies and pickles: torch's own part and what this class adds to it."""
+        own = ("moment_bits", "max_grad_norm", "seed", "grad_norm", "_moments")
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in own}}
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

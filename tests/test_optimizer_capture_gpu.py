@@ -108,3 +108,19 @@ def test_a_training_step_needs_a_step_before_its_capture(gpu):
         captured(graph["positions"])
         torch.cuda.synchronize(gpu)
     assert float(optimizer.moments(first)[2]) == 4.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copy_goes_on_by_itself(gpu, bits):
+    import copy
+    params, optimizer = _optimizer(gpu, bits)
+    optimizer.step()
+    others, other = copy.deepcopy((params, optimizer))
+    for a, b in zip(params, others):
+        b.grad = a.grad.clone()
+    other.step()
+    optimizer.step()
+    assert all(torch.equal(a, b) for a, b in zip(params, others))
+    assert torch.equal(optimizer.grad_norm, other.grad_norm)
+    other.step()
+    assert float(optimizer.moments(params[0])[2]) == 2.0 and float(other.moments(others[0])[2]) == 3.0

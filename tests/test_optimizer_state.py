@@ -1,4 +1,7 @@
 """The optimizer's own bookkeeping, without a GPU: what a loaded state, a copy and a capture do to it."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -59,3 +62,20 @@ def test_a_first_step_is_refused_in_a_capture(monkeypatch):
         assert optimizer.moments(p[0]) is None
     p[0].grad = None
     optimizer.step()                                     # nothing to do
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_keep_everything(copied):
+    p = _params()
+    optimizer = AdamW([{"params": p[:1], "lr": 0.5}, {"params": p[1:]}], moment_bits=8, max_grad_norm=3.0, seed=11)
+    codes = lambda k: (torch.full((256,), k, dtype=torch.uint8), torch.ones(1, dtype=torch.uint8))       # noqa: E731
+    optimizer._moments[1] = (codes(3), codes(5), torch.full((1, 3), 7.0, dtype=torch.float64))
+    q, other = copied((p, optimizer))
+    assert (other.moment_bits, other.max_grad_norm, other.seed) == (8, 3.0, 11) and other.grad_norm is None
+    assert other.param_groups[0]["lr"] == 0.5 and other.param_groups[1]["params"][0] is q[1]
+    assert other._moments[0] is None and other._moments[1][0][0].eq(3).all()
+    other._moments[1][2].zero_()
+    assert optimizer._moments[1][2].eq(7.0).all()                    # tensors of its own
+    other.step()                                                     # (no gradients)
+    state = other.state_dict()
+    assert state["seed"] == 11 and state["moments"][0] is None
