@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import torch
 
+from ictc_o3 import _lib
 from ictc_o3.backends.hip.graph_message import pin_graphs
 from ictc_o3.backends.hip.runtime import require_gpu_fp32, strict_fp32
 
@@ -144,7 +145,6 @@ def check_model(model, *, training=False, capture=False) -> dict:
     if any(p.device.type != "cuda" or p.dtype != torch.float32 for p in model.parameters()):
         reasons.append("All model parameters must already be ROCm GPU FP32")
     try:
-        from ictc_o3 import _lib
         _lib.lib()
     except (OSError, RuntimeError) as exc:
         reasons.append(f"The HIP operator library is unavailable: {exc}")
@@ -242,7 +242,9 @@ class CapturedTrainingStep:
     step) captured once and replayed on new positions.  The optimizer must keep its state on
     the device (``ictc_o3.optim.AdamW``, or ``torch.optim.AdamW(..., capturable=True)``, which may also be
     ``fused=True``: one update kernel for all parameters, 0.3 ms less per cfg-4 step); gradients are released before
-    capture so that backward writes them into the graph's own buffers on every replay."""
+    capture so that backward writes them into the graph's own buffers on every replay.  A replay raises the
+    parameters' version counters as an eager step does: what frozen evaluations keep of the weights (folded
+    gate weights, contraction tables) goes by them."""
 
     def __init__(self, model, optimizer, graph: dict, *, species=None, warmup: int = 3):
         if not all(group.get("capturable", False) for group in optimizer.param_groups):
@@ -259,6 +261,7 @@ class CapturedTrainingStep:
             self._loss = force_loss(prediction, self._graph["positions"].shape[0])
             backward_to_parameters(self._loss, model, self._graph["positions"])
             optimizer.step()
+        self._trained = [p for group in optimizer.param_groups for p in group["params"] if p.grad is not None]
 
     def __call__(self, positions: torch.Tensor, cell=None) -> torch.Tensor:
         """Replays the step on these positions; returns the loss buffer (device, not synchronised)."""
@@ -268,4 +271,5 @@ class CapturedTrainingStep:
         if cell is not None:
             self._graph["cell"].copy_(cell)
         self.graph.replay()
+        _lib.host().written(self._trained, self._trained)
         return self._loss

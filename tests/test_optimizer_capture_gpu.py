@@ -124,3 +124,34 @@ def test_a_copy_goes_on_by_itself(gpu, bits):
     assert torch.equal(optimizer.grad_norm, other.grad_norm)
     other.step()
     assert float(optimizer.moments(params[0])[2]) == 2.0 and float(other.moments(others[0])[2]) == 3.0
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_a_frozen_evaluation_sees_replayed_steps(gpu, fused):
+    """What a frozen model derives from its weights once and keeps (folded gate weights, contraction tables) goes
+    by the weights' versions: replays have to raise them as eager steps do."""
+    import copy
+    from conftest import RTOL_FORCE, assert_rel
+    from ictc_o3.optim import AdamW
+    from mace_hip import CapturedTrainingStep, energy_and_forces
+    from test_mace_gpu import _setup
+    model, graph, _, _ = _setup(gpu, atoms=48)
+    trained = [p for p in model.parameters() if p.requires_grad]
+    optimizer = torch.optim.AdamW(trained, lr=0.02, capturable=True, fused=True) if fused else AdamW(trained, lr=0.02)
+    captured = CapturedTrainingStep(model, optimizer, graph, warmup=1)
+
+    def frozen(m):
+        for p in m.parameters():
+            p.requires_grad_(False)
+        return energy_and_forces(m, **graph)
+
+    first = frozen(model)
+    for _ in range(3):
+        for p in trained:
+            p.requires_grad_(True)
+        captured(graph["positions"])
+        torch.cuda.synchronize(gpu)
+        got, want = frozen(model), frozen(copy.deepcopy(model))      # (a copy derives its own)
+        assert_rel(got["energy"], want["energy"], what="energy")
+        assert_rel(got["forces"], want["forces"], rtol=RTOL_FORCE, what="forces")
+    assert not torch.allclose(got["energy"], first["energy"], rtol=1e-3)
