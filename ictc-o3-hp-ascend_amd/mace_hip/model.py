@@ -290,6 +290,8 @@ def _side_stream(device: torch.device) -> "torch.cuda.Stream":
 
 
 class MaceICTC(nn.Module):
+    block_norm = False      # (of modules pickled before they had it)
+
     def __init__(self, *, channels: int = 128, lmax: int = 3, num_interactions: int = 2, correlation: int = 3,
                  atomic_numbers=tuple(range(1, 11)), cutoff: float = 5.0, avg_num_neighbors: float = 50.0,
                  num_basis: int = 8, cutoff_p: int = 5, readout_hidden: int = 16, block_norm: bool = False):

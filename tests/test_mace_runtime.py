@@ -50,3 +50,11 @@ def test_batch_indices_are_range_checked():
     b[1] = 5                                          # in-place change: version bump, checked again
     with pytest.raises(ValueError):
         _validate_batch(b, 2)
+
+
+def test_models_pickled_before_block_norms_run_without_them():
+    """A whole module that was saved when the model had no block_norm attribute: forward asks for it."""
+    import copy
+    model = _cpu_model()
+    del model.__dict__["block_norm"]
+    assert copy.deepcopy(model).block_norm is False
