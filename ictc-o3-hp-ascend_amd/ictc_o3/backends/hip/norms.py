@@ -114,7 +114,7 @@ class _Layout:
         self.places = (lmax + 1) * channels
         self.place = (degree * channels + torch.cat([torch.arange(channels).repeat_interleave(2 * l + 1)
                                                      for l in range(lmax + 1)])).to(device)
-        self.share = (1.0 / ((lmax + 1) * channels * (2 * degree + 1).double())).float().to(device)
+        self.share = (1.0 / ((lmax + 1) * channels * (2 * degree + 1).double())).to(device)
 
     def spread(self, w):
         return w.reshape(-1, self.places)[:, self.place]
@@ -126,7 +126,11 @@ class _Layout:
 
 def gradient_formula(desc, x, block, gate, post, pre, dh, dy):
     """(dx, dblock, dgate, dpost, dpre) of torch operations: what ``ictc_hip_norm_backward`` computes, from the
-    forward pass's arguments."""
+    forward pass's arguments.  In 64 bits, as the kernels' sums and projections are: what is left of a cotangent
+    along its row (eps / (q + eps) of it for a row with one large entry) is a difference, and in 32 bits its
+    rounding was all that came out (800 times the result at an entry of 300).  The results are rounded once."""
+    dtype = x.dtype
+    x, block, gate, post, pre, dh, dy = (None if t is None else t.double() for t in (x, block, gate, post, pre, dh, dy))
     lay = _Layout(desc.channels, desc.lmax, x.device)
     width, wide = desc.channels * (desc.lmax + 1) ** 2, x.shape[1]
 
@@ -151,11 +155,12 @@ def gradient_formula(desc, x, block, gate, post, pre, dh, dy):
         dpre = lay.gather(rho * dy * h).sum(0).view_as(pre)
     dx = fit(r, wide)
     if block is None:
-        return dx, None, None, None, dpre
+        return dx.to(dtype), None, None, None, dpre.to(dtype)
     db = adjoint(block, rho_b, lay.spread(k.expand(x.shape[0], -1)) * r)
     along = rho_b * lay.gather(r * block) * desc.residual_scale
     dgate = None if gate is None else along * open_ * (1.0 - open_) * post.reshape(1, -1)
-    return dx, db, dgate, (along * open_).sum(0).view_as(post), dpre
+    results = dx, db, dgate, (along * open_).sum(0).view_as(post), dpre
+    return tuple(None if t is None else t.to(dtype) for t in results)
 
 
 class _Gradient(torch.autograd.Function):
