@@ -17,7 +17,8 @@ from ictc_o3.backends.hip.optimizer import MOMENT_BLOCK, adamw_step, gradient_no
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW (decoupled weight decay) with torch.optim's interface.
+    """AdamW (decoupled weight decay) with torch.optim's interface, for contiguous float32 parameters on a GPU.
+    Moments are kept for whole groups (``moments`` gives one parameter's; ``state`` stays empty).
 
     moment_bits: 32 or 8 bits a value (8: blocks of 256 values with a power of two as scale, rounded at
     random from ``seed``).  max_grad_norm: the global norm of all groups' gradients is limited to it
@@ -43,6 +44,9 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
+        if not all(p.is_contiguous() for p in self.param_groups[-1]["params"]):
+            self.param_groups.pop()
+            raise ValueError("parameters must be contiguous")
         self._moments.append(None)
 
     def __getstate__(self):

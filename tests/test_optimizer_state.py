@@ -79,3 +79,16 @@ def test_copies_keep_everything(copied):
     other.step()                                                     # (no gradients)
     state = other.state_dict()
     assert state["seed"] == 11 and state["moments"][0] is None
+
+
+def test_parameters_that_are_not_contiguous_are_refused_when_they_are_given():
+    p = _params(1)
+    bad = torch.nn.Parameter(torch.zeros(4, 3).t())
+    with pytest.raises(ValueError, match="contiguous"):
+        AdamW([*p, bad])
+    optimizer = AdamW(p)
+    with pytest.raises(ValueError, match="contiguous"):
+        optimizer.add_param_group({"params": [bad]})
+    assert len(optimizer.param_groups) == len(optimizer._moments) == 1
+    optimizer.add_param_group({"params": torch.nn.Parameter(torch.zeros(2, 2))})       # a tensor by itself
+    assert len(optimizer.param_groups) == len(optimizer._moments) == 2
