@@ -100,7 +100,8 @@ def _number(value, name: str, below: float = math.inf) -> float:
 def adamw_step(params, grads, exp_avg, exp_avg_sq, progress, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                clip=None, seed=0) -> None:
     """One AdamW step of every parameter with a gradient, in place (a None gradient leaves its
-    parameter, moments and steps as they are).
+    parameter, moments and steps as they are).  One launch updates many tensors side by side: no two of
+    them may overlap.
 
     exp_avg, exp_avg_sq, progress: as ``new_state`` makes them (float32 moments, or pairs of 8-bit codes
     and block exponents; for each parameter its steps t, beta1^t and beta2^t, further rows are left alone).  lr: a number, or a one-element float32 tensor on the device.  clip:

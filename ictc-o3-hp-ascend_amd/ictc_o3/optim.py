@@ -44,9 +44,10 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
-        if not all(p.is_contiguous() for p in self.param_groups[-1]["params"]):
+        params = self.param_groups[-1]["params"]
+        if not all(p.is_contiguous() for p in params) or len({id(p) for p in params}) != len(params):
             self.param_groups.pop()
-            raise ValueError("parameters must be contiguous")
+            raise ValueError("parameters must be contiguous, and each in its group once")
         self._moments.append(None)
 
     def __getstate__(self):

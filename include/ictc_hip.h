@@ -704,7 +704,8 @@ int ictc_hip_gates_weight_grad(const float *grad, int64_t grad_row_stride, const
  *   m <- beta1 m + (1 - beta1) g         v <- beta2 v + (1 - beta2) g^2
  *   p <- (1 - lr weight_decay) p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
  * A clip[1] that is not a number leaves everything as it is.  lr_device, if not null, is one float on the
- * device that takes the place of desc->lr.  A tensor and its gradient may have any float alignment.
+ * device that takes the place of desc->lr.  A tensor and its gradient may have any float alignment; no two
+ * tensors may overlap (they are updated side by side).
  *
  * exp_avg and exp_avg_sq are flat arrays over all `count` tensors (those without a gradient too), each
  * tensor's values starting at the next multiple of ICTC_MOMENT_BLOCK; the values behind a tensor's end

@@ -92,3 +92,10 @@ def test_parameters_that_are_not_contiguous_are_refused_when_they_are_given():
     assert len(optimizer.param_groups) == len(optimizer._moments) == 1
     optimizer.add_param_group({"params": torch.nn.Parameter(torch.zeros(2, 2))})       # a tensor by itself
     assert len(optimizer.param_groups) == len(optimizer._moments) == 2
+
+
+def test_a_parameter_is_in_a_group_once():
+    """One launch updates all of a group's tensors side by side: twice the same one would race with itself."""
+    p = _params()
+    with pytest.raises(ValueError, match="once"):
+        AdamW([p[0], p[1], p[0]])
