@@ -59,7 +59,8 @@ def gradient_norm(grads, max_norm=None) -> torch.Tensor:
         raise ValueError("expected at least one gradient")
     if max_norm is not None and not float(max_norm) > 0.0:
         raise ValueError("max_norm must be positive, or None for no limit")
-    limit = 0.0 if max_norm is None or math.isinf(max_norm) else float(max_norm)
+    # (as a float32: one that rounds to zero would mean no limit)
+    limit = 0.0 if max_norm is None or math.isinf(max_norm) else max(float(max_norm), 2.0 ** -149)
     _, at, sizes, contiguous = _lib.host().addresses(grads, "gradients")
     if not contiguous:
         grads = [g.contiguous() for g in grads]

@@ -155,3 +155,11 @@ def test_a_frozen_evaluation_sees_replayed_steps(gpu, fused):
         assert_rel(got["energy"], want["energy"], what="energy")
         assert_rel(got["forces"], want["forces"], rtol=RTOL_FORCE, what="forces")
     assert not torch.allclose(got["energy"], first["energy"], rtol=1e-3)
+
+
+@pytest.mark.parametrize("limit", [1e-40, 1e-46, 1e-300])
+def test_limits_below_float32_are_limits(gpu, limit):
+    """Below float32's smallest number a limit was passed as zero, which means none."""
+    from ictc_o3 import gradient_norm
+    norm, coefficient = gradient_norm([torch.full((30,), 3.0, device=gpu)], limit).tolist()
+    assert abs(norm - 270.0 ** 0.5) <= 2e-6 * norm and 0.0 <= coefficient <= 2e-41
