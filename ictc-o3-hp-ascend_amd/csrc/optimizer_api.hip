@@ -237,6 +237,15 @@ __device__ __forceinline__ void moments(const StepScalars& c, const float* g, fl
   }
 }
 
+// A parameter behind its step, for the approximate reciprocal r: products and the last sum rounded in one given way.
+// Left to the compiler, variants of the kernel fused different products into the sum, and the last bit of a
+// parameter depended on how many blocks its wave took with it.
+__device__ __forceinline__ float stepped(const StepScalars& c, float p, float m, float r) {
+#pragma clang fp contract(off)
+  const float down = c.rate * m * r;
+  return __builtin_fmaf(c.keep, p, -down);
+}
+
 // The update of U whole blocks (or, with U = 1, of the first `left` of each lane's values): four values a
 // lane and block, all loads before the first store.
 template <bool SMALL, bool STREAM, int U, bool WHOLE>
@@ -282,8 +291,8 @@ __device__ __forceinline__ void update(const StepArgs& a, const StepScalars& c, 
       // them): with the exact ones instructions bound this variant (100 M values: 279 us against 250).
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        p[u][k] = c.keep * p[u][k] -
-                  c.rate * m[u][k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[u][k] * c.inv2) + c.eps);
+        p[u][k] = stepped(c, p[u][k], m[u][k],
+                          __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[u][k] * c.inv2) + c.eps));
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
