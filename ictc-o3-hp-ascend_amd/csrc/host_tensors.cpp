@@ -3,7 +3,7 @@
 //
 // A step over a model's parameters looks at dtype, device, layout, size and address of every
 // parameter and gradient.  From Python that is about 1.3 us a tensor, many times the update itself for
-// hundreds of small ones; here it is about 0.02 us.
+// hundreds of small ones; here it is about 0.025 us (pairs 0.019, written 0.006; 300 tensors).
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -128,9 +128,11 @@ PyObject* guarded(PyObject* self, PyObject* args) {
 }
 
 PyMethodDef methods[] = {
-    {"addresses", guarded<addresses>, METH_VARARGS, "(device, addresses, sizes, contiguous) of a list of FP32 GPU tensors"},
+    {"addresses", guarded<addresses>, METH_VARARGS,
+     "(device, addresses, sizes, contiguous) of a list of FP32 GPU tensors"},
     {"pairs", guarded<pairs>, METH_VARARGS, "(device, parameters, gradients, sizes, values, contiguous) of two lists"},
-    {"written", guarded<written>, METH_VARARGS, "raise the version counters of parameters written through their addresses"},
+    {"written", guarded<written>, METH_VARARGS,
+     "raise the version counters of parameters written through their addresses"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ictc_host_tensors", nullptr, -1, methods};

@@ -34,7 +34,10 @@
 //
 // Measured at C = 128, L = 3 (bytes as each kernel reads and writes them): forward of 32,768 rows 204 us, 5.6 TB/s;
 // of 8,192 rows 48 us (6.0), gradients 81 us with weight gradients (5.4), second derivatives 158 us (4.6: two waves to
-// a SIMD, and 1,900 instructions a wave and row).
+// a SIMD, and 1,900 instructions a wave and row).  The norm alone, 8,192 rows: gradients 43 us (4.7), second
+// derivatives 67 (5.0).  With degrees to 3 registers spill in wider rows: gradients 3.6 to 4.7 TB/s and second
+// derivatives 2.5 to 3.5 at 257 to 512 channels, 2.3 to 3.0 and 1.4 to 1.5 beyond.  These are the present code's; the
+// pairs of times at single choices below are from when each was made, on the code of that time.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -486,10 +489,11 @@ __device__ __forceinline__ void take_back(const float* stash, float (&u)[N], flo
 }
 
 // Where two of the second derivatives' operands wait in LDS: with all degrees to 3 a thread has 112 values, which with
-// what goes beside them did not fit into 256 registers (132 bytes of scratch memory a thread, 212 us for 8,192
-// rows of C = 128 against 172; one wave to a SIMD and 512 registers: 209).  With degrees to 2 they fit (109 us against
-// 112 for 16,384 rows of C = 64), rows that share a wave gain nothing (127 us against 130 at C = 32), and more than
-// 256 threads would take 64 KB and more.
+// what goes beside them do not fit into 256 registers (132 bytes of scratch memory a thread without the LDS, 12 with
+// it: 212 us for 8,192 rows of C = 128 against 172; one wave to a SIMD and 512 registers: 209).  With degrees to 2 they
+// fit (109 us against 112 for 16,384 rows of C = 64), and rows that share a wave gain nothing (127 us against 130 at
+// C = 32).  Rows of more than 256 threads do without it and spill (132 bytes a thread up to 512 threads, 616 beyond,
+// where a thread has 128 registers): 40 to 64 KB of LDS would hold the operands of 320 to 512 threads; not built.
 constexpr bool stashes(int lmax, int wide, bool block, bool next) { return lmax == 3 && wide == 1 && block && next; }
 
 template <int L, int WIDE, bool BLOCK, bool NEXT>
@@ -710,7 +714,7 @@ struct NormShape {
 // gradients 74 against 82; with degrees to 2 98 against 96).
 NormShape shape_of(int channels, int lmax, int64_t rows) {
   NormShape s;
-const bool shared = channels <= (lmax == 3 ? kNormWave / 2 : kNormWave);
+  const bool shared = channels <= (lmax == 3 ? kNormWave / 2 : kNormWave);
   s.wide = shared ? 0 : channels <= most_threads(1) ? 1 : channels <= most_threads(2) ? 2 : 3;
   if (s.wide) {
     s.threads = (channels + kNormWave - 1) / kNormWave * kNormWave;

@@ -3,9 +3,9 @@ reference, whose layers have none): the norm before the first block, and a block
 (norm of the block's output, gate, residual sum, norm before the next block).  Formulas stand in
 ``ictc_hip.h``.
 
-Forward, gradients and the gradients of those (training on forces) each run as one kernel; beyond, and for
-cotangents of weight gradients, the gradients' formulas are composed of torch operations and
-differentiated, so every order stays available.
+Forward, gradients and the gradients of those (training on forces) each run as one kernel; beyond, where the
+second ones are recorded, and for cotangents of weight gradients, the gradients' formulas are composed of torch
+operations in 64 bits and differentiated, so every order stays available.
 """
 from __future__ import annotations
 

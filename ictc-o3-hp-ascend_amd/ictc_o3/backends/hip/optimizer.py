@@ -72,7 +72,8 @@ def gradient_norm(grads, max_norm=None) -> torch.Tensor:
     workspace = torch.empty(doubles, device=device, dtype=torch.float64)
     with _on(device):
         _lib.check(lib.ictc_hip_gradient_norm(
-            at, sizes, n, limit, workspace.data_ptr(), doubles, out.data_ptr(), _lib.stream_of(device)), "ictc_hip_gradient_norm")
+            at, sizes, n, limit, workspace.data_ptr(), doubles, out.data_ptr(), _lib.stream_of(device)),
+            "ictc_hip_gradient_norm")
     return out
 
 
@@ -105,8 +106,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, progress, *, lr, betas=(0.9, 
     them may overlap.
 
     exp_avg, exp_avg_sq, progress: as ``new_state`` makes them (float32 moments, or pairs of 8-bit codes
-    and block exponents; for each parameter its steps t, beta1^t and beta2^t, further rows are left alone).  lr: a number, or a one-element float32 tensor on the device.  clip:
-    ``gradient_norm``'s result, whose coefficient scales the gradients.  seed: of the 8-bit rounding."""
+    and block exponents; for each parameter its steps t, beta1^t and beta2^t, further rows are left alone).
+    lr: a number, or a one-element float32 tensor on the device.  clip: ``gradient_norm``'s result, whose
+    coefficient scales the gradients.  seed: of the 8-bit rounding."""
     params, grads = list(params), list(grads)
     _, p_at, g_at, sizes, values, contiguous = _lib.host().pairs(params, grads, MOMENT_BLOCK)
     if not contiguous:
@@ -117,8 +119,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, progress, *, lr, betas=(0.9, 
     v, v_top, v_bits = _moments(exp_avg_sq, values, device, "exp_avg_sq")
     if bits != v_bits:
         raise ValueError("exp_avg and exp_avg_sq must have the same number of bits")
-    if progress.dim() != 2 or progress.shape[0] < n or progress.shape[1] != 3 or progress.dtype is not torch.float64 or not progress.is_contiguous() \
-            or progress.device != device:
+    if (progress.dim() != 2 or progress.shape[0] < n or progress.shape[1] != 3 or progress.dtype is not torch.float64
+            or not progress.is_contiguous() or progress.device != device):
         raise ValueError(f"progress must be a contiguous float64 tensor of at least {n} rows of 3 beside the "
                          "parameters")
     if clip is not None and (clip.dtype is not torch.float32 or clip.shape != (2,) or clip.device != device

@@ -22,7 +22,8 @@ def _operands(c, lmax, rows, one_large):
 
 
 @pytest.mark.parametrize("block", [True, False])
-@pytest.mark.parametrize("c,lmax,rows,one_large", [(1, 0, 7, False), (1, 0, 7, True), (5, 1, 6, True), (6, 2, 11, False)])
+@pytest.mark.parametrize("c,lmax,rows,one_large", [(1, 0, 7, False), (1, 0, 7, True), (5, 1, 6, True),
+                                                   (6, 2, 11, False)])
 def test_formula_in_single_precision(c, lmax, rows, one_large, block):
     from ictc_o3 import _lib
     from ictc_o3.backends.hip.norms import gradient_formula

@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 NAMES = ("x", "block", "gate", "post", "pre")
 
 
-@pytest.mark.parametrize("c,lmax,rows,one_large", [(1, 0, 7, False), (1, 0, 7, True), (5, 1, 6, True), (70, 2, 11, False)])
+@pytest.mark.parametrize("c,lmax,rows,one_large", [(1, 0, 7, False), (1, 0, 7, True), (5, 1, 6, True),
+                                                   (70, 2, 11, False)])
 def test_composed_orders_keep_what_cancels(gpu, c, lmax, rows, one_large):
     """Second derivatives with a recorded graph, their derivatives, and cotangents of weight gradients, with a row's
     entries alike and with one that is much larger (a cotangent's part along the row then cancels almost wholly)."""
