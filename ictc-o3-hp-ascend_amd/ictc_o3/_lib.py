@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must precede CDLL, see module docstring)
 MAX_PATHS = 128
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libictc_hip.so")
 HOST_PATH = os.path.join(os.path.dirname(LIB_PATH), "ictc_host_tensors.so")
-ABI_VERSION = 27
+ABI_VERSION = 28
 
 
 class TpDesc(ctypes.Structure):
@@ -156,6 +156,12 @@ _SIGNATURES = {
     "ictc_hip_norm_forward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_P] * 7 + [_I64, _P]),
     "ictc_hip_norm_backward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_P] * 13 + [_I64, _I64, _P]),
     "ictc_hip_norm_second": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [_P] * 18 + [_I64, _I64, _P]),
+    "ictc_hip_layer_norm_workspace": (_I64, [ctypes.c_int, _I64]),
+    "ictc_hip_layer_norm_forward": (ctypes.c_int, [_P] * 4 + [ctypes.c_int, ctypes.c_int, ctypes.c_float, _I64, _P]),
+    "ictc_hip_layer_norm_backward": (ctypes.c_int, [_P] * 8 + [_I64, ctypes.c_int, ctypes.c_int, ctypes.c_float, _I64,
+                                                               _P]),
+    "ictc_hip_layer_norm_second": (ctypes.c_int, [_P] * 10 + [_I64, ctypes.c_int, ctypes.c_int, ctypes.c_float, _I64,
+                                                              _P]),
     "ictc_hip_sgemm": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _I64, _I64, _I64, ctypes.c_float, _P, _I64, _P,
                                       _I64, ctypes.c_float, _P, _I64, _P]),
     "ictc_hip_radius_graph_bins": (ctypes.c_int, [ctypes.POINTER(CellGrid), _P, _I64, _P, _P, _P, _P, _P, _P]),

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import torch
 
+from ictc_o3.backends.hip.layer_norm import layer_norm
 from ictc_o3.backends.hip.linear import channel_linear, species_channel_linear
 from ictc_o3.backends.hip.norms import equivariant_norm, gated_residual_norm
 from ictc_o3.backends.hip.optimizer import adamw_step, gradient_norm, moment_values
@@ -281,4 +282,4 @@ __all__ = ["EdgeTensorProduct", "PackedGraphMessage", "GraphMessage", "direction
            "create_symmetric_contraction", "configure_symmetric_contraction",
            "channel_linear", "species_channel_linear", "normalized_silu", "strict_fp32",
            "gradient_norm", "adamw_step", "moment_values",
-           "equivariant_norm", "gated_residual_norm"]
+           "equivariant_norm", "gated_residual_norm", "layer_norm"]

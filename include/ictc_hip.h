@@ -789,6 +789,34 @@ int ictc_hip_norm_second(const ictc_norm_desc* desc, const float* h, const float
                          int64_t workspace_floats, int64_t rows, hipStream_t stream);
 
 /*
+ * Layer norm of rows of `width` columns, with SiLU behind it or nothing (no counterpart in the reference, whose
+ * radial network has none):
+ *   y = f(w xh + b)      xh = (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps)
+ * bias may be null (b = 0), in all calls alike.  Rows are contiguous, at any float's alignment.
+ *
+ *   backward: the gradients to x, weight and bias from grad_y; any output may be null.
+ *   second:   the gradients of <cot_x, dx>, dx being backward's as a function of x, weight, bias and grad_y, to
+ *             x, grad_y, weight and bias; any output may be null.
+ *
+ * Weight gradients need a workspace of ictc_hip_layer_norm_workspace(width, rows) floats (negative: -ictc_status)
+ * and are summed in a fixed order; they are zero for rows = 0.  1 <= width <= ICTC_LAYER_NORM_MAX_WIDTH, eps > 0.
+ */
+#define ICTC_LAYER_NORM_MAX_WIDTH 8192
+#define ICTC_ACTIVATION_NONE 0
+#define ICTC_ACTIVATION_SILU 1
+
+int64_t ictc_hip_layer_norm_workspace(int width, int64_t rows);
+int ictc_hip_layer_norm_forward(const float* x, const float* weight, const float* bias, float* y, int width,
+                                int activation, float eps, int64_t rows, hipStream_t stream);
+int ictc_hip_layer_norm_backward(const float* x, const float* weight, const float* bias, const float* grad_y, float* dx,
+                                 float* dweight, float* dbias, float* workspace, int64_t workspace_floats, int width,
+                                 int activation, float eps, int64_t rows, hipStream_t stream);
+int ictc_hip_layer_norm_second(const float* x, const float* weight, const float* bias, const float* grad_y,
+                               const float* cot_x, float* dx, float* dgrad_y, float* dweight, float* dbias,
+                               float* workspace, int64_t workspace_floats, int width, int activation, float eps,
+                               int64_t rows, hipStream_t stream);
+
+/*
  * Row-major fp32 product C[m,n] = alpha * op(A) op(B) + beta * C on rocBLAS, for the dense
  * channel linears around the operators.  op(A) is [m,k]: A is stored [m,k] (lda >= k) or,
  * with trans_a != 0, [k,m] (lda >= m); likewise B with op(B) [k,n].  Each host thread uses
