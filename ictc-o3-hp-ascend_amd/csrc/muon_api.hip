@@ -1,0 +1,611 @@
+// Orthogonalised updates of matrices: moving averages of gradients brought near an orthogonal matrix by
+// Newton-Schulz products, many matrices at a time, gfx950.
+//
+//   M <- beta M + (1 - beta) g     U = beta M + (1 - beta) g  (or M)     X = U / (|U| + eps)
+//   steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X           (on the shorter side, m <= n)
+//   P <- (1 - lr wd) P - rate X
+//
+// Precision.  A singular value goes through p(s) = a s + b s^3 + c s^5 in every step, so small ones grow by a = 3.4
+// each time and an error of X with them: products in bfloat16 would leave updates with 2 correct digits.  A product
+// here is of float32 accuracy on the float16 matrix cores: x = hi + lo 2^-11 with hi = f16(x) and lo = f16(2^11 (x - hi)),
+// 22 bits or an absolute 2^-36, whichever is larger (entries are near 1 and below, |X| is at most about 1.2), and
+//   x y = hi hi' + 2^-11 (hi lo' + lo hi')  + (2^-22 x y, left out)
+// in two float32 accumulators.  A matrix with |U| below eps, where X stays small, is kept times a power of two (2^e,
+// see exponent_at), so that it has as many bits.  Three products at 16 times the float32 instructions' rate.  (The form that iterates
+// A alone and multiplies X once has a third of the work for wide matrices, but doubles the error's growth: singular values
+// below 1e-3 of the largest come out wrong, 1e-4 of the result at rank-deficient matrices.)
+//
+// All three products are of the form P Q^T with both operands' rows along the reduction (X X^T, A A^T, B (X^T)^T), so
+// one kernel does them; X is kept in both orientations.  A and B are symmetric: only tiles on and above the diagonal
+// are computed.  Every matrix of every tensor takes part in the same launches: `owner` says which matrix a workgroup's
+// tile belongs to.  Sides are padded with zeros to whole tiles, which stay zero.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "ictc_hip.h"
+
+namespace ictc {
+namespace {
+
+constexpr int kMuThreads = 256;
+constexpr int kMuWave = 64;
+constexpr int kTensorsPerLaunch = 48;        // of the table in the kernel's arguments
+constexpr int kPrep = 64;                    // side of a tile of the source
+constexpr int kStep = 32;                    // reduction entries in LDS at a time
+constexpr int64_t kMostBytes = int64_t{2} << 30;     // workspace that a call goes by, unless one tensor needs more
+
+using half8 = _Float16 __attribute__((ext_vector_type(8)));
+using half4 = _Float16 __attribute__((ext_vector_type(4)));
+using f32x16 = float __attribute__((ext_vector_type(16)));
+typedef float mf4 __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr float kLow = 2048.f, kUnlow = 1.f / 2048.f;
+constexpr int kMostExponent = 200;           // (2^-149 is the smallest number)
+
+// One tensor's matrices, as the host describes them.
+struct MuonTensor {
+  const float* src;          // gradient, or the matrix itself
+  float* momentum;           // null: src is the matrix
+  float* out;                // parameter, or the result
+  int64_t base;              // of the first matrix, in bytes of the workspace
+  int32_t rows, cols, batches, first;          // first: index of the first matrix
+  uint32_t prep, sym, apply;                   // first tile of each kind
+  float rate;                // of the update, times the learning rate
+};
+
+struct MuonTable {
+  MuonTensor tensor[kTensorsPerLaunch];
+};
+
+static_assert(sizeof(MuonTable) + 128 <= 4096, "kernel arguments are limited to 4 KB");
+
+// One matrix, in the workspace.
+struct MuonMatrix {
+  const float* src;
+  float* momentum;
+  float* out;
+  char* x;                   // X [mp][np], two planes; then X^T twice [np][mp], A and B [mp][mp]
+  int32_t rows, cols, mp, np;
+  uint32_t prep, prep_tiles, sym, apply;
+  float rate;
+  int32_t transposed;        // more rows than columns
+};
+
+struct MuonArgs {
+  const MuonMatrix* matrices;
+  const uint32_t *prep_owner, *sym_owner, *apply_owner;
+  double* squares;           // of each tile of the source
+  int32_t* exponents;        // of each matrix: X is kept times 2^e at first
+  const float* clip;
+  const float* lr_device;
+  double weight_decay, eps;
+  float beta, rest, lr;      // rest: 1 - beta
+  float a, b, c;
+  int32_t nesterov;
+};
+
+__device__ __forceinline__ bool skipped(const MuonArgs& a) { return a.clip && a.clip[1] != a.clip[1]; }
+
+constexpr int64_t up_to(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// Tiles and bytes of one matrix, with sides padded to multiples of T.
+struct MuonSize {
+  int64_t mp, np, prep, sym, apply, bytes;
+};
+
+template <int T>
+__host__ __device__ MuonSize muon_size(int64_t rows, int64_t cols) {
+  MuonSize s;
+  const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  s.mp = up_to(m, T), s.np = up_to(n, T);
+  s.prep = (s.mp / kPrep) * (s.np / kPrep);
+  const int64_t i = s.mp / T, j = s.np / T;
+  s.sym = i * (i + 1) / 2;
+  s.apply = i * j;
+  s.bytes = 12 * s.mp * s.np + 8 * s.mp * s.mp;
+  return s;
+}
+
+// Descriptions of every matrix of the table's tensors, and the owners of their tiles: a workgroup to a tensor.
+template <int T>
+__global__ void __launch_bounds__(kMuThreads)
+muon_setup_kernel(const MuonTable table, char* __restrict__ workspace, MuonMatrix* __restrict__ matrices,
+                  uint32_t* __restrict__ prep_owner, uint32_t* __restrict__ sym_owner, uint32_t* __restrict__ apply_owner) {
+  const MuonTensor& t = table.tensor[blockIdx.x];
+  const MuonSize s = muon_size<T>(t.rows, t.cols);
+  const int64_t values = static_cast<int64_t>(t.rows) * t.cols;
+  for (int b = threadIdx.x; b < t.batches; b += kMuThreads) {
+    MuonMatrix m;
+    m.src = t.src + b * values;
+    m.momentum = t.momentum ? t.momentum + b * values : nullptr;
+    m.out = t.out + b * values;
+    m.x = workspace + t.base + b * s.bytes;
+    m.rows = t.rows, m.cols = t.cols, m.mp = static_cast<int32_t>(s.mp), m.np = static_cast<int32_t>(s.np);
+    m.prep = t.prep + static_cast<uint32_t>(b * s.prep), m.prep_tiles = static_cast<uint32_t>(s.prep);
+    m.sym = t.sym + static_cast<uint32_t>(b * s.sym);
+    m.apply = t.apply + static_cast<uint32_t>(b * s.apply);
+    m.rate = t.rate;
+    m.transposed = t.rows > t.cols;
+    matrices[t.first + b] = m;
+  }
+  for (int64_t k = threadIdx.x; k < t.batches * s.prep; k += kMuThreads)
+    prep_owner[t.prep + k] = t.first + static_cast<uint32_t>(k / s.prep);
+  for (int64_t k = threadIdx.x; k < t.batches * s.sym; k += kMuThreads)
+    sym_owner[t.sym + k] = t.first + static_cast<uint32_t>(k / s.sym);
+  for (int64_t k = threadIdx.x; k < t.batches * s.apply; k += kMuThreads)
+    apply_owner[t.apply + k] = t.first + static_cast<uint32_t>(k / s.apply);
+}
+
+// A tile of the source: its first row and column there, and what of it there is.
+struct SourceTile {
+  int r0, c0, rows, cols;
+
+  __device__ __forceinline__ SourceTile(const MuonMatrix& m, uint32_t tile) {
+    const int across = (m.transposed ? m.mp : m.np) / kPrep;
+    r0 = static_cast<int>(tile / across) * kPrep;
+    c0 = static_cast<int>(tile % across) * kPrep;
+    rows = m.rows - r0 < 0 ? 0 : m.rows - r0 > kPrep ? kPrep : m.rows - r0;
+    cols = m.cols - c0 < 0 ? 0 : m.cols - c0 > kPrep ? kPrep : m.cols - c0;
+  }
+};
+
+__device__ __forceinline__ double muon_block_sum(double x, double* part) {
+#pragma unroll
+  for (int d = kMuWave / 2; d; d >>= 1) x += __shfl_xor(x, d);
+  if ((threadIdx.x & (kMuWave - 1)) == 0) part[threadIdx.x / kMuWave] = x;
+  __syncthreads();
+  double sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < kMuThreads / kMuWave; ++w) sum += part[w];
+  return sum;
+}
+
+// The moving average and what is orthogonalised; each product and sum rounded for itself.
+__device__ __forceinline__ float averaged(const MuonArgs& a, float m, float g) {
+#pragma clang fp contract(off)
+  return a.beta * m + a.rest * g;
+}
+
+// Moving averages, and the sum of squares (in 64 bits) of each tile of what is orthogonalised.
+__global__ void __launch_bounds__(kMuThreads) muon_average_kernel(const MuonArgs a) {
+  __shared__ double part[kMuThreads / kMuWave];
+  if (skipped(a)) return;
+  const MuonMatrix m = a.matrices[a.prep_owner[blockIdx.x]];
+  const SourceTile t(m, blockIdx.x - m.prep);
+  const float scale = a.clip ? a.clip[1] : 1.f;
+  const int column = threadIdx.x % kPrep;
+  double sum = 0.0;
+  if (column < t.cols)
+    for (int r = threadIdx.x / kPrep; r < t.rows; r += kMuThreads / kPrep) {
+      const int64_t at = static_cast<int64_t>(t.r0 + r) * m.cols + t.c0 + column;
+      float u = m.src[at];
+      if (m.momentum) {
+        const float g = scale * u;
+        u = averaged(a, m.momentum[at], g);
+        m.momentum[at] = u;
+        if (a.nesterov) u = averaged(a, u, g);
+      }
+      sum += static_cast<double>(u) * static_cast<double>(u);
+    }
+  sum = muon_block_sum(sum, part);
+  if (threadIdx.x == 0) a.squares[blockIdx.x] = sum;
+}
+
+__device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
+  hi = static_cast<_Float16>(x);
+  lo = static_cast<_Float16>((x - static_cast<float>(hi)) * kLow);
+}
+
+__device__ __forceinline__ float joined(_Float16 hi, _Float16 lo) {
+  return fmaf(static_cast<float>(lo), kUnlow, static_cast<float>(hi));
+}
+
+// The power of two that X is kept with before a step, from the one at first: |X| <= 2^-e, and a step multiplies it by at
+// most |a| + |b| 4^-e + |c| 16^-e.
+__device__ __forceinline__ int exponent_at(const MuonArgs& a, int e, int step) {
+  for (; step && e; --step) {
+    const float most = fabsf(a.a) + ldexpf(fabsf(a.b), -2 * e) + ldexpf(fabsf(a.c), -4 * e);
+    e -= most > 1.f ? ilogbf(most) + 1 : 0;
+    e = e < 0 ? 0 : e;
+  }
+  return e;
+}
+
+// X in both orientations from the source: tiles go through LDS.
+__global__ void __launch_bounds__(kMuThreads) muon_normalise_kernel(const MuonArgs a) {
+  __shared__ double part[kMuThreads / kMuWave];
+  __shared__ float tile[kPrep][kPrep + 1];
+  if (skipped(a)) return;
+  const uint32_t owner = a.prep_owner[blockIdx.x];
+  const MuonMatrix m = a.matrices[owner];
+  const SourceTile t(m, blockIdx.x - m.prep);
+  double sum = 0.0;
+  for (uint32_t k = threadIdx.x; k < m.prep_tiles; k += kMuThreads) sum += a.squares[m.prep + k];
+  const double norm = sqrt(muon_block_sum(sum, part)), share = norm / (norm + a.eps);
+  const int e = share > 0.0 && share < 0.5 ? min(-ilogb(share) - 1, kMostExponent) : 0;
+  if (threadIdx.x == 0 && blockIdx.x == m.prep) a.exponents[owner] = e;
+  const double inv = ldexp(1.0 / (norm + a.eps), e);
+  const float scale = a.clip ? a.clip[1] : 1.f;
+  const int column = threadIdx.x % kPrep;
+  for (int r = threadIdx.x / kPrep; r < kPrep; r += kMuThreads / kPrep) {
+    float u = 0.f;
+    if (r < t.rows && column < t.cols) {
+      const int64_t at = static_cast<int64_t>(t.r0 + r) * m.cols + t.c0 + column;
+      u = m.src[at];
+      if (m.momentum) u = a.nesterov ? averaged(a, m.momentum[at], scale * u) : m.momentum[at];
+      u = static_cast<float>(u * inv);
+    }
+    tile[r][column] = u;
+  }
+  __syncthreads();
+  const int64_t plane = static_cast<int64_t>(m.mp) * m.np;
+  _Float16* const x = reinterpret_cast<_Float16*>(m.x);
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {           // as it is, and transposed
+    _Float16* to = x + ((side != 0) == (m.transposed != 0) ? 0 : 2 * plane);
+    const int64_t wide = (side != 0) == (m.transposed != 0) ? m.np : m.mp;
+    const int first = side ? t.c0 : t.r0, along = side ? t.r0 : t.c0;
+    for (int k = threadIdx.x; k < kPrep * kPrep / 8; k += kMuThreads) {
+      const int r = k / (kPrep / 8), c = k % (kPrep / 8) * 8;
+      half8 hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        _Float16 h, l;
+        split(side ? tile[c + j][r] : tile[r][c + j], h, l);
+        hi[j] = h, lo[j] = l;
+      }
+      const int64_t at = (first + r) * wide + along + c;
+      *reinterpret_cast<half8*>(to + at) = hi;
+      *reinterpret_cast<half8*>(to + plane + at) = lo;
+    }
+  }
+}
+
+enum MuonPhase { kGram, kPoly, kApply, kLast };
+
+// 16 bytes a lane from global memory to consecutive places of LDS.
+__device__ __forceinline__ void load_to_lds(const _Float16* from, _Float16* to) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t __attribute__((address_space(1)))*>(
+                                       reinterpret_cast<uintptr_t>(from)),
+                                   reinterpret_cast<uint32_t __attribute__((address_space(3)))*>(
+                                       static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to))),
+                                   16, 0, 0);
+}
+
+// One tile of P Q^T: T x T, four waves of (T/2) x (T/2).  Rows of 32 reduction entries (64 bytes) lie in LDS in four groups
+// of 16 bytes, whose order is turned with the row so that 8 rows' groups fill all banks; they come straight from
+// global memory (a lane picks the group that belongs to its place), one step ahead of the products.
+template <int T, int PHASE>
+__global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs a, int step) {
+  constexpr int N = T / 64;                        // 32 x 32 products of a wave, each way
+  constexpr int kPlane = T * kStep;                // halves of one operand plane in LDS
+  __shared__ _Float16 lds[2][4][kPlane];           // P's hi and lo, Q's hi and lo
+  if (skipped(a)) return;
+  constexpr bool kSym = PHASE == kGram || PHASE == kPoly;
+  const uint32_t owner = (kSym ? a.sym_owner : a.apply_owner)[blockIdx.x];
+  const MuonMatrix m = a.matrices[owner];
+  const int parity = step & 1;
+  const uint32_t local = blockIdx.x - (kSym ? m.sym : m.apply);
+  int ti, tj;
+  if constexpr (kSym) {
+    tj = static_cast<int>((sqrtf(8.f * local + 1.f) - 1.f) * 0.5f);
+    while (static_cast<uint32_t>(tj + 1) * (tj + 2) / 2 <= local) ++tj;
+    while (static_cast<uint32_t>(tj) * (tj + 1) / 2 > local) --tj;
+    ti = static_cast<int>(local) - tj * (tj + 1) / 2;
+  } else {
+    const uint32_t down = m.mp / T;
+    ti = static_cast<int>(local % down), tj = static_cast<int>(local / down);
+  }
+  const int64_t plane = static_cast<int64_t>(m.mp) * m.np, square = static_cast<int64_t>(m.mp) * m.mp;
+  _Float16* const x = reinterpret_cast<_Float16*>(m.x);
+  _Float16* const xt = x + 2 * plane * (1 + parity);               // X^T now, and what it becomes
+  _Float16* const xt_next = x + 2 * plane * (2 - parity);
+  _Float16* const gram = x + 6 * plane;
+  _Float16* const poly = gram + 2 * square;
+  const _Float16* const p = PHASE == kGram ? x : PHASE == kPoly ? gram : poly;
+  const _Float16* const q = PHASE == kGram ? x : PHASE == kPoly ? gram : xt;
+  const int64_t p_plane = PHASE == kGram ? plane : square, q_plane = PHASE == kPoly ? square : plane;
+  const int depth = PHASE == kGram ? m.np : m.mp;
+
+  const int lane = threadIdx.x & (kMuWave - 1), wave = threadIdx.x / kMuWave;
+  const int wi = (wave & 1) * (T / 2), wj = (wave >> 1) * (T / 2);
+  const auto fetch = [&](int step, int buffer) {
+    // a wave's load fills 16 rows of a plane; the tile has T / 16 of them for each plane
+#pragma unroll
+    for (int k = 0; k < T / 16; ++k) {
+      const int piece = k * 4 + wave;                 // of 4 planes x T / 16
+      const int which = piece / (T / 16), rows = piece % (T / 16) * 16;
+      const int row = rows + lane / 4, group = (lane & 3) ^ ((row >> 1) & 3);
+      const _Float16* base = which < 2 ? p + which * p_plane + static_cast<int64_t>(ti * T + row) * depth
+                                       : q + (which - 2) * q_plane + static_cast<int64_t>(tj * T + row) * depth;
+      load_to_lds(base + step * kStep + group * 8, &lds[buffer][which][rows * kStep]);
+    }
+  };
+  f32x16 high[N][N] = {}, low[N][N] = {};
+  const int steps = depth / kStep;
+  fetch(0, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int s = 0; s < steps; ++s) {
+    const int buffer = s & 1;
+    if (s + 1 < steps) fetch(s + 1, buffer ^ 1);
+#pragma unroll
+    for (int k = 0; k < kStep / 16; ++k) {
+      half8 op[4][N];
+#pragma unroll
+      for (int which = 0; which < 4; ++which)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const int row = (which < 2 ? wi : wj) + n * 32 + (lane & 31), group = k * 2 + lane / 32;
+          op[which][n] = *reinterpret_cast<const half8*>(&lds[buffer][which][row * kStep + (group ^ ((row >> 1) & 3)) * 8]);
+        }
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) high[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[0][i], op[2][j], high[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[0][i], op[3][j], low[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[1][i], op[2][j], low[i][j], 0, 0, 0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+  // A lane holds rows 8 (k / 4) + 4 (lane / 32) + k % 4 of column lane % 32 of each 32 x 32 product.
+  int shift = 0;                                   // of the result's power of two
+  if constexpr (PHASE != kPoly) {
+    const int first = a.exponents[owner];
+    if (first) {
+      const int e = exponent_at(a, first, step);
+      shift = PHASE == kGram ? -2 * e : PHASE == kApply ? exponent_at(a, first, step + 1) - e : -e;
+    }
+  }
+  float keep = 1.f, rate = 0.f;
+  if constexpr (PHASE == kLast) {
+    if (m.momentum) {
+      const float lr = a.lr_device ? *a.lr_device : a.lr;
+      keep = static_cast<float>(1.0 - static_cast<double>(lr) * a.weight_decay);
+      rate = lr * m.rate;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int k = 0; k < 16; k += 4) {
+        const int row = ti * T + wi + i * 32 + 2 * k + 4 * (lane / 32), column = tj * T + wj + j * 32 + (lane & 31);
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = fmaf(low[i][j][k + r], kUnlow, high[i][j][k + r]);
+        const int64_t across = static_cast<int64_t>(column) * m.mp + row;        // in what has rows of m entries
+        if constexpr (PHASE == kPoly || PHASE == kApply || PHASE == kLast) {
+          const _Float16* old = PHASE == kPoly ? gram : xt;
+          const int64_t old_plane = PHASE == kPoly ? square : plane;
+          const half4 hi = *reinterpret_cast<const half4*>(old + across);
+          const half4 lo = *reinterpret_cast<const half4*>(old + old_plane + across);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            v[r] = PHASE == kPoly ? fmaf(a.b, joined(hi[r], lo[r]), a.c * v[r]) : fmaf(a.a, joined(hi[r], lo[r]), v[r]);
+        }
+        if (PHASE != kPoly && shift) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], shift);
+        }
+        if constexpr (PHASE == kLast) {
+          const int shorter = m.transposed ? m.cols : m.rows, longer = m.transposed ? m.rows : m.cols;
+          if (column < longer) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (row + r < shorter) {
+                float* to = m.out + (m.transposed ? static_cast<int64_t>(column) * m.cols + row + r
+                                                  : static_cast<int64_t>(row + r) * m.cols + column);
+                *to = m.momentum ? keep * *to - rate * v[r] : v[r];
+              }
+          }
+        } else {
+          _Float16* const turned = PHASE == kGram ? gram : PHASE == kPoly ? poly : xt_next;      // [column][row]
+          _Float16* const plain = PHASE == kGram ? gram : PHASE == kPoly ? poly : x;             // [row][column]
+          const int64_t out_plane = PHASE == kApply ? plane : square, wide = PHASE == kApply ? m.np : m.mp;
+          half4 hi, lo;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            _Float16 h, l;
+            split(v[r], h, l);
+            hi[r] = h, lo[r] = l;
+          }
+          *reinterpret_cast<half4*>(turned + across) = hi;
+          *reinterpret_cast<half4*>(turned + out_plane + across) = lo;
+          if (!kSym || ti != tj) {       // (a tile on the diagonal holds its own mirror image)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              plain[(row + r) * wide + column] = hi[r];
+              plain[out_plane + (row + r) * wide + column] = lo[r];
+            }
+          }
+        }
+      }
+}
+
+constexpr int kTile = 64;
+constexpr int64_t kMostSide = 1 << 20;
+constexpr int64_t kMostMatrices = int64_t{1} << 23;
+constexpr int64_t kMostTiles = int64_t{1} << 23;      // of a launch: threads within 32 bits
+
+// Tensors [first, end) of a call whose matrices take part in the same launches, and what they need.
+struct MuonGroup {
+  int64_t end, matrices, prep, sym, apply, bytes;
+
+  // Where the tables and the matrices lie in the workspace.
+  int64_t at_matrices() const { return 0; }
+  int64_t at_prep() const { return up_to(matrices * static_cast<int64_t>(sizeof(MuonMatrix)), 256); }
+  int64_t at_sym() const { return at_prep() + up_to(4 * prep, 256); }
+  int64_t at_apply() const { return at_sym() + up_to(4 * sym, 256); }
+  int64_t at_squares() const { return at_apply() + up_to(4 * apply, 256); }
+  int64_t at_exponents() const { return at_squares() + up_to(8 * prep, 256); }
+  int64_t at_values() const { return at_exponents() + up_to(4 * matrices, 256); }
+  int64_t size() const { return at_values() + bytes; }
+};
+
+// (Tensors that take no part are counted: the groups, and with them the workspace, go by the shapes alone.)
+template <int T>
+MuonGroup muon_group(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t first, int64_t count) {
+  MuonGroup g = {};
+  int64_t k = first;
+  for (; k < count; ++k) {
+    if (!rows[k] || !cols[k] || !batches[k]) continue;
+    const MuonSize s = muon_size<T>(rows[k], cols[k]);
+    const int64_t b = batches[k];
+    if (g.matrices && (g.bytes + b * s.bytes > kMostBytes || g.prep + b * s.prep > kMostTiles)) break;
+    g.matrices += b, g.prep += b * s.prep, g.sym += b * s.sym, g.apply += b * s.apply, g.bytes += b * s.bytes;
+  }
+  g.end = k;
+  return g;
+}
+
+bool muon_valid(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count) {
+  if (count < 0 || count > 0x7fffffff || (count && (!rows || !cols || !batches))) return false;
+  for (int64_t k = 0; k < count; ++k) {
+    if (rows[k] < 0 || rows[k] > kMostSide || cols[k] < 0 || cols[k] > kMostSide || batches[k] < 0 ||
+        batches[k] > kMostMatrices)
+      return false;
+    if (!rows[k] || !cols[k] || !batches[k]) continue;
+    const MuonSize s = muon_size<kTile>(rows[k], cols[k]);
+    if (s.prep > kMostTiles / batches[k]) return false;
+  }
+  return true;
+}
+
+bool muon_valid(const ictc_muon_desc* d, const float* lr_device) {
+  if (!d) return false;
+  for (const double c : d->coefficients)
+    if (!isfinite(c)) return false;
+  return d->beta >= 0.0 && d->beta < 1.0 && d->weight_decay >= 0.0 && d->eps > 0.0 && isfinite(d->eps) &&
+         (lr_device || d->lr >= 0.f) && d->steps >= 1 && d->steps <= ICTC_MUON_MAX_STEPS &&
+         (d->adjust == ICTC_MUON_SHAPE || d->adjust == ICTC_MUON_MATCH_RMS);
+}
+
+int muon_launched() { return hipGetLastError() == hipSuccess ? ICTC_OK : ICTC_ERR_LAUNCH; }
+
+template <int T>
+int64_t muon_workspace(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count) {
+  int64_t most = 0;
+  for (int64_t k = 0; k < count;) {
+    const MuonGroup g = muon_group<T>(rows, cols, batches, k, count);
+    if (g.size() > most) most = g.size();
+    k = g.end;
+  }
+  return most;
+}
+
+template <int T>
+int muon_run(const float* const* src, float* const* momentum, float* const* out, const int64_t* rows,
+             const int64_t* cols, const int64_t* batches, int64_t count, const ictc_muon_desc* d, const float* clip,
+             const float* lr_device, char* ws, int64_t ws_bytes, hipStream_t stream) {
+  MuonArgs a;
+  a.clip = clip, a.lr_device = lr_device;
+  a.weight_decay = d->weight_decay, a.eps = d->eps;
+  a.beta = static_cast<float>(d->beta), a.rest = static_cast<float>(1.0 - d->beta), a.lr = d->lr;
+  a.a = static_cast<float>(d->coefficients[0]), a.b = static_cast<float>(d->coefficients[1]);
+  a.c = static_cast<float>(d->coefficients[2]);
+  a.nesterov = d->nesterov;
+  for (int64_t k = 0; k < count;) {
+    const MuonGroup g = muon_group<T>(rows, cols, batches, k, count);
+    if (g.size() > ws_bytes) return ICTC_ERR_INVALID_ARGUMENT;
+    MuonMatrix* const matrices = reinterpret_cast<MuonMatrix*>(ws + g.at_matrices());
+    uint32_t* const prep = reinterpret_cast<uint32_t*>(ws + g.at_prep());
+    uint32_t* const sym = reinterpret_cast<uint32_t*>(ws + g.at_sym());
+    uint32_t* const apply = reinterpret_cast<uint32_t*>(ws + g.at_apply());
+    a.matrices = matrices, a.prep_owner = prep, a.sym_owner = sym, a.apply_owner = apply;
+    a.squares = reinterpret_cast<double*>(ws + g.at_squares());
+    a.exponents = reinterpret_cast<int32_t*>(ws + g.at_exponents());
+    MuonGroup at = {};       // of the tensors before that take part
+    for (int64_t t = k; t < g.end;) {
+      MuonTable table;
+      int n = 0;
+      for (; t < g.end && n < kTensorsPerLaunch; ++t) {
+        if (!src[t] || !rows[t] || !cols[t] || !batches[t]) continue;
+        const MuonSize s = muon_size<T>(rows[t], cols[t]);
+        const int64_t b = batches[t];
+        const double r = static_cast<double>(rows[t]), c = static_cast<double>(cols[t]);
+        MuonTensor& e = table.tensor[n++];
+        e.src = src[t], e.momentum = momentum ? momentum[t] : nullptr, e.out = out[t];
+        e.base = at.bytes, e.rows = static_cast<int32_t>(rows[t]), e.cols = static_cast<int32_t>(cols[t]);
+        e.batches = static_cast<int32_t>(b), e.first = static_cast<int32_t>(at.matrices);
+        e.prep = static_cast<uint32_t>(at.prep), e.sym = static_cast<uint32_t>(at.sym);
+        e.apply = static_cast<uint32_t>(at.apply);
+        e.rate = static_cast<float>(d->adjust == ICTC_MUON_SHAPE ? sqrt(r > c ? r / c : 1.0) : 0.2 * sqrt(r > c ? r : c));
+        at.matrices += b, at.prep += b * s.prep, at.sym += b * s.sym, at.apply += b * s.apply, at.bytes += b * s.bytes;
+      }
+      if (!n) break;
+      hipLaunchKernelGGL(muon_setup_kernel<T>, dim3(n), dim3(kMuThreads), 0, stream, table, ws + g.at_values(), matrices,
+                         prep, sym, apply);
+      if (const int rc = muon_launched()) return rc;
+    }
+    k = g.end;
+    if (!at.matrices) continue;
+    hipLaunchKernelGGL(muon_average_kernel, dim3(static_cast<unsigned>(at.prep)), dim3(kMuThreads), 0, stream, a);
+    hipLaunchKernelGGL(muon_normalise_kernel, dim3(static_cast<unsigned>(at.prep)), dim3(kMuThreads), 0, stream, a);
+    for (int step = 0; step < d->steps; ++step) {
+      const auto apply_kernel = step + 1 < d->steps ? muon_product_kernel<T, kApply> : muon_product_kernel<T, kLast>;
+      hipLaunchKernelGGL((muon_product_kernel<T, kGram>), dim3(static_cast<unsigned>(at.sym)), dim3(kMuThreads), 0, stream,
+                         a, step);
+      hipLaunchKernelGGL((muon_product_kernel<T, kPoly>), dim3(static_cast<unsigned>(at.sym)), dim3(kMuThreads), 0, stream,
+                         a, step);
+      hipLaunchKernelGGL(apply_kernel, dim3(static_cast<unsigned>(at.apply)), dim3(kMuThreads), 0, stream, a, step);
+      if (const int rc = muon_launched()) return rc;
+    }
+  }
+  return ICTC_OK;
+}
+
+}  // namespace
+}  // namespace ictc
+
+extern "C" {
+
+int64_t ictc_hip_muon_workspace(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count) {
+  using namespace ictc;
+  if (!muon_valid(rows, cols, batches, count)) return -ICTC_ERR_INVALID_ARGUMENT;
+  return muon_workspace<kTile>(rows, cols, batches, count);
+}
+
+int ictc_hip_orthogonalize(const float* const* in, float* const* out, const int64_t* rows, const int64_t* cols,
+                           const int64_t* batches, int64_t count, const ictc_muon_desc* desc, void* workspace,
+                           int64_t workspace_bytes, hipStream_t stream) {
+  using namespace ictc;
+  if (!muon_valid(rows, cols, batches, count) || !muon_valid(desc, nullptr)) return ICTC_ERR_INVALID_ARGUMENT;
+  const int64_t need = muon_workspace<kTile>(rows, cols, batches, count);
+  if (need == 0) return ICTC_OK;
+  if (!in || !out || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < need)
+    return ICTC_ERR_INVALID_ARGUMENT;
+  for (int64_t k = 0; k < count; ++k)
+    if (rows[k] && cols[k] && batches[k] && (!in[k] || !out[k])) return ICTC_ERR_INVALID_ARGUMENT;
+  return muon_run<kTile>(in, nullptr, out, rows, cols, batches, count, desc, nullptr, nullptr,
+                         static_cast<char*>(workspace), workspace_bytes, stream);
+}
+
+int ictc_hip_muon_step(float* const* params, const float* const* grads, float* const* momentum, const int64_t* rows,
+                       const int64_t* cols, const int64_t* batches, int64_t count, const ictc_muon_desc* desc,
+                       const float* clip, const float* lr_device, void* workspace, int64_t workspace_bytes,
+                       hipStream_t stream) {
+  using namespace ictc;
+  if (!muon_valid(rows, cols, batches, count) || !muon_valid(desc, lr_device)) return ICTC_ERR_INVALID_ARGUMENT;
+  const int64_t need = muon_workspace<kTile>(rows, cols, batches, count);
+  if (need == 0) return ICTC_OK;
+  if (!params || !grads || !momentum || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+      workspace_bytes < need)
+    return ICTC_ERR_INVALID_ARGUMENT;
+  for (int64_t k = 0; k < count; ++k)
+    if (rows[k] && cols[k] && batches[k] && grads[k] && (!params[k] || !momentum[k])) return ICTC_ERR_INVALID_ARGUMENT;
+  return muon_run<kTile>(grads, momentum, params, rows, cols, batches, count, desc, clip, lr_device,
+                         static_cast<char*>(workspace), workspace_bytes, stream);
+}
+
+}  // extern "C"

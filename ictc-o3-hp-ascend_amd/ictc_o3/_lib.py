@@ -59,6 +59,20 @@ class AdamwDesc(ctypes.Structure):
     ]
 
 
+class MuonDesc(ctypes.Structure):
+    """Mirror of ``ictc_muon_desc``."""
+    _fields_ = [
+        ("beta", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("coefficients", ctypes.c_double * 3),
+        ("lr", ctypes.c_float),
+        ("nesterov", ctypes.c_int32),
+        ("steps", ctypes.c_int32),
+        ("adjust", ctypes.c_int32),
+    ]
+
+
 class NormDesc(ctypes.Structure):
     """Mirror of ``ictc_norm_desc``."""
     _fields_ = [
@@ -162,6 +176,14 @@ _SIGNATURES = {
                                                                _P]),
     "ictc_hip_layer_norm_second": (ctypes.c_int, [_P] * 10 + [_I64, ctypes.c_int, ctypes.c_int, ctypes.c_float, _I64,
                                                               _P]),
+    "ictc_hip_embedding_forward": (ctypes.c_int, [_P, ctypes.c_int, _P, _P, _I64, ctypes.c_int, ctypes.c_float, _I64,
+                                                  _P]),
+    "ictc_hip_embedding_workspace": (_I64, [_I64, ctypes.c_int, _I64]),
+    "ictc_hip_embedding_table_grad": (ctypes.c_int, [_P, ctypes.c_int, _P, _P, _I64, ctypes.c_int, ctypes.c_float, _I64,
+                                                     _P, _I64, _P]),
+    "ictc_hip_muon_workspace": (_I64, [_P, _P, _P, _I64]),
+    "ictc_hip_orthogonalize": (ctypes.c_int, [_P] * 5 + [_I64, ctypes.POINTER(MuonDesc), _P, _I64, _P]),
+    "ictc_hip_muon_step": (ctypes.c_int, [_P] * 6 + [_I64, ctypes.POINTER(MuonDesc), _P, _P, _P, _I64, _P]),
     "ictc_hip_sgemm": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _I64, _I64, _I64, ctypes.c_float, _P, _I64, _P,
                                       _I64, ctypes.c_float, _P, _I64, _P]),
     "ictc_hip_radius_graph_bins": (ctypes.c_int, [ctypes.POINTER(CellGrid), _P, _I64, _P, _P, _P, _P, _P, _P]),

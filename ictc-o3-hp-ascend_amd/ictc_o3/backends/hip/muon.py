@@ -1,0 +1,126 @@
+"""Orthogonalised updates of many matrices on ``libictc_hip.so`` (``ictc_hip_orthogonalize``,
+``ictc_hip_muon_step``; no counterpart in the reference, whose training loop uses torch's optimizers).  Formulas
+stand in ``ictc_hip.h``.
+
+Nothing here reads from the device or copies to it: the tensors' addresses are kernel arguments, and clipping
+coefficient and (where it is a tensor) the learning rate stay on the device, so a step can be captured into a
+HIP graph.  ``ictc_o3.optim.Muon`` is the optimizer on top.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from array import array
+
+import torch
+
+from ictc_o3 import _lib
+
+from .optimizer import _number, _on
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+MAX_STEPS = 64
+ADJUST = {"original": 0, "match_rms_adamw": 1}
+
+
+def _shapes(tensors, what: str):
+    """Rows, columns and numbers of matrices of tensors [..., rows, columns], as the arrays that the C entry
+    points take (and the three arrays themselves, which have to outlive the call)."""
+    rows, cols, batches = array("q"), array("q"), array("q")
+    for t in tensors:
+        shape = t.shape
+        if len(shape) < 2:
+            raise ValueError(f"{what} must be matrices (or have leading axes that count them)")
+        rows.append(shape[-2])
+        cols.append(shape[-1])
+        batches.append(math.prod(shape[:-2]))
+    return [(ctypes.c_int64 * len(a)).from_buffer(a) if len(a) else None for a in (rows, cols, batches)]
+
+
+def _desc(*, steps, coefficients, eps, beta=0.0, nesterov=False, weight_decay=0.0, lr=0.0, adjust="original"):
+    if isinstance(steps, bool) or not isinstance(steps, int) or not 1 <= steps <= MAX_STEPS:
+        raise ValueError(f"steps must be an integer in [1, {MAX_STEPS}]")
+    if len(coefficients) != 3 or not all(isinstance(c, (int, float)) and math.isfinite(c) for c in coefficients):
+        raise ValueError("coefficients must be three finite numbers")
+    if not _number(eps, "eps") > 0.0:
+        raise ValueError("eps must be positive")
+    if adjust not in ADJUST:
+        raise ValueError(f"adjust must be one of {sorted(ADJUST)}")
+    return _lib.MuonDesc(_number(beta, "beta", 1.0), _number(weight_decay, "weight_decay"), float(eps),
+                         (ctypes.c_double * 3)(*coefficients), _number(lr, "lr"), bool(nesterov), steps, ADJUST[adjust])
+
+
+def _workspace(shapes, count: int, device) -> torch.Tensor:
+    needed = int(_lib.lib().ictc_hip_muon_workspace(*shapes, count))
+    if needed < 0:
+        _lib.check(-needed, "ictc_hip_muon_workspace")
+    # (torch's allocations begin at multiples of 512 bytes)
+    return torch.empty(needed, device=device, dtype=torch.uint8)
+
+
+def orthogonalize(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
+    """Each matrix of a list (tensors [..., rows, columns], leading axes counting matrices) scaled to Frobenius norm
+    1 and brought near an orthogonal one by ``steps`` Newton-Schulz products, as a list of new tensors.  Without
+    gradients."""
+    with torch.no_grad():
+        matrices = list(matrices)
+        if not matrices:
+            return []
+        _, at, _, contiguous = _lib.host().addresses(matrices, "matrices")
+        shapes = _shapes(matrices, "matrices")
+        if not contiguous:
+            matrices = [m.contiguous() for m in matrices]
+            _, at, _, _ = _lib.host().addresses(matrices, "matrices")
+        desc = _desc(steps=steps, coefficients=coefficients, eps=eps)
+        out = [torch.empty_like(m, memory_format=torch.contiguous_format) for m in matrices]
+        n, device = len(matrices), matrices[0].device
+        to = _lib.host().addresses(out, "matrices")[1]
+        ws = _workspace(shapes, n, device)
+        with _on(device):
+            _lib.check(_lib.lib().ictc_hip_orthogonalize(at, to, *shapes, n, ctypes.byref(desc), _lib.ptr(ws), ws.numel(),
+                                                         _lib.stream_of(device)), "ictc_hip_orthogonalize")
+        return out
+
+
+def muon_step(params, grads, momentum, *, lr, beta: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+              steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7, adjust: str = "original", clip=None) -> None:
+    """One step of every parameter with a gradient, in place (a None gradient leaves its parameter and momentum as
+    they are): a moving average of the gradient, orthogonalised as ``orthogonalize`` does, as the update.  The
+    parameters are matrices (or have leading axes that count them); no two of them may overlap.
+
+    momentum: a list of float32 tensors of the parameters' shapes (zeros before the first step).  lr: a number, or a
+    one-element float32 tensor on the device.  adjust: the update's size, "original" for sqrt(max(1, rows / columns))
+    or "match_rms_adamw" for 0.2 sqrt(max(rows, columns)), which gives entries of AdamW's usual size.  clip:
+    ``gradient_norm``'s result, whose coefficient scales the gradients (not a number: nothing changes)."""
+    params, grads, momentum = list(params), list(grads), list(momentum)
+    host = _lib.host()
+    _, p_at, g_at, _, _, contiguous = host.pairs(params, grads, 1)
+    if not contiguous:
+        grads = [g if g is None else g.contiguous() for g in grads]
+        _, p_at, g_at, _, _, _ = host.pairs(params, grads, 1)
+    n, device = len(params), params[0].device
+    shapes = _shapes(params, "parameters")
+    m_device, m_at, _, contiguous = host.addresses(momentum, "momentum")
+    if len(momentum) != n or not contiguous or m_device != device.index \
+            or any(m.shape != p.shape for m, p in zip(momentum, params)):
+        raise ValueError("momentum must hold a contiguous tensor of each parameter's shape beside the parameters")
+    if clip is not None and (clip.dtype is not torch.float32 or clip.shape != (2,) or clip.device != device
+                             or not clip.is_contiguous()):
+        raise ValueError("clip must be gradient_norm's result")
+    lr_device = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.device != device:
+            raise ValueError("a learning rate tensor must hold one FP32 value beside the parameters")
+        lr_device, lr = lr.data_ptr(), 0.0
+    desc = _desc(steps=steps, coefficients=coefficients, eps=eps, beta=beta, nesterov=nesterov,
+                 weight_decay=weight_decay, lr=lr, adjust=adjust)
+    if all(g is None for g in grads):
+        return
+    ws = _workspace(shapes, n, device)
+    with _on(device):
+        _lib.check(_lib.lib().ictc_hip_muon_step(p_at, g_at, m_at, *shapes, n, ctypes.byref(desc), _lib.ptr(clip),
+                                                 lr_device, _lib.ptr(ws), ws.numel(), _lib.stream_of(device)),
+                   "ictc_hip_muon_step")
+    # the kernels write through addresses: tell autograd (and caches keyed on versions) of the change
+    host.written(params, grads)
+    host.written(momentum, grads)

@@ -9,8 +9,10 @@ from __future__ import annotations
 
 import torch
 
+from ictc_o3.backends.hip.embedding import embedding
 from ictc_o3.backends.hip.layer_norm import layer_norm
 from ictc_o3.backends.hip.linear import channel_linear, species_channel_linear
+from ictc_o3.backends.hip.muon import muon_step, orthogonalize
 from ictc_o3.backends.hip.norms import equivariant_norm, gated_residual_norm
 from ictc_o3.backends.hip.optimizer import adamw_step, gradient_norm, moment_values
 from ictc_o3.backends.hip.runtime import require_gpu_fp32, strict_fp32
@@ -281,5 +283,6 @@ def normalized_silu(features, scale=1.):
 __all__ = ["EdgeTensorProduct", "PackedGraphMessage", "GraphMessage", "direction_harmonics",
            "create_symmetric_contraction", "configure_symmetric_contraction",
            "channel_linear", "species_channel_linear", "normalized_silu", "strict_fp32",
-           "gradient_norm", "adamw_step", "moment_values",
-           "equivariant_norm", "gated_residual_norm", "layer_norm"]
+           "gradient_norm", "adamw_step", "moment_values", "orthogonalize", "muon_step",
+           "equivariant_norm", "gated_residual_norm", "layer_norm",
+           "embedding"]

@@ -817,6 +817,66 @@ int ictc_hip_layer_norm_second(const float* x, const float* weight, const float*
                                int64_t rows, hipStream_t stream);
 
 /*
+ * Rows of a table [rows, width] by token, times a scale, and the gradient of the table (the reference's species
+ * embedding is a product with one-hot rows, mace_ictc/models/pure_cartesian_ictd_fix.py:3008-3011):
+ *   out[i] = scale table[t_i]            dtable[v] = scale sum over {i : t_i = v} of grad[i]
+ * The two maps are each other's adjoint.  Tokens are 4- or 8-byte signed integers (index_bytes); one outside
+ * [0, rows) has a row of zeros and no gradient.  dtable is written whole, its sums in a fixed order.  count may be
+ * 0 for the forward pass only.  workspace: ictc_hip_embedding_workspace(rows, width, count) units of 4 bytes
+ * (negative: -ictc_status), 16-byte aligned.  1 <= rows < 2^31 - 1, 1 <= width <= 2^20, count < 2^31 - 4096.
+ */
+int ictc_hip_embedding_forward(const void* tokens, int index_bytes, const float* table, float* out, int64_t rows,
+                               int width, float scale, int64_t count, hipStream_t stream);
+int64_t ictc_hip_embedding_workspace(int64_t rows, int width, int64_t count);
+int ictc_hip_embedding_table_grad(const void* tokens, int index_bytes, const float* grad, float* dtable, int64_t rows,
+                                  int width, float scale, int64_t count, void* workspace, int64_t workspace_units,
+                                  hipStream_t stream);
+
+/*
+ * Orthogonalised updates of matrices (no counterpart in the reference).  A matrix U [m, n] is scaled to
+ * X = U / (|U| + eps), |U| the Frobenius norm, and goes through `steps` of
+ *   X <- a X + (b A + c A A) X,  A = X X^T        (a, b, c) = coefficients; m > n: of the transposed matrix
+ * which brings its singular values near 1.  Products are of float32 accuracy (operands in two float16 parts).
+ *
+ * Host arrays of `count` tensors, each of `batches` contiguous matrices of rows x cols; device addresses in them
+ * are read before the call returns.
+ *
+ * ictc_hip_orthogonalize: out[i] = X of in[i] (they may be the same).
+ *
+ * ictc_hip_muon_step: for every tensor with a gradient (a null one is left out), with g = clip[1] grad (clip null: grad),
+ *   M <- beta M + (1 - beta) g      U = nesterov ? beta M + (1 - beta) g : M
+ *   P <- (1 - lr weight_decay) P - lr s X(U)
+ *   s = sqrt(max(1, rows / cols)) (ICTC_MUON_SHAPE) or 0.2 sqrt(max(rows, cols)) (ICTC_MUON_MATCH_RMS)
+ * A clip[1] that is not a number leaves everything as it is.  lr_device, if not null, is one float on the device
+ * that takes the place of desc->lr.  No two tensors may overlap.
+ *
+ * workspace: ictc_hip_muon_workspace(rows, cols, batches, count) bytes (negative: -ictc_status), 256-byte aligned.
+ */
+#define ICTC_MUON_SHAPE 0
+#define ICTC_MUON_MATCH_RMS 1
+#define ICTC_MUON_MAX_STEPS 64
+
+typedef struct ictc_muon_desc {
+    double beta;               /* [0, 1) */
+    double weight_decay;       /* >= 0 */
+    double eps;                /* > 0 */
+    double coefficients[3];
+    float lr;                  /* >= 0 */
+    int32_t nesterov;
+    int32_t steps;             /* [0, ICTC_MUON_MAX_STEPS] */
+    int32_t adjust;            /* ICTC_MUON_SHAPE or ICTC_MUON_MATCH_RMS */
+} ictc_muon_desc;
+
+int64_t ictc_hip_muon_workspace(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count);
+int ictc_hip_orthogonalize(const float* const* in, float* const* out, const int64_t* rows, const int64_t* cols,
+                           const int64_t* batches, int64_t count, const ictc_muon_desc* desc, void* workspace,
+                           int64_t workspace_bytes, hipStream_t stream);
+int ictc_hip_muon_step(float* const* params, const float* const* grads, float* const* momentum, const int64_t* rows,
+                       const int64_t* cols, const int64_t* batches, int64_t count, const ictc_muon_desc* desc,
+                       const float* clip, const float* lr_device, void* workspace, int64_t workspace_bytes,
+                       hipStream_t stream);
+
+/*
  * Row-major fp32 product C[m,n] = alpha * op(A) op(B) + beta * C on rocBLAS, for the dense
  * channel linears around the operators.  op(A) is [m,k]: A is stored [m,k] (lda >= k) or,
  * with trans_a != 0, [k,m] (lda >= m); likewise B with op(B) [k,n].  Each host thread uses
