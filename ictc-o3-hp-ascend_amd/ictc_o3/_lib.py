@@ -18,6 +18,7 @@ import torch  # noqa: F401  (must precede CDLL, see module docstring)
 MAX_PATHS = 128
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libictc_hip.so")
 HOST_PATH = os.path.join(os.path.dirname(LIB_PATH), "ictc_host_tensors.so")
+LAYERS_PATH = os.path.join(os.path.dirname(LIB_PATH), "ictc_host_layers.so")
 ABI_VERSION = 28
 
 
@@ -227,6 +228,18 @@ def lib() -> ctypes.CDLL:
 
 
 _host = None
+_layers = None
+
+
+def _module(name: str, path: str):
+    """A host module that was built beside the library."""
+    if not os.path.isfile(path):
+        raise RuntimeError(f"{os.path.basename(path)} not found beside {LIB_PATH}; build it with "
+                           "`python ictc-o3-hp-ascend_amd/csrc/build.py`")
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+    loader.exec_module(module)
+    return module
 
 
 def host():
@@ -236,15 +249,30 @@ def host():
         return _host
     with _lock:
         if _host is None:
-            if not os.path.isfile(HOST_PATH):
-                raise RuntimeError(f"{os.path.basename(HOST_PATH)} not found beside {LIB_PATH}; build it with "
-                                   "`python ictc-o3-hp-ascend_amd/csrc/build.py`")
-            loader = importlib.machinery.ExtensionFileLoader("ictc_host_tensors", HOST_PATH)
-            spec = importlib.util.spec_from_loader("ictc_host_tensors", loader)
-            module = importlib.util.module_from_spec(spec)
-            loader.exec_module(module)
-            _host = module
+            _host = _module("ictc_host_tensors", HOST_PATH)
     return _host
+
+
+_LAYER_ENTRIES = ("ictc_hip_status_string", "ictc_hip_layer_norm_workspace", "ictc_hip_layer_norm_forward",
+                  "ictc_hip_layer_norm_backward", "ictc_hip_layer_norm_second", "ictc_hip_embedding_forward",
+                  "ictc_hip_embedding_workspace", "ictc_hip_embedding_table_grad")
+
+
+def layers():
+    """The host module of the layers' autograd nodes (``csrc/host_layers.cpp``), opened once and bound to the
+    library."""
+    global _layers
+    if _layers is not None:
+        return _layers
+    from ictc_o3.backends.hip.layer_norm import composed_gradients
+    handle = lib()
+    with _lock:
+        if _layers is None:
+            module = _module("ictc_host_layers", LAYERS_PATH)
+            module.bind(*[ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in _LAYER_ENTRIES],
+                        composed_gradients)
+            _layers = module
+    return _layers
 
 
 def check(status: int, what: str) -> None:
