@@ -15,10 +15,14 @@
 // A alone and multiplies X once has a third of the work for wide matrices, but doubles the error's growth: singular values
 // below 1e-3 of the largest come out wrong, 1e-4 of the result at rank-deficient matrices.)
 //
-// All three products are of the form P Q^T with both operands' rows along the reduction (X X^T, A A^T, B (X^T)^T), so
+// Matrices with a side of more than 128 (below: the shorter side): all three products are of the form P Q^T with both operands' rows along the reduction (X X^T, A A^T, B (X^T)^T), so
 // one kernel does them; X is kept in both orientations.  A and B are symmetric: only tiles on and above the diagonal
 // are computed.  Every matrix of every tensor takes part in the same launches: `owner` says which matrix a workgroup's
 // tile belongs to.  Sides are padded with zeros to whole tiles, which stay zero.
+//
+// Matrices with a shorter side of up to 128, of which most models have most: two launches a step, bound by latency.  A
+// workgroup keeps 64 columns of X at a time: it multiplies them by B, and adds what they give to the next X X^T at once,
+// from LDS; the other launch, one workgroup to a matrix, adds these parts up in order, and makes A A and B.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -30,7 +34,7 @@ namespace {
 
 constexpr int kMuThreads = 256;
 constexpr int kMuWave = 64;
-constexpr int kTensorsPerLaunch = 48;        // of the table in the kernel's arguments
+constexpr int kTensorsPerLaunch = 44;        // of the table in the kernel's arguments
 constexpr int kPrep = 64;                    // side of a tile of the source
 constexpr int kStep = 32;                    // reduction entries in LDS at a time
 constexpr int64_t kMostBytes = int64_t{2} << 30;     // workspace that a call goes by, unless one tensor needs more
@@ -50,7 +54,7 @@ struct MuonTensor {
   float* out;                // parameter, or the result
   int64_t base;              // of the first matrix, in bytes of the workspace
   int32_t rows, cols, batches, first;          // first: index of the first matrix
-  uint32_t prep, sym, apply;                   // first tile of each kind
+  uint32_t prep, sym, apply, chunk;            // first tile (or chunk of columns) of each kind
   float rate;                // of the update, times the learning rate
 };
 
@@ -60,21 +64,24 @@ struct MuonTable {
 
 static_assert(sizeof(MuonTable) + 128 <= 4096, "kernel arguments are limited to 4 KB");
 
-// One matrix, in the workspace.
+// One matrix, in the workspace.  With a shorter side of up to 128: X^T [np][mp], two planes; B [mp][mp]; the parts of
+// X X^T.  Else: X [mp][np], two planes; then X^T twice [np][mp], A and B [mp][mp].
 struct MuonMatrix {
   const float* src;
   float* momentum;
   float* out;
-  char* x;                   // X [mp][np], two planes; then X^T twice [np][mp], A and B [mp][mp]
+  char* x;
   int32_t rows, cols, mp, np;
-  uint32_t prep, prep_tiles, sym, apply;
+  uint32_t prep, prep_tiles, prep_across;      // tiles of the source
+  uint32_t sym, apply;                         // tiles of products
+  uint32_t chunk, chunks, chunk_parts;         // chunks of columns, of `chunk_parts` times 64
   float rate;
-  int32_t transposed;        // more rows than columns
+  int32_t transposed;                          // more rows than columns
 };
 
 struct MuonArgs {
   const MuonMatrix* matrices;
-  const uint32_t *prep_owner, *sym_owner, *apply_owner;
+  const uint32_t *prep_owner, *sym_owner, *apply_owner, *chunk_owner;
   double* squares;           // of each tile of the source
   int32_t* exponents;        // of each matrix: X is kept times 2^e at first
   const float* clip;
@@ -89,20 +96,41 @@ __device__ __forceinline__ bool skipped(const MuonArgs& a) { return a.clip && a.
 
 constexpr int64_t up_to(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Tiles and bytes of one matrix, with sides padded to multiples of T.
+constexpr int kShort = 128;                  // shorter sides of matrices that are done in chunks of columns
+constexpr int kPart = 64;                    // columns in LDS at a time
+constexpr int kChunks = 24;                  // of a matrix, unless they get longer than kLongest parts
+constexpr int kLongest = 8;
+
+// Tiles and bytes of one matrix; sides padded to multiples of T, or for short ones to 32, 64 or 128 and kPart.
 struct MuonSize {
-  int64_t mp, np, prep, sym, apply, bytes;
+  bool is_short;
+  int64_t mp, np, prep, across, sym, apply, chunks, parts, bytes;
 };
 
 template <int T>
 __host__ __device__ MuonSize muon_size(int64_t rows, int64_t cols) {
   MuonSize s;
   const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  s.is_short = m <= kShort;
+  if (s.is_short) {
+    s.mp = m <= 32 ? 32 : m <= 64 ? 64 : 128, s.np = up_to(n, kPart);
+    s.across = (cols + kPrep - 1) / kPrep;
+    s.prep = (rows + kPrep - 1) / kPrep * s.across;
+    const int64_t all = s.np / kPart, blocks = s.mp / 32;
+    s.parts = (all + kChunks - 1) / kChunks;
+    if (s.parts > kLongest) s.parts = kLongest;
+    s.chunks = (all + s.parts - 1) / s.parts;
+    s.sym = s.apply = 0;
+    s.bytes = up_to(4 * s.np * s.mp + 4 * s.mp * s.mp + s.chunks * (blocks * (blocks + 1) / 2) * 4096, 256);
+    return s;
+  }
   s.mp = up_to(m, T), s.np = up_to(n, T);
+  s.across = (rows > cols ? s.mp : s.np) / kPrep;
   s.prep = (s.mp / kPrep) * (s.np / kPrep);
   const int64_t i = s.mp / T, j = s.np / T;
   s.sym = i * (i + 1) / 2;
   s.apply = i * j;
+  s.chunks = s.parts = 0;
   s.bytes = 12 * s.mp * s.np + 8 * s.mp * s.mp;
   return s;
 }
@@ -111,7 +139,8 @@ __host__ __device__ MuonSize muon_size(int64_t rows, int64_t cols) {
 template <int T>
 __global__ void __launch_bounds__(kMuThreads)
 muon_setup_kernel(const MuonTable table, char* __restrict__ workspace, MuonMatrix* __restrict__ matrices,
-                  uint32_t* __restrict__ prep_owner, uint32_t* __restrict__ sym_owner, uint32_t* __restrict__ apply_owner) {
+                  uint32_t* __restrict__ prep_owner, uint32_t* __restrict__ sym_owner, uint32_t* __restrict__ apply_owner,
+                  uint32_t* __restrict__ chunk_owner) {
   const MuonTensor& t = table.tensor[blockIdx.x];
   const MuonSize s = muon_size<T>(t.rows, t.cols);
   const int64_t values = static_cast<int64_t>(t.rows) * t.cols;
@@ -123,18 +152,23 @@ muon_setup_kernel(const MuonTable table, char* __restrict__ workspace, MuonMatri
     m.x = workspace + t.base + b * s.bytes;
     m.rows = t.rows, m.cols = t.cols, m.mp = static_cast<int32_t>(s.mp), m.np = static_cast<int32_t>(s.np);
     m.prep = t.prep + static_cast<uint32_t>(b * s.prep), m.prep_tiles = static_cast<uint32_t>(s.prep);
+    m.prep_across = static_cast<uint32_t>(s.across);
     m.sym = t.sym + static_cast<uint32_t>(b * s.sym);
     m.apply = t.apply + static_cast<uint32_t>(b * s.apply);
+    m.chunk = t.chunk + static_cast<uint32_t>(b * s.chunks), m.chunks = static_cast<uint32_t>(s.chunks);
+    m.chunk_parts = static_cast<uint32_t>(s.parts);
     m.rate = t.rate;
     m.transposed = t.rows > t.cols;
     matrices[t.first + b] = m;
   }
-  for (int64_t k = threadIdx.x; k < t.batches * s.prep; k += kMuThreads)
-    prep_owner[t.prep + k] = t.first + static_cast<uint32_t>(k / s.prep);
-  for (int64_t k = threadIdx.x; k < t.batches * s.sym; k += kMuThreads)
-    sym_owner[t.sym + k] = t.first + static_cast<uint32_t>(k / s.sym);
-  for (int64_t k = threadIdx.x; k < t.batches * s.apply; k += kMuThreads)
-    apply_owner[t.apply + k] = t.first + static_cast<uint32_t>(k / s.apply);
+  const auto own = [&](uint32_t* owner, uint32_t first, int64_t each) {
+    for (int64_t k = threadIdx.x; k < t.batches * each; k += kMuThreads)
+      owner[first + k] = t.first + static_cast<uint32_t>(k / each);
+  };
+  own(prep_owner, t.prep, s.prep);
+  own(sym_owner, t.sym, s.sym);
+  own(apply_owner, t.apply, s.apply);
+  own(chunk_owner, t.chunk, s.chunks);
 }
 
 // A tile of the source: its first row and column there, and what of it there is.
@@ -142,9 +176,8 @@ struct SourceTile {
   int r0, c0, rows, cols;
 
   __device__ __forceinline__ SourceTile(const MuonMatrix& m, uint32_t tile) {
-    const int across = (m.transposed ? m.mp : m.np) / kPrep;
-    r0 = static_cast<int>(tile / across) * kPrep;
-    c0 = static_cast<int>(tile % across) * kPrep;
+    r0 = static_cast<int>(tile / m.prep_across) * kPrep;
+    c0 = static_cast<int>(tile % m.prep_across) * kPrep;
     rows = m.rows - r0 < 0 ? 0 : m.rows - r0 > kPrep ? kPrep : m.rows - r0;
     cols = m.cols - c0 < 0 ? 0 : m.cols - c0 > kPrep ? kPrep : m.cols - c0;
   }
@@ -167,27 +200,63 @@ __device__ __forceinline__ float averaged(const MuonArgs& a, float m, float g) {
   return a.beta * m + a.rest * g;
 }
 
-// Moving averages, and the sum of squares (in 64 bits) of each tile of what is orthogonalised.
+// Four values of a row at any alignment, or the `count` that there are (zeros for the rest).
+__device__ __forceinline__ mf4 load_quad(const float* p, int count) {
+  mf4 v = {0.f, 0.f, 0.f, 0.f};
+  if (count >= 4) return *reinterpret_cast<const mf4*>(p);
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (j < count) v[j] = p[j];
+  return v;
+}
+
+__device__ __forceinline__ void store_quad(float* p, int count, const mf4& v) {
+  if (count >= 4) {
+    *reinterpret_cast<mf4*>(p) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < count) p[j] = v[j];
+  }
+}
+
+constexpr int kQuadRows = kMuThreads / (kPrep / 4), kPasses = kPrep / kQuadRows;   // a tile's rows at a time, and times
+
+// Moving averages, and the sum of squares (in 64 bits) of each tile of what is orthogonalised.  Bound by memory: 12
+// bytes a value (momentum read and written, gradient read); all loads before the first store.
 __global__ void __launch_bounds__(kMuThreads) muon_average_kernel(const MuonArgs a) {
   __shared__ double part[kMuThreads / kMuWave];
   if (skipped(a)) return;
   const MuonMatrix m = a.matrices[a.prep_owner[blockIdx.x]];
   const SourceTile t(m, blockIdx.x - m.prep);
   const float scale = a.clip ? a.clip[1] : 1.f;
-  const int column = threadIdx.x % kPrep;
+  const int column = threadIdx.x % (kPrep / 4) * 4, count = t.cols - column, first = threadIdx.x / (kPrep / 4);
+  const int64_t from = static_cast<int64_t>(t.r0 + first) * m.cols + t.c0 + column;
+  mf4 u[kPasses], old[kPasses];
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    const int64_t at = from + static_cast<int64_t>(k * kQuadRows) * m.cols;
+    const int there = first + k * kQuadRows < t.rows ? count : 0;
+    u[k] = load_quad(m.src + at, there);
+    if (m.momentum) old[k] = load_quad(m.momentum + at, there);
+  }
   double sum = 0.0;
-  if (column < t.cols)
-    for (int r = threadIdx.x / kPrep; r < t.rows; r += kMuThreads / kPrep) {
-      const int64_t at = static_cast<int64_t>(t.r0 + r) * m.cols + t.c0 + column;
-      float u = m.src[at];
-      if (m.momentum) {
-        const float g = scale * u;
-        u = averaged(a, m.momentum[at], g);
-        m.momentum[at] = u;
-        if (a.nesterov) u = averaged(a, u, g);
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    if (m.momentum) {
+      mf4 g = u[k];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        g[j] *= scale;
+        old[k][j] = u[k][j] = averaged(a, old[k][j], g[j]);
+        if (a.nesterov) u[k][j] = averaged(a, u[k][j], g[j]);
       }
-      sum += static_cast<double>(u) * static_cast<double>(u);
+      store_quad(m.momentum + from + static_cast<int64_t>(k * kQuadRows) * m.cols,
+                 first + k * kQuadRows < t.rows ? count : 0, old[k]);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += static_cast<double>(u[k][j]) * static_cast<double>(u[k][j]);
+  }
   sum = muon_block_sum(sum, part);
   if (threadIdx.x == 0) a.squares[blockIdx.x] = sum;
 }
@@ -212,6 +281,33 @@ __device__ __forceinline__ int exponent_at(const MuonArgs& a, int e, int step) {
   return e;
 }
 
+// What a matrix's values are multiplied by at first (its power of two among it), from its tiles' squares; every
+// workgroup of the matrix calls it, and the one that is told to keeps the exponent.
+__device__ __forceinline__ double first_scale(const MuonArgs& a, const MuonMatrix& m, uint32_t owner, bool keeps,
+                                              double* part) {
+  double sum = 0.0;
+  for (uint32_t k = threadIdx.x; k < m.prep_tiles; k += kMuThreads) sum += a.squares[m.prep + k];
+  const double norm = sqrt(muon_block_sum(sum, part)), share = norm / (norm + a.eps);
+  const int e = share > 0.0 && share < 0.5 ? min(-ilogb(share) - 1, kMostExponent) : 0;
+  if (threadIdx.x == 0 && keeps) a.exponents[owner] = e;
+  return ldexp(1.0 / (norm + a.eps), e);
+}
+
+// Values of what is orthogonalised, from the source and (after muon_average_kernel) the moving average.
+struct Source {
+  mf4 g, m;
+
+  __device__ __forceinline__ void load(const MuonArgs& a, const MuonMatrix& m_, int64_t at, int count) {
+    if (!m_.momentum || a.nesterov) g = load_quad(m_.src + at, count);
+    if (m_.momentum) m = load_quad(m_.momentum + at, count);
+  }
+
+  __device__ __forceinline__ float value(const MuonArgs& a, const MuonMatrix& m_, int j, float scale, double inv) const {
+    const float u = !m_.momentum ? g[j] : a.nesterov ? averaged(a, m[j], scale * g[j]) : m[j];
+    return static_cast<float>(u * inv);
+  }
+};
+
 // X in both orientations from the source: tiles go through LDS.
 __global__ void __launch_bounds__(kMuThreads) muon_normalise_kernel(const MuonArgs a) {
   __shared__ double part[kMuThreads / kMuWave];
@@ -220,24 +316,19 @@ __global__ void __launch_bounds__(kMuThreads) muon_normalise_kernel(const MuonAr
   const uint32_t owner = a.prep_owner[blockIdx.x];
   const MuonMatrix m = a.matrices[owner];
   const SourceTile t(m, blockIdx.x - m.prep);
-  double sum = 0.0;
-  for (uint32_t k = threadIdx.x; k < m.prep_tiles; k += kMuThreads) sum += a.squares[m.prep + k];
-  const double norm = sqrt(muon_block_sum(sum, part)), share = norm / (norm + a.eps);
-  const int e = share > 0.0 && share < 0.5 ? min(-ilogb(share) - 1, kMostExponent) : 0;
-  if (threadIdx.x == 0 && blockIdx.x == m.prep) a.exponents[owner] = e;
-  const double inv = ldexp(1.0 / (norm + a.eps), e);
-  const float scale = a.clip ? a.clip[1] : 1.f;
-  const int column = threadIdx.x % kPrep;
-  for (int r = threadIdx.x / kPrep; r < kPrep; r += kMuThreads / kPrep) {
-    float u = 0.f;
-    if (r < t.rows && column < t.cols) {
-      const int64_t at = static_cast<int64_t>(t.r0 + r) * m.cols + t.c0 + column;
-      u = m.src[at];
-      if (m.momentum) u = a.nesterov ? averaged(a, m.momentum[at], scale * u) : m.momentum[at];
-      u = static_cast<float>(u * inv);
-    }
-    tile[r][column] = u;
+  const int column = threadIdx.x % (kPrep / 4) * 4, first = threadIdx.x / (kPrep / 4);
+  Source source[kPasses];
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    const int r = first + k * kQuadRows;
+    source[k].load(a, m, static_cast<int64_t>(t.r0 + r) * m.cols + t.c0 + column, r < t.rows ? t.cols - column : 0);
   }
+  const double inv = first_scale(a, m, owner, blockIdx.x == m.prep, part);
+  const float scale = a.clip ? a.clip[1] : 1.f;
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tile[first + k * kQuadRows][column + j] = source[k].value(a, m, j, scale, inv);
   __syncthreads();
   const int64_t plane = static_cast<int64_t>(m.mp) * m.np;
   _Float16* const x = reinterpret_cast<_Float16*>(m.x);
@@ -262,7 +353,43 @@ __global__ void __launch_bounds__(kMuThreads) muon_normalise_kernel(const MuonAr
   }
 }
 
-enum MuonPhase { kGram, kPoly, kApply, kLast };
+enum MuonPhase { kGram, kPoly, kApply, kLast, kFirst };
+
+// The power of two that a product's results are multiplied by.
+template <int PHASE>
+__device__ __forceinline__ int shift_of(const MuonArgs& a, uint32_t owner, int step) {
+  if constexpr (PHASE == kPoly || PHASE == kFirst) return 0;
+  const int first = a.exponents[owner];
+  if (!first) return 0;
+  const int e = exponent_at(a, first, step);
+  return PHASE == kGram ? -2 * e : PHASE == kApply ? exponent_at(a, first, step + 1) - e : -e;
+}
+
+// The last step's results: the matrix itself, or a parameter's update.
+struct Update {
+  float keep = 1.f, rate = 0.f;
+
+  __device__ __forceinline__ Update() {}
+  __device__ __forceinline__ Update(const MuonArgs& a, const MuonMatrix& m) {
+    if (!m.momentum) return;
+    const float lr = a.lr_device ? *a.lr_device : a.lr;
+    keep = static_cast<float>(1.0 - static_cast<double>(lr) * a.weight_decay);
+    rate = lr * m.rate;
+  }
+
+  // Rows row .. row + 3 (along the shorter side) of a column.
+  __device__ __forceinline__ void write(const MuonMatrix& m, int row, int column, const float (&v)[4]) const {
+    const int shorter = m.transposed ? m.cols : m.rows, longer = m.transposed ? m.rows : m.cols;
+    if (column >= longer) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (row + r < shorter) {
+        float* to = m.out + (m.transposed ? static_cast<int64_t>(column) * m.cols + row + r
+                                          : static_cast<int64_t>(row + r) * m.cols + column);
+        *to = m.momentum ? keep * *to - rate * v[r] : v[r];
+      }
+  }
+};
 
 // 16 bytes a lane from global memory to consecutive places of LDS.
 __device__ __forceinline__ void load_to_lds(const _Float16* from, _Float16* to) {
@@ -358,22 +485,8 @@ __global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs
   }
 
   // A lane holds rows 8 (k / 4) + 4 (lane / 32) + k % 4 of column lane % 32 of each 32 x 32 product.
-  int shift = 0;                                   // of the result's power of two
-  if constexpr (PHASE != kPoly) {
-    const int first = a.exponents[owner];
-    if (first) {
-      const int e = exponent_at(a, first, step);
-      shift = PHASE == kGram ? -2 * e : PHASE == kApply ? exponent_at(a, first, step + 1) - e : -e;
-    }
-  }
-  float keep = 1.f, rate = 0.f;
-  if constexpr (PHASE == kLast) {
-    if (m.momentum) {
-      const float lr = a.lr_device ? *a.lr_device : a.lr;
-      keep = static_cast<float>(1.0 - static_cast<double>(lr) * a.weight_decay);
-      rate = lr * m.rate;
-    }
-  }
+  const int shift = shift_of<PHASE>(a, owner, step);
+  const Update update = PHASE == kLast ? Update(a, m) : Update();
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -399,16 +512,7 @@ __global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs
           for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], shift);
         }
         if constexpr (PHASE == kLast) {
-          const int shorter = m.transposed ? m.cols : m.rows, longer = m.transposed ? m.rows : m.cols;
-          if (column < longer) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (row + r < shorter) {
-                float* to = m.out + (m.transposed ? static_cast<int64_t>(column) * m.cols + row + r
-                                                  : static_cast<int64_t>(row + r) * m.cols + column);
-                *to = m.momentum ? keep * *to - rate * v[r] : v[r];
-              }
-          }
+          update.write(m, row, column, v);
         } else {
           _Float16* const turned = PHASE == kGram ? gram : PHASE == kPoly ? poly : xt_next;      // [column][row]
           _Float16* const plain = PHASE == kGram ? gram : PHASE == kPoly ? poly : x;             // [row][column]
@@ -433,6 +537,305 @@ __global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs
       }
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// Matrices with a shorter side of up to 128
+// ---------------------------------------------------------------------------------------------------------
+
+// Where the group of 8 halves `group` of row `row` lies in LDS, rows of `groups` such groups: turned with the row, so
+// that the groups that 8 lanes read fill all banks.
+__device__ __forceinline__ int turned_at(int row, int group, int groups) {
+  return (row * groups + (groups == 4 ? group ^ ((row >> 1) & 3) : group ^ (row & 7))) * 8;
+}
+
+// Block `b` of the upper triangle, column by column.
+__device__ __forceinline__ void upper_block(int b, int& i, int& j) {
+  j = b >= 6 ? 3 : b >= 3 ? 2 : b >= 1 ? 1 : 0;
+  i = b - j * (j + 1) / 2;
+}
+
+__device__ __forceinline__ void three_products(const half8& ah, const half8& al, const half8& bh, const half8& bl,
+                                               f32x16& high, f32x16& low) {
+  high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, high, 0, 0, 0);
+  low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, low, 0, 0, 0);
+  low = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, low, 0, 0, 0);
+}
+
+// LDS of a chunk's workgroup: 64 columns of X, their rows along the columns (as they lie in memory), and along the rows.
+struct ShortLds {
+  _Float16 xt[2][kPart * kShort];
+  _Float16 x[2][kShort * kPart];
+  double part[kMuThreads / kMuWave];
+};
+
+// The products of one chunk of columns, MB x 32 rows (see the top).  kFirst: the columns come from the source.
+template <int PHASE, int MB>
+__device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix& m, uint32_t owner, int step,
+                                            ShortLds& lds) {
+  constexpr int M = 32 * MB, kGroups = M / 8, kBlocks = MB * (MB + 1) / 2, kMine = (kBlocks + 3) / 4;
+  constexpr int kTiles = MB == 4 ? 2 : 1;          // 32 x 32 products of a wave
+  const int lane = threadIdx.x & (kMuWave - 1), wave = threadIdx.x / kMuWave, half = lane / 32;
+  const int64_t plane = static_cast<int64_t>(m.np) * M;
+  _Float16* const xt = reinterpret_cast<_Float16*>(m.x);
+  const _Float16* const poly = xt + 2 * plane;
+  const uint32_t chunk = blockIdx.x - m.chunk;
+  const int first = static_cast<int>(chunk * m.chunk_parts), all = m.np / kPart;
+  const int end = first + static_cast<int>(m.chunk_parts) < all ? first + static_cast<int>(m.chunk_parts) : all;
+  const int row0 = (MB == 4 ? wave : MB == 2 ? wave & 1 : 0) * 32;                  // of a wave's products
+  const int col0 = (MB == 4 ? 0 : MB == 2 ? wave >> 1 : wave) * 32;
+  const bool works = MB > 1 || wave < 2;
+
+  double inv = 0.0;
+  float scale = 1.f;
+  if constexpr (PHASE == kFirst) {
+    if (a.clip) scale = a.clip[1];
+  }
+  half8 b_op[2][PHASE == kFirst ? 1 : M / 16];
+  if constexpr (PHASE != kFirst) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int k = 0; k < M / 16; ++k)
+        b_op[p][k] = *reinterpret_cast<const half8*>(poly + p * M * M + (row0 + (lane & 31)) * M + k * 16 + half * 8);
+  }
+  const int shift = shift_of<PHASE>(a, owner, step);
+  const Update update = PHASE == kLast ? Update(a, m) : Update();
+  f32x16 gram_high[kMine] = {}, gram_low[kMine] = {};
+
+  for (int part = first; part < end; ++part) {
+    const int64_t at = static_cast<int64_t>(part) * kPart * M;       // of the columns in X^T
+    if constexpr (PHASE == kFirst) {
+      // rows of the source: of the matrix, or (transposed) of its columns; four values of one at a time
+      constexpr int kQuads = M * kPart / 4 / kMuThreads;
+      Source source[kQuads];
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) {
+        const int k = q * kMuThreads + threadIdx.x;
+        const int i = m.transposed ? k / (M / 4) + part * kPart : k / (kPart / 4);
+        const int j = m.transposed ? k % (M / 4) * 4 : k % (kPart / 4) * 4 + part * kPart;
+        source[q].load(a, m, static_cast<int64_t>(i) * m.cols + j, i < m.rows ? m.cols - j : 0);
+      }
+      if (part == first) inv = first_scale(a, m, owner, chunk == 0, lds.part);
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) {
+        const int k = q * kMuThreads + threadIdx.x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = m.transposed ? k % (M / 4) * 4 + r : k / (kPart / 4);        // of X
+          const int j = m.transposed ? k / (M / 4) : k % (kPart / 4) * 4 + r;
+          _Float16 h, l;
+          split(source[q].value(a, m, r, scale, inv), h, l);
+          const int in_x = turned_at(i, j / 8, kPart / 8) + j % 8, in_xt = turned_at(j, i / 8, kGroups) + i % 8;
+          lds.x[0][in_x] = h, lds.x[1][in_x] = l;
+          lds.xt[0][in_xt] = h, lds.xt[1][in_xt] = l;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        for (int k = threadIdx.x; k < kPart * kGroups; k += kMuThreads)
+          *reinterpret_cast<half8*>(xt + p * plane + at + k * 8) =
+              *reinterpret_cast<const half8*>(&lds.xt[p][turned_at(k / kGroups, k % kGroups, kGroups)]);
+    } else {
+      // a wave's load fills 64 groups of a plane
+#pragma unroll
+      for (int k = 0; k < 2 * kPart * kGroups / 256; ++k) {
+        const int piece = k * 4 + wave, p = piece / (kPart * kGroups / 64), group = piece % (kPart * kGroups / 64) * 64;
+        const int j = (group + lane) / kGroups, turned = (group + lane) % kGroups;
+        const int from = kGroups == 4 ? turned ^ ((j >> 1) & 3) : turned ^ (j & 7);
+        load_to_lds(xt + p * plane + at + (j * kGroups + from) * 8, &lds.xt[p][group * 8]);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (works) {
+        f32x16 high[kTiles] = {}, low[kTiles] = {};
+#pragma unroll
+        for (int k = 0; k < M / 16; ++k)
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const int from = turned_at(col0 + t * 32 + (lane & 31), k * 2 + half, kGroups);
+            three_products(b_op[0][k], b_op[1][k], *reinterpret_cast<const half8*>(&lds.xt[0][from]),
+                           *reinterpret_cast<const half8*>(&lds.xt[1][from]), high[t], low[t]);
+          }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int k = 0; k < 16; k += 4) {
+            const int row = row0 + 2 * k + 4 * half, j = col0 + t * 32 + (lane & 31);
+            const int from = turned_at(j, row / 8, kGroups) + row % 8;
+            const half4 old_hi = *reinterpret_cast<const half4*>(&lds.xt[0][from]);
+            const half4 old_lo = *reinterpret_cast<const half4*>(&lds.xt[1][from]);
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              v[r] = fmaf(a.a, joined(old_hi[r], old_lo[r]), fmaf(low[t][k + r], kUnlow, high[t][k + r]));
+              if (shift) v[r] = ldexpf(v[r], shift);
+            }
+            if constexpr (PHASE == kLast) {
+              update.write(m, row, part * kPart + j, v);
+            } else {
+              half4 hi, lo;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                _Float16 h, l;
+                split(v[r], h, l);
+                hi[r] = h, lo[r] = l;
+                const int to = turned_at(row + r, j / 8, kPart / 8) + j % 8;
+                lds.x[0][to] = h, lds.x[1][to] = l;
+              }
+              *reinterpret_cast<half4*>(xt + at + j * M + row) = hi;
+              *reinterpret_cast<half4*>(xt + plane + at + j * M + row) = lo;
+            }
+          }
+      }
+      __syncthreads();
+    }
+    if constexpr (PHASE != kLast) {
+#pragma unroll
+      for (int q = 0; q < kMine; ++q) {
+        const int b = wave + 4 * q;
+        if (b >= kBlocks) continue;
+        int bi, bj;
+        upper_block(b, bi, bj);
+#pragma unroll
+        for (int k = 0; k < kPart / 16; ++k) {
+          const int i = turned_at(bi * 32 + (lane & 31), k * 2 + half, kPart / 8);
+          const int j = turned_at(bj * 32 + (lane & 31), k * 2 + half, kPart / 8);
+          three_products(*reinterpret_cast<const half8*>(&lds.x[0][i]), *reinterpret_cast<const half8*>(&lds.x[1][i]),
+                         *reinterpret_cast<const half8*>(&lds.x[0][j]), *reinterpret_cast<const half8*>(&lds.x[1][j]),
+                         gram_high[q], gram_low[q]);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  if constexpr (PHASE != kLast) {
+    float* const parts = reinterpret_cast<float*>(xt + 2 * plane + 2 * M * M) + static_cast<int64_t>(chunk) * kBlocks * 1024;
+#pragma unroll
+    for (int q = 0; q < kMine; ++q) {
+      const int b = wave + 4 * q;
+      if (b >= kBlocks) continue;
+#pragma unroll
+      for (int k = 0; k < 16; k += 4) {
+        mf4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = fmaf(gram_low[q][k + r], kUnlow, gram_high[q][k + r]);
+        *reinterpret_cast<mf4*>(parts + b * 1024 + (k / 4 * 64 + lane) * 4) = v;
+      }
+    }
+  }
+}
+
+template <int PHASE>
+__global__ void __launch_bounds__(kMuThreads) muon_chunk_kernel(const MuonArgs a, int step) {
+  __shared__ ShortLds lds;
+  if (skipped(a)) return;
+  const uint32_t owner = a.chunk_owner[blockIdx.x];
+  const MuonMatrix m = a.matrices[owner];
+  if (m.mp == 128) short_chunk<PHASE, 4>(a, m, owner, step, lds);
+  else if (m.mp == 64) short_chunk<PHASE, 2>(a, m, owner, step, lds);
+  else short_chunk<PHASE, 1>(a, m, owner, step, lds);
+}
+
+constexpr int kPolyThreads = 512;
+
+// A from its chunks' parts, in order, and B = b A + c A A: a workgroup to a matrix.
+template <int MB>
+__device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& m, uint32_t owner, int step,
+                                           _Float16 (*lds)[kShort * kShort]) {
+  constexpr int M = 32 * MB, kGroups = M / 8, kBlocks = MB * (MB + 1) / 2, kQuads = kBlocks * 256;
+  constexpr int kMine = (kQuads + kPolyThreads - 1) / kPolyThreads;
+  const int lane = threadIdx.x & (kMuWave - 1), wave = threadIdx.x / kMuWave, half = lane / 32;
+  const int64_t plane = static_cast<int64_t>(m.np) * M;
+  _Float16* const poly = reinterpret_cast<_Float16*>(m.x) + 2 * plane;
+  const float* const parts = reinterpret_cast<const float*>(poly + 2 * M * M);
+  const int shift = shift_of<kGram>(a, owner, step);
+  mf4 sum[kMine] = {};
+  constexpr int kAhead = MB == 4 ? 4 : 12;         // chunks whose parts are on their way at a time
+  for (uint32_t first = 0; first < m.chunks; first += kAhead) {
+    mf4 v[kAhead][kMine];
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c)
+#pragma unroll
+      for (int q = 0; q < kMine; ++q) {
+        const int quad = q * kPolyThreads + threadIdx.x;
+        v[c][q] = mf4{0.f, 0.f, 0.f, 0.f};
+        if (quad < kQuads && first + c < m.chunks)
+          v[c][q] = *reinterpret_cast<const mf4*>(parts + (static_cast<int64_t>(first + c) * kQuads + quad) * 4);
+      }
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c)
+#pragma unroll
+      for (int q = 0; q < kMine; ++q)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[q][r] += v[c][q][r];
+  }
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) {
+    const int quad = q * kPolyThreads + threadIdx.x;
+    if (quad >= kQuads) continue;
+    int bi, bj;
+    upper_block(quad / 256, bi, bj);
+    const int of = quad % 64, row = bi * 32 + quad % 256 / 64 * 8 + 4 * (of / 32), column = bj * 32 + (of & 31);
+    half4 hi, lo;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      _Float16 h, l;
+      split(shift ? ldexpf(sum[q][r], shift) : sum[q][r], h, l);
+      hi[r] = h, lo[r] = l;
+      if (bi != bj) {
+        const int to = turned_at(row + r, column / 8, kGroups) + column % 8;
+        lds[0][to] = h, lds[1][to] = l;
+      }
+    }
+    const int to = turned_at(column, row / 8, kGroups) + row % 8;
+    *reinterpret_cast<half4*>(&lds[0][to]) = hi;
+    *reinterpret_cast<half4*>(&lds[1][to]) = lo;
+  }
+  __syncthreads();
+  for (int b = wave; b < kBlocks; b += kPolyThreads / kMuWave) {
+    int bi, bj;
+    upper_block(b, bi, bj);
+    f32x16 high = {}, low = {};
+#pragma unroll
+    for (int k = 0; k < M / 16; ++k) {
+      const int i = turned_at(bi * 32 + (lane & 31), k * 2 + half, kGroups);
+      const int j = turned_at(bj * 32 + (lane & 31), k * 2 + half, kGroups);
+      three_products(*reinterpret_cast<const half8*>(&lds[0][i]), *reinterpret_cast<const half8*>(&lds[1][i]),
+                     *reinterpret_cast<const half8*>(&lds[0][j]), *reinterpret_cast<const half8*>(&lds[1][j]), high, low);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) {
+      const int row = bi * 32 + 2 * k + 4 * half, column = bj * 32 + (lane & 31);
+      const int from = turned_at(column, row / 8, kGroups) + row % 8;
+      const half4 old_hi = *reinterpret_cast<const half4*>(&lds[0][from]);
+      const half4 old_lo = *reinterpret_cast<const half4*>(&lds[1][from]);
+      half4 hi, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        _Float16 h, l;
+        split(fmaf(a.b, joined(old_hi[r], old_lo[r]), a.c * fmaf(low[k + r], kUnlow, high[k + r])), h, l);
+        hi[r] = h, lo[r] = l;
+        if (bi != bj) {
+          poly[(row + r) * M + column] = h;
+          poly[M * M + (row + r) * M + column] = l;
+        }
+      }
+      *reinterpret_cast<half4*>(poly + column * M + row) = hi;
+      *reinterpret_cast<half4*>(poly + M * M + column * M + row) = lo;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kPolyThreads) muon_short_poly_kernel(const MuonArgs a, uint32_t first, int step) {
+  __shared__ _Float16 lds[2][kShort * kShort];
+  if (skipped(a)) return;
+  const uint32_t owner = first + blockIdx.x;
+  const MuonMatrix m = a.matrices[owner];
+  if (m.mp == 128) short_poly<4>(a, m, owner, step, lds);
+  else if (m.mp == 64) short_poly<2>(a, m, owner, step, lds);
+  else short_poly<1>(a, m, owner, step, lds);
+}
+
 constexpr int kTile = 64;
 constexpr int64_t kMostSide = 1 << 20;
 constexpr int64_t kMostMatrices = int64_t{1} << 23;
@@ -440,14 +843,19 @@ constexpr int64_t kMostTiles = int64_t{1} << 23;      // of a launch: threads wi
 
 // Tensors [first, end) of a call whose matrices take part in the same launches, and what they need.
 struct MuonGroup {
-  int64_t end, matrices, prep, sym, apply, bytes;
+  int64_t end, matrices, prep, sym, apply, chunks, bytes;
+
+  void add(const MuonSize& s, int64_t batches) {
+    matrices += batches, prep += batches * s.prep, sym += batches * s.sym, apply += batches * s.apply;
+    chunks += batches * s.chunks, bytes += batches * s.bytes;
+  }
 
   // Where the tables and the matrices lie in the workspace.
-  int64_t at_matrices() const { return 0; }
   int64_t at_prep() const { return up_to(matrices * static_cast<int64_t>(sizeof(MuonMatrix)), 256); }
   int64_t at_sym() const { return at_prep() + up_to(4 * prep, 256); }
   int64_t at_apply() const { return at_sym() + up_to(4 * sym, 256); }
-  int64_t at_squares() const { return at_apply() + up_to(4 * apply, 256); }
+  int64_t at_chunk() const { return at_apply() + up_to(4 * apply, 256); }
+  int64_t at_squares() const { return at_chunk() + up_to(4 * chunks, 256); }
   int64_t at_exponents() const { return at_squares() + up_to(8 * prep, 256); }
   int64_t at_values() const { return at_exponents() + up_to(4 * matrices, 256); }
   int64_t size() const { return at_values() + bytes; }
@@ -463,7 +871,7 @@ MuonGroup muon_group(const int64_t* rows, const int64_t* cols, const int64_t* ba
     const MuonSize s = muon_size<T>(rows[k], cols[k]);
     const int64_t b = batches[k];
     if (g.matrices && (g.bytes + b * s.bytes > kMostBytes || g.prep + b * s.prep > kMostTiles)) break;
-    g.matrices += b, g.prep += b * s.prep, g.sym += b * s.sym, g.apply += b * s.apply, g.bytes += b * s.bytes;
+    g.add(s, b);
   }
   g.end = k;
   return g;
@@ -518,47 +926,65 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
   for (int64_t k = 0; k < count;) {
     const MuonGroup g = muon_group<T>(rows, cols, batches, k, count);
     if (g.size() > ws_bytes) return ICTC_ERR_INVALID_ARGUMENT;
-    MuonMatrix* const matrices = reinterpret_cast<MuonMatrix*>(ws + g.at_matrices());
-    uint32_t* const prep = reinterpret_cast<uint32_t*>(ws + g.at_prep());
-    uint32_t* const sym = reinterpret_cast<uint32_t*>(ws + g.at_sym());
-    uint32_t* const apply = reinterpret_cast<uint32_t*>(ws + g.at_apply());
-    a.matrices = matrices, a.prep_owner = prep, a.sym_owner = sym, a.apply_owner = apply;
+    MuonMatrix* const matrices = reinterpret_cast<MuonMatrix*>(ws);
+    const auto owners = [&](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
+    uint32_t* const prep = owners(g.at_prep());
+    uint32_t* const sym = owners(g.at_sym());
+    uint32_t* const apply = owners(g.at_apply());
+    uint32_t* const chunk = owners(g.at_chunk());
+    a.matrices = matrices, a.prep_owner = prep, a.sym_owner = sym, a.apply_owner = apply, a.chunk_owner = chunk;
     a.squares = reinterpret_cast<double*>(ws + g.at_squares());
     a.exponents = reinterpret_cast<int32_t*>(ws + g.at_exponents());
-    MuonGroup at = {};       // of the tensors before that take part
-    for (int64_t t = k; t < g.end;) {
-      MuonTable table;
-      int n = 0;
-      for (; t < g.end && n < kTensorsPerLaunch; ++t) {
+    // those that take part, the ones with long shorter sides first
+    MuonGroup at = {}, longs = {};
+    MuonTable table;
+    int n = 0;
+    const auto send = [&]() {
+      if (n)
+        hipLaunchKernelGGL(muon_setup_kernel<T>, dim3(n), dim3(kMuThreads), 0, stream, table, ws + g.at_values(), matrices,
+                           prep, sym, apply, chunk);
+      n = 0;
+      return muon_launched();
+    };
+    for (int shorts = 0; shorts < 2; ++shorts) {
+      for (int64_t t = k; t < g.end; ++t) {
         if (!src[t] || !rows[t] || !cols[t] || !batches[t]) continue;
         const MuonSize s = muon_size<T>(rows[t], cols[t]);
-        const int64_t b = batches[t];
+        if (s.is_short != (shorts != 0)) continue;
         const double r = static_cast<double>(rows[t]), c = static_cast<double>(cols[t]);
         MuonTensor& e = table.tensor[n++];
         e.src = src[t], e.momentum = momentum ? momentum[t] : nullptr, e.out = out[t];
         e.base = at.bytes, e.rows = static_cast<int32_t>(rows[t]), e.cols = static_cast<int32_t>(cols[t]);
-        e.batches = static_cast<int32_t>(b), e.first = static_cast<int32_t>(at.matrices);
+        e.batches = static_cast<int32_t>(batches[t]), e.first = static_cast<int32_t>(at.matrices);
         e.prep = static_cast<uint32_t>(at.prep), e.sym = static_cast<uint32_t>(at.sym);
-        e.apply = static_cast<uint32_t>(at.apply);
+        e.apply = static_cast<uint32_t>(at.apply), e.chunk = static_cast<uint32_t>(at.chunks);
         e.rate = static_cast<float>(d->adjust == ICTC_MUON_SHAPE ? sqrt(r > c ? r / c : 1.0) : 0.2 * sqrt(r > c ? r : c));
-        at.matrices += b, at.prep += b * s.prep, at.sym += b * s.sym, at.apply += b * s.apply, at.bytes += b * s.bytes;
+        at.add(s, batches[t]);
+        if (n == kTensorsPerLaunch)
+          if (const int rc = send()) return rc;
       }
-      if (!n) break;
-      hipLaunchKernelGGL(muon_setup_kernel<T>, dim3(n), dim3(kMuThreads), 0, stream, table, ws + g.at_values(), matrices,
-                         prep, sym, apply);
-      if (const int rc = muon_launched()) return rc;
+      if (!shorts) longs = at;
     }
+    if (const int rc = send()) return rc;
     k = g.end;
     if (!at.matrices) continue;
+    const auto launch = [&](void (*kernel)(MuonArgs, int), int64_t grid, int step) {
+      if (grid) hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kMuThreads), 0, stream, a, step);
+    };
     hipLaunchKernelGGL(muon_average_kernel, dim3(static_cast<unsigned>(at.prep)), dim3(kMuThreads), 0, stream, a);
-    hipLaunchKernelGGL(muon_normalise_kernel, dim3(static_cast<unsigned>(at.prep)), dim3(kMuThreads), 0, stream, a);
+    if (longs.matrices)
+      hipLaunchKernelGGL(muon_normalise_kernel, dim3(static_cast<unsigned>(longs.prep)), dim3(kMuThreads), 0, stream, a);
+    launch(muon_chunk_kernel<kFirst>, at.chunks, 0);
     for (int step = 0; step < d->steps; ++step) {
-      const auto apply_kernel = step + 1 < d->steps ? muon_product_kernel<T, kApply> : muon_product_kernel<T, kLast>;
-      hipLaunchKernelGGL((muon_product_kernel<T, kGram>), dim3(static_cast<unsigned>(at.sym)), dim3(kMuThreads), 0, stream,
-                         a, step);
-      hipLaunchKernelGGL((muon_product_kernel<T, kPoly>), dim3(static_cast<unsigned>(at.sym)), dim3(kMuThreads), 0, stream,
-                         a, step);
-      hipLaunchKernelGGL(apply_kernel, dim3(static_cast<unsigned>(at.apply)), dim3(kMuThreads), 0, stream, a, step);
+      const bool last = step + 1 == d->steps;
+      launch(muon_product_kernel<T, kGram>, longs.sym, step);
+      launch(muon_product_kernel<T, kPoly>, longs.sym, step);
+      launch(last ? muon_product_kernel<T, kLast> : muon_product_kernel<T, kApply>, longs.apply, step);
+      const uint32_t first = static_cast<uint32_t>(longs.matrices);
+      if (at.matrices > longs.matrices)
+        hipLaunchKernelGGL(muon_short_poly_kernel, dim3(static_cast<unsigned>(at.matrices - longs.matrices)),
+                           dim3(kPolyThreads), 0, stream, a, first, step);
+      launch(last ? muon_chunk_kernel<kLast> : muon_chunk_kernel<kApply>, at.chunks, step);
       if (const int rc = muon_launched()) return rc;
     }
   }
