@@ -7,13 +7,15 @@
 //
 // Precision.  A singular value goes through p(s) = a s + b s^3 + c s^5 in every step, so small ones grow by a = 3.4
 // each time and an error of X with them: products in bfloat16 would leave updates with 2 correct digits.  A product
-// here is of float32 accuracy on the float16 matrix cores: x = hi + lo 2^-11 with hi = f16(x) and lo = f16(2^11 (x - hi)),
-// 22 bits or an absolute 2^-36, whichever is larger (entries are near 1 and below, |X| is at most about 1.2), and
-//   x y = hi hi' + 2^-11 (hi lo' + lo hi')  + (2^-22 x y, left out)
-// in two float32 accumulators.  A matrix with |U| below eps, where X stays small, is kept times a power of two (2^e,
-// see exponent_at), so that it has as many bits.  Three products at 16 times the float32 instructions' rate.  (The form that iterates
-// A alone and multiplies X once has a third of the work for wide matrices, but doubles the error's growth: singular values
-// below 1e-3 of the largest come out wrong, 1e-4 of the result at rank-deficient matrices.)
+// here is of float32 accuracy on the float16 matrix cores: 2^11 x = hi + lo with hi = f16(2^11 x) and lo = f16(2^11 x - hi),
+// 22 bits or an absolute 2^-36, whichever is larger (entries of X and A are near 1 and below), and
+//   x y = 2^-22 (hi hi' + hi lo' + lo hi')  + (2^-22 x y, left out)
+// in one float32 accumulator.  Three products at 16 times the float32 instructions' rate.  What a power of two is chosen
+// for grows at most 32-fold: |X| stays near 1 with coefficients for which the iteration is of use.  A matrix with |U|
+// below eps, where X stays small, is kept times another power of two (2^e, see exponent_at), so that it has as many
+// bits.  (The form that iterates A alone and multiplies X once has a third of the work for wide matrices, but doubles
+// the error's growth: singular values below 1e-3 of the largest come out wrong, 1e-4 of the result at rank-deficient
+// matrices.)
 //
 // Matrices with a side of more than 128 (below: the shorter side): all three products are of the form P Q^T with both operands' rows along the reduction (X X^T, A A^T, B (X^T)^T), so
 // one kernel does them; X is kept in both orientations.  A and B are symmetric: only tiles on and above the diagonal
@@ -44,7 +46,7 @@ using half4 = _Float16 __attribute__((ext_vector_type(4)));
 using f32x16 = float __attribute__((ext_vector_type(16)));
 typedef float mf4 __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr float kLow = 2048.f, kUnlow = 1.f / 2048.f;
+constexpr float kScale = 2048.f, kUnscale = 1.f / kScale;      // of X and A as they are kept
 constexpr int kMostExponent = 200;           // (2^-149 is the smallest number)
 
 // One tensor's matrices, as the host describes them.
@@ -89,6 +91,7 @@ struct MuonArgs {
   double weight_decay, eps;
   float beta, rest, lr;      // rest: 1 - beta
   float a, b, c;
+  float b_kept, c_kept, unpoly;      // b and c for B as it is kept, from A and A A as they are; B's scale, inverse
   int32_t nesterov;
 };
 
@@ -263,11 +266,11 @@ __global__ void __launch_bounds__(kMuThreads) muon_average_kernel(const MuonArgs
 
 __device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
   hi = static_cast<_Float16>(x);
-  lo = static_cast<_Float16>((x - static_cast<float>(hi)) * kLow);
+  lo = static_cast<_Float16>(x - static_cast<float>(hi));
 }
 
 __device__ __forceinline__ float joined(_Float16 hi, _Float16 lo) {
-  return fmaf(static_cast<float>(lo), kUnlow, static_cast<float>(hi));
+  return static_cast<float>(hi) + static_cast<float>(lo);
 }
 
 // The power of two that X is kept with before a step, from the one at first: |X| <= 2^-e, and a step multiplies it by at
@@ -290,7 +293,7 @@ __device__ __forceinline__ double first_scale(const MuonArgs& a, const MuonMatri
   const double norm = sqrt(muon_block_sum(sum, part)), share = norm / (norm + a.eps);
   const int e = share > 0.0 && share < 0.5 ? min(-ilogb(share) - 1, kMostExponent) : 0;
   if (threadIdx.x == 0 && keeps) a.exponents[owner] = e;
-  return ldexp(1.0 / (norm + a.eps), e);
+  return ldexp(kScale / (norm + a.eps), e);
 }
 
 // Values of what is orthogonalised, from the source and (after muon_average_kernel) the moving average.
@@ -386,7 +389,8 @@ struct Update {
       if (row + r < shorter) {
         float* to = m.out + (m.transposed ? static_cast<int64_t>(column) * m.cols + row + r
                                           : static_cast<int64_t>(row + r) * m.cols + column);
-        *to = m.momentum ? keep * *to - rate * v[r] : v[r];
+        const float x = v[r] * kUnscale;
+        *to = m.momentum ? keep * *to - rate * x : x;
       }
   }
 };
@@ -404,7 +408,7 @@ __device__ __forceinline__ void load_to_lds(const _Float16* from, _Float16* to) 
 // of 16 bytes, whose order is turned with the row so that 8 rows' groups fill all banks; they come straight from
 // global memory (a lane picks the group that belongs to its place), one step ahead of the products.
 template <int T, int PHASE>
-__global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs a, int step) {
+__global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonArgs a, int step) {
   constexpr int N = T / 64;                        // 32 x 32 products of a wave, each way
   constexpr int kPlane = T * kStep;                // halves of one operand plane in LDS
   __shared__ _Float16 lds[2][4][kPlane];           // P's hi and lo, Q's hi and lo
@@ -449,7 +453,7 @@ __global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs
       load_to_lds(base + step * kStep + group * 8, &lds[buffer][which][rows * kStep]);
     }
   };
-  f32x16 high[N][N] = {}, low[N][N] = {};
+  f32x16 acc[N][N] = {};
   const int steps = depth / kStep;
   fetch(0, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -467,18 +471,14 @@ __global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs
           const int row = (which < 2 ? wi : wj) + n * 32 + (lane & 31), group = k * 2 + lane / 32;
           op[which][n] = *reinterpret_cast<const half8*>(&lds[buffer][which][row * kStep + (group ^ ((row >> 1) & 3)) * 8]);
         }
+      // (hi lo', lo hi', hi hi': consecutive instructions go to different accumulators)
 #pragma unroll
-      for (int i = 0; i < N; ++i)
+      for (int q = 0; q < 3; ++q)
 #pragma unroll
-        for (int j = 0; j < N; ++j) high[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[0][i], op[2][j], high[i][j], 0, 0, 0);
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < N; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[0][i], op[3][j], low[i][j], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < N; ++j) low[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[1][i], op[2][j], low[i][j], 0, 0, 0);
+          for (int j = 0; j < N; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[q == 1 ? 1 : 0][i], op[q == 0 ? 3 : 2][j], acc[i][j], 0, 0, 0);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs
         const int row = ti * T + wi + i * 32 + 2 * k + 4 * (lane / 32), column = tj * T + wj + j * 32 + (lane & 31);
         float v[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = fmaf(low[i][j][k + r], kUnlow, high[i][j][k + r]);
+        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][k + r];
         const int64_t across = static_cast<int64_t>(column) * m.mp + row;        // in what has rows of m entries
         if constexpr (PHASE == kPoly || PHASE == kApply || PHASE == kLast) {
           const _Float16* old = PHASE == kPoly ? gram : xt;
@@ -505,7 +505,11 @@ __global__ void __launch_bounds__(kMuThreads) muon_product_kernel(const MuonArgs
           const half4 lo = *reinterpret_cast<const half4*>(old + old_plane + across);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            v[r] = PHASE == kPoly ? fmaf(a.b, joined(hi[r], lo[r]), a.c * v[r]) : fmaf(a.a, joined(hi[r], lo[r]), v[r]);
+            v[r] = PHASE == kPoly ? fmaf(a.b_kept, joined(hi[r], lo[r]), a.c_kept * v[r])
+                                  : fmaf(a.a, joined(hi[r], lo[r]), a.unpoly * v[r]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] *= kUnscale;
         }
         if (PHASE != kPoly && shift) {
 #pragma unroll
@@ -554,10 +558,10 @@ __device__ __forceinline__ void upper_block(int b, int& i, int& j) {
 }
 
 __device__ __forceinline__ void three_products(const half8& ah, const half8& al, const half8& bh, const half8& bl,
-                                               f32x16& high, f32x16& low) {
-  high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, high, 0, 0, 0);
-  low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, low, 0, 0, 0);
-  low = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, low, 0, 0, 0);
+                                               f32x16& acc) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
 }
 
 // LDS of a chunk's workgroup: 64 columns of X, their rows along the columns (as they lie in memory), and along the rows.
@@ -599,7 +603,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
   }
   const int shift = shift_of<PHASE>(a, owner, step);
   const Update update = PHASE == kLast ? Update(a, m) : Update();
-  f32x16 gram_high[kMine] = {}, gram_low[kMine] = {};
+  f32x16 gram[kMine] = {};
 
   for (int part = first; part < end; ++part) {
     const int64_t at = static_cast<int64_t>(part) * kPart * M;       // of the columns in X^T
@@ -647,14 +651,14 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       if (works) {
-        f32x16 high[kTiles] = {}, low[kTiles] = {};
+        f32x16 acc[kTiles] = {};
 #pragma unroll
         for (int k = 0; k < M / 16; ++k)
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
             const int from = turned_at(col0 + t * 32 + (lane & 31), k * 2 + half, kGroups);
             three_products(b_op[0][k], b_op[1][k], *reinterpret_cast<const half8*>(&lds.xt[0][from]),
-                           *reinterpret_cast<const half8*>(&lds.xt[1][from]), high[t], low[t]);
+                           *reinterpret_cast<const half8*>(&lds.xt[1][from]), acc[t]);
           }
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
@@ -667,7 +671,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
             float v[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              v[r] = fmaf(a.a, joined(old_hi[r], old_lo[r]), fmaf(low[t][k + r], kUnlow, high[t][k + r]));
+              v[r] = fmaf(a.a, joined(old_hi[r], old_lo[r]), a.unpoly * acc[t][k + r]);
               if (shift) v[r] = ldexpf(v[r], shift);
             }
             if constexpr (PHASE == kLast) {
@@ -702,7 +706,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
           const int j = turned_at(bj * 32 + (lane & 31), k * 2 + half, kPart / 8);
           three_products(*reinterpret_cast<const half8*>(&lds.x[0][i]), *reinterpret_cast<const half8*>(&lds.x[1][i]),
                          *reinterpret_cast<const half8*>(&lds.x[0][j]), *reinterpret_cast<const half8*>(&lds.x[1][j]),
-                         gram_high[q], gram_low[q]);
+                         gram[q]);
         }
       }
       __syncthreads();
@@ -718,7 +722,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
       for (int k = 0; k < 16; k += 4) {
         mf4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = fmaf(gram_low[q][k + r], kUnlow, gram_high[q][k + r]);
+        for (int r = 0; r < 4; ++r) v[r] = gram[q][k + r] * kUnscale;
         *reinterpret_cast<mf4*>(parts + b * 1024 + (k / 4 * 64 + lane) * 4) = v;
       }
     }
@@ -795,13 +799,13 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
   for (int b = wave; b < kBlocks; b += kPolyThreads / kMuWave) {
     int bi, bj;
     upper_block(b, bi, bj);
-    f32x16 high = {}, low = {};
+    f32x16 acc = {};
 #pragma unroll
     for (int k = 0; k < M / 16; ++k) {
       const int i = turned_at(bi * 32 + (lane & 31), k * 2 + half, kGroups);
       const int j = turned_at(bj * 32 + (lane & 31), k * 2 + half, kGroups);
       three_products(*reinterpret_cast<const half8*>(&lds[0][i]), *reinterpret_cast<const half8*>(&lds[1][i]),
-                     *reinterpret_cast<const half8*>(&lds[0][j]), *reinterpret_cast<const half8*>(&lds[1][j]), high, low);
+                     *reinterpret_cast<const half8*>(&lds[0][j]), *reinterpret_cast<const half8*>(&lds[1][j]), acc);
     }
 #pragma unroll
     for (int k = 0; k < 16; k += 4) {
@@ -813,7 +817,7 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         _Float16 h, l;
-        split(fmaf(a.b, joined(old_hi[r], old_lo[r]), a.c * fmaf(low[k + r], kUnlow, high[k + r])), h, l);
+        split(fmaf(a.b_kept, joined(old_hi[r], old_lo[r]), a.c_kept * acc[k + r]), h, l);
         hi[r] = h, lo[r] = l;
         if (bi != bj) {
           poly[(row + r) * M + column] = h;
@@ -836,9 +840,9 @@ __global__ void __launch_bounds__(kPolyThreads) muon_short_poly_kernel(const Muo
   else short_poly<1>(a, m, owner, step, lds);
 }
 
-constexpr int kTile = 64;
 constexpr int64_t kMostSide = 1 << 20;
 constexpr int64_t kMostMatrices = int64_t{1} << 23;
+constexpr int64_t kFewTiles = 512;
 constexpr int64_t kMostTiles = int64_t{1} << 23;      // of a launch: threads within 32 bits
 
 // Tensors [first, end) of a call whose matrices take part in the same launches, and what they need.
@@ -884,7 +888,7 @@ bool muon_valid(const int64_t* rows, const int64_t* cols, const int64_t* batches
         batches[k] > kMostMatrices)
       return false;
     if (!rows[k] || !cols[k] || !batches[k]) continue;
-    const MuonSize s = muon_size<kTile>(rows[k], cols[k]);
+    const MuonSize s = muon_size<128>(rows[k], cols[k]);
     if (s.prep > kMostTiles / batches[k]) return false;
   }
   return true;
@@ -901,6 +905,15 @@ bool muon_valid(const ictc_muon_desc* d, const float* lr_device) {
 
 int muon_launched() { return hipGetLastError() == hipSuccess ? ICTC_OK : ICTC_ERR_LAUNCH; }
 
+// Whether products go by tiles of 128 x 128 (and sides are padded to that): where these alone fill the chip twice.  They
+// read half as much from LDS for a product as tiles of 64 x 64.
+bool large_tiles(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count) {
+  int64_t tiles = 0;
+  for (int64_t k = 0; k < count; ++k)
+    if (rows[k] && cols[k] && batches[k]) tiles += batches[k] * muon_size<128>(rows[k], cols[k]).apply;
+  return tiles >= kFewTiles;
+}
+
 template <int T>
 int64_t muon_workspace(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count) {
   int64_t most = 0;
@@ -910,6 +923,11 @@ int64_t muon_workspace(const int64_t* rows, const int64_t* cols, const int64_t* 
     k = g.end;
   }
   return most;
+}
+
+int64_t muon_workspace(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count) {
+  return large_tiles(rows, cols, batches, count) ? muon_workspace<128>(rows, cols, batches, count)
+                                                 : muon_workspace<64>(rows, cols, batches, count);
 }
 
 template <int T>
@@ -922,6 +940,12 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
   a.beta = static_cast<float>(d->beta), a.rest = static_cast<float>(1.0 - d->beta), a.lr = d->lr;
   a.a = static_cast<float>(d->coefficients[0]), a.b = static_cast<float>(d->coefficients[1]);
   a.c = static_cast<float>(d->coefficients[2]);
+  // B as it is kept: below 2^15 for |X| up to 1.5
+  const double most = 2.25 * fabs(d->coefficients[1]) + 5.0625 * fabs(d->coefficients[2]);
+  const double poly = most > 16.0 ? ldexp(kScale, -ilogb(most / 16.0) - 1) : kScale;
+  a.b_kept = static_cast<float>(d->coefficients[1] * poly / kScale);
+  a.c_kept = static_cast<float>(d->coefficients[2] * poly / kScale / kScale);
+  a.unpoly = static_cast<float>(1.0 / poly);
   a.nesterov = d->nesterov;
   for (int64_t k = 0; k < count;) {
     const MuonGroup g = muon_group<T>(rows, cols, batches, k, count);
@@ -999,7 +1023,7 @@ extern "C" {
 int64_t ictc_hip_muon_workspace(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count) {
   using namespace ictc;
   if (!muon_valid(rows, cols, batches, count)) return -ICTC_ERR_INVALID_ARGUMENT;
-  return muon_workspace<kTile>(rows, cols, batches, count);
+  return muon_workspace(rows, cols, batches, count);
 }
 
 int ictc_hip_orthogonalize(const float* const* in, float* const* out, const int64_t* rows, const int64_t* cols,
@@ -1007,13 +1031,14 @@ int ictc_hip_orthogonalize(const float* const* in, float* const* out, const int6
                            int64_t workspace_bytes, hipStream_t stream) {
   using namespace ictc;
   if (!muon_valid(rows, cols, batches, count) || !muon_valid(desc, nullptr)) return ICTC_ERR_INVALID_ARGUMENT;
-  const int64_t need = muon_workspace<kTile>(rows, cols, batches, count);
+  const int64_t need = muon_workspace(rows, cols, batches, count);
   if (need == 0) return ICTC_OK;
   if (!in || !out || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < need)
     return ICTC_ERR_INVALID_ARGUMENT;
   for (int64_t k = 0; k < count; ++k)
     if (rows[k] && cols[k] && batches[k] && (!in[k] || !out[k])) return ICTC_ERR_INVALID_ARGUMENT;
-  return muon_run<kTile>(in, nullptr, out, rows, cols, batches, count, desc, nullptr, nullptr,
+  const auto run = large_tiles(rows, cols, batches, count) ? muon_run<128> : muon_run<64>;
+  return run(in, nullptr, out, rows, cols, batches, count, desc, nullptr, nullptr,
                          static_cast<char*>(workspace), workspace_bytes, stream);
 }
 
@@ -1023,14 +1048,15 @@ int ictc_hip_muon_step(float* const* params, const float* const* grads, float* c
                        hipStream_t stream) {
   using namespace ictc;
   if (!muon_valid(rows, cols, batches, count) || !muon_valid(desc, lr_device)) return ICTC_ERR_INVALID_ARGUMENT;
-  const int64_t need = muon_workspace<kTile>(rows, cols, batches, count);
+  const int64_t need = muon_workspace(rows, cols, batches, count);
   if (need == 0) return ICTC_OK;
   if (!params || !grads || !momentum || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
       workspace_bytes < need)
     return ICTC_ERR_INVALID_ARGUMENT;
   for (int64_t k = 0; k < count; ++k)
     if (rows[k] && cols[k] && batches[k] && grads[k] && (!params[k] || !momentum[k])) return ICTC_ERR_INVALID_ARGUMENT;
-  return muon_run<kTile>(grads, momentum, params, rows, cols, batches, count, desc, clip, lr_device,
+  const auto run = large_tiles(rows, cols, batches, count) ? muon_run<128> : muon_run<64>;
+  return run(grads, momentum, params, rows, cols, batches, count, desc, clip, lr_device,
                          static_cast<char*>(workspace), workspace_bytes, stream);
 }
 
