@@ -29,6 +29,10 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include "ictc_hip.h"
 
 namespace ictc {
@@ -404,20 +408,32 @@ __device__ __forceinline__ void load_to_lds(const _Float16* from, _Float16* to) 
                                    16, 0, 0);
 }
 
+// Workgroups go to the 8 XCDs in turn, and each has a cache of its own: 32 tiles in a row, which share rows of their
+// operands, go to the same one.
+constexpr uint32_t kXcds = 8, kUnit = 32;
+
+__device__ __forceinline__ uint32_t tile_of(uint32_t block) {
+  return (block / (kXcds * kUnit) * kXcds + block % kXcds) * kUnit + block / kXcds % kUnit;
+}
+
+int64_t tile_grid(int64_t tiles) { return up_to(tiles, kXcds * kUnit); }
+
 // One tile of P Q^T: T x T, four waves of (T/2) x (T/2).  Rows of 32 reduction entries (64 bytes) lie in LDS in four groups
 // of 16 bytes, whose order is turned with the row so that 8 rows' groups fill all banks; they come straight from
 // global memory (a lane picks the group that belongs to its place), one step ahead of the products.
 template <int T, int PHASE>
-__global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonArgs a, int step) {
+__global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonArgs a, uint32_t tiles, int step) {
   constexpr int N = T / 64;                        // 32 x 32 products of a wave, each way
   constexpr int kPlane = T * kStep;                // halves of one operand plane in LDS
   __shared__ _Float16 lds[2][4][kPlane];           // P's hi and lo, Q's hi and lo
   if (skipped(a)) return;
   constexpr bool kSym = PHASE == kGram || PHASE == kPoly;
-  const uint32_t owner = (kSym ? a.sym_owner : a.apply_owner)[blockIdx.x];
+  const uint32_t tile = tile_of(blockIdx.x);
+  if (tile >= tiles) return;
+  const uint32_t owner = (kSym ? a.sym_owner : a.apply_owner)[tile];
   const MuonMatrix m = a.matrices[owner];
   const int parity = step & 1;
-  const uint32_t local = blockIdx.x - (kSym ? m.sym : m.apply);
+  const uint32_t local = tile - (kSym ? m.sym : m.apply);
   int ti, tj;
   if constexpr (kSym) {
     tj = static_cast<int>((sqrtf(8.f * local + 1.f) - 1.f) * 0.5f);
@@ -970,9 +986,14 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
       n = 0;
       return muon_launched();
     };
+    // (and of those the longest first: their tiles take longest)
+    std::vector<int64_t> order;
+    for (int64_t t = k; t < g.end; ++t)
+      if (src[t] && rows[t] && cols[t] && batches[t]) order.push_back(t);
+    const auto longer = [&](int64_t t) { return rows[t] > cols[t] ? rows[t] : cols[t]; };
+    std::stable_sort(order.begin(), order.end(), [&](int64_t x, int64_t y) { return longer(x) > longer(y); });
     for (int shorts = 0; shorts < 2; ++shorts) {
-      for (int64_t t = k; t < g.end; ++t) {
-        if (!src[t] || !rows[t] || !cols[t] || !batches[t]) continue;
+      for (const int64_t t : order) {
         const MuonSize s = muon_size<T>(rows[t], cols[t]);
         if (s.is_short != (shorts != 0)) continue;
         const double r = static_cast<double>(rows[t]), c = static_cast<double>(cols[t]);
@@ -995,15 +1016,20 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
     const auto launch = [&](void (*kernel)(MuonArgs, int), int64_t grid, int step) {
       if (grid) hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kMuThreads), 0, stream, a, step);
     };
+    const auto product = [&](void (*kernel)(MuonArgs, uint32_t, int), int64_t tiles, int step) {
+      if (tiles)
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tile_grid(tiles))), dim3(kMuThreads), 0, stream, a,
+                           static_cast<uint32_t>(tiles), step);
+    };
     hipLaunchKernelGGL(muon_average_kernel, dim3(static_cast<unsigned>(at.prep)), dim3(kMuThreads), 0, stream, a);
     if (longs.matrices)
       hipLaunchKernelGGL(muon_normalise_kernel, dim3(static_cast<unsigned>(longs.prep)), dim3(kMuThreads), 0, stream, a);
     launch(muon_chunk_kernel<kFirst>, at.chunks, 0);
     for (int step = 0; step < d->steps; ++step) {
       const bool last = step + 1 == d->steps;
-      launch(muon_product_kernel<T, kGram>, longs.sym, step);
-      launch(muon_product_kernel<T, kPoly>, longs.sym, step);
-      launch(last ? muon_product_kernel<T, kLast> : muon_product_kernel<T, kApply>, longs.apply, step);
+      product(muon_product_kernel<T, kGram>, longs.sym, step);
+      product(muon_product_kernel<T, kPoly>, longs.sym, step);
+      product(last ? muon_product_kernel<T, kLast> : muon_product_kernel<T, kApply>, longs.apply, step);
       const uint32_t first = static_cast<uint32_t>(longs.matrices);
       if (at.matrices > longs.matrices)
         hipLaunchKernelGGL(muon_short_poly_kernel, dim3(static_cast<unsigned>(at.matrices - longs.matrices)),
@@ -1013,6 +1039,19 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
     }
   }
   return ICTC_OK;
+}
+
+// (No C++ exception leaves through the C interface.)
+int muon_call(const float* const* src, float* const* momentum, float* const* out, const int64_t* rows,
+              const int64_t* cols, const int64_t* batches, int64_t count, const ictc_muon_desc* d, const float* clip,
+              const float* lr_device, void* ws, int64_t ws_bytes, hipStream_t stream) {
+  const auto run = large_tiles(rows, cols, batches, count) ? muon_run<128> : muon_run<64>;
+  try {
+    return run(src, momentum, out, rows, cols, batches, count, d, clip, lr_device, static_cast<char*>(ws), ws_bytes,
+               stream);
+  } catch (const std::bad_alloc&) {
+    return ICTC_ERR_LAUNCH;
+  }
 }
 
 }  // namespace
@@ -1037,9 +1076,8 @@ int ictc_hip_orthogonalize(const float* const* in, float* const* out, const int6
     return ICTC_ERR_INVALID_ARGUMENT;
   for (int64_t k = 0; k < count; ++k)
     if (rows[k] && cols[k] && batches[k] && (!in[k] || !out[k])) return ICTC_ERR_INVALID_ARGUMENT;
-  const auto run = large_tiles(rows, cols, batches, count) ? muon_run<128> : muon_run<64>;
-  return run(in, nullptr, out, rows, cols, batches, count, desc, nullptr, nullptr,
-                         static_cast<char*>(workspace), workspace_bytes, stream);
+  return muon_call(in, nullptr, out, rows, cols, batches, count, desc, nullptr, nullptr, workspace, workspace_bytes,
+                   stream);
 }
 
 int ictc_hip_muon_step(float* const* params, const float* const* grads, float* const* momentum, const int64_t* rows,
@@ -1055,9 +1093,8 @@ int ictc_hip_muon_step(float* const* params, const float* const* grads, float* c
     return ICTC_ERR_INVALID_ARGUMENT;
   for (int64_t k = 0; k < count; ++k)
     if (rows[k] && cols[k] && batches[k] && grads[k] && (!params[k] || !momentum[k])) return ICTC_ERR_INVALID_ARGUMENT;
-  const auto run = large_tiles(rows, cols, batches, count) ? muon_run<128> : muon_run<64>;
-  return run(grads, momentum, params, rows, cols, batches, count, desc, clip, lr_device,
-                         static_cast<char*>(workspace), workspace_bytes, stream);
+  return muon_call(grads, momentum, params, rows, cols, batches, count, desc, clip, lr_device, workspace,
+                   workspace_bytes, stream);
 }
 
 }  // extern "C"
