@@ -85,6 +85,14 @@ struct MuonMatrix {
   int32_t transposed;                          // more rows than columns
 };
 
+// The first kind keeps planes of hi and lo parts; the second one 32 hi parts and their 32 lo parts side by side (kPair
+// halves apart), so that a tile's load of 32 reduction entries takes whole lines of memory.
+constexpr int kPair = 32;
+
+__host__ __device__ constexpr int64_t paired_at(int64_t row, int64_t column, int64_t wide) {
+  return (row * wide + column / kPair * kPair) * 2 + column % kPair;
+}
+
 struct MuonArgs {
   const MuonMatrix* matrices;
   const uint32_t *prep_owner, *sym_owner, *apply_owner, *chunk_owner;
@@ -337,11 +345,11 @@ __global__ void __launch_bounds__(kMuThreads) muon_normalise_kernel(const MuonAr
 #pragma unroll
     for (int j = 0; j < 4; ++j) tile[first + k * kQuadRows][column + j] = source[k].value(a, m, j, scale, inv);
   __syncthreads();
-  const int64_t plane = static_cast<int64_t>(m.mp) * m.np;
+  const int64_t values = static_cast<int64_t>(m.mp) * m.np;
   _Float16* const x = reinterpret_cast<_Float16*>(m.x);
 #pragma unroll
   for (int side = 0; side < 2; ++side) {           // as it is, and transposed
-    _Float16* to = x + ((side != 0) == (m.transposed != 0) ? 0 : 2 * plane);
+    _Float16* to = x + ((side != 0) == (m.transposed != 0) ? 0 : 2 * values);
     const int64_t wide = (side != 0) == (m.transposed != 0) ? m.np : m.mp;
     const int first = side ? t.c0 : t.r0, along = side ? t.r0 : t.c0;
     for (int k = threadIdx.x; k < kPrep * kPrep / 8; k += kMuThreads) {
@@ -353,9 +361,9 @@ __global__ void __launch_bounds__(kMuThreads) muon_normalise_kernel(const MuonAr
         split(side ? tile[c + j][r] : tile[r][c + j], h, l);
         hi[j] = h, lo[j] = l;
       }
-      const int64_t at = (first + r) * wide + along + c;
+      const int64_t at = paired_at(first + r, along + c, wide);
       *reinterpret_cast<half8*>(to + at) = hi;
-      *reinterpret_cast<half8*>(to + plane + at) = lo;
+      *reinterpret_cast<half8*>(to + at + kPair) = lo;
     }
   }
 }
@@ -418,14 +426,13 @@ __device__ __forceinline__ uint32_t tile_of(uint32_t block) {
 
 int64_t tile_grid(int64_t tiles) { return up_to(tiles, kXcds * kUnit); }
 
-// One tile of P Q^T: T x T, four waves of (T/2) x (T/2).  Rows of 32 reduction entries (64 bytes) lie in LDS in four groups
-// of 16 bytes, whose order is turned with the row so that 8 rows' groups fill all banks; they come straight from
-// global memory (a lane picks the group that belongs to its place), one step ahead of the products.
+// One tile of P Q^T: T x T, four waves of (T/2) x (T/2).  Rows of 32 reduction entries (128 bytes with both parts) lie in
+// LDS in eight groups of 16 bytes, whose order is turned with the row so that 16 rows' groups fill all banks; they come
+// straight from global memory (a lane picks the group that belongs to its place), one step ahead of the products.
 template <int T, int PHASE>
 __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonArgs a, uint32_t tiles, int step) {
   constexpr int N = T / 64;                        // 32 x 32 products of a wave, each way
-  constexpr int kPlane = T * kStep;                // halves of one operand plane in LDS
-  __shared__ _Float16 lds[2][4][kPlane];           // P's hi and lo, Q's hi and lo
+  __shared__ _Float16 lds[2][2][T * 2 * kStep];    // rows of P and of Q, hi and lo parts
   if (skipped(a)) return;
   constexpr bool kSym = PHASE == kGram || PHASE == kPoly;
   const uint32_t tile = tile_of(blockIdx.x);
@@ -444,29 +451,29 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
     const uint32_t down = m.mp / T;
     ti = static_cast<int>(local % down), tj = static_cast<int>(local / down);
   }
-  const int64_t plane = static_cast<int64_t>(m.mp) * m.np, square = static_cast<int64_t>(m.mp) * m.mp;
+  const int64_t values = static_cast<int64_t>(m.mp) * m.np;
   _Float16* const x = reinterpret_cast<_Float16*>(m.x);
-  _Float16* const xt = x + 2 * plane * (1 + parity);               // X^T now, and what it becomes
-  _Float16* const xt_next = x + 2 * plane * (2 - parity);
-  _Float16* const gram = x + 6 * plane;
-  _Float16* const poly = gram + 2 * square;
+  _Float16* const xt = x + 2 * values * (1 + parity);               // X^T now, and what it becomes
+  _Float16* const xt_next = x + 2 * values * (2 - parity);
+  _Float16* const gram = x + 6 * values;
+  _Float16* const poly = gram + 2 * static_cast<int64_t>(m.mp) * m.mp;
   const _Float16* const p = PHASE == kGram ? x : PHASE == kPoly ? gram : poly;
   const _Float16* const q = PHASE == kGram ? x : PHASE == kPoly ? gram : xt;
-  const int64_t p_plane = PHASE == kGram ? plane : square, q_plane = PHASE == kPoly ? square : plane;
   const int depth = PHASE == kGram ? m.np : m.mp;
 
   const int lane = threadIdx.x & (kMuWave - 1), wave = threadIdx.x / kMuWave;
   const int wi = (wave & 1) * (T / 2), wj = (wave >> 1) * (T / 2);
+  // (16 lanes read 16 rows at a time, from 64 banks: the groups of every other row are in the same ones)
+  const auto turned = [](int row) { return (row >> 1) & 7; };
   const auto fetch = [&](int step, int buffer) {
-    // a wave's load fills 16 rows of a plane; the tile has T / 16 of them for each plane
+    // a wave's load fills 8 rows, both parts of them; the tile has T / 8 of them for each operand
 #pragma unroll
     for (int k = 0; k < T / 16; ++k) {
-      const int piece = k * 4 + wave;                 // of 4 planes x T / 16
-      const int which = piece / (T / 16), rows = piece % (T / 16) * 16;
-      const int row = rows + lane / 4, group = (lane & 3) ^ ((row >> 1) & 3);
-      const _Float16* base = which < 2 ? p + which * p_plane + static_cast<int64_t>(ti * T + row) * depth
-                                       : q + (which - 2) * q_plane + static_cast<int64_t>(tj * T + row) * depth;
-      load_to_lds(base + step * kStep + group * 8, &lds[buffer][which][rows * kStep]);
+      const int piece = k * 4 + wave, which = piece / (T / 8), first = piece % (T / 8) * 8;
+      const int row = first + lane / 8, group = (lane & 7) ^ turned(row);
+      const _Float16* base = which ? q + static_cast<int64_t>(tj * T + row) * depth * 2
+                                   : p + static_cast<int64_t>(ti * T + row) * depth * 2;
+      load_to_lds(base + step * (2 * kStep) + group * 8, &lds[buffer][which][first * 2 * kStep]);
     }
   };
   f32x16 acc[N][N] = {};
@@ -477,25 +484,28 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
   for (int s = 0; s < steps; ++s) {
     const int buffer = s & 1;
     if (s + 1 < steps) fetch(s + 1, buffer ^ 1);
+    // all of a step's operands are on their way before the first product waits for its own
+    half8 op[kStep / 16][4][N];
 #pragma unroll
-    for (int k = 0; k < kStep / 16; ++k) {
-      half8 op[4][N];
+    for (int k = 0; k < kStep / 16; ++k)
 #pragma unroll
       for (int which = 0; which < 4; ++which)
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-          const int row = (which < 2 ? wi : wj) + n * 32 + (lane & 31), group = k * 2 + lane / 32;
-          op[which][n] = *reinterpret_cast<const half8*>(&lds[buffer][which][row * kStep + (group ^ ((row >> 1) & 3)) * 8]);
+          const int row = (which < 2 ? wi : wj) + n * 32 + (lane & 31), group = (which & 1) * 4 + k * 2 + lane / 32;
+          op[k][which][n] = *reinterpret_cast<const half8*>(&lds[buffer][which / 2][row * 2 * kStep + (group ^ turned(row)) * 8]);
         }
+#pragma unroll
+    for (int k = 0; k < kStep / 16; ++k)
       // (hi lo', lo hi', hi hi': consecutive instructions go to different accumulators)
 #pragma unroll
-      for (int q = 0; q < 3; ++q)
+      for (int c = 0; c < 3; ++c)
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
           for (int j = 0; j < N; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[q == 1 ? 1 : 0][i], op[q == 0 ? 3 : 2][j], acc[i][j], 0, 0, 0);
-    }
+            acc[i][j] =
+                __builtin_amdgcn_mfma_f32_32x32x16_f16(op[k][c == 1 ? 1 : 0][i], op[k][c == 0 ? 3 : 2][j], acc[i][j], 0, 0, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
@@ -513,12 +523,11 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
         float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = acc[i][j][k + r];
-        const int64_t across = static_cast<int64_t>(column) * m.mp + row;        // in what has rows of m entries
+        const int64_t across = paired_at(column, row, m.mp);                     // in what has rows of m entries
         if constexpr (PHASE == kPoly || PHASE == kApply || PHASE == kLast) {
           const _Float16* old = PHASE == kPoly ? gram : xt;
-          const int64_t old_plane = PHASE == kPoly ? square : plane;
           const half4 hi = *reinterpret_cast<const half4*>(old + across);
-          const half4 lo = *reinterpret_cast<const half4*>(old + old_plane + across);
+          const half4 lo = *reinterpret_cast<const half4*>(old + across + kPair);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             v[r] = PHASE == kPoly ? fmaf(a.b_kept, joined(hi[r], lo[r]), a.c_kept * v[r])
@@ -534,9 +543,9 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
         if constexpr (PHASE == kLast) {
           update.write(m, row, column, v);
         } else {
-          _Float16* const turned = PHASE == kGram ? gram : PHASE == kPoly ? poly : xt_next;      // [column][row]
+          _Float16* const mirror = PHASE == kGram ? gram : PHASE == kPoly ? poly : xt_next;      // [column][row]
           _Float16* const plain = PHASE == kGram ? gram : PHASE == kPoly ? poly : x;             // [row][column]
-          const int64_t out_plane = PHASE == kApply ? plane : square, wide = PHASE == kApply ? m.np : m.mp;
+          const int64_t wide = PHASE == kApply ? m.np : m.mp;
           half4 hi, lo;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -544,13 +553,14 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
             split(v[r], h, l);
             hi[r] = h, lo[r] = l;
           }
-          *reinterpret_cast<half4*>(turned + across) = hi;
-          *reinterpret_cast<half4*>(turned + out_plane + across) = lo;
+          *reinterpret_cast<half4*>(mirror + across) = hi;
+          *reinterpret_cast<half4*>(mirror + across + kPair) = lo;
           if (!kSym || ti != tj) {       // (a tile on the diagonal holds its own mirror image)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              plain[(row + r) * wide + column] = hi[r];
-              plain[out_plane + (row + r) * wide + column] = lo[r];
+              const int64_t at = paired_at(row + r, column, wide);
+              plain[at] = hi[r];
+              plain[at + kPair] = lo[r];
             }
           }
         }
@@ -562,9 +572,11 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
 // ---------------------------------------------------------------------------------------------------------
 
 // Where the group of 8 halves `group` of row `row` lies in LDS, rows of `groups` such groups: turned with the row, so
-// that the groups that 8 lanes read fill all banks.
+// that the groups that 16 lanes read fill all 64 banks.
+__device__ __forceinline__ int turn_of(int row, int groups) { return row / (16 / groups) & (groups - 1); }
+
 __device__ __forceinline__ int turned_at(int row, int group, int groups) {
-  return (row * groups + (groups == 4 ? group ^ ((row >> 1) & 3) : group ^ (row & 7))) * 8;
+  return (row * groups + (group ^ turn_of(row, groups))) * 8;
 }
 
 // Block `b` of the upper triangle, column by column.
@@ -660,8 +672,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
 #pragma unroll
       for (int k = 0; k < 2 * kPart * kGroups / 256; ++k) {
         const int piece = k * 4 + wave, p = piece / (kPart * kGroups / 64), group = piece % (kPart * kGroups / 64) * 64;
-        const int j = (group + lane) / kGroups, turned = (group + lane) % kGroups;
-        const int from = kGroups == 4 ? turned ^ ((j >> 1) & 3) : turned ^ (j & 7);
+        const int j = (group + lane) / kGroups, from = (group + lane) % kGroups ^ turn_of(j, kGroups);
         load_to_lds(xt + p * plane + at + (j * kGroups + from) * 8, &lds.xt[p][group * 8]);
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
