@@ -392,15 +392,32 @@ struct Update {
     rate = lr * m.rate;
   }
 
-  // Rows row .. row + 3 (along the shorter side) of a column.
-  __device__ __forceinline__ void write(const MuonMatrix& m, int row, int column, const float (&v)[4]) const {
-    const int shorter = m.transposed ? m.cols : m.rows, longer = m.transposed ? m.rows : m.cols;
-    if (column >= longer) return;
+  // Consecutive results along a row of the result, from (row, column) on.
+  template <int N>
+  __device__ __forceinline__ void write(const MuonMatrix& m, int row, int column, const float (&v)[N]) const {
+    if (row >= m.rows) return;
+    float* const to = m.out + static_cast<int64_t>(row) * m.cols + column;
+#pragma unroll
+    for (int q = 0; q < N; q += 4) {
+      const int count = m.cols - column - q;
+      if (count <= 0) return;
+      mf4 t = m.momentum ? load_quad(to + q, count) : mf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[r] = m.momentum ? keep * t[r] - rate * (v[q + r] * kUnscale) : v[q + r] * kUnscale;
+      store_quad(to + q, count, t);
+    }
+  }
+
+  // Four consecutive results along the shorter side.
+  __device__ __forceinline__ void write_short(const MuonMatrix& m, int row, int column, const float (&v)[4]) const {
+    if (m.transposed) {
+      write<4>(m, column, row, v);
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (row + r < shorter) {
-        float* to = m.out + (m.transposed ? static_cast<int64_t>(column) * m.cols + row + r
-                                          : static_cast<int64_t>(row + r) * m.cols + column);
+      if (row + r < m.rows && column < m.cols) {
+        float* const to = m.out + static_cast<int64_t>(row + r) * m.cols + column;
         const float x = v[r] * kUnscale;
         *to = m.momentum ? keep * *to - rate * x : x;
       }
@@ -426,13 +443,40 @@ __device__ __forceinline__ uint32_t tile_of(uint32_t block) {
 
 int64_t tile_grid(int64_t tiles) { return up_to(tiles, kXcds * kUnit); }
 
+// At most N of the wave's loads are still on their way, and then all waves go on: a barrier that leaves the others in
+// flight (__syncthreads waits for all).
+template <int N>
+__device__ __forceinline__ void wait_for_loads() {
+  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+  else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// All waves have their operands out of LDS.
+__device__ __forceinline__ void wait_for_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Where an entry of a tile of results lies in LDS: rows of a column side by side, in groups of four that are turned with
+// the column, so that neither 16 columns' groups nor 16 groups of 8 columns' single entries meet in a bank.
+template <int T>
+__device__ __forceinline__ int tile_at(int column, int row) {
+  return column * T + (row ^ (((column ^ (column >> 3)) & 15) * 4));
+}
+
 // One tile of P Q^T: T x T, four waves of (T/2) x (T/2).  Rows of 32 reduction entries (128 bytes with both parts) lie in
 // LDS in eight groups of 16 bytes, whose order is turned with the row so that 16 rows' groups fill all banks; they come
 // straight from global memory (a lane picks the group that belongs to its place), one step ahead of the products.
 template <int T, int PHASE>
 __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonArgs a, uint32_t tiles, int step) {
   constexpr int N = T / 64;                        // 32 x 32 products of a wave, each way
-  __shared__ _Float16 lds[2][2][T * 2 * kStep];    // rows of P and of Q, hi and lo parts
+  __shared__ __align__(16) _Float16 lds[2][2][T * 2 * kStep];     // rows of P and of Q, hi and lo parts
+  static_assert(sizeof(lds) >= sizeof(float) * T * T);
+  float* const results = reinterpret_cast<float*>(lds);             // of the tile, behind the last step
   if (skipped(a)) return;
   constexpr bool kSym = PHASE == kGram || PHASE == kPoly;
   const uint32_t tile = tile_of(blockIdx.x);
@@ -465,7 +509,7 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
   const int wi = (wave & 1) * (T / 2), wj = (wave >> 1) * (T / 2);
   // (16 lanes read 16 rows at a time, from 64 banks: the groups of every other row are in the same ones)
   const auto turned = [](int row) { return (row >> 1) & 7; };
-  const auto fetch = [&](int step, int buffer) {
+  const auto fetch = [&](int at, int buffer) {
     // a wave's load fills 8 rows, both parts of them; the tile has T / 8 of them for each operand
 #pragma unroll
     for (int k = 0; k < T / 16; ++k) {
@@ -473,18 +517,19 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
       const int row = first + lane / 8, group = (lane & 7) ^ turned(row);
       const _Float16* base = which ? q + static_cast<int64_t>(tj * T + row) * depth * 2
                                    : p + static_cast<int64_t>(ti * T + row) * depth * 2;
-      load_to_lds(base + step * (2 * kStep) + group * 8, &lds[buffer][which][first * 2 * kStep]);
+      load_to_lds(base + at * (2 * kStep) + group * 8, &lds[buffer][which][first * 2 * kStep]);
     }
   };
+  // Two steps' rows are in LDS or on their way there.  A step's operands go to registers as a whole, so that its place
+  // in LDS is free for the step after the next while its products run.
+  constexpr int kLoads = T / 16;                   // of a wave and step
   f32x16 acc[N][N] = {};
   const int steps = depth / kStep;
   fetch(0, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  if (steps > 1) fetch(1, 1);
   for (int s = 0; s < steps; ++s) {
     const int buffer = s & 1;
-    if (s + 1 < steps) fetch(s + 1, buffer ^ 1);
-    // all of a step's operands are on their way before the first product waits for its own
+    if (s + 1 < steps) wait_for_loads<kLoads>(); else wait_for_loads<0>();
     half8 op[kStep / 16][4][N];
 #pragma unroll
     for (int k = 0; k < kStep / 16; ++k)
@@ -495,6 +540,10 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
           const int row = (which < 2 ? wi : wj) + n * 32 + (lane & 31), group = (which & 1) * 4 + k * 2 + lane / 32;
           op[k][which][n] = *reinterpret_cast<const half8*>(&lds[buffer][which / 2][row * 2 * kStep + (group ^ turned(row)) * 8]);
         }
+    if (s + 2 < steps) {
+      wait_for_lds();
+      fetch(s + 2, buffer);
+    }
 #pragma unroll
     for (int k = 0; k < kStep / 16; ++k)
       // (hi lo', lo hi', hi hi': consecutive instructions go to different accumulators)
@@ -506,65 +555,103 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
           for (int j = 0; j < N; ++j)
             acc[i][j] =
                 __builtin_amdgcn_mfma_f32_32x32x16_f16(op[k][c == 1 ? 1 : 0][i], op[k][c == 0 ? 3 : 2][j], acc[i][j], 0, 0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
   }
+  __syncthreads();
 
-  // A lane holds rows 8 (k / 4) + 4 (lane / 32) + k % 4 of column lane % 32 of each 32 x 32 product.
-  const int shift = shift_of<PHASE>(a, owner, step);
-  const Update update = PHASE == kLast ? Update(a, m) : Update();
+  // Results leave through LDS, in whole lines.  A lane holds rows 8 (k / 4) + 4 (lane / 32) + k % 4 of column lane % 32 of
+  // each 32 x 32 product.
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j)
 #pragma unroll
       for (int k = 0; k < 16; k += 4) {
-        const int row = ti * T + wi + i * 32 + 2 * k + 4 * (lane / 32), column = tj * T + wj + j * 32 + (lane & 31);
-        float v[4];
+        const int row = wi + i * 32 + 2 * k + 4 * (lane / 32), column = wj + j * 32 + (lane & 31);
+        mf4 v;
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = acc[i][j][k + r];
-        const int64_t across = paired_at(column, row, m.mp);                     // in what has rows of m entries
-        if constexpr (PHASE == kPoly || PHASE == kApply || PHASE == kLast) {
-          const _Float16* old = PHASE == kPoly ? gram : xt;
-          const half4 hi = *reinterpret_cast<const half4*>(old + across);
-          const half4 lo = *reinterpret_cast<const half4*>(old + across + kPair);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            v[r] = PHASE == kPoly ? fmaf(a.b_kept, joined(hi[r], lo[r]), a.c_kept * v[r])
-                                  : fmaf(a.a, joined(hi[r], lo[r]), a.unpoly * v[r]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] *= kUnscale;
-        }
-        if (PHASE != kPoly && shift) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], shift);
-        }
-        if constexpr (PHASE == kLast) {
-          update.write(m, row, column, v);
-        } else {
-          _Float16* const mirror = PHASE == kGram ? gram : PHASE == kPoly ? poly : xt_next;      // [column][row]
-          _Float16* const plain = PHASE == kGram ? gram : PHASE == kPoly ? poly : x;             // [row][column]
-          const int64_t wide = PHASE == kApply ? m.np : m.mp;
-          half4 hi, lo;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            _Float16 h, l;
-            split(v[r], h, l);
-            hi[r] = h, lo[r] = l;
-          }
-          *reinterpret_cast<half4*>(mirror + across) = hi;
-          *reinterpret_cast<half4*>(mirror + across + kPair) = lo;
-          if (!kSym || ti != tj) {       // (a tile on the diagonal holds its own mirror image)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int64_t at = paired_at(row + r, column, wide);
-              plain[at] = hi[r];
-              plain[at + kPair] = lo[r];
-            }
-          }
-        }
+        *reinterpret_cast<mf4*>(&results[tile_at<T>(column, row)]) = v;
       }
+  __syncthreads();
+  const int shift = shift_of<PHASE>(a, owner, step);
+  const Update update = PHASE == kLast ? Update(a, m) : Update();
+  // columns of the tile, 8 rows of one at a time: rows of what has its rows along the shorter side
+  for (int unit = threadIdx.x; unit < T * T / 8; unit += kMuThreads) {
+    const int column = unit / (T / 8), row = unit % (T / 8) * 8;
+    const int64_t across = paired_at(tj * T + column, ti * T + row, m.mp);
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; q += 4) {
+      const mf4 t = *reinterpret_cast<const mf4*>(&results[tile_at<T>(column, row + q)]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[q + r] = t[r];
+    }
+    if constexpr (PHASE == kGram) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] *= kUnscale;
+    } else {
+      const _Float16* old = (PHASE == kPoly ? gram : xt) + across;
+      const half8 hi = *reinterpret_cast<const half8*>(old), lo = *reinterpret_cast<const half8*>(old + kPair);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        v[r] = PHASE == kPoly ? fmaf(a.b_kept, joined(hi[r], lo[r]), a.c_kept * v[r])
+                              : fmaf(a.a, joined(hi[r], lo[r]), a.unpoly * v[r]);
+    }
+    if (PHASE != kPoly && shift) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = ldexpf(v[r], shift);
+    }
+    uint32_t kept[8];
+    if constexpr (PHASE == kLast) {
+      if (m.transposed) update.write<8>(m, tj * T + column, ti * T + row, v);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) kept[r] = __float_as_uint(v[r]);
+    } else {
+      _Float16* const mirror = (PHASE == kGram ? gram : PHASE == kPoly ? poly : xt_next) + across;
+      half8 hi, lo;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        _Float16 h, l;
+        split(v[r], h, l);
+        hi[r] = h, lo[r] = l;
+        kept[r] = __builtin_bit_cast(uint16_t, h) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, l)) << 16;
+      }
+      *reinterpret_cast<half8*>(mirror) = hi;
+      *reinterpret_cast<half8*>(mirror + kPair) = lo;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; q += 4)
+      *reinterpret_cast<mf4*>(&results[tile_at<T>(column, row + q)]) =
+          mf4{__uint_as_float(kept[q]), __uint_as_float(kept[q + 1]), __uint_as_float(kept[q + 2]),
+              __uint_as_float(kept[q + 3])};
+  }
+  if (kSym ? ti == tj : PHASE == kLast && m.transposed) return;      // (a tile on the diagonal holds its mirror image)
+  __syncthreads();
+  // rows of the tile, 8 columns of one at a time
+  _Float16* const plain = PHASE == kGram ? gram : PHASE == kPoly ? poly : x;
+  const int64_t wide = PHASE == kApply ? m.np : m.mp;
+  for (int unit = threadIdx.x; unit < T * T / 8; unit += kMuThreads) {
+    const int row = unit / (T / 8), column = unit % (T / 8) * 8;
+    uint32_t kept[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) kept[r] = __float_as_uint(results[tile_at<T>(column + r, row)]);
+    if constexpr (PHASE == kLast) {
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = __uint_as_float(kept[r]);
+      update.write<8>(m, ti * T + row, tj * T + column, v);
+    } else {
+      half8 hi, lo;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        hi[r] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(kept[r]));
+        lo[r] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(kept[r] >> 16));
+      }
+      _Float16* const to = plain + paired_at(ti * T + row, tj * T + column, wide);
+      *reinterpret_cast<half8*>(to) = hi;
+      *reinterpret_cast<half8*>(to + kPair) = lo;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -702,7 +789,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
               if (shift) v[r] = ldexpf(v[r], shift);
             }
             if constexpr (PHASE == kLast) {
-              update.write(m, row, part * kPart + j, v);
+              update.write_short(m, row, part * kPart + j, v);
             } else {
               half4 hi, lo;
 #pragma unroll
