@@ -1078,9 +1078,9 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
     MuonTable table;
     int n = 0;
     const auto send = [&]() {
-      if (n)
-        hipLaunchKernelGGL(muon_setup_kernel<T>, dim3(n), dim3(kMuThreads), 0, stream, table, ws + g.at_values(), matrices,
-                           prep, sym, apply, chunk);
+      if (!n) return static_cast<int>(ICTC_OK);
+      hipLaunchKernelGGL(muon_setup_kernel<T>, dim3(n), dim3(kMuThreads), 0, stream, table, ws + g.at_values(), matrices,
+                         prep, sym, apply, chunk);
       n = 0;
       return muon_launched();
     };

@@ -26,6 +26,14 @@ block of a residual stream, for stacks of more interactions than plain sums carr
 with s = 1 / sqrt(interactions), the readouts on y_{t+1}, and the norms, gate and sum of a block's end in one
 kernel (``gated_residual_norm``).
 
+``radial_norm=True`` (no counterpart in the reference; off by default) gives each hidden layer of the radial MLP a
+layer norm before its SiLU, for deeper training at larger learning rates, and with ``edge_species`` the first one a
+row of a table for each pair of species, which the gates otherwise do not see:
+
+  h = silu(norm(W1 bessel(r) + T[s_src, s_dst])),  then twice h = silu(norm(W h));  gates = W4 (u(r) h)
+
+with the cutoff envelope u on the last hidden layer, since a normalised layer does not vanish with its input.
+
 Dense layers (radial MLP, channel linears, readouts) go through ``mace_hip.linear`` (one GEMM
 per layer and degree; weight gradients reduced in row blocks).  The edge directions and the
 Bessel x cutoff embedding come from ``mace_hip.embedding`` (one HIP kernel per derivative order).
@@ -45,7 +53,7 @@ bit-identical from run to run.
 from __future__ import annotations
 
 import math
-from typing import Dict, List, Optional
+from typing import Dict, List, NamedTuple, Optional
 
 import torch
 import torch.nn as nn
@@ -53,8 +61,10 @@ import torch.nn.functional as F
 
 from ictc_o3.backends.hip.degree_linear import (DegreeLinearPlan, degree_linear, degree_linear_adjoint,
                                                  degree_linear_mul_ir)
+from ictc_o3.backends.hip.embedding import embedding
 from ictc_o3.backends.hip.graph_message import message_bonds, packed_graph_message
 from ictc_o3.backends.hip.harmonics import direction_harmonics_packed
+from ictc_o3.backends.hip.layer_norm import layer_norm
 from ictc_o3.backends.hip.norms import equivariant_norm, gated_residual_norm
 from ictc_o3.backends.hip.radial_message import fold_projection, packed_radial_graph_message
 from ictc_o3.basis.ictd_irreps import EdgeWeightedPathPreservingTensorProduct
@@ -66,7 +76,7 @@ from .activation import silu
 from .embedding import edge_embedding
 from .geometry import edge_vectors, one_hot_rows
 from .linear import Linear, linear
-from .radial import bessel_embedding
+from .radial import bessel_embedding, polynomial_cutoff
 
 SILU_SCALE = 1.6791767923989418   # _Normalize2MomSiLU (pure_cartesian_ictd_fix.py:610-619)
 
@@ -80,6 +90,27 @@ def tp_paths(input_lmax: int, edge_lmax: int, target_lmax: int):
 class NormalizedSiLU(nn.Module):
     def forward(self, x):
         return F.silu(x) * SILU_SCALE
+
+
+class NormSiLU(nn.Module):
+    """Layer norm and the SiLU behind it, one kernel (``layer_norm``)."""
+
+    def __init__(self, width: int):
+        super().__init__()
+        self.weight, self.bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, activation="silu")
+
+
+class EdgeExtras(NamedTuple):
+    """What a normalised radial MLP takes beside the radial features: the cutoff envelope [E], and the edges' pairs
+    of species (s_src S + s_dst) where the model has a table of them."""
+    envelope: torch.Tensor
+    pairs: Optional[torch.Tensor]
+
+    def tensors(self):
+        return [t for t in self if t is not None]
 
 
 def _mace_linear(fan_in: int, fan_out: int) -> Linear:
@@ -166,9 +197,12 @@ class IrrepsLinear(nn.Module):
 
 
 class Interaction(nn.Module):
+    radial_norm = edge_species = False      # (of modules pickled before they had them)
+
     def __init__(self, *, channels: int, input_lmax: int, edge_lmax: int, num_elements: int, num_basis: int,
-                 avg_num_neighbors: float):
+                 avg_num_neighbors: float, radial_norm: bool = False, edge_species: bool = False):
         super().__init__()
+        self.radial_norm, self.edge_species = bool(radial_norm), bool(edge_species)
         self.channels, self.input_lmax, self.edge_lmax = channels, input_lmax, edge_lmax
         self.avg_num_neighbors = float(avg_num_neighbors)
         self.linear_up = ChannelLinear(channels, input_lmax)
@@ -177,9 +211,11 @@ class Interaction(nn.Module):
         with torch.no_grad():
             self.tp.weight.fill_(1.0)          # _init_path_tp_weight_to_one_, then frozen
         self.tp.weight.requires_grad_(False)
-        self.fc = nn.Sequential(_mace_linear(num_basis, 64), NormalizedSiLU(), _mace_linear(64, 64),
-                                NormalizedSiLU(), _mace_linear(64, 64), NormalizedSiLU(),
-                                _mace_linear(64, self.tp.num_paths * channels))
+        activation = (lambda: NormSiLU(64)) if self.radial_norm else NormalizedSiLU
+        self.fc = nn.Sequential(_mace_linear(num_basis, 64), activation(), _mace_linear(64, 64), activation(),
+                                _mace_linear(64, 64), activation(), _mace_linear(64, self.tp.num_paths * channels))
+        if self.edge_species:
+            self.edge_embedding = nn.Parameter(torch.randn(num_elements * num_elements, 64))
         self.message_linear = MessageLinear(self.tp.path_counts_by_l, channels, edge_lmax)
         # None: the gates are one [E, P*C] tensor; an int: radial streaming over receiver ranges of
         # at most that many edges (the reference's _ascend_edge_chunk_size)
@@ -187,14 +223,21 @@ class Interaction(nn.Module):
         self._gate_weight = None   # (weights' identity and version, folded last-layer weight) when frozen
         self.self_connection = SpeciesLinear(num_elements, channels)
 
-    def radial_hidden(self, edge_feats):
+    def radial_hidden(self, edge_feats, extras=None):
         """self.fc up to its last Linear: (the last layer's input [E, 64], its weight [P*C, 64]),
         each normalised SiLU's constant folded into the next layer's weight instead of scaling
         the [E, 64] activations.  On the GPU the three layers and their activations run as one
         kernel per derivative order (mace_hip.radial_mlp)."""
-        return self._hidden(edge_feats), self.fc[-1].weight * SILU_SCALE
+        return self._hidden(edge_feats, extras), self.fc[-1].weight * SILU_SCALE
 
-    def _hidden(self, edge_feats):
+    def _hidden(self, edge_feats, extras=None):
+        if self.radial_norm:
+            h = self.fc[0](edge_feats)
+            if self.edge_species:
+                h = h + embedding(extras.pairs, self.edge_embedding)
+            for module in self.fc[1:-1]:
+                h = module(h)
+            return h * extras.envelope.unsqueeze(1)
         layers = [m for m in self.fc if isinstance(m, nn.Linear)]
         w = [lin.weight for lin in layers]
         if len(layers) == 4 and radial_mlp.supported(edge_feats, *w[:3]):
@@ -204,18 +247,18 @@ class Interaction(nn.Module):
             h = linear(silu(h), lin.weight * SILU_SCALE)
         return silu(h)
 
-    def radial_mlp(self, edge_feats):
+    def radial_mlp(self, edge_feats, extras=None):
         """self.fc on the edge features: the gates [E, P*C]."""
-        hidden, weight = self.radial_hidden(edge_feats)
+        hidden, weight = self.radial_hidden(edge_feats, extras)
         return linear(hidden, weight)
 
-    def message_gates(self, edge_feats):
+    def message_gates(self, edge_feats, extras=None):
         """The gates times the TP's frozen path weight (the reference's gates * weight,
         ``backends/ascend/packed_tensor_product.py:163-164``), folded into the rows of the radial
         MLP's last weight ([P*C, 64]) rather than applied to the [E, P*C] gates.  With no gradient
         to either weight the folded [P*C, 64] weight is kept until one of them is replaced or
         modified in place."""
-        hidden = self._hidden(edge_feats)
+        hidden = self._hidden(edge_feats, extras)
         last = self.fc[-1].weight
         if torch.is_grad_enabled() and (last.requires_grad or self.tp.weight.requires_grad):
             return linear(hidden, last * SILU_SCALE * self.tp.weight.reshape(-1, 1))
@@ -228,9 +271,11 @@ class Interaction(nn.Module):
         """The bond rows the message forward derives from the harmonics (see forward's bonds)."""
         return message_bonds(self.tp.hip_plan(self.input_lmax, self.edge_lmax), harmonics)
 
-    def forward(self, h, harmonics, edge_feats, src, dst, mask, species, scalars=None, gates=None, bonds=None):
+    def forward(self, h, harmonics, edge_feats, src, dst, mask, species, scalars=None, gates=None, bonds=None,
+                extras=None):
         """mask: the reference multiplies the gates by (r <= r_max) (:1801-1808).  The radial
-        features carry the cutoff envelope, exactly 0 from r_max on, and fc has no biases, so
+        features carry the cutoff envelope, exactly 0 from r_max on, and fc has no biases (a
+        normalised one is multiplied by the envelope behind them), so
         the gates are already exactly 0 wherever the mask is 0: the product is an identity and
         is skipped (mask is accepted for the signature).  scalars: h's l = 0 block as its own
         tensor when the caller has it (the previous product's), so the self connection does not
@@ -242,12 +287,12 @@ class Interaction(nn.Module):
         plan = self.tp.hip_plan(self.input_lmax, self.edge_lmax)
         if self.edge_chunk_size is None:
             if gates is None:
-                gates = self.message_gates(edge_feats)
+                gates = self.message_gates(edge_feats, extras)
             m = packed_graph_message(plan, x1, harmonics, gates, src, dst, nodes_dst=n, bonds=bonds)
         else:
             # the radial MLP's last layer produced one receiver range at a time inside the message
             # (reference capacity mode, capacity_message.py:109-179): no [E, P*C] gate tensor
-            hidden, weight = self.radial_hidden(edge_feats)
+            hidden, weight = self.radial_hidden(edge_feats, extras)
             weight, _ = fold_projection(self.tp, plan, weight, None)
             m = packed_radial_graph_message(plan, x1, harmonics, hidden, weight, None, src, dst, nodes_dst=n,
                                             edge_chunk_size=self.edge_chunk_size)
@@ -290,12 +335,16 @@ def _side_stream(device: torch.device) -> "torch.cuda.Stream":
 
 
 class MaceICTC(nn.Module):
-    block_norm = False      # (of modules pickled before they had it)
+    block_norm = radial_norm = edge_species = False      # (of modules pickled before they had them)
 
     def __init__(self, *, channels: int = 128, lmax: int = 3, num_interactions: int = 2, correlation: int = 3,
                  atomic_numbers=tuple(range(1, 11)), cutoff: float = 5.0, avg_num_neighbors: float = 50.0,
-                 num_basis: int = 8, cutoff_p: int = 5, readout_hidden: int = 16, block_norm: bool = False):
+                 num_basis: int = 8, cutoff_p: int = 5, readout_hidden: int = 16, block_norm: bool = False,
+                 radial_norm: bool = False, edge_species: bool = False):
         super().__init__()
+        if edge_species and not radial_norm:
+            raise ValueError("edge_species needs radial_norm (gates that vanish at the cutoff)")
+        self.radial_norm, self.edge_species = bool(radial_norm), bool(edge_species)
         self.channels, self.lmax, self.cutoff = int(channels), int(lmax), float(cutoff)
         self.num_basis, self.cutoff_p = int(num_basis), int(cutoff_p)
         # radial MLPs and gates on a second stream beside the interactions (GPU, whole gates)
@@ -313,7 +362,8 @@ class MaceICTC(nn.Module):
         for t, target in enumerate(targets):
             self.interactions.append(Interaction(channels=self.channels, input_lmax=0 if t == 0 else self.lmax,
                                                  edge_lmax=self.lmax, num_elements=self.num_elements,
-                                                 num_basis=self.num_basis, avg_num_neighbors=avg_num_neighbors))
+                                                 num_basis=self.num_basis, avg_num_neighbors=avg_num_neighbors,
+                                                 radial_norm=radial_norm, edge_species=edge_species))
             self.products.append(Product(channels=self.channels, lmax=self.lmax, target_lmax=target,
                                          correlation=correlation, num_elements=self.num_elements))
         # EquivariantScalarReadoutSO3 (pure_cartesian_ictd_layers.py:46-70) per inner layer and the
@@ -381,7 +431,13 @@ class MaceICTC(nn.Module):
             h = linear(one_hot_rows(species, self.num_elements), self.node_embedding.weight)
         else:
             h = self.node_embedding.weight.t().index_select(0, species)
-        side = self._side_work(edge_feats, harmonics)
+        extras = None
+        if self.radial_norm:
+            pairs = None
+            if self.edge_species:
+                pairs = species.index_select(0, edge_src) * self.num_elements + species.index_select(0, edge_dst)
+            extras = EdgeExtras(polynomial_cutoff(vec.norm(dim=1), self.cutoff, self.cutoff_p), pairs)
+        side = self._side_work(edge_feats, harmonics, extras)
         energy = None
         if self.block_norm:
             stream, h = h, equivariant_norm(h, self.input_norm, channels=self.channels)
@@ -394,7 +450,7 @@ class MaceICTC(nn.Module):
                 gates, bonds, ready = side[t]
                 torch.cuda.current_stream(pos.device).wait_event(ready)
             message, sc = interaction(h, harmonics, edge_feats, edge_src, edge_dst, mask, species, scalars,
-                                      gates, bonds)
+                                      gates, bonds, extras)
             if self.block_norm:
                 gate = self.block_gates[t](scalars)
                 stream, h = gated_residual_norm(stream, product(message, sc, species)[0], gate,
@@ -430,7 +486,7 @@ class MaceICTC(nn.Module):
         w_lin = self.layer_readouts[len(self.interactions) - 2].weight
         return w_lin.shape[0] == 1 and readout_supported(scalars, scalars, w_lin, lin1.weight, lin2.weight)
 
-    def _side_work(self, edge_feats, harmonics):
+    def _side_work(self, edge_feats, harmonics, extras=None):
         """Each interaction's message gates (radial MLP and its [E, P*C] last layer) and bond rows,
         issued on a second stream: they depend only on the edge features and harmonics, so
         interaction t+1's run beside interaction t's message, contraction and linears, and the
@@ -446,7 +502,7 @@ class MaceICTC(nn.Module):
         out = []
         with torch.cuda.stream(side):
             for interaction in self.interactions:
-                gates = interaction.message_gates(edge_feats)
+                gates = interaction.message_gates(edge_feats, extras)
                 bonds = interaction.message_bonds(harmonics)
                 ev = torch.cuda.Event()
                 ev.record(side)
@@ -455,6 +511,23 @@ class MaceICTC(nn.Module):
             gates.record_stream(main)
             if bonds is not None:
                 bonds.record_stream(main)
-        for t in (edge_feats, harmonics):   # read on the side stream: not reusable on the main one before
+        read = (edge_feats, harmonics, *(() if extras is None else extras.tensors()))
+        for t in read:   # read on the side stream: not reusable on the main one before
             t.record_stream(side)
         return out
+
+
+def split_parameters(model: nn.Module):
+    """(matrices, others) of a model's trained parameters: the weights of its linear maps, whose updates can be
+    orthogonalised (``ictc_o3.optim.Muon``), and everything else (tables, per-channel weights, norms, biases, maps of
+    one output) for an optimizer of single values."""
+    maps = []
+    for module in model.modules():
+        if isinstance(module, (ChannelLinear, MessageLinear, IrrepsLinear)):
+            maps += list(module.weights)
+        elif isinstance(module, SpeciesLinear) or (isinstance(module, nn.Linear)
+                                                   and module is not getattr(model, "node_embedding", None)):
+            maps.append(module.weight)
+    matrices = {id(p) for p in maps if p.dim() >= 2 and min(p.shape[-2:]) > 1}
+    trained = [p for p in model.parameters() if p.requires_grad]
+    return [p for p in trained if id(p) in matrices], [p for p in trained if id(p) not in matrices]

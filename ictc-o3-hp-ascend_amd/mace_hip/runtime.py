@@ -29,9 +29,11 @@ from .model import MaceICTC
 
 def create_model(*, channels=64, lmax=3, edge_lmax=None, num_interactions=2, correlation=3,
                  atomic_numbers=(1, 6, 8), cutoff=5.0, avg_num_neighbors=50.0, device="cuda",
-                 dtype=torch.float32, seed=None, block_norm=False) -> MaceICTC:
-    """The model with the reference's arguments; ``block_norm`` (no counterpart there) gives every block norms
-    before and after it, a gate and a residual stream (see ``mace_hip.model``)."""
+                 dtype=torch.float32, seed=None, block_norm=False, radial_norm=False,
+                 edge_species=False) -> MaceICTC:
+    """The model with the reference's arguments; ``block_norm`` (no counterpart there, as the next two) gives every
+    block norms before and after it, a gate and a residual stream, ``radial_norm`` the radial MLPs' hidden layers
+    layer norms, and ``edge_species`` those a table for the pairs of species (see ``mace_hip.model``)."""
     if dtype != torch.float32:
         raise ValueError("the HIP operators compute in float32")
     if not isinstance(num_interactions, int) or isinstance(num_interactions, bool) or num_interactions < 1:
@@ -48,7 +50,7 @@ def create_model(*, channels=64, lmax=3, edge_lmax=None, num_interactions=2, cor
         torch.manual_seed(int(seed))
     model = MaceICTC(channels=channels, lmax=lmax, num_interactions=num_interactions, correlation=correlation,
                      atomic_numbers=atomic_numbers, cutoff=cutoff, avg_num_neighbors=avg_num_neighbors,
-                     block_norm=block_norm)
+                     block_norm=block_norm, radial_norm=radial_norm, edge_species=edge_species)
     return model.to(device=device, dtype=dtype)
 
 
@@ -240,7 +242,7 @@ class CapturedEnergyAndForces:
 class CapturedTrainingStep:
     """One force-loss training step (energy + forces with create_graph, loss backward, optimizer
     step) captured once and replayed on new positions.  The optimizer must keep its state on
-    the device (``ictc_o3.optim.AdamW``, or ``torch.optim.AdamW(..., capturable=True)``, which may also be
+    the device (``ictc_o3.optim.AdamW``, ``Muon`` or both ``Together``, or ``torch.optim.AdamW(..., capturable=True)``, which may also be
     ``fused=True``: one update kernel for all parameters, 0.3 ms less per cfg-4 step); gradients are released before
     capture so that backward writes them into the graph's own buffers on every replay.  A replay raises the
     parameters' version counters as an eager step does: what frozen evaluations keep of the weights (folded
