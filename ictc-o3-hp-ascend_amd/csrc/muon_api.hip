@@ -66,9 +66,11 @@ struct MuonTensor {
 
 struct MuonTable {
   MuonTensor tensor[kTensorsPerLaunch];
+  int32_t count;
 };
 
-static_assert(sizeof(MuonTable) + 128 <= 4096, "kernel arguments are limited to 4 KB");
+static_assert(sizeof(MuonTable) + 320 <= 4096, "kernel arguments are limited to 4 KB");
+static_assert(kTensorsPerLaunch <= kMuWave, "a wave looks through the table");
 
 // One matrix, in the workspace.  With a shorter side of up to 128: X^T [np][mp], two planes; B [mp][mp]; the parts of
 // X X^T.  Else: X [mp][np], two planes; then X^T twice [np][mp], A and B [mp][mp].
@@ -80,9 +82,10 @@ struct MuonMatrix {
   int32_t rows, cols, mp, np;
   uint32_t prep, prep_tiles, prep_across;      // tiles of the source
   uint32_t sym, apply;                         // tiles of products
-  uint32_t chunk, chunks, chunk_parts;         // chunks of columns, of `chunk_parts` times 64
+  uint32_t chunk, chunks, chunk_parts;         // chunks of columns, of `chunk_parts` times kPart
   float rate;
   int32_t transposed;                          // more rows than columns
+  uint32_t owner;                              // its index
 };
 
 // The first kind keeps planes of hi and lo parts; the second one 32 hi parts and their 32 lo parts side by side (kPair
@@ -95,7 +98,8 @@ __host__ __device__ constexpr int64_t paired_at(int64_t row, int64_t column, int
 
 struct MuonArgs {
   const MuonMatrix* matrices;
-  const uint32_t *prep_owner, *sym_owner, *apply_owner, *chunk_owner;
+  const MuonMatrix* chunks;  // the matrix of each chunk of columns (a copy: one load less to wait for)
+  const uint32_t *prep_owner, *sym_owner, *apply_owner;
   double* squares;           // of each tile of the source
   int32_t* exponents;        // of each matrix: X is kept times 2^e at first
   const float* clip;
@@ -112,9 +116,10 @@ __device__ __forceinline__ bool skipped(const MuonArgs& a) { return a.clip && a.
 constexpr int64_t up_to(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 constexpr int kShort = 128;                  // shorter sides of matrices that are done in chunks of columns
-constexpr int kPart = 64;                    // columns in LDS at a time
+constexpr int kPart = 128;                   // columns in LDS at a time
 constexpr int kChunks = 24;                  // of a matrix, unless they get longer than kLongest parts
-constexpr int kLongest = 8;
+constexpr int kLongest = 4;
+constexpr int kShortThreads = 512;
 
 // Tiles and bytes of one matrix; sides padded to multiples of T, or for short ones to 32, 64 or 128 and kPart.
 struct MuonSize {
@@ -150,40 +155,51 @@ __host__ __device__ MuonSize muon_size(int64_t rows, int64_t cols) {
   return s;
 }
 
-// Descriptions of every matrix of the table's tensors, and the owners of their tiles: a workgroup to a tensor.
+// Where the descriptions and the owners of tiles lie.
+struct MuonTables {
+  char* workspace;
+  MuonMatrix *matrices, *chunks;
+  uint32_t *prep_owner, *sym_owner, *apply_owner;
+};
+
 template <int T>
-__global__ void __launch_bounds__(kMuThreads)
-muon_setup_kernel(const MuonTable table, char* __restrict__ workspace, MuonMatrix* __restrict__ matrices,
-                  uint32_t* __restrict__ prep_owner, uint32_t* __restrict__ sym_owner, uint32_t* __restrict__ apply_owner,
-                  uint32_t* __restrict__ chunk_owner) {
-  const MuonTensor& t = table.tensor[blockIdx.x];
-  const MuonSize s = muon_size<T>(t.rows, t.cols);
+__device__ __forceinline__ MuonMatrix matrix_of(const MuonTensor& t, const MuonSize& s, char* workspace, int b) {
   const int64_t values = static_cast<int64_t>(t.rows) * t.cols;
+  MuonMatrix m;
+  m.src = t.src + b * values;
+  m.momentum = t.momentum ? t.momentum + b * values : nullptr;
+  m.out = t.out + b * values;
+  m.x = workspace + t.base + b * s.bytes;
+  m.rows = t.rows, m.cols = t.cols, m.mp = static_cast<int32_t>(s.mp), m.np = static_cast<int32_t>(s.np);
+  m.prep = t.prep + static_cast<uint32_t>(b * s.prep), m.prep_tiles = static_cast<uint32_t>(s.prep);
+  m.prep_across = static_cast<uint32_t>(s.across);
+  m.sym = t.sym + static_cast<uint32_t>(b * s.sym);
+  m.apply = t.apply + static_cast<uint32_t>(b * s.apply);
+  m.chunk = t.chunk + static_cast<uint32_t>(b * s.chunks), m.chunks = static_cast<uint32_t>(s.chunks);
+  m.chunk_parts = static_cast<uint32_t>(s.parts);
+  m.rate = t.rate;
+  m.transposed = t.rows > t.cols;
+  m.owner = t.first + static_cast<uint32_t>(b);
+  return m;
+}
+
+// Descriptions of a tensor's matrices, and the owners of their tiles.
+template <int T>
+__device__ __forceinline__ void describe(const MuonTensor& t, const MuonTables& to) {
+  const MuonSize s = muon_size<T>(t.rows, t.cols);
   for (int b = threadIdx.x; b < t.batches; b += kMuThreads) {
-    MuonMatrix m;
-    m.src = t.src + b * values;
-    m.momentum = t.momentum ? t.momentum + b * values : nullptr;
-    m.out = t.out + b * values;
-    m.x = workspace + t.base + b * s.bytes;
-    m.rows = t.rows, m.cols = t.cols, m.mp = static_cast<int32_t>(s.mp), m.np = static_cast<int32_t>(s.np);
-    m.prep = t.prep + static_cast<uint32_t>(b * s.prep), m.prep_tiles = static_cast<uint32_t>(s.prep);
-    m.prep_across = static_cast<uint32_t>(s.across);
-    m.sym = t.sym + static_cast<uint32_t>(b * s.sym);
-    m.apply = t.apply + static_cast<uint32_t>(b * s.apply);
-    m.chunk = t.chunk + static_cast<uint32_t>(b * s.chunks), m.chunks = static_cast<uint32_t>(s.chunks);
-    m.chunk_parts = static_cast<uint32_t>(s.parts);
-    m.rate = t.rate;
-    m.transposed = t.rows > t.cols;
-    matrices[t.first + b] = m;
+    const MuonMatrix m = matrix_of<T>(t, s, to.workspace, b);
+    to.matrices[m.owner] = m;
   }
+  for (int64_t k = threadIdx.x; k < t.batches * s.chunks; k += kMuThreads)
+    to.chunks[t.chunk + k] = matrix_of<T>(t, s, to.workspace, static_cast<int>(k / s.chunks));
   const auto own = [&](uint32_t* owner, uint32_t first, int64_t each) {
     for (int64_t k = threadIdx.x; k < t.batches * each; k += kMuThreads)
       owner[first + k] = t.first + static_cast<uint32_t>(k / each);
   };
-  own(prep_owner, t.prep, s.prep);
-  own(sym_owner, t.sym, s.sym);
-  own(apply_owner, t.apply, s.apply);
-  own(chunk_owner, t.chunk, s.chunks);
+  if (!s.is_short) own(to.prep_owner, t.prep, s.prep);
+  own(to.sym_owner, t.sym, s.sym);
+  own(to.apply_owner, t.apply, s.apply);
 }
 
 // A tile of the source: its first row and column there, and what of it there is.
@@ -198,6 +214,7 @@ struct SourceTile {
   }
 };
 
+template <int THREADS = kMuThreads>
 __device__ __forceinline__ double muon_block_sum(double x, double* part) {
 #pragma unroll
   for (int d = kMuWave / 2; d; d >>= 1) x += __shfl_xor(x, d);
@@ -205,7 +222,7 @@ __device__ __forceinline__ double muon_block_sum(double x, double* part) {
   __syncthreads();
   double sum = 0.0;
 #pragma unroll
-  for (int w = 0; w < kMuThreads / kMuWave; ++w) sum += part[w];
+  for (int w = 0; w < THREADS / kMuWave; ++w) sum += part[w];
   return sum;
 }
 
@@ -238,12 +255,26 @@ __device__ __forceinline__ void store_quad(float* p, int count, const mf4& v) {
 constexpr int kQuadRows = kMuThreads / (kPrep / 4), kPasses = kPrep / kQuadRows;   // a tile's rows at a time, and times
 
 // Moving averages, and the sum of squares (in 64 bits) of each tile of what is orthogonalised.  Bound by memory: 12
-// bytes a value (momentum read and written, gradient read); all loads before the first store.
-__global__ void __launch_bounds__(kMuThreads) muon_average_kernel(const MuonArgs a) {
+// bytes a value (momentum read and written, gradient read); all loads before the first store.  The last workgroups
+// describe the table's tensors, one each, for the launches behind.
+template <int T>
+__global__ void __launch_bounds__(kMuThreads)
+muon_average_kernel(const MuonTable table, const MuonArgs a, const MuonTables to, uint32_t first_tile, uint32_t tiles) {
   __shared__ double part[kMuThreads / kMuWave];
+  if (blockIdx.x >= tiles) {
+    describe<T>(table.tensor[blockIdx.x - tiles], to);
+    return;
+  }
   if (skipped(a)) return;
-  const MuonMatrix m = a.matrices[a.prep_owner[blockIdx.x]];
-  const SourceTile t(m, blockIdx.x - m.prep);
+  // the tensor that the tile is of: the last one that begins at or before it
+  const uint32_t tile = first_tile + blockIdx.x;
+  const int lane = threadIdx.x & (kMuWave - 1);
+  const int at = __builtin_amdgcn_readfirstlane(
+      __popcll(__ballot(lane < table.count && table.tensor[lane < table.count ? lane : 0].prep <= tile)) - 1);
+  const MuonTensor& tensor = table.tensor[at];
+  const MuonSize size = muon_size<T>(tensor.rows, tensor.cols);
+  const MuonMatrix m = matrix_of<T>(tensor, size, nullptr, static_cast<int>((tile - tensor.prep) / static_cast<uint32_t>(size.prep)));
+  const SourceTile t(m, tile - m.prep);
   const float scale = a.clip ? a.clip[1] : 1.f;
   const int column = threadIdx.x % (kPrep / 4) * 4, count = t.cols - column, first = threadIdx.x / (kPrep / 4);
   const int64_t from = static_cast<int64_t>(t.r0 + first) * m.cols + t.c0 + column;
@@ -273,7 +304,7 @@ __global__ void __launch_bounds__(kMuThreads) muon_average_kernel(const MuonArgs
     for (int j = 0; j < 4; ++j) sum += static_cast<double>(u[k][j]) * static_cast<double>(u[k][j]);
   }
   sum = muon_block_sum(sum, part);
-  if (threadIdx.x == 0) a.squares[blockIdx.x] = sum;
+  if (threadIdx.x == 0) a.squares[tile] = sum;
 }
 
 __device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
@@ -298,11 +329,12 @@ __device__ __forceinline__ int exponent_at(const MuonArgs& a, int e, int step) {
 
 // What a matrix's values are multiplied by at first (its power of two among it), from its tiles' squares; every
 // workgroup of the matrix calls it, and the one that is told to keeps the exponent.
+template <int THREADS = kMuThreads>
 __device__ __forceinline__ double first_scale(const MuonArgs& a, const MuonMatrix& m, uint32_t owner, bool keeps,
                                               double* part) {
   double sum = 0.0;
-  for (uint32_t k = threadIdx.x; k < m.prep_tiles; k += kMuThreads) sum += a.squares[m.prep + k];
-  const double norm = sqrt(muon_block_sum(sum, part)), share = norm / (norm + a.eps);
+  for (uint32_t k = threadIdx.x; k < m.prep_tiles; k += THREADS) sum += a.squares[m.prep + k];
+  const double norm = sqrt(muon_block_sum<THREADS>(sum, part)), share = norm / (norm + a.eps);
   const int e = share > 0.0 && share < 0.5 ? min(-ilogb(share) - 1, kMostExponent) : 0;
   if (threadIdx.x == 0 && keeps) a.exponents[owner] = e;
   return ldexp(kScale / (norm + a.eps), e);
@@ -407,21 +439,6 @@ struct Update {
       store_quad(to + q, count, t);
     }
   }
-
-  // Four consecutive results along the shorter side.
-  __device__ __forceinline__ void write_short(const MuonMatrix& m, int row, int column, const float (&v)[4]) const {
-    if (m.transposed) {
-      write<4>(m, column, row, v);
-      return;
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (row + r < m.rows && column < m.cols) {
-        float* const to = m.out + static_cast<int64_t>(row + r) * m.cols + column;
-        const float x = v[r] * kUnscale;
-        *to = m.momentum ? keep * *to - rate * x : x;
-      }
-  }
 };
 
 // 16 bytes a lane from global memory to consecutive places of LDS.
@@ -465,7 +482,7 @@ __device__ __forceinline__ void wait_for_lds() {
 // the column, so that neither 16 columns' groups nor 16 groups of 8 columns' single entries meet in a bank.
 template <int T>
 __device__ __forceinline__ int tile_at(int column, int row) {
-  return column * T + (row ^ (((column ^ (column >> 3)) & 15) * 4));
+  return column * T + (row ^ (((column ^ (column >> 3)) & (T < 64 ? T / 4 - 1 : 15)) * 4));
 }
 
 // One tile of P Q^T: T x T, four waves of (T/2) x (T/2).  Rows of 32 reduction entries (128 bytes with both parts) lie in
@@ -679,18 +696,37 @@ __device__ __forceinline__ void three_products(const half8& ah, const half8& al,
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
 }
 
-// LDS of a chunk's workgroup: 64 columns of X, their rows along the columns (as they lie in memory), and along the rows.
+// LDS of a chunk's workgroup: kPart columns of X, as their rows lie in X^T; the last step's results.
 struct ShortLds {
   _Float16 xt[2][kPart * kShort];
-  _Float16 x[2][kShort * kPart];
-  double part[kMuThreads / kMuWave];
+  double part[kShortThreads / kMuWave];
 };
+
+using short4v = short __attribute__((ext_vector_type(4)));
+
+// Eight entries along the columns of a row of X (a lane's operand for X X^T), from rows of X^T in LDS: the hardware turns
+// blocks of 4 of its rows and 16 of its columns as it reads them, 16 lanes to a block.  row0: first of the wave's 32 rows
+// of X; j0: first of 16 columns, of which a lane has those from 8 (lane / 32) on.
+__device__ __forceinline__ half8 turned_operand(const _Float16* plane, int row0, int j0, int groups) {
+  const int lane = threadIdx.x & (kMuWave - 1), of = lane & 15;
+  const int row = row0 + (lane & 16) + (of & 3) * 4, j = j0 + lane / 32 * 8 + of / 4;
+  half8 v;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const _Float16* const from = plane + turned_at(j + 4 * q, row / 8, groups) + row % 8;
+    const short4v t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<short4v __attribute__((address_space(3)))*>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from))));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[4 * q + r] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(t[r]));
+  }
+  return v;
+}
 
 // The products of one chunk of columns, MB x 32 rows (see the top).  kFirst: the columns come from the source.
 template <int PHASE, int MB>
-__device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix& m, uint32_t owner, int step,
-                                            ShortLds& lds) {
-  constexpr int M = 32 * MB, kGroups = M / 8, kBlocks = MB * (MB + 1) / 2, kMine = (kBlocks + 3) / 4;
+__device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix& m, int step, ShortLds& lds) {
+  constexpr int kWaves = kShortThreads / kMuWave;
+  constexpr int M = 32 * MB, kGroups = M / 8, kBlocks = MB * (MB + 1) / 2, kMine = (kBlocks + kWaves - 1) / kWaves;
   constexpr int kTiles = MB == 4 ? 2 : 1;          // 32 x 32 products of a wave
   const int lane = threadIdx.x & (kMuWave - 1), wave = threadIdx.x / kMuWave, half = lane / 32;
   const int64_t plane = static_cast<int64_t>(m.np) * M;
@@ -699,73 +735,66 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
   const uint32_t chunk = blockIdx.x - m.chunk;
   const int first = static_cast<int>(chunk * m.chunk_parts), all = m.np / kPart;
   const int end = first + static_cast<int>(m.chunk_parts) < all ? first + static_cast<int>(m.chunk_parts) : all;
-  const int row0 = (MB == 4 ? wave : MB == 2 ? wave & 1 : 0) * 32;                  // of a wave's products
-  const int col0 = (MB == 4 ? 0 : MB == 2 ? wave >> 1 : wave) * 32;
-  const bool works = MB > 1 || wave < 2;
-
-  double inv = 0.0;
-  float scale = 1.f;
-  if constexpr (PHASE == kFirst) {
-    if (a.clip) scale = a.clip[1];
-  }
-  half8 b_op[2][PHASE == kFirst ? 1 : M / 16];
-  if constexpr (PHASE != kFirst) {
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int k = 0; k < M / 16; ++k)
-        b_op[p][k] = *reinterpret_cast<const half8*>(poly + p * M * M + (row0 + (lane & 31)) * M + k * 16 + half * 8);
-  }
-  const int shift = shift_of<PHASE>(a, owner, step);
-  const Update update = PHASE == kLast ? Update(a, m) : Update();
+  const int row0 = wave % MB * 32, col0 = wave / MB * (32 * kTiles);        // of a wave's products
+  const bool works = col0 < kPart;
   f32x16 gram[kMine] = {};
 
   for (int part = first; part < end; ++part) {
-    const int64_t at = static_cast<int64_t>(part) * kPart * M;       // of the columns in X^T
+    _Float16* const columns = xt + static_cast<int64_t>(part) * kPart * M;
     if constexpr (PHASE == kFirst) {
       // rows of the source: of the matrix, or (transposed) of its columns; four values of one at a time
-      constexpr int kQuads = M * kPart / 4 / kMuThreads;
+      constexpr int kQuads = M * kPart / 4 / kShortThreads;
       Source source[kQuads];
 #pragma unroll
       for (int q = 0; q < kQuads; ++q) {
-        const int k = q * kMuThreads + threadIdx.x;
+        const int k = q * kShortThreads + threadIdx.x;
         const int i = m.transposed ? k / (M / 4) + part * kPart : k / (kPart / 4);
         const int j = m.transposed ? k % (M / 4) * 4 : k % (kPart / 4) * 4 + part * kPart;
         source[q].load(a, m, static_cast<int64_t>(i) * m.cols + j, i < m.rows ? m.cols - j : 0);
       }
-      if (part == first) inv = first_scale(a, m, owner, chunk == 0, lds.part);
+      const float scale = a.clip ? a.clip[1] : 1.f;
+      const double inv = first_scale<kShortThreads>(a, m, m.owner, chunk == 0 && part == first, lds.part);
 #pragma unroll
       for (int q = 0; q < kQuads; ++q) {
-        const int k = q * kMuThreads + threadIdx.x;
+        const int k = q * kShortThreads + threadIdx.x;
+        half4 hi, lo;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = m.transposed ? k % (M / 4) * 4 + r : k / (kPart / 4);        // of X
-          const int j = m.transposed ? k / (M / 4) : k % (kPart / 4) * 4 + r;
           _Float16 h, l;
           split(source[q].value(a, m, r, scale, inv), h, l);
-          const int in_x = turned_at(i, j / 8, kPart / 8) + j % 8, in_xt = turned_at(j, i / 8, kGroups) + i % 8;
-          lds.x[0][in_x] = h, lds.x[1][in_x] = l;
-          lds.xt[0][in_xt] = h, lds.xt[1][in_xt] = l;
+          hi[r] = h, lo[r] = l;
+        }
+        if (m.transposed) {
+          const int i = k % (M / 4) * 4, to = turned_at(k / (M / 4), i / 8, kGroups) + i % 8;
+          *reinterpret_cast<half4*>(&lds.xt[0][to]) = hi;
+          *reinterpret_cast<half4*>(&lds.xt[1][to]) = lo;
+        } else {
+          const int i = k / (kPart / 4), j = k % (kPart / 4) * 4;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int to = turned_at(j + r, i / 8, kGroups) + i % 8;
+            lds.xt[0][to] = hi[r], lds.xt[1][to] = lo[r];
+          }
         }
       }
-      __syncthreads();
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-        for (int k = threadIdx.x; k < kPart * kGroups; k += kMuThreads)
-          *reinterpret_cast<half8*>(xt + p * plane + at + k * 8) =
-              *reinterpret_cast<const half8*>(&lds.xt[p][turned_at(k / kGroups, k % kGroups, kGroups)]);
     } else {
       // a wave's load fills 64 groups of a plane
 #pragma unroll
-      for (int k = 0; k < 2 * kPart * kGroups / 256; ++k) {
-        const int piece = k * 4 + wave, p = piece / (kPart * kGroups / 64), group = piece % (kPart * kGroups / 64) * 64;
-        const int j = (group + lane) / kGroups, from = (group + lane) % kGroups ^ turn_of(j, kGroups);
-        load_to_lds(xt + p * plane + at + (j * kGroups + from) * 8, &lds.xt[p][group * 8]);
+      for (int k = 0; k < 2 * kPart * kGroups / kShortThreads; ++k) {
+        const int piece = k * kWaves + wave, p = piece / (kPart * kGroups / 64), group = piece % (kPart * kGroups / 64) * 64;
+        const int j = (group + lane) / kGroups, turned = (group + lane) % kGroups ^ turn_of(j, kGroups);
+        load_to_lds(columns + p * plane + (j * kGroups + turned) * 8, &lds.xt[p][group * 8]);
       }
+      half8 b_op[2][M / 16];
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int k = 0; k < M / 16; ++k)
+          b_op[p][k] = *reinterpret_cast<const half8*>(poly + p * M * M + (row0 + (lane & 31)) * M + k * 16 + half * 8);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
+      f32x16 acc[kTiles] = {};
       if (works) {
-        f32x16 acc[kTiles] = {};
 #pragma unroll
         for (int k = 0; k < M / 16; ++k)
 #pragma unroll
@@ -774,63 +803,89 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
             three_products(b_op[0][k], b_op[1][k], *reinterpret_cast<const half8*>(&lds.xt[0][from]),
                            *reinterpret_cast<const half8*>(&lds.xt[1][from]), acc[t]);
           }
+      }
+      const int shift = shift_of<PHASE>(a, m.owner, step);
+      __syncthreads();         // all products have their operands: their places take the results
+      if (works) {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
           for (int k = 0; k < 16; k += 4) {
             const int row = row0 + 2 * k + 4 * half, j = col0 + t * 32 + (lane & 31);
-            const int from = turned_at(j, row / 8, kGroups) + row % 8;
-            const half4 old_hi = *reinterpret_cast<const half4*>(&lds.xt[0][from]);
-            const half4 old_lo = *reinterpret_cast<const half4*>(&lds.xt[1][from]);
-            float v[4];
+            const int at = turned_at(j, row / 8, kGroups) + row % 8;
+            half4 hi = *reinterpret_cast<const half4*>(&lds.xt[0][at]), lo = *reinterpret_cast<const half4*>(&lds.xt[1][at]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              v[r] = fmaf(a.a, joined(old_hi[r], old_lo[r]), a.unpoly * acc[t][k + r]);
-              if (shift) v[r] = ldexpf(v[r], shift);
-            }
-            if constexpr (PHASE == kLast) {
-              update.write_short(m, row, part * kPart + j, v);
-            } else {
-              half4 hi, lo;
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
+              float v = fmaf(a.a, joined(hi[r], lo[r]), a.unpoly * acc[t][k + r]);
+              if (shift) v = ldexpf(v, shift);
+              if constexpr (PHASE == kLast) {
+                acc[t][k + r] = v;
+              } else {
                 _Float16 h, l;
-                split(v[r], h, l);
+                split(v, h, l);
                 hi[r] = h, lo[r] = l;
-                const int to = turned_at(row + r, j / 8, kPart / 8) + j % 8;
-                lds.x[0][to] = h, lds.x[1][to] = l;
               }
-              *reinterpret_cast<half4*>(xt + at + j * M + row) = hi;
-              *reinterpret_cast<half4*>(xt + plane + at + j * M + row) = lo;
+            }
+            if constexpr (PHASE != kLast) {
+              *reinterpret_cast<half4*>(&lds.xt[0][at]) = hi;
+              *reinterpret_cast<half4*>(&lds.xt[1][at]) = lo;
             }
           }
       }
-      __syncthreads();
+      if constexpr (PHASE == kLast) {
+        __syncthreads();
+        float* const results = reinterpret_cast<float*>(lds.xt);
+        static_assert(sizeof(lds.xt) >= sizeof(float) * kPart * M);
+        if (works) {
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int k = 0; k < 16; k += 4)
+              *reinterpret_cast<mf4*>(&results[tile_at<M>(col0 + t * 32 + (lane & 31), row0 + 2 * k + 4 * half)]) =
+                  mf4{acc[t][k], acc[t][k + 1], acc[t][k + 2], acc[t][k + 3]};
+        }
+        __syncthreads();
+        const Update update(a, m);
+        for (int unit = threadIdx.x; unit < kPart * M / 8; unit += kShortThreads) {
+          float v[8];
+          const int j = m.transposed ? unit / (M / 8) : unit % (kPart / 8) * 8;
+          const int i = m.transposed ? unit % (M / 8) * 8 : unit / (kPart / 8);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) v[r] = results[m.transposed ? tile_at<M>(j, i + r) : tile_at<M>(j + r, i)];
+          if (m.transposed) update.write<8>(m, part * kPart + j, i, v); else update.write<8>(m, i, part * kPart + j, v);
+        }
+      }
     }
+    __syncthreads();
     if constexpr (PHASE != kLast) {
 #pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int k = 0; k < kPart * kGroups / kShortThreads; ++k) {
+          const int group = k * kShortThreads + threadIdx.x;
+          *reinterpret_cast<half8*>(columns + p * plane + group * 8) =
+              *reinterpret_cast<const half8*>(&lds.xt[p][turned_at(group / kGroups, group % kGroups, kGroups)]);
+        }
+#pragma unroll
       for (int q = 0; q < kMine; ++q) {
-        const int b = wave + 4 * q;
+        const int b = wave + kWaves * q;
         if (b >= kBlocks) continue;
         int bi, bj;
         upper_block(b, bi, bj);
-#pragma unroll
-        for (int k = 0; k < kPart / 16; ++k) {
-          const int i = turned_at(bi * 32 + (lane & 31), k * 2 + half, kPart / 8);
-          const int j = turned_at(bj * 32 + (lane & 31), k * 2 + half, kPart / 8);
-          three_products(*reinterpret_cast<const half8*>(&lds.x[0][i]), *reinterpret_cast<const half8*>(&lds.x[1][i]),
-                         *reinterpret_cast<const half8*>(&lds.x[0][j]), *reinterpret_cast<const half8*>(&lds.x[1][j]),
+#pragma unroll 2
+        for (int k = 0; k < kPart; k += 16)
+          three_products(turned_operand(lds.xt[0], bi * 32, k, kGroups), turned_operand(lds.xt[1], bi * 32, k, kGroups),
+                         turned_operand(lds.xt[0], bj * 32, k, kGroups), turned_operand(lds.xt[1], bj * 32, k, kGroups),
                          gram[q]);
-        }
       }
-      __syncthreads();
+      if (part + 1 < end) __syncthreads();
     }
   }
   if constexpr (PHASE != kLast) {
     float* const parts = reinterpret_cast<float*>(xt + 2 * plane + 2 * M * M) + static_cast<int64_t>(chunk) * kBlocks * 1024;
 #pragma unroll
     for (int q = 0; q < kMine; ++q) {
-      const int b = wave + 4 * q;
+      const int b = wave + kWaves * q;
       if (b >= kBlocks) continue;
 #pragma unroll
       for (int k = 0; k < 16; k += 4) {
@@ -844,14 +899,13 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
 }
 
 template <int PHASE>
-__global__ void __launch_bounds__(kMuThreads) muon_chunk_kernel(const MuonArgs a, int step) {
-  __shared__ ShortLds lds;
+__global__ void __launch_bounds__(kShortThreads) muon_chunk_kernel(const MuonArgs a, int step) {
+  __shared__ __align__(16) ShortLds lds;
   if (skipped(a)) return;
-  const uint32_t owner = a.chunk_owner[blockIdx.x];
-  const MuonMatrix m = a.matrices[owner];
-  if (m.mp == 128) short_chunk<PHASE, 4>(a, m, owner, step, lds);
-  else if (m.mp == 64) short_chunk<PHASE, 2>(a, m, owner, step, lds);
-  else short_chunk<PHASE, 1>(a, m, owner, step, lds);
+  const MuonMatrix m = a.chunks[blockIdx.x];
+  if (m.mp == 128) short_chunk<PHASE, 4>(a, m, step, lds);
+  else if (m.mp == 64) short_chunk<PHASE, 2>(a, m, step, lds);
+  else short_chunk<PHASE, 1>(a, m, step, lds);
 }
 
 constexpr int kPolyThreads = 512;
@@ -973,7 +1027,7 @@ struct MuonGroup {
   int64_t at_sym() const { return at_prep() + up_to(4 * prep, 256); }
   int64_t at_apply() const { return at_sym() + up_to(4 * sym, 256); }
   int64_t at_chunk() const { return at_apply() + up_to(4 * apply, 256); }
-  int64_t at_squares() const { return at_chunk() + up_to(4 * chunks, 256); }
+  int64_t at_squares() const { return at_chunk() + up_to(chunks * static_cast<int64_t>(sizeof(MuonMatrix)), 256); }
   int64_t at_exponents() const { return at_squares() + up_to(8 * prep, 256); }
   int64_t at_values() const { return at_exponents() + up_to(4 * matrices, 256); }
   int64_t size() const { return at_values() + bytes; }
@@ -1069,19 +1123,21 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
     uint32_t* const prep = owners(g.at_prep());
     uint32_t* const sym = owners(g.at_sym());
     uint32_t* const apply = owners(g.at_apply());
-    uint32_t* const chunk = owners(g.at_chunk());
-    a.matrices = matrices, a.prep_owner = prep, a.sym_owner = sym, a.apply_owner = apply, a.chunk_owner = chunk;
+    MuonMatrix* const chunk = reinterpret_cast<MuonMatrix*>(ws + g.at_chunk());
+    a.matrices = matrices, a.prep_owner = prep, a.sym_owner = sym, a.apply_owner = apply, a.chunks = chunk;
+    const MuonTables tables{ws + g.at_values(), matrices, chunk, prep, sym, apply};
     a.squares = reinterpret_cast<double*>(ws + g.at_squares());
     a.exponents = reinterpret_cast<int32_t*>(ws + g.at_exponents());
     // those that take part, the ones with long shorter sides first
     MuonGroup at = {}, longs = {};
     MuonTable table;
-    int n = 0;
+    table.count = 0;
+    int64_t sent = 0;        // tiles of the tables before
     const auto send = [&]() {
-      if (!n) return static_cast<int>(ICTC_OK);
-      hipLaunchKernelGGL(muon_setup_kernel<T>, dim3(n), dim3(kMuThreads), 0, stream, table, ws + g.at_values(), matrices,
-                         prep, sym, apply, chunk);
-      n = 0;
+      if (!table.count) return static_cast<int>(ICTC_OK);
+      hipLaunchKernelGGL(muon_average_kernel<T>, dim3(static_cast<unsigned>(at.prep - sent + table.count)), dim3(kMuThreads),
+                         0, stream, table, a, tables, static_cast<uint32_t>(sent), static_cast<uint32_t>(at.prep - sent));
+      table.count = 0, sent = at.prep;
       return muon_launched();
     };
     // (and of those the longest first: their tiles take longest)
@@ -1095,7 +1151,7 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
         const MuonSize s = muon_size<T>(rows[t], cols[t]);
         if (s.is_short != (shorts != 0)) continue;
         const double r = static_cast<double>(rows[t]), c = static_cast<double>(cols[t]);
-        MuonTensor& e = table.tensor[n++];
+        MuonTensor& e = table.tensor[table.count++];
         e.src = src[t], e.momentum = momentum ? momentum[t] : nullptr, e.out = out[t];
         e.base = at.bytes, e.rows = static_cast<int32_t>(rows[t]), e.cols = static_cast<int32_t>(cols[t]);
         e.batches = static_cast<int32_t>(batches[t]), e.first = static_cast<int32_t>(at.matrices);
@@ -1103,7 +1159,7 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
         e.apply = static_cast<uint32_t>(at.apply), e.chunk = static_cast<uint32_t>(at.chunks);
         e.rate = static_cast<float>(d->adjust == ICTC_MUON_SHAPE ? sqrt(r > c ? r / c : 1.0) : 0.2 * sqrt(r > c ? r : c));
         at.add(s, batches[t]);
-        if (n == kTensorsPerLaunch)
+        if (table.count == kTensorsPerLaunch)
           if (const int rc = send()) return rc;
       }
       if (!shorts) longs = at;
@@ -1112,14 +1168,13 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
     k = g.end;
     if (!at.matrices) continue;
     const auto launch = [&](void (*kernel)(MuonArgs, int), int64_t grid, int step) {
-      if (grid) hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kMuThreads), 0, stream, a, step);
+      if (grid) hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kShortThreads), 0, stream, a, step);
     };
     const auto product = [&](void (*kernel)(MuonArgs, uint32_t, int), int64_t tiles, int step) {
       if (tiles)
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tile_grid(tiles))), dim3(kMuThreads), 0, stream, a,
                            static_cast<uint32_t>(tiles), step);
     };
-    hipLaunchKernelGGL(muon_average_kernel, dim3(static_cast<unsigned>(at.prep)), dim3(kMuThreads), 0, stream, a);
     if (longs.matrices)
       hipLaunchKernelGGL(muon_normalise_kernel, dim3(static_cast<unsigned>(longs.prep)), dim3(kMuThreads), 0, stream, a);
     launch(muon_chunk_kernel<kFirst>, at.chunks, 0);
