@@ -696,6 +696,13 @@ __device__ __forceinline__ void three_products(const half8& ah, const half8& al,
   acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
 }
 
+// Where an entry of B lies: in the order in which a wave's lanes take it as an operand, 32 rows and 16 columns at a
+// time, so that a load is one piece of memory.
+template <int M>
+__device__ __forceinline__ int operand_at(int row, int column) {
+  return ((row / 32 * (M / 16) + column / 16) * 64 + column % 16 / 8 * 32 + row % 32) * 8 + column % 8;
+}
+
 // LDS of a chunk's workgroup: kPart columns of X, as their rows lie in X^T; the last step's results.
 struct ShortLds {
   _Float16 xt[2][kPart * kShort];
@@ -790,7 +797,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
       for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int k = 0; k < M / 16; ++k)
-          b_op[p][k] = *reinterpret_cast<const half8*>(poly + p * M * M + (row0 + (lane & 31)) * M + k * 16 + half * 8);
+          b_op[p][k] = *reinterpret_cast<const half8*>(poly + p * M * M + operand_at<M>(row0, k * 16) + lane * 8);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       f32x16 acc[kTiles] = {};
@@ -988,12 +995,12 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
         split(fmaf(a.b_kept, joined(old_hi[r], old_lo[r]), a.c_kept * acc[k + r]), h, l);
         hi[r] = h, lo[r] = l;
         if (bi != bj) {
-          poly[(row + r) * M + column] = h;
-          poly[M * M + (row + r) * M + column] = l;
+          poly[operand_at<M>(row + r, column)] = h;
+          poly[M * M + operand_at<M>(row + r, column)] = l;
         }
       }
-      *reinterpret_cast<half4*>(poly + column * M + row) = hi;
-      *reinterpret_cast<half4*>(poly + M * M + column * M + row) = lo;
+      *reinterpret_cast<half4*>(poly + operand_at<M>(column, row)) = hi;
+      *reinterpret_cast<half4*>(poly + M * M + operand_at<M>(column, row)) = lo;
     }
   }
 }
