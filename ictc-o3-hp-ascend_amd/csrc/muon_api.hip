@@ -327,17 +327,28 @@ __device__ __forceinline__ int exponent_at(const MuonArgs& a, int e, int step) {
   return e;
 }
 
-// What a matrix's values are multiplied by at first (its power of two among it), from its tiles' squares; every
-// workgroup of the matrix calls it, and the one that is told to keeps the exponent.
+// What a matrix's values are multiplied by at first, as a float in [1, 2) and a power of two (floats of any norm stay
+// in range).
+struct Scale {
+  float mantissa;
+  int exponent;
+
+  __device__ __forceinline__ float of(float x) const { return ldexpf(x * mantissa, exponent); }
+};
+
+// That scale from the matrix's tiles' squares (its power of two among it); every workgroup of the matrix calls it, and
+// the one that is told to keeps the exponent.
 template <int THREADS = kMuThreads>
-__device__ __forceinline__ double first_scale(const MuonArgs& a, const MuonMatrix& m, uint32_t owner, bool keeps,
+__device__ __forceinline__ Scale first_scale(const MuonArgs& a, const MuonMatrix& m, uint32_t owner, bool keeps,
                                               double* part) {
   double sum = 0.0;
   for (uint32_t k = threadIdx.x; k < m.prep_tiles; k += THREADS) sum += a.squares[m.prep + k];
   const double norm = sqrt(muon_block_sum<THREADS>(sum, part)), share = norm / (norm + a.eps);
   const int e = share > 0.0 && share < 0.5 ? min(-ilogb(share) - 1, kMostExponent) : 0;
   if (threadIdx.x == 0 && keeps) a.exponents[owner] = e;
-  return ldexp(kScale / (norm + a.eps), e);
+  const double scale = kScale / (norm + a.eps);
+  const int power = ilogb(scale);
+  return {static_cast<float>(ldexp(scale, -power)), power + e};
 }
 
 // Values of what is orthogonalised, from the source and (after muon_average_kernel) the moving average.
@@ -349,9 +360,8 @@ struct Source {
     if (m_.momentum) m = load_quad(m_.momentum + at, count);
   }
 
-  __device__ __forceinline__ float value(const MuonArgs& a, const MuonMatrix& m_, int j, float scale, double inv) const {
-    const float u = !m_.momentum ? g[j] : a.nesterov ? averaged(a, m[j], scale * g[j]) : m[j];
-    return static_cast<float>(u * inv);
+  __device__ __forceinline__ float value(const MuonArgs& a, const MuonMatrix& m_, int j, float scale, const Scale& first) const {
+    return first.of(!m_.momentum ? g[j] : a.nesterov ? averaged(a, m[j], scale * g[j]) : m[j]);
   }
 };
 
@@ -370,7 +380,7 @@ __global__ void __launch_bounds__(kMuThreads) muon_normalise_kernel(const MuonAr
     const int r = first + k * kQuadRows;
     source[k].load(a, m, static_cast<int64_t>(t.r0 + r) * m.cols + t.c0 + column, r < t.rows ? t.cols - column : 0);
   }
-  const double inv = first_scale(a, m, owner, blockIdx.x == m.prep, part);
+  const Scale inv = first_scale(a, m, owner, blockIdx.x == m.prep, part);
   const float scale = a.clip ? a.clip[1] : 1.f;
 #pragma unroll
   for (int k = 0; k < kPasses; ++k)
@@ -750,37 +760,41 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
     _Float16* const columns = xt + static_cast<int64_t>(part) * kPart * M;
     if constexpr (PHASE == kFirst) {
       // rows of the source: of the matrix, or (transposed) of its columns; four values of one at a time
-      constexpr int kQuads = M * kPart / 4 / kShortThreads;
-      Source source[kQuads];
-#pragma unroll
-      for (int q = 0; q < kQuads; ++q) {
-        const int k = q * kShortThreads + threadIdx.x;
-        const int i = m.transposed ? k / (M / 4) + part * kPart : k / (kPart / 4);
-        const int j = m.transposed ? k % (M / 4) * 4 : k % (kPart / 4) * 4 + part * kPart;
-        source[q].load(a, m, static_cast<int64_t>(i) * m.cols + j, i < m.rows ? m.cols - j : 0);
-      }
+      // (a loop, not straight code: instructions that run once have to be fetched, too)
+      constexpr int kQuads = M * kPart / 4 / kShortThreads, kAtOnce = kQuads < 4 ? kQuads : 4;
       const float scale = a.clip ? a.clip[1] : 1.f;
-      const double inv = first_scale<kShortThreads>(a, m, m.owner, chunk == 0 && part == first, lds.part);
+      const Scale inv = first_scale<kShortThreads>(a, m, m.owner, chunk == 0 && part == first, lds.part);
+#pragma unroll 1
+      for (int base = 0; base < kQuads; base += kAtOnce) {
+        Source source[kAtOnce];
 #pragma unroll
-      for (int q = 0; q < kQuads; ++q) {
-        const int k = q * kShortThreads + threadIdx.x;
-        half4 hi, lo;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          _Float16 h, l;
-          split(source[q].value(a, m, r, scale, inv), h, l);
-          hi[r] = h, lo[r] = l;
+        for (int q = 0; q < kAtOnce; ++q) {
+          const int k = (base + q) * kShortThreads + threadIdx.x;
+          const int i = m.transposed ? k / (M / 4) + part * kPart : k / (kPart / 4);
+          const int j = m.transposed ? k % (M / 4) * 4 : k % (kPart / 4) * 4 + part * kPart;
+          source[q].load(a, m, static_cast<int64_t>(i) * m.cols + j, i < m.rows ? m.cols - j : 0);
         }
-        if (m.transposed) {
-          const int i = k % (M / 4) * 4, to = turned_at(k / (M / 4), i / 8, kGroups) + i % 8;
-          *reinterpret_cast<half4*>(&lds.xt[0][to]) = hi;
-          *reinterpret_cast<half4*>(&lds.xt[1][to]) = lo;
-        } else {
-          const int i = k / (kPart / 4), j = k % (kPart / 4) * 4;
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+          const int k = (base + q) * kShortThreads + threadIdx.x;
+          half4 hi, lo;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int to = turned_at(j + r, i / 8, kGroups) + i % 8;
-            lds.xt[0][to] = hi[r], lds.xt[1][to] = lo[r];
+            _Float16 h, l;
+            split(source[q].value(a, m, r, scale, inv), h, l);
+            hi[r] = h, lo[r] = l;
+          }
+          if (m.transposed) {
+            const int i = k % (M / 4) * 4, to = turned_at(k / (M / 4), i / 8, kGroups) + i % 8;
+            *reinterpret_cast<half4*>(&lds.xt[0][to]) = hi;
+            *reinterpret_cast<half4*>(&lds.xt[1][to]) = lo;
+          } else {
+            const int i = k / (kPart / 4), j = k % (kPart / 4) * 4;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int to = turned_at(j + r, i / 8, kGroups) + i % 8;
+              lds.xt[0][to] = hi[r], lds.xt[1][to] = lo[r];
+            }
           }
         }
       }
