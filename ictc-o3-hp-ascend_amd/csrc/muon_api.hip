@@ -360,6 +360,18 @@ struct Source {
     if (m_.momentum) m = load_quad(m_.momentum + at, count);
   }
 
+  // Four of a column, as many of them as there are.
+  __device__ __forceinline__ void load_down(const MuonArgs& a, const MuonMatrix& m_, int64_t at, int count) {
+    g = m = mf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < count) {
+        const int64_t from = at + static_cast<int64_t>(r) * m_.cols;
+        if (!m_.momentum || a.nesterov) g[r] = m_.src[from];
+        if (m_.momentum) m[r] = m_.momentum[from];
+      }
+  }
+
   __device__ __forceinline__ float value(const MuonArgs& a, const MuonMatrix& m_, int j, float scale, const Scale& first) const {
     return first.of(!m_.momentum ? g[j] : a.nesterov ? averaged(a, m[j], scale * g[j]) : m[j]);
   }
@@ -759,7 +771,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
   for (int part = first; part < end; ++part) {
     _Float16* const columns = xt + static_cast<int64_t>(part) * kPart * M;
     if constexpr (PHASE == kFirst) {
-      // rows of the source: of the matrix, or (transposed) of its columns; four values of one at a time
+      // four values of a column of X at a time: of a row of the source if it is transposed, else of four rows
       // (a loop, not straight code: instructions that run once have to be fetched, too)
       constexpr int kQuads = M * kPart / 4 / kShortThreads, kAtOnce = kQuads < 4 ? kQuads : 4;
       const float scale = a.clip ? a.clip[1] : 1.f;
@@ -770,9 +782,13 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
 #pragma unroll
         for (int q = 0; q < kAtOnce; ++q) {
           const int k = (base + q) * kShortThreads + threadIdx.x;
-          const int i = m.transposed ? k / (M / 4) + part * kPart : k / (kPart / 4);
-          const int j = m.transposed ? k % (M / 4) * 4 : k % (kPart / 4) * 4 + part * kPart;
-          source[q].load(a, m, static_cast<int64_t>(i) * m.cols + j, i < m.rows ? m.cols - j : 0);
+          if (m.transposed) {
+            const int row = k / (M / 4) + part * kPart, column = k % (M / 4) * 4;
+            source[q].load(a, m, static_cast<int64_t>(row) * m.cols + column, row < m.rows ? m.cols - column : 0);
+          } else {
+            const int row = k / kPart * 4, column = k % kPart + part * kPart;
+            source[q].load_down(a, m, static_cast<int64_t>(row) * m.cols + column, column < m.cols ? m.rows - row : 0);
+          }
         }
 #pragma unroll
         for (int q = 0; q < kAtOnce; ++q) {
@@ -784,18 +800,10 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
             split(source[q].value(a, m, r, scale, inv), h, l);
             hi[r] = h, lo[r] = l;
           }
-          if (m.transposed) {
-            const int i = k % (M / 4) * 4, to = turned_at(k / (M / 4), i / 8, kGroups) + i % 8;
-            *reinterpret_cast<half4*>(&lds.xt[0][to]) = hi;
-            *reinterpret_cast<half4*>(&lds.xt[1][to]) = lo;
-          } else {
-            const int i = k / (kPart / 4), j = k % (kPart / 4) * 4;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int to = turned_at(j + r, i / 8, kGroups) + i % 8;
-              lds.xt[0][to] = hi[r], lds.xt[1][to] = lo[r];
-            }
-          }
+          const int i = m.transposed ? k % (M / 4) * 4 : k / kPart * 4, j = m.transposed ? k / (M / 4) : k % kPart;
+          const int to = turned_at(j, i / 8, kGroups) + i % 8;
+          *reinterpret_cast<half4*>(&lds.xt[0][to]) = hi;
+          *reinterpret_cast<half4*>(&lds.xt[1][to]) = lo;
         }
       }
     } else {
