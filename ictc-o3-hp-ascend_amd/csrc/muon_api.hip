@@ -232,23 +232,34 @@ __device__ __forceinline__ float averaged(const MuonArgs& a, float m, float g) {
   return a.beta * m + a.rest * g;
 }
 
+// Global memory behind addresses that come out of memory, which the compiler cannot tell from LDS by itself.
+template <typename V, typename T>
+__device__ __forceinline__ V from_global(const T* p) {
+  return *reinterpret_cast<const V __attribute__((address_space(1)))*>(reinterpret_cast<uintptr_t>(p));
+}
+
+template <typename V, typename T>
+__device__ __forceinline__ void to_global(T* p, const V& v) {
+  *reinterpret_cast<V __attribute__((address_space(1)))*>(reinterpret_cast<uintptr_t>(p)) = v;
+}
+
 // Four values of a row at any alignment, or the `count` that there are (zeros for the rest).
 __device__ __forceinline__ mf4 load_quad(const float* p, int count) {
   mf4 v = {0.f, 0.f, 0.f, 0.f};
-  if (count >= 4) return *reinterpret_cast<const mf4*>(p);
+  if (count >= 4) return from_global<mf4>(p);
 #pragma unroll
   for (int j = 0; j < 3; ++j)
-    if (j < count) v[j] = p[j];
+    if (j < count) v[j] = from_global<float>(p + j);
   return v;
 }
 
 __device__ __forceinline__ void store_quad(float* p, int count, const mf4& v) {
   if (count >= 4) {
-    *reinterpret_cast<mf4*>(p) = v;
+    to_global<mf4>(p, v);
   } else {
 #pragma unroll
     for (int j = 0; j < 3; ++j)
-      if (j < count) p[j] = v[j];
+      if (j < count) to_global<float>(p + j, v[j]);
   }
 }
 
@@ -367,8 +378,8 @@ struct Source {
     for (int r = 0; r < 4; ++r)
       if (r < count) {
         const int64_t from = at + static_cast<int64_t>(r) * m_.cols;
-        if (!m_.momentum || a.nesterov) g[r] = m_.src[from];
-        if (m_.momentum) m[r] = m_.momentum[from];
+        if (!m_.momentum || a.nesterov) g[r] = from_global<float>(m_.src + from);
+        if (m_.momentum) m[r] = from_global<float>(m_.momentum + from);
       }
   }
 
@@ -416,8 +427,8 @@ __global__ void __launch_bounds__(kMuThreads) muon_normalise_kernel(const MuonAr
         hi[j] = h, lo[j] = l;
       }
       const int64_t at = paired_at(first + r, along + c, wide);
-      *reinterpret_cast<half8*>(to + at) = hi;
-      *reinterpret_cast<half8*>(to + at + kPair) = lo;
+      to_global<half8>(to + at, hi);
+      to_global<half8>(to + at + kPair, lo);
     }
   }
 }
@@ -544,7 +555,7 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
   const _Float16* const q = PHASE == kGram ? x : PHASE == kPoly ? gram : xt;
   const int depth = PHASE == kGram ? m.np : m.mp;
 
-  const int lane = threadIdx.x & (kMuWave - 1), wave = threadIdx.x / kMuWave;
+  const int lane = threadIdx.x & (kMuWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kMuWave);
   const int wi = (wave & 1) * (T / 2), wj = (wave >> 1) * (T / 2);
   // (16 lanes read 16 rows at a time, from 64 banks: the groups of every other row are in the same ones)
   const auto turned = [](int row) { return (row >> 1) & 7; };
@@ -630,7 +641,7 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
       for (int r = 0; r < 8; ++r) v[r] *= kUnscale;
     } else {
       const _Float16* old = (PHASE == kPoly ? gram : xt) + across;
-      const half8 hi = *reinterpret_cast<const half8*>(old), lo = *reinterpret_cast<const half8*>(old + kPair);
+      const half8 hi = from_global<half8>(old), lo = from_global<half8>(old + kPair);
 #pragma unroll
       for (int r = 0; r < 8; ++r)
         v[r] = PHASE == kPoly ? fmaf(a.b_kept, joined(hi[r], lo[r]), a.c_kept * v[r])
@@ -655,8 +666,8 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
         hi[r] = h, lo[r] = l;
         kept[r] = __builtin_bit_cast(uint16_t, h) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, l)) << 16;
       }
-      *reinterpret_cast<half8*>(mirror) = hi;
-      *reinterpret_cast<half8*>(mirror + kPair) = lo;
+      to_global<half8>(mirror, hi);
+      to_global<half8>(mirror + kPair, lo);
     }
 #pragma unroll
     for (int q = 0; q < 8; q += 4)
@@ -687,8 +698,8 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
         lo[r] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(kept[r] >> 16));
       }
       _Float16* const to = plain + paired_at(ti * T + row, tj * T + column, wide);
-      *reinterpret_cast<half8*>(to) = hi;
-      *reinterpret_cast<half8*>(to + kPair) = lo;
+      to_global<half8>(to, hi);
+      to_global<half8>(to + kPair, lo);
     }
   }
 }
@@ -711,11 +722,12 @@ __device__ __forceinline__ void upper_block(int b, int& i, int& j) {
   i = b - j * (j + 1) / 2;
 }
 
+// (Two accumulators: a product waits for the one before it in the same accumulator twice as long as it takes to issue.)
 __device__ __forceinline__ void three_products(const half8& ah, const half8& al, const half8& bh, const half8& bl,
-                                               f32x16& acc) {
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+                                               f32x16& high, f32x16& low) {
+  low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, low, 0, 0, 0);
+  high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, high, 0, 0, 0);
+  low = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, low, 0, 0, 0);
 }
 
 // Where an entry of B lies: in the order in which a wave's lanes take it as an operand, 32 rows and 16 columns at a
@@ -757,7 +769,8 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
   constexpr int kWaves = kShortThreads / kMuWave;
   constexpr int M = 32 * MB, kGroups = M / 8, kBlocks = MB * (MB + 1) / 2, kMine = (kBlocks + kWaves - 1) / kWaves;
   constexpr int kTiles = MB == 4 ? 2 : 1;          // 32 x 32 products of a wave
-  const int lane = threadIdx.x & (kMuWave - 1), wave = threadIdx.x / kMuWave, half = lane / 32;
+  const int lane = threadIdx.x & (kMuWave - 1), half = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kMuWave);
   const int64_t plane = static_cast<int64_t>(m.np) * M;
   _Float16* const xt = reinterpret_cast<_Float16*>(m.x);
   const _Float16* const poly = xt + 2 * plane;
@@ -819,19 +832,22 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
       for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int k = 0; k < M / 16; ++k)
-          b_op[p][k] = *reinterpret_cast<const half8*>(poly + p * M * M + operand_at<M>(row0, k * 16) + lane * 8);
+          b_op[p][k] = from_global<half8>(poly + p * M * M + operand_at<M>(row0, k * 16) + lane * 8);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       f32x16 acc[kTiles] = {};
       if (works) {
+        f32x16 low[kTiles] = {};
 #pragma unroll
         for (int k = 0; k < M / 16; ++k)
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
             const int from = turned_at(col0 + t * 32 + (lane & 31), k * 2 + half, kGroups);
             three_products(b_op[0][k], b_op[1][k], *reinterpret_cast<const half8*>(&lds.xt[0][from]),
-                           *reinterpret_cast<const half8*>(&lds.xt[1][from]), acc[t]);
+                           *reinterpret_cast<const half8*>(&lds.xt[1][from]), acc[t], low[t]);
           }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) acc[t] += low[t];
       }
       const int shift = shift_of<PHASE>(a, m.owner, step);
       __syncthreads();         // all products have their operands: their places take the results
@@ -892,8 +908,8 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
 #pragma unroll
         for (int k = 0; k < kPart * kGroups / kShortThreads; ++k) {
           const int group = k * kShortThreads + threadIdx.x;
-          *reinterpret_cast<half8*>(columns + p * plane + group * 8) =
-              *reinterpret_cast<const half8*>(&lds.xt[p][turned_at(group / kGroups, group % kGroups, kGroups)]);
+          to_global<half8>(columns + p * plane + group * 8,
+                           *reinterpret_cast<const half8*>(&lds.xt[p][turned_at(group / kGroups, group % kGroups, kGroups)]));
         }
 #pragma unroll
       for (int q = 0; q < kMine; ++q) {
@@ -901,11 +917,13 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
         if (b >= kBlocks) continue;
         int bi, bj;
         upper_block(b, bi, bj);
+        f32x16 low = {};
 #pragma unroll 2
         for (int k = 0; k < kPart; k += 16)
           three_products(turned_operand(lds.xt[0], bi * 32, k, kGroups), turned_operand(lds.xt[1], bi * 32, k, kGroups),
                          turned_operand(lds.xt[0], bj * 32, k, kGroups), turned_operand(lds.xt[1], bj * 32, k, kGroups),
-                         gram[q]);
+                         gram[q], low);
+        gram[q] += low;
       }
       if (part + 1 < end) __syncthreads();
     }
@@ -921,7 +939,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
         mf4 v;
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = gram[q][k + r] * kUnscale;
-        *reinterpret_cast<mf4*>(parts + b * 1024 + (k / 4 * 64 + lane) * 4) = v;
+        to_global<mf4>(parts + b * 1024 + (k / 4 * 64 + lane) * 4, v);
       }
     }
   }
@@ -945,7 +963,8 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
                                            _Float16 (*lds)[kShort * kShort]) {
   constexpr int M = 32 * MB, kGroups = M / 8, kBlocks = MB * (MB + 1) / 2, kQuads = kBlocks * 256;
   constexpr int kMine = (kQuads + kPolyThreads - 1) / kPolyThreads;
-  const int lane = threadIdx.x & (kMuWave - 1), wave = threadIdx.x / kMuWave, half = lane / 32;
+  const int lane = threadIdx.x & (kMuWave - 1), half = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kMuWave);
   const int64_t plane = static_cast<int64_t>(m.np) * M;
   _Float16* const poly = reinterpret_cast<_Float16*>(m.x) + 2 * plane;
   const float* const parts = reinterpret_cast<const float*>(poly + 2 * M * M);
@@ -961,7 +980,7 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
         const int quad = q * kPolyThreads + threadIdx.x;
         v[c][q] = mf4{0.f, 0.f, 0.f, 0.f};
         if (quad < kQuads && first + c < m.chunks)
-          v[c][q] = *reinterpret_cast<const mf4*>(parts + (static_cast<int64_t>(first + c) * kQuads + quad) * 4);
+          v[c][q] = from_global<mf4>(parts + (static_cast<int64_t>(first + c) * kQuads + quad) * 4);
       }
 #pragma unroll
     for (int c = 0; c < kAhead; ++c)
@@ -993,17 +1012,28 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
     *reinterpret_cast<half4*>(&lds[1][to]) = lo;
   }
   __syncthreads();
-  for (int b = wave; b < kBlocks; b += kPolyThreads / kMuWave) {
-    int bi, bj;
-    upper_block(b, bi, bj);
-    f32x16 acc = {};
+  // (a wave's blocks side by side)
+  constexpr int kWaves = kPolyThreads / kMuWave, kEach = (kBlocks + kWaves - 1) / kWaves;
+  f32x16 acc[kEach] = {}, low[kEach] = {};
 #pragma unroll
-    for (int k = 0; k < M / 16; ++k) {
+  for (int k = 0; k < M / 16; ++k)
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const int b = wave + q * kWaves;
+      if (b >= kBlocks) continue;
+      int bi, bj;
+      upper_block(b, bi, bj);
       const int i = turned_at(bi * 32 + (lane & 31), k * 2 + half, kGroups);
       const int j = turned_at(bj * 32 + (lane & 31), k * 2 + half, kGroups);
       three_products(*reinterpret_cast<const half8*>(&lds[0][i]), *reinterpret_cast<const half8*>(&lds[1][i]),
-                     *reinterpret_cast<const half8*>(&lds[0][j]), *reinterpret_cast<const half8*>(&lds[1][j]), acc);
+                     *reinterpret_cast<const half8*>(&lds[0][j]), *reinterpret_cast<const half8*>(&lds[1][j]), acc[q], low[q]);
     }
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) {
+    const int b = wave + q * kWaves;
+    if (b >= kBlocks) continue;
+    int bi, bj;
+    upper_block(b, bi, bj);
 #pragma unroll
     for (int k = 0; k < 16; k += 4) {
       const int row = bi * 32 + 2 * k + 4 * half, column = bj * 32 + (lane & 31);
@@ -1014,15 +1044,15 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         _Float16 h, l;
-        split(fmaf(a.b_kept, joined(old_hi[r], old_lo[r]), a.c_kept * acc[k + r]), h, l);
+        split(fmaf(a.b_kept, joined(old_hi[r], old_lo[r]), a.c_kept * (acc[q][k + r] + low[q][k + r])), h, l);
         hi[r] = h, lo[r] = l;
         if (bi != bj) {
-          poly[operand_at<M>(row + r, column)] = h;
-          poly[M * M + operand_at<M>(row + r, column)] = l;
+          to_global<_Float16>(poly + operand_at<M>(row + r, column), h);
+          to_global<_Float16>(poly + M * M + operand_at<M>(row + r, column), l);
         }
       }
-      *reinterpret_cast<half4*>(poly + operand_at<M>(column, row)) = hi;
-      *reinterpret_cast<half4*>(poly + M * M + operand_at<M>(column, row)) = lo;
+      to_global<half4>(poly + operand_at<M>(column, row), hi);
+      to_global<half4>(poly + M * M + operand_at<M>(column, row), lo);
     }
   }
 }
