@@ -24,7 +24,9 @@
 //
 // Matrices with a shorter side of up to 128, of which most models have most: two launches a step, bound by latency.  A
 // workgroup keeps 64 columns of X at a time: it multiplies them by B, and adds what they give to the next X X^T at once,
-// from LDS; the other launch, one workgroup to a matrix, adds these parts up in order, and makes A A and B.
+// from LDS; the other launch, one workgroup to a matrix, adds these parts up in order, and makes A A and B.  (Done by
+// the workgroup that is the last of its matrix to leave its part, it saves a launch, but what makes the parts of
+// others visible within one costs more: a step of the C128 / lmax 3 model's matrices 35 us against 23.)
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

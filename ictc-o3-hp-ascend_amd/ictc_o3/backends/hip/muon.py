@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from array import array
 
 import torch
 
@@ -21,20 +20,6 @@ from .optimizer import _number, _on
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_STEPS = 64
 ADJUST = {"original": 0, "match_rms_adamw": 1}
-
-
-def _shapes(tensors, what: str):
-    """Rows, columns and numbers of matrices of tensors [..., rows, columns], as the arrays that the C entry
-    points take (and the three arrays themselves, which have to outlive the call)."""
-    rows, cols, batches = array("q"), array("q"), array("q")
-    for t in tensors:
-        shape = t.shape
-        if len(shape) < 2:
-            raise ValueError(f"{what} must be matrices (or have leading axes that count them)")
-        rows.append(shape[-2])
-        cols.append(shape[-1])
-        batches.append(math.prod(shape[:-2]))
-    return [(ctypes.c_int64 * len(a)).from_buffer(a) if len(a) else None for a in (rows, cols, batches)]
 
 
 def _desc(*, steps, coefficients, eps, beta=0.0, nesterov=False, weight_decay=0.0, lr=0.0, adjust="original"):
@@ -66,18 +51,17 @@ def orthogonalize(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: f
         matrices = list(matrices)
         if not matrices:
             return []
-        _, at, _, contiguous = _lib.host().addresses(matrices, "matrices")
-        shapes = _shapes(matrices, "matrices")
+        host = _lib.host()
+        _, at, *shapes, contiguous = host.matrices(matrices, "matrices")
         if not contiguous:
             matrices = [m.contiguous() for m in matrices]
-            _, at, _, _ = _lib.host().addresses(matrices, "matrices")
+            _, at, *shapes, _ = host.matrices(matrices, "matrices")
         desc = _desc(steps=steps, coefficients=coefficients, eps=eps)
-        out = [torch.empty_like(m, memory_format=torch.contiguous_format) for m in matrices]
         n, device = len(matrices), matrices[0].device
-        to = _lib.host().addresses(out, "matrices")[1]
-        ws = _workspace(shapes, n, device)
         with _on(device):
-            _lib.check(_lib.lib().ictc_hip_orthogonalize(at, to, *shapes, n, ctypes.byref(desc), _lib.ptr(ws), ws.numel(),
+            out, to = host.alike(matrices)
+            ws = _workspace(shapes, n, device)
+            _lib.check(_lib.lib().ictc_hip_orthogonalize(at, to, *shapes, n, ctypes.byref(desc), ws.data_ptr(), ws.numel(),
                                                          _lib.stream_of(device)), "ictc_hip_orthogonalize")
         return out
 
@@ -99,10 +83,9 @@ def muon_step(params, grads, momentum, *, lr, beta: float = 0.95, nesterov: bool
         grads = [g if g is None else g.contiguous() for g in grads]
         _, p_at, g_at, _, _, _ = host.pairs(params, grads, 1)
     n, device = len(params), params[0].device
-    shapes = _shapes(params, "parameters")
-    m_device, m_at, _, contiguous = host.addresses(momentum, "momentum")
-    if len(momentum) != n or not contiguous or m_device != device.index \
-            or any(m.shape != p.shape for m, p in zip(momentum, params)):
+    _, _, *shapes, _ = host.matrices(params, "parameters")
+    m_device, m_at, *m_shapes, contiguous = host.matrices(momentum, "momentum")
+    if len(momentum) != n or not contiguous or m_device != device.index or m_shapes != shapes:
         raise ValueError("momentum must hold a contiguous tensor of each parameter's shape beside the parameters")
     if clip is not None and (clip.dtype is not torch.float32 or clip.shape != (2,) or clip.device != device
                              or not clip.is_contiguous()):
