@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 #include <exception>
 #include <optional>
@@ -316,9 +317,30 @@ variable_list TableGrad::backward(AutogradContext* ctx, variable_list tops) {
 // Python's interface
 // ---------------------------------------------------------------------------------------------------------
 
+// What a caller gave wrong: a ValueError.
+struct Refused : std::invalid_argument {
+  using std::invalid_argument::invalid_argument;
+};
+
 const Tensor& tensor(PyObject* o) {
-  if (!THPVariable_Check(o)) throw std::invalid_argument("expected a tensor");
+  if (!THPVariable_Check(o)) throw Refused("expected a tensor");
   return THPVariable_Unpack(o);
+}
+
+void require_gpu_fp32(const Tensor& t, const Tensor& beside) {
+  if (!t.is_cuda() || t.scalar_type() != at::kFloat || t.layout() != at::kStrided)
+    throw Refused("ictc_o3 HIP operators require FP32 tensors on a ROCm GPU; precision is never changed automatically");
+  if (t.device() != beside.device()) throw Refused("All operands must be on the same GPU");
+}
+
+// A Python number as a double (bool is none).
+double number(PyObject* o, const char* what) {
+  const double v = PyBool_Check(o) || !(PyFloat_Check(o) || PyLong_Check(o)) ? NAN : PyFloat_AsDouble(o);
+  if (!std::isfinite(v)) {
+    PyErr_Clear();
+    throw Refused(what);
+  }
+  return v;
 }
 
 // bind(status_string, norm workspace, forward, backward, second, embedding forward, workspace, table_grad, formula)
@@ -341,32 +363,50 @@ PyObject* bind(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// layer_norm(features [..., W], weight, bias or None, activation, eps), arguments checked by the caller
+// layer_norm(features [..., W], weight, bias or None, activation, eps)
 PyObject* layer_norm(PyObject*, PyObject* args) {
-  PyObject *x, *weight, *bias;
+  PyObject *x, *weight, *bias, *given_eps;
   int activation;
-  double eps;
-  if (!PyArg_ParseTuple(args, "OOOid", &x, &weight, &bias, &activation, &eps)) return nullptr;
+  if (!PyArg_ParseTuple(args, "OOOiO", &x, &weight, &bias, &activation, &given_eps)) return nullptr;
   if (!lib.norm_forward) throw std::runtime_error("the host module is not bound to the library");
+  const double eps = number(given_eps, "eps must be a positive number");
+  if (!(static_cast<float>(eps) > 0.f) || !std::isfinite(static_cast<float>(eps)))
+    throw Refused("eps must be a positive number");
   const Tensor& features = tensor(x);
-  std::optional<Tensor> b;
-  if (bias != Py_None) b = tensor(bias).contiguous();
+  if (features.dim() < 1 || features.size(-1) < 1 || features.size(-1) > ICTC_LAYER_NORM_MAX_WIDTH)
+    throw Refused("features must have between 1 and " + std::to_string(ICTC_LAYER_NORM_MAX_WIDTH) + " columns");
   const int64_t width = features.size(-1);
+  const auto check_weight = [&](const Tensor& w) {
+    if (w.dim() != 1 || w.size(0) != width)
+      throw Refused("weight and bias must have shape [" + std::to_string(width) + "]");
+    require_gpu_fp32(w, features);
+  };
+  require_gpu_fp32(features, features);
+  check_weight(tensor(weight));
+  std::optional<Tensor> b;
+  if (bias != Py_None) {
+    check_weight(tensor(bias));
+    b = tensor(bias).contiguous();
+  }
   const bool rows = features.dim() == 2;
   const Tensor y = LayerNorm::apply(rows ? features.contiguous() : features.reshape({-1, width}).contiguous(),
                                     tensor(weight).contiguous(), b, activation, eps);
   return THPVariable_Wrap(rows ? y : y.view(features.sizes()));
 }
 
-// embedding(table, tokens of any shape, scale), arguments checked by the caller
+// embedding(tokens of any shape, table, scale)
 PyObject* embedding(PyObject*, PyObject* args) {
-  PyObject *table, *tokens;
-  double scale;
-  if (!PyArg_ParseTuple(args, "OOd", &table, &tokens, &scale)) return nullptr;
+  PyObject *given_tokens, *given_table, *given_scale;
+  if (!PyArg_ParseTuple(args, "OOO", &given_tokens, &given_table, &given_scale)) return nullptr;
   if (!lib.embedding_forward) throw std::runtime_error("the host module is not bound to the library");
-  const Tensor& t = tensor(tokens);
+  const Tensor &t = tensor(given_tokens), &table = tensor(given_table);
+  if (table.dim() != 2 || table.size(0) < 1 || table.size(1) < 1) throw Refused("the table must have shape [rows, width]");
+  if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) throw Refused("tokens must be int32 or int64");
+  const double scale = number(given_scale, "scale must be a finite number");
+  require_gpu_fp32(table, table);
+  if (t.device() != table.device()) throw Refused("All operands must be on the same GPU");
   const bool flat = t.dim() == 1;
-  const Tensor y = Lookup::apply(tensor(table).contiguous(), flat ? t.contiguous() : t.reshape({-1}).contiguous(), scale);
+  const Tensor y = Lookup::apply(table.contiguous(), flat ? t.contiguous() : t.reshape({-1}).contiguous(), scale);
   if (flat) return THPVariable_Wrap(y);
   auto shape = t.sizes().vec();
   shape.push_back(y.size(1));
@@ -378,6 +418,9 @@ template <PyObject* (*F)(PyObject*, PyObject*)>
 PyObject* guarded(PyObject* self, PyObject* args) {
   try {
     return F(self, args);
+  } catch (const Refused& e) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, e.what());
+    return nullptr;
   } catch (const std::exception& e) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;

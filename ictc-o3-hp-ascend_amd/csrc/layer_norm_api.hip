@@ -328,7 +328,7 @@ struct LnShape {
 LnShape ln_shape(int width, int64_t rows) {
   LnShape s;
   const int quads = (width + 3) / 4;
-  s.wide = quads <= 4 * kRowWave ? 0 : quads <= 4 * kLnThreads ? 1 : 2;
+  s.wide = quads <= 2 * kRowWave ? 0 : quads <= 4 * kLnThreads ? 1 : 2;
   if (s.wide) {
     s.threads = ln_block(s.wide);
     s.groups = 1;
@@ -357,8 +357,9 @@ LnKernel ln_kernel(int order) {
 template <bool SILU>
 LnKernel ln_kernel(int order, const LnShape& s) {
   if (s.wide == 0)
-    return s.k == 1 ? ln_kernel<1, 0, SILU>(order) : s.k == 2 ? ln_kernel<2, 0, SILU>(order) : ln_kernel<4, 0, SILU>(order);
-  if (s.wide == 1) return s.k == 2 ? ln_kernel<2, 1, SILU>(order) : ln_kernel<4, 1, SILU>(order);
+    return s.k == 1 ? ln_kernel<1, 0, SILU>(order) : ln_kernel<2, 0, SILU>(order);
+  if (s.wide == 1)
+    return s.k == 1 ? ln_kernel<1, 1, SILU>(order) : s.k == 2 ? ln_kernel<2, 1, SILU>(order) : ln_kernel<4, 1, SILU>(order);
   return ln_kernel<2, 2, SILU>(order);
 }
 

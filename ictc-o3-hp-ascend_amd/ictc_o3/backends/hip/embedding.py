@@ -7,26 +7,16 @@ The lookup and the table's gradient are linear and each other's adjoint: their a
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from ictc_o3 import _lib
 
-from .runtime import require_gpu_fp32
+from .runtime import require_ordinary_autograd
 
 
 def embedding(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
     """scale * table[tokens] for int32 or int64 tokens of any shape and a table [rows, width]: [..., width].  Tokens
     outside [0, rows) (padding) give rows of zeros and have no gradient.  The table's gradient is dense and
     bit-identical from run to run."""
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
-        raise ValueError("the table must have shape [rows, width]")
-    if tokens.dtype not in (torch.int32, torch.int64):
-        raise ValueError("tokens must be int32 or int64")
-    if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not math.isfinite(scale):
-        raise ValueError("scale must be a finite number")
-    require_gpu_fp32(table)
-    if tokens.device != table.device:
-        raise ValueError("All operands must be on the same GPU")
-    return _lib.layers().embedding(table, tokens, scale)
+    require_ordinary_autograd()
+    return _lib.layers().embedding(tokens, table, scale)

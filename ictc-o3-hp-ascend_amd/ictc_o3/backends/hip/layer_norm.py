@@ -8,16 +8,14 @@ stays available.
 """
 from __future__ import annotations
 
-import math
 from typing import Optional
 
 import torch
 
 from ictc_o3 import _lib
 
-from .runtime import require_gpu_fp32
+from .runtime import require_ordinary_autograd
 
-MAX_WIDTH = 8192
 ACTIVATIONS = {None: 0, "silu": 1}
 
 
@@ -63,15 +61,5 @@ def layer_norm(features: torch.Tensor, weight: torch.Tensor, bias: Optional[torc
     with SiLU behind it where ``activation`` is "silu", for features [..., W], weight [W] and bias [W] or None."""
     if activation not in ACTIVATIONS:
         raise ValueError('activation must be None or "silu"')
-    if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not eps > 0.0 or not math.isfinite(eps):
-        raise ValueError("eps must be a positive number")
-    if features.dim() < 1 or not 1 <= features.shape[-1] <= MAX_WIDTH:
-        raise ValueError(f"features must have between 1 and {MAX_WIDTH} columns")
-    width = features.shape[-1]
-    if weight.shape != (width,) or (bias is not None and bias.shape != (width,)):
-        raise ValueError(f"weight and bias must have shape [{width}]")
-    if bias is None:
-        require_gpu_fp32(features, weight)
-    else:
-        require_gpu_fp32(features, weight, bias)
+    require_ordinary_autograd()
     return _lib.layers().layer_norm(features, weight, bias, ACTIVATIONS[activation], eps)

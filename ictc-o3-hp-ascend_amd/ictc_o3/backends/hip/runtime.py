@@ -16,6 +16,11 @@ def require_gpu_fp32(*values: torch.Tensor) -> None:
                          "precision is never changed automatically")
     if any(v.device != values[0].device for v in values):
         raise ValueError("All operands must be on the same GPU")
+    require_ordinary_autograd()
+
+
+def require_ordinary_autograd() -> None:
+    """The part of ``require_gpu_fp32`` that is not about operands."""
     if torch.is_autocast_enabled("cuda"):
         raise ValueError("ictc_o3 HIP operators require autocast to be disabled")
     if torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active():
