@@ -29,6 +29,7 @@ namespace {
 constexpr int kLnThreads = 256;              // of a workgroup whose rows fit into a wave, or of a row
 constexpr int kLnWideThreads = 1024;
 constexpr int kLnGroups = 1024;              // workgroups that leave partial weight gradients
+constexpr float kLog2E = 0x1.715476p+0f, kLog2ELow = 0x1.4ae0cp-26f, kLn2 = 0x1.62e43p-1f;
 
 typedef float lf4 __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -99,9 +100,14 @@ struct Columns {
   __device__ __forceinline__ bool valid(int i) const { return i % 4 < count[i / 4]; }
 };
 
-// sigmoid(z) and sigmoid(-z), both to their last bits.
+// sigmoid(z) and sigmoid(-z), both to their last bits but one: q = e^-|z| as a power of two of a product in two parts
+// (beyond 200 nothing changes), and a reciprocal with one step of Newton's.  With expf and a division a third of all
+// instructions is theirs (forward, 20,000 x 1,000: 43 us against 35).
 __device__ __forceinline__ void sigmoids(float z, float& open, float& closed) {
-  const float q = expf(-fabsf(z)), inv = 1.f / (1.f + q);
+  const float size = -fminf(fabsf(z), 200.f), high = size * kLog2E;
+  const float low = fmaf(size, kLog2E, -high) + size * kLog2ELow;
+  const float power = __builtin_amdgcn_exp2f(high), q = fmaf(power, low * kLn2, power), d = 1.f + q;
+  const float near = __builtin_amdgcn_rcpf(d), inv = fmaf(fmaf(-d, near, 1.f), near, near);
   open = z < 0.f ? q * inv : inv;
   closed = z < 0.f ? inv : q * inv;
 }
@@ -238,7 +244,7 @@ __global__ void __launch_bounds__(ln_block(WIDE)) layer_norm_backward_kernel(con
 }
 
 template <int K, int WIDE, bool SILU>
-__global__ void __launch_bounds__(ln_block(WIDE)) layer_norm_second_kernel(const LayerNormArgs a) {
+__global__ void __launch_bounds__(ln_block(WIDE), K == 1 ? 4 : 1) layer_norm_second_kernel(const LayerNormArgs a) {
   __shared__ double lds[WIDE ? 2 * kSums * kMaxWaves : 1];
   int turn = 0;
   const Columns<K, WIDE> c(a);
