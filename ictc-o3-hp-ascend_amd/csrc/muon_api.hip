@@ -485,9 +485,10 @@ __device__ __forceinline__ void load_to_lds(const _Float16* from, _Float16* to) 
                                    16, 0, 0);
 }
 
-// Workgroups go to the 8 XCDs in turn, and each has a cache of its own: 32 tiles in a row, which share rows of their
-// operands, go to the same one.
-constexpr uint32_t kXcds = 8, kUnit = 32;
+// Workgroups go to the 8 XCDs in turn, and each has a cache of its own: 16 tiles in a row, which share rows of their
+// operands, go to the same one (X X^T of 24 matrices of 1 to 4 million values 209 us, with 32 in a row 236 for the
+// imbalance of long reductions, without 250).
+constexpr uint32_t kXcds = 8, kUnit = 16;
 
 __device__ __forceinline__ uint32_t tile_of(uint32_t block) {
   return (block / (kXcds * kUnit) * kXcds + block % kXcds) * kUnit + block / kXcds % kUnit;

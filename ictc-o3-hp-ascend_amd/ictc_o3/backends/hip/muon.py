@@ -46,7 +46,7 @@ def _workspace(shapes, count: int, device) -> torch.Tensor:
 def orthogonalize(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
     """Each matrix of a list (tensors [..., rows, columns], leading axes counting matrices) scaled to Frobenius norm
     1 and brought near an orthogonal one by ``steps`` Newton-Schulz products, as a list of new tensors.  Without
-    gradients."""
+    gradients.  The coefficients have to keep singular values below 5 (beyond, a result is not a number)."""
     with torch.no_grad():
         matrices = list(matrices)
         if not matrices:

@@ -191,3 +191,33 @@ def test_refusals(gpu):
                  lambda: embedding(tokens, table, scale="1"), lambda: embedding(tokens, table, scale=True)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_inference_and_changed_tokens(gpu):
+    from ictc_o3.operators import embedding
+    tokens, table, dy = (t.to(gpu) for t in _case(50, 6, 16, 14))
+    with torch.inference_mode():
+        assert torch.equal(embedding(tokens, table, scale=2.0), table[tokens] * 2.0)
+    leaf = table.requires_grad_()
+    y = embedding(tokens, leaf)
+    tokens.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, leaf, dy)
+
+
+def test_two_streams_at_once(gpu):
+    from ictc_o3.operators import embedding
+    cases = [tuple(t.to(gpu) for t in _case(60000, rows, 64, rows)) for rows in (90, 4000)]
+    leaves = [c[1].requires_grad_() for c in cases]
+    work = lambda c, leaf: torch.autograd.grad(embedding(c[0], leaf), leaf, c[2])[0]     # noqa: E731
+    want = [work(c, leaf).clone() for c, leaf in zip(cases, leaves)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for s, c, leaf in zip(streams, cases, leaves):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(work(c, leaf))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

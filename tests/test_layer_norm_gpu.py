@@ -255,3 +255,49 @@ def test_refusals(gpu):
             call()
     with torch.autocast("cuda"), pytest.raises(ValueError):
         layer_norm(x, w)
+
+
+def test_inference_and_no_grad(gpu):
+    from ictc_o3.operators import layer_norm
+    t = _leaves(_inputs(64, 30, 6), gpu, torch.float32)
+    want = layer_norm(t["x"], t["w"], t["b"])
+    with torch.no_grad():
+        assert torch.equal(layer_norm(t["x"], t["w"], t["b"]), want.detach())
+    with torch.inference_mode():
+        fresh = t["x"].clone()
+        assert torch.equal(layer_norm(fresh, t["w"], t["b"]), want)
+    assert want.requires_grad
+
+
+def test_two_streams_at_once(gpu):
+    """Passes side by side have workspaces of their own."""
+    from ictc_o3.operators import layer_norm
+    cases = [_leaves(_inputs(64, 40000, 30 + k), gpu, torch.float32) for k in range(2)]
+
+    def work(t):
+        return torch.autograd.grad(layer_norm(t["x"], t["w"], t["b"], activation="silu"), [t["x"], t["w"], t["b"]], t["dy"])
+
+    want = [[g.clone() for g in work(t)] for t in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for s, t in zip(streams, cases):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(work(t))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+def test_changed_inputs_are_noticed(gpu):
+    """An input that was changed in place after the forward pass is refused by the backward pass."""
+    from ictc_o3.operators import layer_norm
+    t = _leaves(_inputs(16, 5, 2), gpu, torch.float32)
+    x = t["x"].detach().clone().requires_grad_()
+    held = x * 1.0
+    y = layer_norm(held, t["w"], t["b"])
+    with torch.no_grad():
+        held.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, x, t["dy"])

@@ -241,3 +241,55 @@ def test_refusals(gpu):
         with pytest.raises(ValueError):
             call()
     assert torch.equal(p, x) and torch.equal(m, x)
+
+
+def test_two_streams_at_once(gpu):
+    from ictc_o3.operators import orthogonalize
+    cases = [[_draw(s, k).to(gpu) for k, s in enumerate(shapes)]
+             for shapes in ([(64, 900), (128, 128), (30, 30)], [(300, 700), (90, 400)])]
+    want = [[x.clone() for x in orthogonalize(c)] for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, cases):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(orthogonalize(c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+def test_in_place_and_the_same_matrix_twice(gpu):
+    """What reads a matrix twice may; a captured step's moving averages go on from replay to replay."""
+    from ictc_o3.operators import muon_step, orthogonalize
+    u = _draw((70, 90), 1).to(gpu)
+    a, b = orthogonalize([u, u])
+    assert torch.equal(a, b)
+    p, m = _draw((70, 90), 2).to(gpu), torch.zeros(70, 90, device=gpu)
+    q, n = p.clone(), m.clone()
+    rate = torch.tensor([0.1], device=gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        muon_step([p], [u], [m], lr=rate)
+        muon_step([q], [u], [n], lr=rate)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        muon_step([p], [u], [m], lr=rate)
+    for k in range(3):
+        u.copy_(_draw((70, 90), 10 + k))
+        rate.fill_(0.1 / (k + 1))
+        graph.replay()
+        muon_step([q], [u.clone()], [n], lr=0.1 / (k + 1))
+        torch.cuda.synchronize()
+        # (the rate as a float32 tensor and as a number: the same bits)
+        assert torch.equal(p, q) and torch.equal(m, n)
+
+
+def test_coefficients_beyond_the_range(gpu):
+    """Singular values that grow without bound are seen as such."""
+    from ictc_o3.operators import orthogonalize
+    got, other = orthogonalize([_draw((40, 40), 3).to(gpu), torch.zeros(8, 8, device=gpu)], steps=8, coefficients=(4.0, 0.0, 0.0))
+    assert not got.isfinite().all() and not other.any()
