@@ -131,12 +131,11 @@ PyObject* matrices(PyObject*, PyObject* args) {
                        contiguous ? Py_True : Py_False);
 }
 
-// alike(tensors) -> (new contiguous tensors of their shapes, addresses)
+// alike(tensors) -> new contiguous tensors of their shapes
 PyObject* alike(PyObject*, PyObject* args) {
   PyObject* list;
   if (!PyArg_ParseTuple(args, "O!", &PyList_Type, &list)) return nullptr;
   const Py_ssize_t n = PyList_GET_SIZE(list);
-  std::vector<int64_t> at(n);
   PyObject* made = PyList_New(n);
   if (!made) return nullptr;
   try {
@@ -146,15 +145,13 @@ PyObject* alike(PyObject*, PyObject* args) {
         Py_DECREF(made);
         return nullptr;
       }
-      const at::Tensor y = at::empty(t->sizes(), t->options());
-      at[i] = reinterpret_cast<int64_t>(y.const_data_ptr());
-      PyList_SET_ITEM(made, i, THPVariable_Wrap(y));
+      PyList_SET_ITEM(made, i, THPVariable_Wrap(at::empty(t->sizes(), t->options())));
     }
   } catch (...) {
     Py_DECREF(made);
     throw;
   }
-  return Py_BuildValue("NN", made, bytes_of(at));
+  return made;
 }
 
 // written(params, grads): raises the version counter of every parameter whose gradient is not None.
@@ -188,7 +185,7 @@ PyMethodDef methods[] = {
     {"pairs", guarded<pairs>, METH_VARARGS, "(device, parameters, gradients, sizes, values, contiguous) of two lists"},
     {"matrices", guarded<matrices>, METH_VARARGS,
      "(device, addresses, rows, columns, batches, contiguous) of a list of matrices"},
-    {"alike", guarded<alike>, METH_VARARGS, "(new contiguous tensors, addresses) of a list's shapes"},
+    {"alike", guarded<alike>, METH_VARARGS, "new contiguous tensors of a list's shapes"},
     {"written", guarded<written>, METH_VARARGS,
      "raise the version counters of parameters written through their addresses"},
     {nullptr, nullptr, 0, nullptr}};

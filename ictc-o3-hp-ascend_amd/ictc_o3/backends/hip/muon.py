@@ -19,6 +19,7 @@ from .optimizer import _number, _on
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_STEPS = 64
+SHORT = 128           # shorter sides that the kernels do in chunks of columns
 ADJUST = {"original": 0, "match_rms_adamw": 1}
 
 
@@ -43,6 +44,42 @@ def _workspace(shapes, count: int, device) -> torch.Tensor:
     return torch.empty(needed, device=device, dtype=torch.uint8)
 
 
+_SIDE_STREAMS = {}
+
+
+def _side_stream(device: torch.device):
+    """One default-priority side stream per device, created once, and another one for captures: work that is issued
+    elsewhere meanwhile must not end up in a graph."""
+    key = device.index, torch.cuda.is_current_stream_capturing()
+    stream = _SIDE_STREAMS.get(key)
+    if stream is None:
+        stream = _SIDE_STREAMS[key] = torch.cuda.Stream(device=device)
+    return stream
+
+
+def _both_kinds(shapes, device, run) -> None:
+    """run(places) for the matrices whose shorter side is up to SHORT, which have launches of their own, and for the
+    others; where there are both, on two streams side by side (both are bound by the latency of their launches: 12
+    matrices of 1 to 1,501 rows and columns 188 us against 257 one after the other)."""
+    rows, columns = (memoryview(b).cast("q") for b in shapes[:2])
+    kinds = ([], [])
+    for k, (r, c) in enumerate(zip(rows, columns)):
+        kinds[min(r, c) <= SHORT].append(k)
+    if not kinds[0] or not kinds[1]:
+        run(None)
+        return
+    here, side = torch.cuda.current_stream(device), _side_stream(device)
+    side.wait_stream(here)
+    with torch.cuda.stream(side):
+        run(kinds[1])
+    run(kinds[0])
+    here.wait_stream(side)
+
+
+def _at(values, places):
+    return values if places is None else [values[k] for k in places]
+
+
 def orthogonalize(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
     """Each matrix of a list (tensors [..., rows, columns], leading axes counting matrices) scaled to Frobenius norm
     1 and brought near an orthogonal one by ``steps`` Newton-Schulz products, as a list of new tensors.  Without
@@ -52,17 +89,23 @@ def orthogonalize(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: f
         if not matrices:
             return []
         host = _lib.host()
-        _, at, *shapes, contiguous = host.matrices(matrices, "matrices")
+        _, _, *shapes, contiguous = host.matrices(matrices, "matrices")
         if not contiguous:
             matrices = [m.contiguous() for m in matrices]
-            _, at, *shapes, _ = host.matrices(matrices, "matrices")
         desc = _desc(steps=steps, coefficients=coefficients, eps=eps)
-        n, device = len(matrices), matrices[0].device
+        device = matrices[0].device
+
+        def run(places):
+            own = _at(matrices, places)
+            _, at, *sizes, _ = host.matrices(own, "matrices")
+            _, to, *_ = host.matrices(_at(out, places), "matrices")
+            ws = _workspace(sizes, len(own), device)
+            _lib.check(_lib.lib().ictc_hip_orthogonalize(at, to, *sizes, len(own), ctypes.byref(desc), ws.data_ptr(),
+                                                         ws.numel(), _lib.stream_of(device)), "ictc_hip_orthogonalize")
+
         with _on(device):
-            out, to = host.alike(matrices)
-            ws = _workspace(shapes, n, device)
-            _lib.check(_lib.lib().ictc_hip_orthogonalize(at, to, *shapes, n, ctypes.byref(desc), ws.data_ptr(), ws.numel(),
-                                                         _lib.stream_of(device)), "ictc_hip_orthogonalize")
+            out = host.alike(matrices)
+            _both_kinds(shapes, device, run)
         return out
 
 
@@ -78,13 +121,12 @@ def muon_step(params, grads, momentum, *, lr, beta: float = 0.95, nesterov: bool
     ``gradient_norm``'s result, whose coefficient scales the gradients (not a number: nothing changes)."""
     params, grads, momentum = list(params), list(grads), list(momentum)
     host = _lib.host()
-    _, p_at, g_at, _, _, contiguous = host.pairs(params, grads, 1)
+    _, _, _, _, _, contiguous = host.pairs(params, grads, 1)
     if not contiguous:
         grads = [g if g is None else g.contiguous() for g in grads]
-        _, p_at, g_at, _, _, _ = host.pairs(params, grads, 1)
     n, device = len(params), params[0].device
     _, _, *shapes, _ = host.matrices(params, "parameters")
-    m_device, m_at, *m_shapes, contiguous = host.matrices(momentum, "momentum")
+    m_device, _, *m_shapes, contiguous = host.matrices(momentum, "momentum")
     if len(momentum) != n or not contiguous or m_device != device.index or m_shapes != shapes:
         raise ValueError("momentum must hold a contiguous tensor of each parameter's shape beside the parameters")
     if clip is not None and (clip.dtype is not torch.float32 or clip.shape != (2,) or clip.device != device
@@ -99,11 +141,18 @@ def muon_step(params, grads, momentum, *, lr, beta: float = 0.95, nesterov: bool
                  weight_decay=weight_decay, lr=lr, adjust=adjust)
     if all(g is None for g in grads):
         return
-    ws = _workspace(shapes, n, device)
-    with _on(device):
-        _lib.check(_lib.lib().ictc_hip_muon_step(p_at, g_at, m_at, *shapes, n, ctypes.byref(desc), _lib.ptr(clip),
+
+    def run(places):
+        own = _at(params, places)
+        _, p_at, g_at, _, _, _ = host.pairs(own, _at(grads, places), 1)
+        _, m_at, *sizes, _ = host.matrices(_at(momentum, places), "momentum")
+        ws = _workspace(sizes, len(own), device)
+        _lib.check(_lib.lib().ictc_hip_muon_step(p_at, g_at, m_at, *sizes, len(own), ctypes.byref(desc), _lib.ptr(clip),
                                                  lr_device, _lib.ptr(ws), ws.numel(), _lib.stream_of(device)),
                    "ictc_hip_muon_step")
+
+    with _on(device):
+        _both_kinds(shapes, device, run)
     # the kernels write through addresses: tell autograd (and caches keyed on versions) of the change
     host.written(params, grads)
     host.written(momentum, grads)

@@ -293,3 +293,31 @@ def test_coefficients_beyond_the_range(gpu):
     from ictc_o3.operators import orthogonalize
     got, other = orthogonalize([_draw((40, 40), 3).to(gpu), torch.zeros(8, 8, device=gpu)], steps=8, coefficients=(4.0, 0.0, 0.0))
     assert not got.isfinite().all() and not other.any()
+
+
+def test_both_kinds_of_matrices_captured(gpu):
+    """Matrices with short and with long shorter sides, which run on two streams, in a graph; and in between them
+    eager calls on another stream."""
+    from ictc_o3.operators import muon_step
+    shapes = [(40, 300), (200, 300), (3, 64, 64), (150, 150)]
+    first = [[_draw(s, 10 * j + k, scale).to(gpu) for k, s in enumerate(shapes)] for j, scale in ((1, 0.1), (2, 0.01), (3, 0.0))]
+    second = [[t.clone() for t in ts] for ts in first]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        muon_step(*first, lr=0.1)
+        muon_step(*second, lr=0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        muon_step(*first, lr=0.1)
+    for seed in range(3):
+        for k, (g, h) in enumerate(zip(first[1], second[1])):
+            g.copy_(_draw(g.shape, 100 * seed + k, 0.01))
+            h.copy_(g)
+        graph.replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            muon_step(*second, lr=0.1)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(first, second) for a, b in zip(x, y))
