@@ -17,16 +17,21 @@
 // the error's growth: singular values below 1e-3 of the largest come out wrong, 1e-4 of the result at rank-deficient
 // matrices.)
 //
-// Matrices with a side of more than 128 (below: the shorter side): all three products are of the form P Q^T with both operands' rows along the reduction (X X^T, A A^T, B (X^T)^T), so
-// one kernel does them; X is kept in both orientations.  A and B are symmetric: only tiles on and above the diagonal
-// are computed.  Every matrix of every tensor takes part in the same launches: `owner` says which matrix a workgroup's
-// tile belongs to.  Sides are padded with zeros to whole tiles, which stay zero.
+// Matrices with a shorter side of more than 128: all three products are of the form P Q^T with both operands' rows along
+// the reduction (X X^T, A A^T, B (X^T)^T), so one kernel does them; X is kept in both orientations.  A and B are
+// symmetric: only tiles on and above the diagonal are computed.  Every matrix of every tensor takes part in the same
+// launches: `owner` says which matrix a workgroup's tile belongs to.  Sides are padded with zeros to whole tiles, which
+// stay zero.  16 matrices of 1024 x 1024 and 8 of 1024 x 4096: average 106 us and normalise 169 (2.8 and 2.4 TB/s), then
+// each step X X^T 204, B 111, B X 358 us, 850 TFLOP/s of float16 instructions over all (a large float16 product of the
+// library 1,090): B X moves 12 bytes an entry in its epilogue (130 us at a copy's rate) and its operands through the L2
+// (171 us at the 19 TB/s it gives) for 123 us of instructions.
 //
 // Matrices with a shorter side of up to 128, of which most models have most: two launches a step, bound by latency.  A
-// workgroup keeps 64 columns of X at a time: it multiplies them by B, and adds what they give to the next X X^T at once,
-// from LDS; the other launch, one workgroup to a matrix, adds these parts up in order, and makes A A and B.  (Done by
-// the workgroup that is the last of its matrix to leave its part, it saves a launch, but what makes the parts of
-// others visible within one costs more: a step of the C128 / lmax 3 model's matrices 35 us against 23.)
+// workgroup keeps 128 columns of X at a time: it multiplies them by B, and adds what they give to the next X X^T at
+// once, from LDS; the other launch, one workgroup to a matrix, adds these parts up in order, and makes A A and B: 6.6
+// and 4.6 us for the 29 matrices (64 rows or columns) of a C64 / lmax 2 model, 11.7 and 8.5 for the 47 (128) of a C128 /
+// lmax 3 one.  (Done by the workgroup that is the last of its matrix to leave its part, it saves a launch, but what makes
+// the parts of others visible within one costs more: a step of the C128 model's matrices 35 us against 23.)
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -726,12 +731,21 @@ __device__ __forceinline__ void upper_block(int b, int& i, int& j) {
 }
 
 // (Two accumulators: a product waits for the one before it in the same accumulator twice as long as it takes to issue.)
-// FOURTH: with lo lo', for sides of up to 32, where too few terms are added up for what is left out to cancel (the
-// result's error at 1 x 77 and 8 x 64 1.5 times that of float32 products without it, and the same with it).
-template <bool FOURTH>
+// SINGLE: float32 products of the parts' sums, for sides of up to 32, where too few terms are added up for what is left
+// out to cancel: the result's error at 8 x 64 is 5.6e-7 of its norm, 6.4e-7 with the three products and lo lo', 6.2e-7 in
+// plain float32; these short matrices' workgroups wait for the larger ones' either way.  (Which of 16 columns a lane's
+// value is does not matter, as both operands have the same.)
+template <bool SINGLE>
 __device__ __forceinline__ void three_products(const half8& ah, const half8& al, const half8& bh, const half8& bl,
                                                f32x16& high, f32x16& low) {
-  if constexpr (FOURTH) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bl, low, 0, 0, 0);
+  if constexpr (SINGLE) {
+#pragma unroll
+    for (int r = 0; r < 8; r += 2) {
+      high = __builtin_amdgcn_mfma_f32_32x32x2f32(joined(ah[r], al[r]), joined(bh[r], bl[r]), high, 0, 0, 0);
+      low = __builtin_amdgcn_mfma_f32_32x32x2f32(joined(ah[r + 1], al[r + 1]), joined(bh[r + 1], bl[r + 1]), low, 0, 0, 0);
+    }
+    return;
+  }
   low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, low, 0, 0, 0);
   high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, high, 0, 0, 0);
   low = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, low, 0, 0, 0);
