@@ -18,8 +18,8 @@ EPS = 1e-5
 # width (one column, parts of a group of four, parts of a wave, whole ones, two and four groups a thread, rows of
 # 4 and 16 waves), rows (one, less than a workgroup's, more than the workgroups with partial sums hold)
 SHAPES = [(1, 3), (2, 9), (3, 300), (4, 1), (5, 70), (7, 2000), (16, 33), (63, 17), (64, 20000), (65, 40), (128, 130),
-          (255, 9), (256, 65), (257, 33), (510, 12), (512, 40), (1001, 21), (1024, 9), (1025, 5), (2048, 6), (2050, 7),
-          (4096, 3), (4099, 5), (8192, 2)]
+          (255, 9), (256, 65), (257, 33), (510, 12), (512, 40), (513, 20), (601, 37), (768, 5000), (769, 6), (1001,
+          21), (1024, 9), (1025, 5), (2048, 6), (2050, 7), (4096, 3), (4099, 5), (8192, 2)]
 
 
 def _formula(x, w, b, silu):
