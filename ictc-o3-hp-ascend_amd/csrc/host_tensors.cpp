@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <exception>
 #include <vector>
@@ -131,6 +132,41 @@ PyObject* matrices(PyObject*, PyObject* args) {
                        contiguous ? Py_True : Py_False);
 }
 
+// apart(params, momentum, grads): refuses written memory (params, momentum) that another one of the lists' tensors
+// overlaps, of those whose gradient is not None.  Gradients may share memory with each other.
+PyObject* apart(PyObject*, PyObject* args) {
+  PyObject* lists[3];
+  if (!PyArg_ParseTuple(args, "O!O!O!", &PyList_Type, &lists[0], &PyList_Type, &lists[1], &PyList_Type, &lists[2]))
+    return nullptr;
+  struct Piece {
+    uintptr_t from, to;
+    bool written;
+  };
+  std::vector<Piece> pieces;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(lists[2]); ++i) {
+    if (PyList_GET_ITEM(lists[2], i) == Py_None) continue;
+    for (int k = 0; k < 3; ++k) {
+      if (i >= PyList_GET_SIZE(lists[k])) continue;
+      const at::Tensor* t = item(lists[k], i, false, "parameters, momentum and gradients");
+      if (!t) return nullptr;
+      if (t->numel() == 0) continue;
+      const uintptr_t from = reinterpret_cast<uintptr_t>(t->const_data_ptr());
+      pieces.push_back({from, from + t->numel() * sizeof(float), k < 2});
+    }
+  }
+  std::sort(pieces.begin(), pieces.end(), [](const Piece& a, const Piece& b) { return a.from < b.from; });
+  uintptr_t written = 0, any = 0;      // where what begins earlier ends
+  for (const Piece& p : pieces) {
+    if (p.from < (p.written ? any : written)) {
+      PyErr_SetString(PyExc_ValueError, "parameters and momentum must not overlap each other or the gradients");
+      return nullptr;
+    }
+    any = std::max(any, p.to);
+    if (p.written) written = std::max(written, p.to);
+  }
+  Py_RETURN_NONE;
+}
+
 // alike(tensors) -> new contiguous tensors of their shapes
 PyObject* alike(PyObject*, PyObject* args) {
   PyObject* list;
@@ -185,6 +221,7 @@ PyMethodDef methods[] = {
     {"pairs", guarded<pairs>, METH_VARARGS, "(device, parameters, gradients, sizes, values, contiguous) of two lists"},
     {"matrices", guarded<matrices>, METH_VARARGS,
      "(device, addresses, rows, columns, batches, contiguous) of a list of matrices"},
+    {"apart", guarded<apart>, METH_VARARGS, "refuse parameters and momentum that overlap"},
     {"alike", guarded<alike>, METH_VARARGS, "new contiguous tensors of a list's shapes"},
     {"written", guarded<written>, METH_VARARGS,
      "raise the version counters of parameters written through their addresses"},

@@ -70,10 +70,12 @@ def _both_kinds(shapes, device, run) -> None:
         return
     here, side = torch.cuda.current_stream(device), _side_stream(device)
     side.wait_stream(here)
-    with torch.cuda.stream(side):
-        run(kinds[1])
-    run(kinds[0])
-    here.wait_stream(side)
+    try:
+        with torch.cuda.stream(side):
+            run(kinds[1])
+        run(kinds[0])
+    finally:
+        here.wait_stream(side)
 
 
 def _at(values, places):
@@ -113,7 +115,8 @@ def muon_step(params, grads, momentum, *, lr, beta: float = 0.95, nesterov: bool
               steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7, adjust: str = "original", clip=None) -> None:
     """One step of every parameter with a gradient, in place (a None gradient leaves its parameter and momentum as
     they are): a moving average of the gradient, orthogonalised as ``orthogonalize`` does, as the update.  The
-    parameters are matrices (or have leading axes that count them); no two of them may overlap.
+    parameters are matrices (or have leading axes that count them).  What is written, parameters and momentum, must
+    not overlap each other or a gradient.
 
     momentum: a list of float32 tensors of the parameters' shapes (zeros before the first step).  lr: a number, or a
     one-element float32 tensor on the device.  adjust: the update's size, "original" for sqrt(max(1, rows / columns))
@@ -137,6 +140,7 @@ def muon_step(params, grads, momentum, *, lr, beta: float = 0.95, nesterov: bool
         if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.device != device:
             raise ValueError("a learning rate tensor must hold one FP32 value beside the parameters")
         lr_device, lr = lr.data_ptr(), 0.0
+    host.apart(params, momentum, grads)
     desc = _desc(steps=steps, coefficients=coefficients, eps=eps, beta=beta, nesterov=nesterov,
                  weight_decay=weight_decay, lr=lr, adjust=adjust)
     if all(g is None for g in grads):

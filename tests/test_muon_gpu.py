@@ -321,3 +321,19 @@ def test_both_kinds_of_matrices_captured(gpu):
             muon_step(*second, lr=0.1)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for x, y in zip(first, second) for a, b in zip(x, y))
+
+
+def test_written_memory_that_overlaps_is_refused(gpu):
+    from ictc_o3.operators import muon_step
+    flat = _draw((8, 20), 5).to(gpu)
+    kept = flat.clone()
+    p, q, m, n = flat[:2], flat[2:4], flat[4:6], flat[6:]      # side by side
+    g = _draw((2, 20), 6).to(gpu)
+    for params, grads, momentum in (([p, p], [g, g], [m, q]), ([p, flat[1:3]], [g, g], [m, flat[4:6]]), ([p], [g], [p]),
+                                    ([p, q], [g, g], [m, m]), ([p], [p], [m]), ([p], [m], [m]),
+                                    ([p, q], [g, flat[1:3]], [m, flat[5:7]])):
+        with pytest.raises(ValueError, match="overlap"):
+            muon_step(params, grads, momentum, lr=0.1)
+    assert torch.equal(flat, kept)
+    muon_step([p, p, q], [g, None, g], [m, m, n[:2]], lr=0.1)  # without a gradient nothing is written; gradients may be one
+    assert not any(torch.equal(a, b) for a, b in zip(flat.split(2), kept.split(2)))
