@@ -21,7 +21,7 @@
 // the reduction (X X^T, A A^T, B (X^T)^T), so one kernel does them; X is kept in both orientations.  A and B are
 // symmetric: only tiles on and above the diagonal are computed.  Every matrix of every tensor takes part in the same
 // launches: `owner` says which matrix a workgroup's tile belongs to.  Sides are padded with zeros to whole tiles, which
-// stay zero.  16 matrices of 1024 x 1024 and 8 of 1024 x 4096: average 106 us and normalise 169 (2.8 and 2.4 TB/s), then
+// stay zero.  16 matrices of 1024 x 1024 and 8 of 1024 x 4096: average 106 us and normalise 169 (5.7 and 4.8 TB/s), then
 // each step X X^T 204, B 111, B X 358 us, 850 TFLOP/s of float16 instructions over all (a large float16 product of the
 // library 1,090): B X moves 12 bytes an entry in its epilogue (130 us at a copy's rate) and its operands through the L2
 // (171 us at the 19 TB/s it gives) for 123 us of instructions.
