@@ -10,7 +10,7 @@
 // here is of float32 accuracy on the float16 matrix cores: 2^11 x = hi + lo with hi = f16(2^11 x) and lo = f16(2^11 x - hi),
 // 22 bits or an absolute 2^-36, whichever is larger (entries of X and A are near 1 and below), and
 //   x y = 2^-22 (hi hi' + hi lo' + lo hi')  + (2^-22 x y, left out)
-// in one float32 accumulator.  Three products at 16 times the float32 instructions' rate.  What a power of two is chosen
+// in one float32 accumulator (sides of up to 32: float32 products).  Three products at 16 times the float32 instructions' rate.  What a power of two is chosen
 // for grows at most 32-fold: |X| stays near 1 with coefficients for which the iteration is of use.  A matrix with |U|
 // below eps, where X stays small, is kept times another power of two (2^e, see exponent_at), so that it has as many
 // bits.  (The form that iterates A alone and multiplies X once has a third of the work for wide matrices, but doubles
@@ -332,6 +332,27 @@ __device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
 
 __device__ __forceinline__ float joined(_Float16 hi, _Float16 lo) {
   return static_cast<float>(hi) + static_cast<float>(lo);
+}
+
+// The same, or (SINGLE: sides of up to 32, whose products are float32 ones) the two halves of a float's bits, in the same
+// places.
+template <bool SINGLE>
+__device__ __forceinline__ void split_for(float x, _Float16& hi, _Float16& lo) {
+  if constexpr (SINGLE) {
+    const uint32_t bits = __float_as_uint(x);
+    hi = __builtin_bit_cast(_Float16, static_cast<uint16_t>(bits >> 16));
+    lo = __builtin_bit_cast(_Float16, static_cast<uint16_t>(bits));
+  } else {
+    split(x, hi, lo);
+  }
+}
+
+template <bool SINGLE>
+__device__ __forceinline__ float joined_for(_Float16 hi, _Float16 lo) {
+  if constexpr (SINGLE)
+    return __uint_as_float(static_cast<uint32_t>(__builtin_bit_cast(uint16_t, hi)) << 16 | __builtin_bit_cast(uint16_t, lo));
+  else
+    return joined(hi, lo);
 }
 
 // The power of two that X is kept with before a step, from the one at first: |X| <= 2^-e, and a step multiplies it by at
@@ -731,18 +752,20 @@ __device__ __forceinline__ void upper_block(int b, int& i, int& j) {
 }
 
 // (Two accumulators: a product waits for the one before it in the same accumulator twice as long as it takes to issue.)
-// SINGLE: float32 products of the parts' sums, for sides of up to 32, where too few terms are added up for what is left
-// out to cancel: the result's error at 8 x 64 is 5.6e-7 of its norm, 6.4e-7 with the three products and lo lo', 6.2e-7 in
-// plain float32; these short matrices' workgroups wait for the larger ones' either way.  (Which of 16 columns a lane's
-// value is does not matter, as both operands have the same.)
+// SINGLE: float32 products of float32 values, for sides of up to 32, where too few terms are added up for what is left
+// out to cancel.  Errors of 64 x 8, 2 x 40 and 5 x 5 with columns of different size 5.3, 4.4 and 5.1e-7 of the result's
+// norm; 6.1, 6.5 and 6.2 with values of two halves, more with the three products; 6.6, 6.1 and 5.7 with library products
+// in float32.  These matrices' workgroups wait for the larger ones' either way.  (Which of 16 columns a lane's value is
+// does not matter, as both operands have the same.)
 template <bool SINGLE>
 __device__ __forceinline__ void three_products(const half8& ah, const half8& al, const half8& bh, const half8& bl,
                                                f32x16& high, f32x16& low) {
   if constexpr (SINGLE) {
 #pragma unroll
     for (int r = 0; r < 8; r += 2) {
-      high = __builtin_amdgcn_mfma_f32_32x32x2f32(joined(ah[r], al[r]), joined(bh[r], bl[r]), high, 0, 0, 0);
-      low = __builtin_amdgcn_mfma_f32_32x32x2f32(joined(ah[r + 1], al[r + 1]), joined(bh[r + 1], bl[r + 1]), low, 0, 0, 0);
+      high = __builtin_amdgcn_mfma_f32_32x32x2f32(joined_for<true>(ah[r], al[r]), joined_for<true>(bh[r], bl[r]), high, 0, 0, 0);
+      low = __builtin_amdgcn_mfma_f32_32x32x2f32(joined_for<true>(ah[r + 1], al[r + 1]),
+                                                 joined_for<true>(bh[r + 1], bl[r + 1]), low, 0, 0, 0);
     }
     return;
   }
@@ -831,7 +854,7 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             _Float16 h, l;
-            split(source[q].value(a, m, r, scale, inv), h, l);
+            split_for<MB == 1>(source[q].value(a, m, r, scale, inv), h, l);
             hi[r] = h, lo[r] = l;
           }
           const int i = m.transposed ? k % (M / 4) * 4 : k / kPart * 4, j = m.transposed ? k / (M / 4) : k % kPart;
@@ -882,13 +905,13 @@ __device__ __forceinline__ void short_chunk(const MuonArgs& a, const MuonMatrix&
             half4 hi = *reinterpret_cast<const half4*>(&lds.xt[0][at]), lo = *reinterpret_cast<const half4*>(&lds.xt[1][at]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              float v = fmaf(a.a, joined(hi[r], lo[r]), a.unpoly * acc[t][k + r]);
+              float v = fmaf(a.a, joined_for<MB == 1>(hi[r], lo[r]), a.unpoly * acc[t][k + r]);
               if (shift) v = ldexpf(v, shift);
               if constexpr (PHASE == kLast) {
                 acc[t][k + r] = v;
               } else {
                 _Float16 h, l;
-                split(v, h, l);
+                split_for<MB == 1>(v, h, l);
                 hi[r] = h, lo[r] = l;
               }
             }
@@ -1021,7 +1044,7 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       _Float16 h, l;
-      split(shift ? ldexpf(sum[q][r], shift) : sum[q][r], h, l);
+      split_for<MB == 1>(shift ? ldexpf(sum[q][r], shift) : sum[q][r], h, l);
       hi[r] = h, lo[r] = l;
       if (bi != bj) {
         const int to = turned_at(row + r, column / 8, kGroups) + column % 8;
@@ -1065,7 +1088,8 @@ __device__ __forceinline__ void short_poly(const MuonArgs& a, const MuonMatrix& 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         _Float16 h, l;
-        split(fmaf(a.b_kept, joined(old_hi[r], old_lo[r]), a.c_kept * (acc[q][k + r] + low[q][k + r])), h, l);
+        const float old = joined_for<MB == 1>(old_hi[r], old_lo[r]);
+        split_for<MB == 1>(fmaf(a.b_kept, old, a.c_kept * (acc[q][k + r] + low[q][k + r])), h, l);
         hi[r] = h, lo[r] = l;
         if (bi != bj) {
           to_global<_Float16>(poly + operand_at<M>(row + r, column), h);

@@ -85,7 +85,7 @@ def _at(values, places):
 def orthogonalize(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
     """Each matrix of a list (tensors [..., rows, columns], leading axes counting matrices) scaled to Frobenius norm
     1 and brought near an orthogonal one by ``steps`` Newton-Schulz products, as a list of new tensors.  Without
-    gradients.  The coefficients have to keep singular values below 5 (beyond, a result is not a number)."""
+    gradients.  The coefficients have to keep singular values below 5 (beyond, a result may not be a number)."""
     with torch.no_grad():
         matrices = list(matrices)
         if not matrices:

@@ -837,7 +837,7 @@ int ictc_hip_embedding_table_grad(const void* tokens, int index_bytes, const flo
  * X = U / (|U| + eps), |U| the Frobenius norm, and goes through `steps` of
  *   X <- a X + (b A + c A A) X,  A = X X^T        (a, b, c) = coefficients; m > n: of the transposed matrix
  * which brings its singular values near 1.  Products are of float32 accuracy (operands in two float16 parts, for which
- * coefficients have to keep singular values below 5: beyond, results are not a number).
+ * coefficients have to keep singular values below 5: beyond, results may not be numbers).
  *
  * Host arrays of `count` tensors, each of `batches` contiguous matrices of rows x cols; device addresses in them
  * are read before the call returns.
