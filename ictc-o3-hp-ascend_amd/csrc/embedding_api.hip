@@ -19,10 +19,10 @@
 // Parts are added up in 64 bits.
 //
 // Bound by memory: dy and the table are read once, y and dT written once; the sort moves 8 to 16 bytes a token
-// and pass.  500,001 tokens of 64 columns, 7,921 rows: lookup 22.5 us (5.8 TB/s), sort 35 (seven launches of 3 to 11,
-// bound by latency), sums 30 (4.3 TB/s), parts 7.  65,537 tokens of 512 columns, 50,000 rows: 36 us (7.4 TB/s; the
-// table's rows repeat), sort 28, sums 39 (4.9), parts 15.  105,634 tokens of 64 columns, 100 rows: lookup 7.4, sums 15,
-// parts 11 (sorted by all workgroups together: 15 + 17 + 33).
+// and pass.  500,001 tokens of 64 columns, 7,921 rows: lookup 22 us (5.9 TB/s), sort 29 (six launches of 3 to 10,
+// bound by latency), sums 28 (4.6 TB/s), parts 7.  65,537 tokens of 512 columns, 50,000 rows: 36 us (7.4 TB/s; the
+// table's rows repeat), sort 21, sums 34 to 39, parts 15.  105,634 tokens of 64 columns, 100 rows: lookup 7.2, sums 14,
+// parts 10 (sorted by all workgroups together: 15 + 17 + 33).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -35,7 +35,8 @@ constexpr int kEmbWave = 64;
 constexpr int kEmbThreads = 256;
 constexpr int kEmbWaves = kEmbThreads / kEmbWave;
 constexpr int kRadix = 256;                  // digits of 8 bits
-constexpr int kRounds = 8;                   // of a wave over its part of a tile
+constexpr int kRounds = 4;                   // of a wave over its part of a tile (8: sorts of 500,001 and 65,537 tokens
+                                             // 32 and 27 us against 29 and 21; 2: 31 and 18)
 constexpr int kTile = kRounds * kEmbThreads;
 constexpr int kLoads = 8;                    // rows on their way at a time
 constexpr int kParts = 16;                   // parts of a row on their way at a time
