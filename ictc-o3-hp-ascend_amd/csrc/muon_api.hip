@@ -50,7 +50,7 @@ constexpr int kMuWave = 64;
 constexpr int kTensorsPerLaunch = 44;        // of the table in the kernel's arguments
 constexpr int kPrep = 64;                    // side of a tile of the source
 constexpr int kStep = 32;                    // reduction entries in LDS at a time
-constexpr int64_t kMostBytes = int64_t{2} << 30;     // workspace that a call goes by, unless one tensor needs more
+constexpr int64_t kMostBytes = int64_t{2} << 30;     // workspace that a call goes by, unless one matrix needs more
 
 using half8 = _Float16 __attribute__((ext_vector_type(8)));
 using half4 = _Float16 __attribute__((ext_vector_type(4)));
@@ -1116,10 +1116,17 @@ constexpr int64_t kMostSide = 1 << 20;
 constexpr int64_t kMostMatrices = int64_t{1} << 23;
 constexpr int64_t kFewTiles = 512;
 constexpr int64_t kMostTiles = int64_t{1} << 23;      // of a launch: threads within 32 bits
+constexpr int64_t kMostChunks = (int64_t{1} << 31) / (kShortThreads > kPolyThreads ? kShortThreads : kPolyThreads);
 
-// Tensors [first, end) of a call whose matrices take part in the same launches, and what they need.
+// A matrix of a call: of which tensor, and which of its matrices.
+struct MuonPlace {
+  int64_t tensor, matrix;
+};
+
+// A call's matrices up to `end` that take part in the same launches, and what they need.
 struct MuonGroup {
-  int64_t end, matrices, prep, sym, apply, chunks, bytes;
+  MuonPlace end;
+  int64_t matrices, prep, sym, apply, chunks, bytes;
 
   void add(const MuonSize& s, int64_t batches) {
     matrices += batches, prep += batches * s.prep, sym += batches * s.sym, apply += batches * s.apply;
@@ -1137,19 +1144,28 @@ struct MuonGroup {
   int64_t size() const { return at_values() + bytes; }
 };
 
-// (Tensors that take no part are counted: the groups, and with them the workspace, go by the shapes alone.)
+// (Tensors that take no part are counted: the groups, and with them the workspace, go by the shapes alone.)  A stack
+// of matrices is split where the group is full, so that no launch and no workspace grows with its length.
 template <int T>
-MuonGroup muon_group(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t first, int64_t count) {
+MuonGroup muon_group(const int64_t* rows, const int64_t* cols, const int64_t* batches, MuonPlace first, int64_t count) {
   MuonGroup g = {};
-  int64_t k = first;
-  for (; k < count; ++k) {
-    if (!rows[k] || !cols[k] || !batches[k]) continue;
-    const MuonSize s = muon_size<T>(rows[k], cols[k]);
-    const int64_t b = batches[k];
-    if (g.matrices && (g.bytes + b * s.bytes > kMostBytes || g.prep + b * s.prep > kMostTiles)) break;
-    g.add(s, b);
+  MuonPlace at = first;
+  while (at.tensor < count) {
+    const int64_t k = at.tensor;
+    if (rows[k] && cols[k] && at.matrix < batches[k]) {
+      const MuonSize s = muon_size<T>(rows[k], cols[k]);
+      int64_t fits = std::min({batches[k] - at.matrix, (kMostBytes - g.bytes) / s.bytes, (kMostTiles - g.prep) / s.prep,
+                               kMostChunks - g.matrices});
+      if (s.chunks) fits = std::min(fits, (kMostChunks - g.chunks) / s.chunks);
+      if (!g.matrices) fits = std::max(fits, int64_t{1});
+      if (fits <= 0) break;
+      g.add(s, fits);
+      at.matrix += fits;
+      if (at.matrix < batches[k]) break;
+    }
+    ++at.tensor, at.matrix = 0;
   }
-  g.end = k;
+  g.end = at;
   return g;
 }
 
@@ -1161,7 +1177,7 @@ bool muon_valid(const int64_t* rows, const int64_t* cols, const int64_t* batches
       return false;
     if (!rows[k] || !cols[k] || !batches[k]) continue;
     const MuonSize s = muon_size<128>(rows[k], cols[k]);
-    if (s.prep > kMostTiles / batches[k]) return false;
+    if (s.prep > kMostTiles) return false;
   }
   return true;
 }
@@ -1189,10 +1205,10 @@ bool large_tiles(const int64_t* rows, const int64_t* cols, const int64_t* batche
 template <int T>
 int64_t muon_workspace(const int64_t* rows, const int64_t* cols, const int64_t* batches, int64_t count) {
   int64_t most = 0;
-  for (int64_t k = 0; k < count;) {
-    const MuonGroup g = muon_group<T>(rows, cols, batches, k, count);
+  for (MuonPlace at = {}; at.tensor < count;) {
+    const MuonGroup g = muon_group<T>(rows, cols, batches, at, count);
     if (g.size() > most) most = g.size();
-    k = g.end;
+    at = g.end;
   }
   return most;
 }
@@ -1219,8 +1235,8 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
   a.c_kept = static_cast<float>(d->coefficients[2] * poly / kScale / kScale);
   a.unpoly = static_cast<float>(1.0 / poly);
   a.nesterov = d->nesterov;
-  for (int64_t k = 0; k < count;) {
-    const MuonGroup g = muon_group<T>(rows, cols, batches, k, count);
+  for (MuonPlace from = {}; from.tensor < count;) {
+    const MuonGroup g = muon_group<T>(rows, cols, batches, from, count);
     if (g.size() > ws_bytes) return ICTC_ERR_INVALID_ARGUMENT;
     MuonMatrix* const matrices = reinterpret_cast<MuonMatrix*>(ws);
     const auto owners = [&](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
@@ -1245,31 +1261,37 @@ int muon_run(const float* const* src, float* const* momentum, float* const* out,
       return muon_launched();
     };
     // (and of those the longest first: their tiles take longest)
-    std::vector<int64_t> order;
-    for (int64_t t = k; t < g.end; ++t)
-      if (src[t] && rows[t] && cols[t] && batches[t]) order.push_back(t);
+    struct Piece {
+      int64_t tensor, first, batches;
+    };
+    std::vector<Piece> order;
+    for (MuonPlace p = from; p.tensor < count && p.tensor <= g.end.tensor; ++p.tensor, p.matrix = 0) {
+      const int64_t t = p.tensor, stop = t < g.end.tensor ? batches[t] : g.end.matrix;
+      if (src[t] && rows[t] && cols[t] && p.matrix < stop) order.push_back({t, p.matrix, stop - p.matrix});
+    }
     const auto longer = [&](int64_t t) { return rows[t] > cols[t] ? rows[t] : cols[t]; };
-    std::stable_sort(order.begin(), order.end(), [&](int64_t x, int64_t y) { return longer(x) > longer(y); });
+    std::stable_sort(order.begin(), order.end(), [&](const Piece& x, const Piece& y) { return longer(x.tensor) > longer(y.tensor); });
     for (int shorts = 0; shorts < 2; ++shorts) {
-      for (const int64_t t : order) {
+      for (const Piece& piece : order) {
+        const int64_t t = piece.tensor, before = piece.first * rows[t] * cols[t];
         const MuonSize s = muon_size<T>(rows[t], cols[t]);
         if (s.is_short != (shorts != 0)) continue;
         const double r = static_cast<double>(rows[t]), c = static_cast<double>(cols[t]);
         MuonTensor& e = table.tensor[table.count++];
-        e.src = src[t], e.momentum = momentum ? momentum[t] : nullptr, e.out = out[t];
+        e.src = src[t] + before, e.momentum = momentum ? momentum[t] + before : nullptr, e.out = out[t] + before;
         e.base = at.bytes, e.rows = static_cast<int32_t>(rows[t]), e.cols = static_cast<int32_t>(cols[t]);
-        e.batches = static_cast<int32_t>(batches[t]), e.first = static_cast<int32_t>(at.matrices);
+        e.batches = static_cast<int32_t>(piece.batches), e.first = static_cast<int32_t>(at.matrices);
         e.prep = static_cast<uint32_t>(at.prep), e.sym = static_cast<uint32_t>(at.sym);
         e.apply = static_cast<uint32_t>(at.apply), e.chunk = static_cast<uint32_t>(at.chunks);
         e.rate = static_cast<float>(d->adjust == ICTC_MUON_SHAPE ? sqrt(r > c ? r / c : 1.0) : 0.2 * sqrt(r > c ? r : c));
-        at.add(s, batches[t]);
+        at.add(s, piece.batches);
         if (table.count == kTensorsPerLaunch)
           if (const int rc = send()) return rc;
       }
       if (!shorts) longs = at;
     }
     if (const int rc = send()) return rc;
-    k = g.end;
+    from = g.end;
     if (!at.matrices) continue;
     const auto launch = [&](void (*kernel)(MuonArgs, int), int64_t grid, int step) {
       if (grid) hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kShortThreads), 0, stream, a, step);

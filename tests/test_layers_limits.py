@@ -1,0 +1,26 @@
+"""What the layers and orthogonalised updates ask for and refuse, without a GPU: workspaces that do not grow with what
+a call could be split by, and numbers that are none."""
+import ctypes
+
+import pytest
+
+
+def _lib():
+    from ictc_o3 import _lib as binding
+    return binding.lib()
+
+
+def _muon_workspace(*shapes):
+    n = len(shapes)
+    return _lib().ictc_hip_muon_workspace(*[(ctypes.c_int64 * n)(*column) for column in zip(*shapes)], n)
+
+
+@pytest.mark.parametrize("rows,cols", [(8, 8), (64, 64), (1, 5000), (128, 300), (200, 300)])
+def test_workspace_of_a_stack_is_bounded(rows, cols):
+    """A stack's matrices go through the workspace in groups: 2 GiB of values, and the tables beside them, 1 % of that."""
+    at_once, most = _muon_workspace((rows, cols, 1)), 2 ** 31 * 1.02
+    assert 0 < at_once < 2 ** 26
+    for matrices in (100_000, (1 << 23) - 1, 1 << 23):
+        assert at_once < _muon_workspace((rows, cols, matrices)) <= most
+    # beside other tensors, and with empty ones between
+    assert 0 < _muon_workspace((5, 7, 3), (rows, cols, 1 << 20), (0, 4, 2), (rows, cols, 1 << 20), (700, 600, 2)) <= most

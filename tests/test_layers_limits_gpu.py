@@ -1,0 +1,36 @@
+"""Layer norm, embedding and orthogonalised updates at the ends of what they take: stacks of matrices that are split."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _draw(shape, seed, gpu, scale=1.0):
+    return scale * torch.randn(*shape, device=gpu, generator=torch.Generator(device=gpu).manual_seed(seed))
+
+
+@pytest.mark.parametrize("shape,parts", [((200_000, 8, 8), 7), ((90, 300, 5000), 4)], ids=["short", "long"])
+def test_stacks_in_several_groups(gpu, shape, parts):
+    """A stack that takes several turns in the workspace has the bits of its parts alone, whatever lies beside it."""
+    from ictc_o3.operators import orthogonalize
+    u, other = _draw(shape, 1, gpu), _draw((50, 60), 2, gpu)
+    got = orthogonalize([other, u, other])
+    want = torch.cat([orthogonalize([p])[0] for p in u.chunk(parts)])
+    assert torch.equal(got[1], want)
+    assert torch.equal(got[0], got[2]) and torch.equal(got[0], orthogonalize([other])[0])
+
+
+def test_steps_of_stacks_in_several_groups(gpu):
+    """Parameters and momentum of every part are written once, those without a gradient not at all."""
+    from ictc_o3.operators import muon_step
+    shapes = [(120_000, 4, 9), (70_000, 12, 5), (3, 20, 20)]
+    first = [[_draw(s, 10 * j + k, gpu, scale) for k, s in enumerate(shapes)]
+             for j, scale in ((1, 0.1), (2, 0.01), (3, 0.005))]
+    grads = [first[1][0], None, first[1][2]]
+    second = [[t.clone() for t in ts] for ts in first]
+    muon_step(first[0], grads, first[2], lr=0.1)
+    for k in (0, 2):
+        for p, g, m in zip(*(ts[k].chunk(5) for ts in second)):
+            muon_step([p], [g], [m], lr=0.1)
+    for ts, us in ((first[0], second[0]), (first[2], second[2])):
+        assert all(torch.equal(t, u) for t, u in zip(ts, us))
