@@ -10,9 +10,10 @@
 // tokens, split evenly over its groups of lanes; a group reads the gradient's rows in sorted order, writes the runs that lie
 // within its share, and leaves its first and its last one in LDS, where runs over several groups are joined.
 //
-//   * Up to 255 rows (species, few pairs): a workgroup sorts its own tokens, in LDS, and leaves a part for each row it
-//     meets; the second launch adds every row's parts up in order.  The sort then costs no launch and no traffic.
-//   * More rows: a radix sort of all tokens by 8 bits a pass (histogram, scan, scatter; stable).  Runs within a workgroup
+//   * Up to 255 rows (species, few pairs) of up to 64 columns, or with few tokens (see sorts_locally): a workgroup sorts its
+//     own tokens, in LDS, and leaves a part for each row it meets; the second launch adds every row's parts up in order.
+//     The sort then costs no launch and no traffic.
+//   * Else: a radix sort of all tokens by 8 bits a pass (histogram, scan, scatter; stable).  Runs within a workgroup
 //     are written at once.  One that goes on into the next workgroup's tokens leaves its part in that one's `head`,
 //     or in `tail` of the one in which it begins; the last launch adds a row's parts up in order and writes zeros for
 //     rows without tokens.
@@ -43,6 +44,8 @@ constexpr int kParts = 16;                   // parts of a row on their way at a
 constexpr int kShare = 32;                   // sorted tokens of a group of lanes at most
 constexpr int kLong = 32;                    // parts of a row that one group adds up
 constexpr int kFewRows = kRadix - 1;         // rows of tables whose tokens are sorted by the workgroup (and padding)
+constexpr int kFewColumns = 64;
+constexpr int64_t kFewValues = int64_t{1} << 21;      // of the gradient
 constexpr int kMostLocal = 512;              // tokens of such a workgroup
 constexpr int kRowGrid = 2048;               // workgroups that rows with parts are spread over
 constexpr int kAhead = 4;                    // rows of a lookup's group of lanes at a time
@@ -580,6 +583,16 @@ struct Split {
   }
 };
 
+// Whether workgroups sort their own tokens.  The wider the rows, the fewer tokens a workgroup has, the more of them are of
+// different rows and the more of the gradient's size its parts have (they are written and read again, and 255 rows of 256
+// columns and more would take twice its size), against a sort of all tokens whose launches cost 8 us.  Of 100 rows,
+// us here / with all sorted: 64 columns, 2,048 tokens 12 / 19, 65,536 21 / 24, 300,000 38 / 39; 128 columns 11 / 19,
+// (20,000) 25 / 20, 29 / 28 and 94 / 48; 512 columns 12 / 19, (20,000) 32 / 29, 79 / 39 and 501 / 121; 10 and 255 rows
+// of 512 columns, 300,000 tokens 472 / 126 and 499 / 123.
+bool sorts_locally(int64_t rows, int width, int64_t count) {
+  return rows <= kFewRows && (width <= kFewColumns || count * width <= kFewValues);
+}
+
 // Where everything lies in the workspace, in 4-byte units.
 struct EmbeddingSpace {
   int64_t keys[2], places[2], counts, totals, spans, met, parts, size;
@@ -588,7 +601,7 @@ struct EmbeddingSpace {
 
   EmbeddingSpace(int64_t rows, int width, int64_t count, const Split& split) {
     tiles = static_cast<int>((count + kTile - 1) / kTile);
-    local = rows <= kFewRows;
+    local = sorts_locally(rows, width, count);
     int64_t at = 0;
     const auto take = [&](int64_t n) {
       const int64_t first = at;

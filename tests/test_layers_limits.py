@@ -24,3 +24,13 @@ def test_workspace_of_a_stack_is_bounded(rows, cols):
         assert at_once < _muon_workspace((rows, cols, matrices)) <= most
     # beside other tensors, and with empty ones between
     assert 0 < _muon_workspace((5, 7, 3), (rows, cols, 1 << 20), (0, 4, 2), (rows, cols, 1 << 20), (700, 600, 2)) <= most
+
+
+@pytest.mark.parametrize("rows", [1, 2, 100, 254, 255, 256, 1000])
+@pytest.mark.parametrize("width", [1, 4, 63, 64, 65, 128, 256, 1000, 1024, 4096])
+def test_workspace_of_a_table_gradient_is_bounded(rows, width):
+    """Parts of rows stay within 64 MiB or about half of the gradient's size (255 of 512 tokens may be of different rows),
+    beside what goes by tokens (keys and places twice, counts) and rows (spans) alone."""
+    for count in (1, 2048, 20_000, 65_536, 300_000, 4_000_000, 100_000_000):
+        units = _lib().ictc_hip_embedding_workspace(rows, width, count)
+        assert 0 < units <= max(2 ** 24, 0.52 * count * width) + 5 * count + 3 * rows + 4096, (count, units)

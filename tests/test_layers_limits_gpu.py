@@ -1,6 +1,9 @@
-"""Layer norm, embedding and orthogonalised updates at the ends of what they take: stacks of matrices that are split."""
+"""Layer norm, embedding and orthogonalised updates at the ends of what they take: stacks of matrices that are split, and
+tables on both sides of the rule by which their tokens are sorted."""
 import pytest
 import torch
+
+from test_embedding_gpu import _case, _check_gradient
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +37,16 @@ def test_steps_of_stacks_in_several_groups(gpu):
             muon_step([p], [g], [m], lr=0.1)
     for ts, us in ((first[0], second[0]), (first[2], second[2])):
         assert all(torch.equal(t, u) for t, u in zip(ts, us))
+
+
+@pytest.mark.parametrize("count,rows,width", [(40_000, 255, 64), (40_000, 255, 65), (40_000, 256, 64), (8192, 255, 256),
+                                              (8193, 255, 256), (8193, 1, 256), (8193, 200, 300), (20_000, 3, 513)])
+def test_few_rows_of_many_columns(gpu, count, rows, width):
+    """Tolerance: test_embedding_gpu's.  Some tokens lie outside the table."""
+    from ictc_o3.operators import embedding
+    tokens, table, dy = _case(count, rows, width, count + rows + width)
+    tokens[::13] = -1
+    leaf, at, top = table.to(gpu).requires_grad_(), tokens.to(gpu), dy.to(gpu)
+    first, second = (torch.autograd.grad(embedding(at, leaf, scale=0.5), leaf, top)[0] for _ in range(2))
+    _check_gradient(first, tokens, dy, rows, 0.5)
+    assert torch.equal(first, second)
