@@ -50,3 +50,17 @@ def test_few_rows_of_many_columns(gpu, count, rows, width):
     first, second = (torch.autograd.grad(embedding(at, leaf, scale=0.5), leaf, top)[0] for _ in range(2))
     _check_gradient(first, tokens, dy, rows, 0.5)
     assert torch.equal(first, second)
+
+
+@pytest.mark.parametrize("shape", [(64, 3000), (3000, 40), (128, 2000), (300, 2000), (20, 3000)], ids=str)
+def test_values_between_products_keep_both_parts(gpu, shape):
+    """With coefficients (3 / 4, 0, 0) the iteration leaves X times 3 / 4 a step, through all its roundings, one by one: the
+    scale's, its product, and in each step what is kept of X (2^-23, or an absolute 2^-36) and the product's: none of
+    10^5 values is off by more."""
+    from ictc_o3.operators import orthogonalize
+    u = _draw(shape, 1, gpu)
+    for steps in (1, 2, 3):
+        got, = orthogonalize([u], steps=steps, coefficients=(0.75, 0.0, 0.0))
+        want = u.double() / (u.double().norm() + 1e-7) * 0.75 ** steps
+        bound = (2 * 2.0 ** -24 + steps * (2.0 ** -23 + 2.0 ** -24)) * 1.001 * want.abs() + steps * 2.0 ** -36
+        assert bool(((got.double() - want).abs() <= bound).all()), ((got.double() - want).abs() / bound).max()
