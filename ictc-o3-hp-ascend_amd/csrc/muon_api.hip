@@ -370,13 +370,13 @@ __device__ __forceinline__ int exponent_at(const MuonArgs& a, int e, int step) {
   return e;
 }
 
-// What a matrix's values are multiplied by at first, as a float in [1, 2) and a power of two (floats of any norm stay
-// in range).
+// What a matrix's values are multiplied by at first, as a float in [1, 2) and a power of two, which comes first: with
+// both a value is at most 2^11 (|X| <= 1), so floats of any size stay in range, and the smallest lose no bits.
 struct Scale {
   float mantissa;
   int exponent;
 
-  __device__ __forceinline__ float of(float x) const { return ldexpf(x * mantissa, exponent); }
+  __device__ __forceinline__ float of(float x) const { return ldexpf(x, exponent) * mantissa; }
 };
 
 // That scale from the matrix's tiles' squares (its power of two among it); every workgroup of the matrix calls it, and

@@ -1,9 +1,10 @@
-"""Layer norm, embedding and orthogonalised updates at the ends of what they take: stacks of matrices that are split, and
-tables on both sides of the rule by which their tokens are sorted."""
+"""Layer norm, embedding and orthogonalised updates at the ends of what they take: stacks of matrices that are split,
+tables on both sides of the rule by which their tokens are sorted, matrices of float32's largest and smallest numbers."""
 import pytest
 import torch
 
 from test_embedding_gpu import _case, _check_gradient
+from test_muon_gpu import _check, _exact
 
 pytestmark = pytest.mark.gpu
 
@@ -50,6 +51,20 @@ def test_few_rows_of_many_columns(gpu, count, rows, width):
     first, second = (torch.autograd.grad(embedding(at, leaf, scale=0.5), leaf, top)[0] for _ in range(2))
     _check_gradient(first, tokens, dy, rows, 0.5)
     assert torch.equal(first, second)
+
+
+@pytest.mark.parametrize("scale", [3.4e38, -2.5e38, 1e-42, 1e-44], ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (40, 70), (200, 300), (150, 140)], ids=str)
+def test_largest_and_smallest_numbers(gpu, shape, scale):
+    """Entries up to float32's last power of two, and ones that are below its normal range (then X stays far below 1).
+    Tolerance: test_muon_gpu's (results are at least 3.4^5 1e-44 / eps, far above float32's smallest number)."""
+    from ictc_o3.operators import orthogonalize
+    u = torch.rand(*shape, generator=torch.Generator().manual_seed(1), dtype=torch.float64) * 2 - 1
+    u[0, 0] = 1.0
+    u = (u * scale).float()
+    assert u.isfinite().all() and u[0, 0] != 0
+    got, = orthogonalize([u.to(gpu)])
+    _check(got, _exact(u))
 
 
 @pytest.mark.parametrize("shape", [(64, 3000), (3000, 40), (128, 2000), (300, 2000), (20, 3000)], ids=str)
