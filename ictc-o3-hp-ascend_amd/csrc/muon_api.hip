@@ -389,7 +389,7 @@ __device__ __forceinline__ Scale first_scale(const MuonArgs& a, const MuonMatrix
   const double norm = sqrt(muon_block_sum<THREADS>(sum, part)), share = norm / (norm + a.eps);
   const int e = share > 0.0 && share < 0.5 ? min(-ilogb(share) - 1, kMostExponent) : 0;
   if (threadIdx.x == 0 && keeps) a.exponents[owner] = e;
-  const double scale = kScale / (norm + a.eps);
+  const double scale = norm == 0.0 ? 1.0 : kScale / (norm + a.eps);      // (zeros stay zeros, however small eps is)
   const int power = ilogb(scale);
   return {static_cast<float>(ldexp(scale, -power)), power + e};
 }

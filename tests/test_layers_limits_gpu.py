@@ -79,3 +79,14 @@ def test_values_between_products_keep_both_parts(gpu, shape):
         want = u.double() / (u.double().norm() + 1e-7) * 0.75 ** steps
         bound = (2 * 2.0 ** -24 + steps * (2.0 ** -23 + 2.0 ** -24)) * 1.001 * want.abs() + steps * 2.0 ** -36
         assert bool(((got.double() - want).abs() <= bound).all()), ((got.double() - want).abs() / bound).max()
+
+
+def test_zeros_with_the_smallest_eps(gpu):
+    """Any positive eps is allowed: 1 / eps need not be a number."""
+    from ictc_o3.operators import muon_step, orthogonalize
+    shapes = [(1, 1), (5, 6), (3, 60, 70), (150, 140)]
+    for got in orthogonalize([torch.zeros(*s, device=gpu) for s in shapes], eps=1e-320):
+        assert not got.any()
+    p, g, m = torch.ones(20, 30, device=gpu), torch.zeros(20, 30, device=gpu), torch.zeros(20, 30, device=gpu)
+    muon_step([p], [g], [m], lr=0.5, weight_decay=0.5, eps=1e-320)
+    assert bool((p == 0.75).all()) and not m.any()
