@@ -17,7 +17,7 @@
 //     are written at once.  One that goes on into the next workgroup's tokens leaves its part in that one's `head`,
 //     or in `tail` of the one in which it begins; the last launch adds a row's parts up in order and writes zeros for
 //     rows without tokens.
-// Parts are added up in 64 bits.
+// Up to 32 tokens of a share and then up to 32 shares are added up in float32, the parts they leave in 64 bits.
 //
 // Bound by memory: dy and the table are read once, y and dT written once; the sort moves 8 to 16 bytes a token
 // and pass.  500,001 tokens of 64 columns, 7,921 rows: lookup 22 us (5.9 TB/s), sort 29 (six launches of 3 to 10,
@@ -42,6 +42,9 @@ constexpr int kTile = kRounds * kEmbThreads;
 constexpr int kLoads = 8;                    // rows on their way at a time
 constexpr int kParts = 16;                   // parts of a row on their way at a time
 constexpr int kShare = 32;                   // sorted tokens of a group of lanes at most
+constexpr int kLeast = 8;                    // lanes of a group that sums them: at most 32 groups, which are joined one after
+                                             // another (400,000 tokens of 4 columns, 200 rows 33 us, with one lane 66; of
+                                             // 16 columns, 30 rows 28 against 26)
 constexpr int kLong = 32;                    // parts of a row that one group adds up
 constexpr int kFewRows = kRadix - 1;         // rows of tables whose tokens are sorted by the workgroup (and padding)
 constexpr int kFewColumns = 64;
@@ -573,7 +576,8 @@ struct Split {
   int threads, columns, share, size, workgroups;
 
   Split(int width, int64_t count) {
-    threads = row_threads(width), columns = (width + 4 * threads - 1) / (4 * threads);
+    threads = row_threads(width) < kLeast ? kLeast : row_threads(width);
+    columns = (width + 4 * threads - 1) / (4 * threads);
     const int groups = kEmbThreads / threads;
     share = kShare;
     while (share > kLoads && count / (static_cast<int64_t>(groups) * share) * columns < kFill) share /= 2;

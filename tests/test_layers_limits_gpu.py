@@ -90,3 +90,18 @@ def test_zeros_with_the_smallest_eps(gpu):
     p, g, m = torch.ones(20, 30, device=gpu), torch.zeros(20, 30, device=gpu), torch.zeros(20, 30, device=gpu)
     muon_step([p], [g], [m], lr=0.5, weight_decay=0.5, eps=1e-320)
     assert bool((p == 0.75).all()) and not m.any()
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("width,share", [(1, 2), (8, 4), (64, 8)])
+def test_many_small_sums_behind_a_large_one(gpu, rows, width, share):
+    """What every group of a workgroup's lanes adds, just under half of a float32 step of the sum so far, is not lost:
+    the bound of test_embedding_gpu, 64 additions in float32, whatever the number of groups."""
+    from ictc_o3.operators import embedding
+    dy = torch.full((512, width), 0.98 * 2.0 ** -24 / share)
+    dy[:share] = 0.0
+    dy[0] = 1.0
+    tokens = torch.zeros(512, dtype=torch.int64)
+    leaf = torch.zeros(rows, width, device=gpu, requires_grad=True)
+    got, = torch.autograd.grad(embedding(tokens.to(gpu), leaf), leaf, dy.to(gpu))
+    _check_gradient(got, tokens, dy, rows, 1.0)
