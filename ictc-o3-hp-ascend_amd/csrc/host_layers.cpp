@@ -336,7 +336,7 @@ void require_gpu_fp32(const Tensor& t, const Tensor& beside) {
 // A Python number as a double (bool is none).
 double number(PyObject* o, const char* what) {
   const double v = PyBool_Check(o) || !(PyFloat_Check(o) || PyLong_Check(o)) ? NAN : PyFloat_AsDouble(o);
-  if (!std::isfinite(v)) {
+  if (!std::isfinite(v) || PyErr_Occurred()) {       // (an integer beyond a double's range is -1 with an exception)
     PyErr_Clear();
     throw Refused(what);
   }

@@ -3,6 +3,7 @@ a call could be split by, and numbers that are none."""
 import ctypes
 
 import pytest
+import torch
 
 
 def _lib():
@@ -34,3 +35,13 @@ def test_workspace_of_a_table_gradient_is_bounded(rows, width):
     for count in (1, 2048, 20_000, 65_536, 300_000, 4_000_000, 100_000_000):
         units = _lib().ictc_hip_embedding_workspace(rows, width, count)
         assert 0 < units <= max(2 ** 24, 0.52 * count * width) + 5 * count + 3 * rows + 4096, (count, units)
+
+
+def test_integers_beyond_a_double_are_refused():
+    """As what they are, with nothing pending behind the refusal."""
+    from ictc_o3 import embedding, layer_norm
+    for large in (10 ** 400, -10 ** 400):
+        with pytest.raises(ValueError, match="scale must be a finite number"):
+            embedding(torch.zeros(2, dtype=torch.int64), torch.ones(3, 4), scale=large)
+        with pytest.raises(ValueError, match="eps must be a positive number"):
+            layer_norm(torch.ones(2, 4), torch.ones(4), eps=large)
