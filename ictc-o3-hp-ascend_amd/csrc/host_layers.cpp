@@ -333,10 +333,10 @@ void require_gpu_fp32(const Tensor& t, const Tensor& beside) {
   if (t.device() != beside.device()) throw Refused("All operands must be on the same GPU");
 }
 
-// A Python number as a double (bool is none).
+// A Python number as a double that is finite as a float, too (bool is none).
 double number(PyObject* o, const char* what) {
   const double v = PyBool_Check(o) || !(PyFloat_Check(o) || PyLong_Check(o)) ? NAN : PyFloat_AsDouble(o);
-  if (!std::isfinite(v) || PyErr_Occurred()) {       // (an integer beyond a double's range is -1 with an exception)
+  if (!std::isfinite(static_cast<float>(v)) || PyErr_Occurred()) {       // (an integer beyond a double's range is -1 with an exception)
     PyErr_Clear();
     throw Refused(what);
   }
@@ -370,8 +370,7 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
   if (!PyArg_ParseTuple(args, "OOOiO", &x, &weight, &bias, &activation, &given_eps)) return nullptr;
   if (!lib.norm_forward) throw std::runtime_error("the host module is not bound to the library");
   const double eps = number(given_eps, "eps must be a positive number");
-  if (!(static_cast<float>(eps) > 0.f) || !std::isfinite(static_cast<float>(eps)))
-    throw Refused("eps must be a positive number");
+  if (!(static_cast<float>(eps) > 0.f)) throw Refused("eps must be a positive number");
   const Tensor& features = tensor(x);
   if (features.dim() < 1 || features.size(-1) < 1 || features.size(-1) > ICTC_LAYER_NORM_MAX_WIDTH)
     throw Refused("features must have between 1 and " + std::to_string(ICTC_LAYER_NORM_MAX_WIDTH) + " columns");

@@ -45,3 +45,13 @@ def test_integers_beyond_a_double_are_refused():
             embedding(torch.zeros(2, dtype=torch.int64), torch.ones(3, 4), scale=large)
         with pytest.raises(ValueError, match="eps must be a positive number"):
             layer_norm(torch.ones(2, 4), torch.ones(4), eps=large)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, 2 ** 128])
+def test_scales_beyond_float32_are_refused(scale):
+    """The kernels take the scale as a float32: one that is none there would give infinities for every token."""
+    from ictc_o3 import embedding, layer_norm
+    with pytest.raises(ValueError, match="scale must be a finite number"):
+        embedding(torch.zeros(2, dtype=torch.int64), torch.ones(3, 4), scale=scale)
+    with pytest.raises(ValueError, match="eps must be a positive number"):
+        layer_norm(torch.ones(2, 4), torch.ones(4), eps=abs(scale))
