@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -120,6 +121,7 @@ variable_list composed(const Spec& s, const variable_list& inputs, const bool (&
   const PyGILState_STATE state = PyGILState_Ensure();
   PyObject* result = nullptr;
   variable_list grads(4);
+  std::optional<python_error> error;      // (an exception of the formula's goes on as what it is)
   bool failed = false;
   {
     PyObject* ins = PyTuple_New(4);
@@ -132,18 +134,11 @@ variable_list composed(const Spec& s, const variable_list& inputs, const bool (&
     Py_XDECREF(tops);
     Py_XDECREF(needs);
   }
-  std::string message;
-  if (!result || !PyTuple_Check(result) || PyTuple_GET_SIZE(result) != 4) {
+  if (!result) {
+    error.emplace();
+    error->persist();
+  } else if (!PyTuple_Check(result) || PyTuple_GET_SIZE(result) != 4) {
     failed = true;
-    PyObject *type, *value, *trace;
-    PyErr_Fetch(&type, &value, &trace);
-    PyObject* text = value ? PyObject_Str(value) : nullptr;
-    message = text && PyUnicode_AsUTF8(text) ? PyUnicode_AsUTF8(text) : "the composed gradients failed";
-    Py_XDECREF(text);
-    Py_XDECREF(type);
-    Py_XDECREF(value);
-    Py_XDECREF(trace);
-    PyErr_Clear();
   } else {
     for (int k = 0; k < 4; ++k) {
       PyObject* g = PyTuple_GET_ITEM(result, k);
@@ -152,7 +147,8 @@ variable_list composed(const Spec& s, const variable_list& inputs, const bool (&
   }
   Py_XDECREF(result);
   PyGILState_Release(state);
-  if (failed) throw std::runtime_error(message);
+  if (error) throw *error;
+  if (failed) throw std::runtime_error("the composed gradients are not four");
   return grads;
 }
 
@@ -418,12 +414,11 @@ PyObject* guarded(PyObject* self, PyObject* args) {
   try {
     return F(self, args);
   } catch (const Refused& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, e.what());
-    return nullptr;
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+    PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const std::exception&) {      // (memory that ran out, a hook's own exception: each as torch's calls raise it)
+    torch::translate_exception_to_python(std::current_exception());
   }
+  return nullptr;
 }
 
 PyMethodDef methods[] = {

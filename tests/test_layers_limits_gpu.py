@@ -105,3 +105,24 @@ def test_many_small_sums_behind_a_large_one(gpu, rows, width, share):
     leaf = torch.zeros(rows, width, device=gpu, requires_grad=True)
     got, = torch.autograd.grad(embedding(tokens.to(gpu), leaf), leaf, dy.to(gpu))
     _check_gradient(got, tokens, dy, rows, 1.0)
+
+
+def test_exceptions_keep_their_types(gpu, monkeypatch):
+    """Memory that runs out, and what the composed formulas or a hook raise, reach the caller as what they are."""
+    from ictc_o3.backends.hip import layer_norm as module
+    from ictc_o3.operators import embedding, layer_norm
+    with pytest.raises(torch.OutOfMemoryError):          # 800 GB
+        embedding(torch.zeros(200_000, dtype=torch.int64, device=gpu), torch.zeros(2, 1 << 20, device=gpu))
+
+    def fails(*args):
+        raise KeyError("none")
+
+    x, w = _draw((3, 8), 1, gpu).requires_grad_(), torch.ones(8, device=gpu, requires_grad=True)
+    dw, = torch.autograd.grad(layer_norm(x, w), w, torch.ones(3, 8, device=gpu), create_graph=True)
+    with monkeypatch.context() as patch:
+        patch.setattr(module, "gradient_formula", fails)
+        with pytest.raises(KeyError, match="none"):
+            torch.autograd.grad(dw.sum(), x, retain_graph=True)
+    assert torch.autograd.grad(dw.sum(), x)[0].shape == x.shape
+    with torch.autograd.graph.saved_tensors_hooks(fails, lambda t: t), pytest.raises(KeyError, match="none"):
+        layer_norm(x, w)
