@@ -76,7 +76,7 @@ from .activation import silu
 from .embedding import edge_embedding
 from .geometry import edge_vectors, one_hot_rows
 from .linear import Linear, linear
-from .radial import bessel_embedding, polynomial_cutoff
+from .radial import bessel_embedding, cutoff_envelope
 
 SILU_SCALE = 1.6791767923989418   # _Normalize2MomSiLU (pure_cartesian_ictd_fix.py:610-619)
 
@@ -436,7 +436,7 @@ class MaceICTC(nn.Module):
             pairs = None
             if self.edge_species:
                 pairs = species.index_select(0, edge_src) * self.num_elements + species.index_select(0, edge_dst)
-            extras = EdgeExtras(polynomial_cutoff(vec.norm(dim=1), self.cutoff, self.cutoff_p), pairs)
+            extras = EdgeExtras(cutoff_envelope(vec, self.cutoff, self.cutoff_p), pairs)
         side = self._side_work(edge_feats, harmonics, extras)
         energy = None
         if self.block_norm:

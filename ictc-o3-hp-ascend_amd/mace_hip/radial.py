@@ -23,6 +23,15 @@ def polynomial_cutoff(r: torch.Tensor, r_max: float, p: int = 5) -> torch.Tensor
     return env * (r < float(r_max)).to(r.dtype)
 
 
+def cutoff_envelope(vec: torch.Tensor, r_max: float, p: int = 5) -> torch.Tensor:
+    """``polynomial_cutoff`` of the lengths of [E, 3] vectors, differentiable as often as p allows at length zero, too,
+    where torch's norm has no second derivative: below 1e-6 r_max the envelope is 1 to all digits (its derivatives up to
+    the order p - 1 vanish at 0, the second one is below 1e-15 there) and its derivatives are taken as zero."""
+    near = vec.detach().norm(dim=1) < 1e-6 * r_max
+    apart = torch.where(near.unsqueeze(1), torch.full_like(vec, 0.5 * r_max), vec)
+    return torch.where(near, torch.ones_like(vec[:, 0]), polynomial_cutoff(apart.norm(dim=1), r_max, p))
+
+
 def bessel_embedding(r: torch.Tensor, *, r_max: float, num_basis: int = 8, cutoff_p: int | None = 5,
                      sqrt_num_basis_norm: bool = False) -> torch.Tensor:
     """[E] edge lengths -> [E, num_basis]."""

@@ -126,3 +126,20 @@ def test_exceptions_keep_their_types(gpu, monkeypatch):
     assert torch.autograd.grad(dw.sum(), x)[0].shape == x.shape
     with torch.autograd.graph.saved_tensors_hooks(fails, lambda t: t), pytest.raises(KeyError, match="none"):
         layer_norm(x, w)
+
+
+@pytest.mark.parametrize("radial_norm", [False, True])
+def test_atoms_in_one_place(gpu, radial_norm):
+    """Two atoms at the same point: energies, forces and the force loss's gradients, those to the positions among them
+    (its second derivatives in the edges' lengths), are numbers."""
+    from mace_hip import create_model, energy_and_forces, force_loss
+    model = create_model(channels=32, lmax=2, num_interactions=2, correlation=2, cutoff=4.0, device=gpu, seed=1,
+                         radial_norm=radial_norm, edge_species=radial_norm)
+    pos = torch.tensor([[0.0, 0, 0], [0, 0, 0], [1.5, 0.3, 0.2], [0.1, 1.7, -0.4]], device=gpu, requires_grad=True)
+    src, dst = (t.to(gpu) for t in (~torch.eye(4, dtype=torch.bool)).nonzero().unbind(1))
+    out = energy_and_forces(model, pos, torch.tensor([1, 6, 8, 1], device=gpu), torch.zeros(4, dtype=torch.int64, device=gpu),
+                            src, dst, torch.zeros(12, 3, device=gpu), 50.0 * torch.eye(3, device=gpu)[None], training=True)
+    force_loss(out, 4).backward()
+    grads = {"positions": pos.grad, **{n: p.grad for n, p in model.named_parameters() if p.requires_grad}}
+    for name, t in {**out, **grads}.items():
+        assert bool(t.isfinite().all()), name
