@@ -138,8 +138,8 @@ class AdamW(torch.optim.Optimizer):
 class Muon(torch.optim.Optimizer):
     """Muon (moving averages of the gradients, orthogonalised, as updates; decoupled weight decay) with torch.optim's
     interface, for contiguous float32 matrices on a GPU: parameters of two axes, or of more, whose leading ones
-    count matrices.  Arguments beyond ``muon_step``'s as for ``AdamW``; ``state`` holds each parameter's
-    ``momentum_buffer``."""
+    count matrices.  Arguments beyond ``muon_step``'s as for ``AdamW``; ``adjust_lr_fn`` None is "original";
+    ``state`` holds each parameter's ``momentum_buffer``.  States are interchangeable with ``torch.optim.Muon``'s."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, *, ns_steps=5,
                  ns_coefficients=COEFFICIENTS, eps=1e-7, adjust_lr_fn="original", max_grad_norm=None):
@@ -153,8 +153,8 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("weight_decay must not be negative, and eps must be positive")
         if not isinstance(ns_steps, int) or not 1 <= ns_steps <= MAX_STEPS or len(ns_coefficients) != 3:
             raise ValueError(f"ns_steps must be an integer in [1, {MAX_STEPS}], and ns_coefficients three numbers")
-        if adjust_lr_fn not in ADJUST:
-            raise ValueError(f"adjust_lr_fn must be one of {sorted(ADJUST)}")
+        if adjust_lr_fn is not None and adjust_lr_fn not in ADJUST:
+            raise ValueError(f"adjust_lr_fn must be None or one of {sorted(ADJUST)}")
         self.max_grad_norm, self.grad_norm = max_grad_norm, None
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       ns_steps=ns_steps, ns_coefficients=tuple(ns_coefficients), eps=eps,
@@ -194,7 +194,7 @@ class Muon(torch.optim.Optimizer):
             muon_step([p for p, _ in own], [g for _, g in own], [self.state[p]["momentum_buffer"] for p, _ in own],
                       lr=group["lr"], beta=group["momentum"], nesterov=group["nesterov"],
                       weight_decay=group["weight_decay"], steps=group["ns_steps"], coefficients=group["ns_coefficients"],
-                      eps=group["eps"], adjust=group["adjust_lr_fn"], clip=clip)
+                      eps=group["eps"], adjust=group["adjust_lr_fn"] or "original", clip=clip)
         return loss
 
     @torch.no_grad()
@@ -202,6 +202,10 @@ class Muon(torch.optim.Optimizer):
         """Restores hyperparameters and momentum.  Buffers and learning rate tensors that exist are overwritten in
         place, so a captured step goes on from what was loaded (numbers among its hyperparameters are part of the
         graph: a rate that has to follow is a tensor)."""
+        own = self.defaults.keys() - {"capturable"}      # (every step can be captured; other programs do not say so)
+        if any(own - group.keys() for group in state_dict["param_groups"]) \
+                or any("momentum_buffer" not in s for s in state_dict["state"].values()):
+            raise ValueError("the state is not that of a Muon optimizer")
         kept = {p: s["momentum_buffer"] for p, s in self.state.items()}
         rates = [group["lr"] for group in self.param_groups]
         _check_shared_rates(rates, state_dict["param_groups"])
@@ -211,6 +215,8 @@ class Muon(torch.optim.Optimizer):
                 if buffer is not None and buffer.shape != p.shape:
                     raise ValueError("the state belongs to parameters of other sizes")
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            group["capturable"] = True
         _restore_rates(rates, self.param_groups)
         for p, buffer in kept.items():
             loaded = self.state[p].get("momentum_buffer")

@@ -143,3 +143,27 @@ def test_atoms_in_one_place(gpu, radial_norm):
     grads = {"positions": pos.grad, **{n: p.grad for n, p in model.named_parameters() if p.requires_grad}}
     for name, t in {**out, **grads}.items():
         assert bool(t.isfinite().all()), name
+
+
+def test_steps_from_a_torch_optimizers_state(gpu):
+    """A state of torch.optim.Muon (no size rule named, nothing about captures) goes on, eagerly and captured."""
+    from ictc_o3.optim import Muon
+    grad = _draw((20, 30), 5, gpu, 0.1)
+    leaves = [torch.nn.Parameter(_draw((20, 30), 4, gpu)) for _ in range(3)]
+    theirs = torch.optim.Muon([leaves[0]], lr=0.05)
+    leaves[0].grad = grad.clone()
+    theirs.step()
+    own = [Muon([p], adjust_lr_fn=rule) for p, rule in zip(leaves[1:], (None, "original"))]
+    for p, o in zip(leaves[1:], own):
+        o.load_state_dict(theirs.state_dict())
+        p.grad = grad.clone()
+        o.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        own[0].step()
+    for _ in range(3):
+        graph.replay()
+        own[1].step()
+        torch.cuda.synchronize()
+        assert torch.equal(leaves[1], leaves[2])
+    assert not torch.equal(leaves[1], _draw((20, 30), 4, gpu))
