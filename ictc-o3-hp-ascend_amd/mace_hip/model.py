@@ -30,9 +30,10 @@ kernel (``gated_residual_norm``).
 layer norm before its SiLU, for deeper training at larger learning rates, and with ``edge_species`` the first one a
 row of a table for each pair of species, which the gates otherwise do not see:
 
-  h = silu(norm(W1 bessel(r) + T[s_src, s_dst])),  then twice h = silu(norm(W h));  gates = W4 (u(r) h)
+  h = silu(norm(W1 bessel(r) + T[s_src, s_dst])),  then twice h = silu(norm(W h));  gates = c W4 (u(r) h)
 
-with the cutoff envelope u on the last hidden layer, since a normalised layer does not vanish with its input.
+with the cutoff envelope u on the last hidden layer, since a normalised layer does not vanish with its input, and c the
+normalised SiLU's constant (1.679, which gives silu of a normal variable a mean square of 1).
 
 Dense layers (radial MLP, channel linears, readouts) go through ``mace_hip.linear`` (one GEMM
 per layer and degree; weight gradients reduced in row blocks).  The edge directions and the

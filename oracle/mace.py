@@ -9,6 +9,9 @@ self connection), the product block (:1145-1195 with the module's bridge-U contr
 ``_add_product_self_connection`` :94-118) and the readouts (:1434-1449,
 ``pure_cartesian_ictd_layers.py:46-70``); energy and forces as ``hp/runtime.py:84-119``.
 
+A state with weights of norms in the radial networks (``fc.1.weight`` and so on; no counterpart in the reference)
+has these between its linear layers, and with ``edge_embedding`` a row for each pair of species in the first one.
+
 Every equivariant operation goes through this package's own oracles (TensorProductOracle,
 SymmetricContractionOracle, ictc_basis.direction_harmonics_all); the parameters are read by
 name from a state dict, so the oracle evaluates exactly the function the GPU model holds.
@@ -91,6 +94,26 @@ class MaceOracle:
                 self.scs[t].u[(l, nu)] = self.p[f"{pre}.U_matrix_{nu}"].to(torch.float64)
         return w
 
+    def radial_gates(self, pre, feats, r, pairs):
+        """Interaction ``pre``'s gates [E, P*C] from the radial features, lengths and pairs of species of the edges."""
+        p = self.p
+        if f"{pre}.fc.1.weight" not in p:
+            g = feats
+            for k in (0, 2, 4):
+                g = _silu(g @ p[f"{pre}.fc.{k}.weight"].t())
+            return g @ p[f"{pre}.fc.6.weight"].t()
+        g = feats @ p[f"{pre}.fc.0.weight"].t()
+        if f"{pre}.edge_embedding" in p:
+            g = g + p[f"{pre}.edge_embedding"][pairs]
+        for k in (1, 3, 5):
+            if k > 1:
+                g = g @ p[f"{pre}.fc.{k - 1}.weight"].t()
+            g = g - g.mean(1, keepdim=True)
+            z = g / (g.square().mean(1, keepdim=True) + 1e-5).sqrt() * p[f"{pre}.fc.{k}.weight"] + p[f"{pre}.fc.{k}.bias"]
+            g = z * torch.sigmoid(z)
+        g = g * polynomial_cutoff(r, self.cutoff, self.cutoff_p)[:, None]
+        return SILU_SCALE * g @ p[f"{pre}.fc.6.weight"].t()
+
     def atomic_energies(self, pos, species, src, dst, shifts, cell, batch):
         p, C, L = self.p, self.C, self.L
         vec = pos[dst] - pos[src] + torch.einsum("ni,nij->nj", shifts, cell[batch[src]])
@@ -108,10 +131,7 @@ class MaceOracle:
             target = L if t < self.T - 1 else 0
             hb = _blocks(h, C, lin)
             x1 = {l: torch.einsum("oc,ncm->nom", p[f"{pre}.linear_up.weights.{l}"], hb[l]) for l in hb}
-            g = feats
-            for k in (0, 2, 4):
-                g = _silu(g @ p[f"{pre}.fc.{k}.weight"].t())
-            gates = g @ p[f"{pre}.fc.6.weight"].t()
+            gates = self.radial_gates(pre, feats, r, species[src] * self.S + species[dst])
             m = self.tps[t].graph_message_blocks(x1, harm, gates, src, dst, mask, nodes=pos.shape[0])
             msg = {l: torch.einsum("oc,ncm->nom", p[f"{pre}.message_linear.weights.{l}"], m[l]) / self.avg
                    for l in range(L + 1)}
