@@ -642,7 +642,10 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
   __syncthreads();
 
   // Results leave through LDS, in whole lines.  A lane holds rows 8 (k / 4) + 4 (lane / 32) + k % 4 of column lane % 32 of
-  // each 32 x 32 product.
+  // each 32 x 32 product.  Below the diagonal of a symmetric result stands the mirror image of what is above it, in blocks
+  // of 64 within a tile as in whole tiles (hi lo' and lo hi' are added up in another order there): a matrix has the same
+  // bits with both sizes of tiles, whatever else is in the call.
+  const bool mirrors = kSym && T > 64 && ti == tj;
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -653,7 +656,11 @@ __global__ void __launch_bounds__(kMuThreads, 2) muon_product_kernel(const MuonA
         mf4 v;
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = acc[i][j][k + r];
-        *reinterpret_cast<mf4*>(&results[tile_at<T>(column, row)]) = v;
+        if (!mirrors || wi <= wj) *reinterpret_cast<mf4*>(&results[tile_at<T>(column, row)]) = v;
+        if (mirrors && wi < wj) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) results[tile_at<T>(row + r, column)] = v[r];
+        }
       }
   __syncthreads();
   const int shift = shift_of<PHASE>(a, owner, step);

@@ -167,3 +167,13 @@ def test_steps_from_a_torch_optimizers_state(gpu):
         torch.cuda.synchronize()
         assert torch.equal(leaves[1], leaves[2])
     assert not torch.equal(leaves[1], _draw((20, 30), 4, gpu))
+
+
+def test_bits_do_not_depend_on_company(gpu):
+    """Alone (tiles of 64), and beside matrices that fill the chip (tiles of 128)."""
+    from ictc_o3.operators import orthogonalize
+    us = [_draw(s, k, gpu) for k, s in enumerate(((64, 300), (130, 130), (512, 200), (9, 9), (300, 257), (1024, 1024),
+                                                  (3, 150, 700), (128, 129), (129, 128)))]
+    many = [_draw((1024, 1024), 100, gpu)] * 10
+    for a, b in zip([orthogonalize([u])[0] for u in us], orthogonalize(us + many)):
+        assert torch.equal(a, b), tuple(a.shape)
