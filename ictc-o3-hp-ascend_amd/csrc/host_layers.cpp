@@ -52,6 +52,9 @@ hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.
 const float* in(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 float* out(const Tensor& t) { return t.defined() ? t.mutable_data_ptr<float>() : nullptr; }
 
+// As the kernels read it: rows one after another, and no sign that is only noted (torch.imag of a conjugate).
+Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
+
 Tensor given(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
 
 // The workspace of a call, or nothing for a size of 0.
@@ -200,7 +203,7 @@ struct LayerNormGradient : torch::autograd::Function<LayerNormGradient> {
     } else if (cots[0].defined()) {
       if (!s.activation) need[2] = false;          // without an activation the bias is in none of the gradients
       if (need[0] || need[1] || need[2] || need[3])
-        grads = norm_second(s, inputs[0], inputs[1], inputs[2], inputs[3], cots[0].contiguous(), need);
+        grads = norm_second(s, inputs[0], inputs[1], inputs[2], inputs[3], dense(cots[0]), need);
     }
     return {grads[0], grads[1], grads[2], grads[3], Tensor(), Tensor(), Tensor()};
   }
@@ -223,7 +226,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     bool need[3];
     needed(ctx, inputs[2].defined(), need);
     if (!tops[0].defined() || !(need[0] || need[1] || need[2])) return grads;
-    const Tensor dy = tops[0].contiguous();
+    const Tensor dy = dense(tops[0]);
     if (at::GradMode::is_enabled()) {
       const std::optional<Tensor> bias = inputs[2].defined() ? std::optional<Tensor>(inputs[2]) : std::nullopt;
       const int64_t mask = need[0] | need[1] << 1 | need[2] << 2;
@@ -287,7 +290,7 @@ Tensor Lookup::forward(AutogradContext* ctx, const Tensor& table, const Tensor& 
 
 variable_list Lookup::backward(AutogradContext* ctx, variable_list tops) {
   if (!tops[0].defined()) return {Tensor(), Tensor(), Tensor()};
-  const Tensor tokens = ctx->get_saved_variables()[0], grad = tops[0].contiguous();
+  const Tensor tokens = ctx->get_saved_variables()[0], grad = dense(tops[0]);
   const int64_t rows = ctx->saved_data["rows"].toInt();
   const double scale = ctx->saved_data["scale"].toDouble();
   return {at::GradMode::is_enabled() ? TableGrad::apply(grad, tokens, rows, scale) : table_grad(grad, tokens, rows, scale),
@@ -303,7 +306,7 @@ Tensor TableGrad::forward(AutogradContext* ctx, const Tensor& grad, const Tensor
 
 variable_list TableGrad::backward(AutogradContext* ctx, variable_list tops) {
   if (!tops[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-  const Tensor tokens = ctx->get_saved_variables()[0], cot = tops[0].contiguous();
+  const Tensor tokens = ctx->get_saved_variables()[0], cot = dense(tops[0]);
   const double scale = ctx->saved_data["scale"].toDouble();
   return {at::GradMode::is_enabled() ? Lookup::apply(cot, tokens, scale) : lookup(cot, tokens, scale), Tensor(), Tensor(),
           Tensor()};
@@ -381,11 +384,11 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
   std::optional<Tensor> b;
   if (bias != Py_None) {
     check_weight(tensor(bias));
-    b = tensor(bias).contiguous();
+    b = dense(tensor(bias));
   }
   const bool rows = features.dim() == 2;
-  const Tensor y = LayerNorm::apply(rows ? features.contiguous() : features.reshape({-1, width}).contiguous(),
-                                    tensor(weight).contiguous(), b, activation, eps);
+  const Tensor y = LayerNorm::apply(dense(rows ? features : features.reshape({-1, width})),
+                                    dense(tensor(weight)), b, activation, eps);
   return THPVariable_Wrap(rows ? y : y.view(features.sizes()));
 }
 
@@ -401,7 +404,7 @@ PyObject* embedding(PyObject*, PyObject* args) {
   require_gpu_fp32(table, table);
   if (t.device() != table.device()) throw Refused("All operands must be on the same GPU");
   const bool flat = t.dim() == 1;
-  const Tensor y = Lookup::apply(table.contiguous(), flat ? t.contiguous() : t.reshape({-1}).contiguous(), scale);
+  const Tensor y = Lookup::apply(dense(table), flat ? t.contiguous() : t.reshape({-1}).contiguous(), scale);
   if (flat) return THPVariable_Wrap(y);
   auto shape = t.sizes().vec();
   shape.push_back(y.size(1));

@@ -24,7 +24,7 @@ const at::Tensor* item(PyObject* list, Py_ssize_t i, bool none, const char* what
     return nullptr;
   }
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.is_cuda() || t.scalar_type() != at::kFloat || t.layout() != at::kStrided) {
+  if (!t.is_cuda() || t.scalar_type() != at::kFloat || t.layout() != at::kStrided || t.is_neg()) {
     PyErr_Format(PyExc_ValueError, "%s must be dense FP32 tensors on a ROCm GPU", what);
     return nullptr;
   }

@@ -177,3 +177,24 @@ def test_bits_do_not_depend_on_company(gpu):
     many = [_draw((1024, 1024), 100, gpu)] * 10
     for a, b in zip([orthogonalize([u])[0] for u in us], orthogonalize(us + many)):
         assert torch.equal(a, b), tuple(a.shape)
+
+
+def test_signs_that_are_only_noted(gpu):
+    """The imaginary part of a conjugate is a view with its sign noted: taken as the numbers that it stands for, or refused
+    where addresses are all that is read."""
+    from ictc_o3.operators import embedding, gradient_norm, layer_norm, muon_step, orthogonalize
+    z = torch.complex(torch.zeros(1, 1, device=gpu), torch.full((1, 1), 2.0, device=gpu))
+    noted = torch.imag(z.conj())
+    assert noted.is_neg() and noted.is_contiguous() and noted.item() == -2.0
+    token, one, zero = torch.zeros(1, dtype=torch.int64, device=gpu), torch.ones(1, device=gpu), torch.zeros(1, device=gpu)
+    assert embedding(token, noted).item() == -2.0
+    assert layer_norm(torch.ones(1, 1, device=gpu), one, noted[0]).item() == -2.0
+    leaf = torch.ones(1, 1, device=gpu, requires_grad=True)
+    assert torch.autograd.grad(embedding(token, leaf), leaf, noted)[0].item() == -2.0
+    bias = zero.clone().requires_grad_()
+    assert torch.autograd.grad(layer_norm(leaf, one, bias), bias, noted)[0].item() == -2.0
+    own = [torch.ones(1, 1, device=gpu) for _ in range(2)]
+    for call in (lambda: orthogonalize([noted]), lambda: gradient_norm([noted]), lambda: muon_step([own[0]], [noted], [own[1]], lr=0.1),
+                 lambda: muon_step([noted], [own[0]], [own[1]], lr=0.1)):
+        with pytest.raises(ValueError):
+            call()
