@@ -7,15 +7,18 @@
 //
 // Precision.  A singular value goes through p(s) = a s + b s^3 + c s^5 in every step, so small ones grow by a = 3.4
 // each time and an error of X with them: products in bfloat16 would leave updates with 2 correct digits.  A product
-// here is of float32 accuracy on the float16 matrix cores: 2^11 x = hi + lo with hi = f16(2^11 x) and lo = f16(2^11 x - hi),
+// here is of about float32 accuracy on the float16 matrix cores: 2^11 x = hi + lo with hi = f16(2^11 x) and lo = f16(2^11 x - hi),
 // 22 bits or an absolute 2^-36, whichever is larger (entries of X and A are near 1 and below), and
 //   x y = 2^-22 (hi hi' + hi lo' + lo hi')  + (2^-22 x y, left out)
-// in one float32 accumulator (sides of up to 32: float32 products).  Three products at 16 times the float32 instructions' rate.  What a power of two is chosen
-// for grows at most 32-fold: |X| stays near 1 with coefficients for which the iteration is of use.  A matrix with |U|
-// below eps, where X stays small, is kept times another power of two (2^e, see exponent_at), so that it has as many
-// bits.  (The form that iterates A alone and multiplies X once has a third of the work for wide matrices, but doubles
-// the error's growth: singular values below 1e-3 of the largest come out wrong, 1e-4 of the result at rank-deficient
-// matrices.)
+// in one float32 accumulator (sides of up to 32: float32 products).  Three products at 16 times the float32 instructions'
+// rate.  Against 64 bits, errors of 14 kinds of matrices, rank-deficient ones among them, are 0.56 to 1.52 times those of
+// a float32 iteration on the CPU (0.43 to 1.14 times with this card's library products): the bits that x has less than a
+// float's 24 weigh less than the roundings of float32 sums, but they do weigh at sides of 200 and more.  What a power of
+// two is chosen for grows at most 32-fold: |X| stays near 1 with coefficients for which the iteration is of use.  A
+// matrix with |U| below eps, where X stays small, is kept times another power of two (2^e, see exponent_at), so that it
+// has as many bits.  (The form that iterates A alone and multiplies X once has a third of the work for wide matrices, but
+// doubles the error's growth: singular values below 1e-3 of the largest come out wrong, 1e-4 of the result at
+// rank-deficient matrices.)
 //
 // Matrices with a shorter side of more than 128: all three products are of the form P Q^T with both operands' rows along
 // the reduction (X X^T, A A^T, B (X^T)^T), so one kernel does them; X is kept in both orientations.  A and B are
@@ -23,8 +26,9 @@
 // launches: `owner` says which matrix a workgroup's tile belongs to.  Sides are padded with zeros to whole tiles, which
 // stay zero.  16 matrices of 1024 x 1024 and 8 of 1024 x 4096: average 106 us and normalise 169 (5.7 and 4.8 TB/s), then
 // each step X X^T 204, B 111, B X 358 us, 850 TFLOP/s of float16 instructions over all (a large float16 product of the
-// library 1,090): B X moves 12 bytes an entry in its epilogue (130 us at a copy's rate) and its operands through the L2
-// (171 us at the 19 TB/s it gives) for 123 us of instructions.
+// library 1,090).  By the counters B X reads 0.92 GB from memory (three times X^T and B: several XCDs take the same rows) and
+// writes 0.40 (3.7 TB/s), takes 4.2 GB from the L2 (12 TB/s of 19) and keeps the matrix cores busy for 41 % of the cycles:
+// none of them alone is the bound.
 //
 // Matrices with a shorter side of up to 128, of which most models have most: two launches a step, bound by latency.  A
 // workgroup keeps 128 columns of X at a time: it multiplies them by B, and adds what they give to the next X X^T at
@@ -87,7 +91,7 @@ struct MuonMatrix {
   float* out;
   char* x;
   int32_t rows, cols, mp, np;
-  uint32_t prep, prep_tiles, prep_across;      // tiles of the source
+  uint32_t prep, prep_across;                  // tiles of the source
   uint32_t sym, apply;                         // tiles of products
   uint32_t chunk, chunks, chunk_parts;         // chunks of columns, of `chunk_parts` times kPart
   float rate;
@@ -178,8 +182,7 @@ __device__ __forceinline__ MuonMatrix matrix_of(const MuonTensor& t, const MuonS
   m.out = t.out + b * values;
   m.x = workspace + t.base + b * s.bytes;
   m.rows = t.rows, m.cols = t.cols, m.mp = static_cast<int32_t>(s.mp), m.np = static_cast<int32_t>(s.np);
-  m.prep = t.prep + static_cast<uint32_t>(b * s.prep), m.prep_tiles = static_cast<uint32_t>(s.prep);
-  m.prep_across = static_cast<uint32_t>(s.across);
+  m.prep = t.prep + static_cast<uint32_t>(b * s.prep), m.prep_across = static_cast<uint32_t>(s.across);
   m.sym = t.sym + static_cast<uint32_t>(b * s.sym);
   m.apply = t.apply + static_cast<uint32_t>(b * s.apply);
   m.chunk = t.chunk + static_cast<uint32_t>(b * s.chunks), m.chunks = static_cast<uint32_t>(s.chunks);
@@ -385,7 +388,10 @@ template <int THREADS = kMuThreads>
 __device__ __forceinline__ Scale first_scale(const MuonArgs& a, const MuonMatrix& m, uint32_t owner, bool keeps,
                                               double* part) {
   double sum = 0.0;
-  for (uint32_t k = threadIdx.x; k < m.prep_tiles; k += THREADS) sum += a.squares[m.prep + k];
+  // (the tiles that the source has, not those of its padding, which goes by the call's other matrices)
+  const uint32_t across = (m.cols + kPrep - 1) / kPrep, tiles = (m.rows + kPrep - 1) / kPrep * across;
+  for (uint32_t k = threadIdx.x; k < tiles; k += THREADS)
+    sum += a.squares[m.prep + (across == m.prep_across ? k : k / across * m.prep_across + k % across)];
   const double norm = sqrt(muon_block_sum<THREADS>(sum, part)), share = norm / (norm + a.eps);
   const int e = share > 0.0 && share < 0.5 ? min(-ilogb(share) - 1, kMostExponent) : 0;
   if (threadIdx.x == 0 && keeps) a.exponents[owner] = e;
