@@ -23,7 +23,7 @@
 // and pass.  500,001 tokens of 64 columns, 7,921 rows: lookup 22 us (5.9 TB/s), sort 29 (six launches of 3 to 10,
 // bound by latency), sums 28 (4.6 TB/s), parts 7.  65,537 tokens of 512 columns, 50,000 rows: 36 us (7.4 TB/s; the
 // table's rows repeat), sort 21, sums 34 to 39, parts 15.  105,634 tokens of 64 columns, 100 rows: lookup 7.2, sums 14,
-// parts 10 (sorted by all workgroups together: 15 + 17 + 33).
+// parts 10.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

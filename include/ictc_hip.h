@@ -836,8 +836,9 @@ int ictc_hip_embedding_table_grad(const void* tokens, int index_bytes, const flo
  * Orthogonalised updates of matrices (no counterpart in the reference).  A matrix U [m, n] is scaled to
  * X = U / (|U| + eps), |U| the Frobenius norm, and goes through `steps` of
  *   X <- a X + (b A + c A A) X,  A = X X^T        (a, b, c) = coefficients; m > n: of the transposed matrix
- * which brings its singular values near 1.  Products are of float32 accuracy (operands in two float16 parts, for which
- * coefficients have to keep singular values below 5: beyond, results may not be numbers).
+ * which brings its singular values near 1.  Products are of about float32 accuracy (operands in two float16 parts, 22 bits
+ * and more: results' errors are 0.4 to 1.5 times those of float32 products; coefficients have to keep singular values below
+ * 5: beyond, results may not be numbers).  A matrix's result does not depend on what else is in the call.
  *
  * Host arrays of `count` tensors, each of `batches` contiguous matrices of rows x cols; device addresses in them
  * are read before the call returns.
@@ -851,7 +852,9 @@ int ictc_hip_embedding_table_grad(const void* tokens, int index_bytes, const flo
  * A clip[1] that is not a number leaves everything as it is.  lr_device, if not null, is one float on the device
  * that takes the place of desc->lr.  No two tensors may overlap.
  *
- * workspace: ictc_hip_muon_workspace(rows, cols, batches, count) bytes (negative: -ictc_status), 256-byte aligned.
+ * workspace: ictc_hip_muon_workspace(rows, cols, batches, count) bytes (negative: -ictc_status), 256-byte aligned: what
+ * the matrices need, 24 KB each at least, or about 2 GiB (more if one matrix does), through which longer lists and
+ * stacks go in turn.
  */
 #define ICTC_MUON_SHAPE 0
 #define ICTC_MUON_MATCH_RMS 1
@@ -864,7 +867,7 @@ typedef struct ictc_muon_desc {
     double coefficients[3];
     float lr;                  /* >= 0 */
     int32_t nesterov;
-    int32_t steps;             /* [0, ICTC_MUON_MAX_STEPS] */
+    int32_t steps;             /* [1, ICTC_MUON_MAX_STEPS] */
     int32_t adjust;            /* ICTC_MUON_SHAPE or ICTC_MUON_MATCH_RMS */
 } ictc_muon_desc;
 
